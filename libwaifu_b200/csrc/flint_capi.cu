@@ -20,6 +20,7 @@
 #include "block_sm100.cuh"
 #include "skinny_sm100.cuh"
 #include "attention_sm100.cuh"
+#include "cache_attention_sm100.cuh"
 #include "elementwise_sm100.cuh"
 #include "fewrow_tc_sm100.cuh"
 #include "peer_sm100.cuh"
@@ -169,6 +170,8 @@ struct DeviceState {
   // (zero between launches). Made once, on the first GEMM, and kept.
   float *sk_partials = nullptr;
   uint32_t *sk_counters = nullptr;
+  // Counters of the attention over a key-value cache (zero between calls), made on its first call and kept.
+  uint32_t *cache_counters = nullptr;
   // Upload destinations on their way back to the pool: a block taken on the copy stream goes back
   // in that stream's order (so that the next upload reuses it at once), but only after the compute
   // stream's last use of it has completed, which `used` marks; nothing waits, the list is swept
@@ -304,10 +307,11 @@ uint32_t *status_word() {
 // has been looked up on this device, 0 before. The caller has synchronised the stream.
 uint32_t take_static_status();
 
-// A GEMM that gave up on a wait may have left some of the stream-K counters counted up.
+// A kernel that gave up on a wait may have left some of the stream-K or key-value cache counters counted up.
 void rezero_stream_k_counters() {
   std::lock_guard<std::mutex> lock(g_mutex);
   if (g_dev.sk_counters) cudaMemsetAsync(g_dev.sk_counters, 0, gemm_stream_k_counter_words() * sizeof(uint32_t), 0);
+  if (g_dev.cache_counters) cudaMemsetAsync(g_dev.cache_counters, 0, kCacheCounters * sizeof(uint32_t), 0);
 }
 
 // A kernel that gave up on a wait in an earlier call is reported by the next call.
@@ -2438,6 +2442,337 @@ int32_t fl_attention(fl_operators_t operators, fl_tensor_view_t q_h, fl_tensor_v
     cudaError_t e = attention(a, &why);
     if (e != cudaSuccess) cuda_check(e, (std::string("attention: ") + why).c_str());
     g_block_launches += plan.launches;
+    return clear_error();
+  });
+}
+
+// ---- attention over a key-value cache, and eviction from it ------------------------------------
+
+namespace {
+
+// The workspace of these entry points: a block of its own, grown like the scratch arena and in stream 0's order. A
+// call's launches go out under the lock, so that two threads' calls do not interleave in it.
+std::mutex g_cache_mutex;
+uint8_t *g_cache_block = nullptr;
+size_t g_cache_cap = 0;
+
+uint8_t *cache_workspace_locked(size_t bytes) {
+  if (bytes > g_cache_cap) {
+    ensure_pool();
+    const size_t cap = bytes + bytes / 4 + (1 << 20);
+    if (g_cache_block) {
+      cuda_check(cudaFreeAsync(g_cache_block, 0), "cudaFreeAsync(workspace)");
+      g_cache_block = nullptr;
+      g_cache_cap = 0;
+    }
+    void *p = nullptr;
+    cuda_check(cudaMallocAsync(&p, cap, 0), "cudaMallocAsync(workspace)");
+    g_cache_block = static_cast<uint8_t *>(p);
+    g_cache_cap = cap;
+  }
+  return g_cache_block;
+}
+
+uint32_t *cache_counters() {
+  ensure_pool();
+  std::lock_guard<std::mutex> lock(g_mutex);
+  if (!g_dev.cache_counters) {
+    void *p = nullptr;
+    cuda_check(cudaMallocAsync(&p, kCacheCounters * sizeof(uint32_t), 0), "cudaMallocAsync(counters)");
+    cuda_check(cudaMemsetAsync(p, 0, kCacheCounters * sizeof(uint32_t), 0), "cudaMemsetAsync(counters)");
+    g_dev.cache_counters = static_cast<uint32_t *>(p);
+  }
+  return g_dev.cache_counters;
+}
+
+// Whether the bytes two views reach meet.
+bool views_overlap(const fl_tensor_view_impl_t &a, const fl_tensor_view_impl_t &b) {
+  auto end = [](const fl_tensor_view_impl_t &v) {
+    int64_t last = 0;
+    for (size_t i = 0; i < v.shape.size(); ++i) last += static_cast<int64_t>(v.shape[i] - 1) * v.stride[i];
+    return raw_ptr(v) + (last + 1) * dtype_size(v.data->dtype);
+  };
+  if (numel_of(a) == 0 || numel_of(b) == 0) return false;
+  return raw_ptr(a) < end(b) && raw_ptr(b) < end(a);
+}
+
+void check_lens(const fl_tensor_view_impl_t &lens, int batch, const char *what) {
+  if (dtype_of(lens) != FL_DTYPE_INT32 || lens.shape != std::vector<int32_t>{batch} || !is_contiguous(lens)) {
+    invalid(std::string(what) + " is not a contiguous <int32>(" + std::to_string(batch) + ")");
+  }
+  if (device_of(lens) != FL_DEVICE_CUDA) invalid(std::string(what) + " is not on the operators' device");
+}
+
+// A float (batch, kv_heads, length) whose last dimension is contiguous.
+void check_weights(const fl_tensor_view_impl_t &w, int batch, int kv_heads, int length, const char *what) {
+  const std::vector<int32_t> shape{batch, kv_heads, length};
+  if (dtype_of(w) != FL_DTYPE_FLOAT || w.shape != shape) invalid(std::string(what) + " is not <float>" + shape_string(shape));
+  if (device_of(w) != FL_DEVICE_CUDA) invalid(std::string(what) + " is not on the operators' device");
+  if (length > 1 && w.stride[2] != 1) invalid(std::string(what) + "'s last dimension is not contiguous");
+}
+
+// No dimension of a written operand, or of one read through a tensor map, is repeated by a stride of 0.
+void check_not_repeated(const fl_tensor_view_impl_t &v, const char *what) {
+  for (size_t i = 0; i < v.shape.size(); ++i) {
+    if (v.shape[i] > 1 && v.stride[i] == 0) invalid(std::string(what) + " repeats a dimension through a stride of 0 (a broadcast view)");
+  }
+}
+
+// Rows are read and written sixteen bytes at a time.
+void check_rows(const fl_tensor_view_impl_t &v, const char *what) {
+  const size_t last = v.shape.size() - 1;
+  if (v.shape[last] > 1 && v.stride[last] != 1) invalid(std::string(what) + "'s last dimension is not contiguous");
+  if (!aligned16(raw_ptr(v))) invalid(std::string(what) + " does not start on a 16-byte boundary");
+  for (size_t i = 0; i < last; ++i) {
+    if (v.shape[i] > 1 && v.stride[i] % 8 != 0) invalid(std::string(what) + " has a stride that is not a multiple of 8 elements");
+  }
+}
+
+constexpr int kMaxCacheKeys = 1 << 30;
+
+// The checks and fields the three attention entry points share.
+CacheAttentionArgs cache_attention_args(fl_operators_t operators, fl_tensor_view_t q_h, fl_tensor_view_t k_h, fl_tensor_view_t v_h,
+                                        fl_tensor_view_t kv_lens_h, fl_tensor_view_t out_h) {
+  if (!operators) invalid("operators is null");
+  const fl_tensor_view_impl_t &q = deref(q_h);
+  const fl_tensor_view_impl_t &k = deref(k_h);
+  const fl_tensor_view_impl_t &v = deref(v_h);
+  const fl_tensor_view_impl_t &out = deref(out_h);
+  const struct { const fl_tensor_view_impl_t *view; const char *name; } all[4] = {{&q, "q"}, {&k, "k"}, {&v, "v"}, {&out, "out"}};
+  for (const auto &t : all) {
+    if (t.view->shape.size() != 4) invalid("attention: q, k, v and out are four-dimensional");
+    if (device_of(*t.view) != FL_DEVICE_CUDA) invalid("an operand is not on the operators' device");
+    if (!is_half_type(dtype_of(*t.view)) || dtype_of(*t.view) != dtype_of(q)) {
+      invalid("attention: this library takes <float16> or <bfloat16> operands of one type");
+    }
+  }
+  CacheAttentionArgs a = {};
+  a.batch = q.shape[0];
+  a.heads = q.shape[1];
+  a.q_len = q.shape[2];
+  a.head_dim = q.shape[3];
+  a.kv_heads = k.shape[1];
+  a.kv_len = k.shape[2];
+  if (k.shape[0] != a.batch || k.shape[3] != a.head_dim || v.shape != k.shape) invalid("attention: k and v disagree with q or each other");
+  if (out.shape != q.shape) invalid("attention: out is not of q's shape");
+  if (a.head_dim != 64 && a.head_dim != 128) invalid("attention: head_dim is not 64 or 128 (not implemented in this library)");
+  if (a.heads <= 0 || a.kv_heads <= 0 || a.heads % a.kv_heads != 0) {
+    invalid("attention: the query heads are not a multiple of the key-value heads");
+  }
+  if (a.kv_len <= 0) invalid("attention: no keys");
+  if (a.kv_len > kMaxCacheKeys) invalid("attention: more than 2^30 keys");
+  for (const auto &t : all) check_rows(*t.view, t.name);
+  for (const auto &t : all) check_not_repeated(*t.view, t.name);
+  if (kv_lens_h) {
+    const fl_tensor_view_impl_t &lens = deref(kv_lens_h);
+    check_lens(lens, a.batch, "kv_lens");
+    a.kv_lens = reinterpret_cast<const int32_t *>(raw_ptr(lens));
+  }
+  a.q = raw_ptr(q);
+  a.k = raw_ptr(k);
+  a.v = raw_ptr(v);
+  a.out = raw_ptr(out);
+  a.is_bf16 = dtype_of(q) == FL_DTYPE_BFLOAT16;
+  for (int i = 0; i < 3; ++i) {
+    a.q_stride[i] = q.stride[i];
+    a.k_stride[i] = k.stride[i];
+    a.v_stride[i] = v.stride[i];
+    a.out_stride[i] = out.stride[i];
+  }
+  a.window = a.kv_len;
+  return a;
+}
+
+int32_t run_cache_attention(CacheAttentionArgs &a) {
+  require_kernels();
+  check_earlier_kernel_status();
+  if (a.batch == 0 || a.q_len == 0) return clear_error();
+  a.status = status_word();
+  a.stream = 0;
+  const char *why = "";
+  if (!cache_attention_supported(a, &why)) invalid(std::string("attention: ") + why + " (not implemented in this library)");
+  a.counters = cache_counters();
+  std::lock_guard<std::mutex> lock(g_cache_mutex);
+  a.workspace = cache_workspace_locked(cache_attention_workspace_bytes(a));
+  int launches = 0;
+  const cudaError_t e = cache_attention(a, &why, &launches);
+  g_block_launches += launches;
+  if (e != cudaSuccess) cuda_check(e, (std::string("attention: ") + why).c_str());
+  return clear_error();
+}
+
+}  // namespace
+
+int32_t fl_attention_window(fl_operators_t operators, fl_tensor_view_t q, fl_tensor_view_t k, fl_tensor_view_t v,
+                            fl_tensor_view_t kv_lens, int32_t window, int32_t sinks, fl_tensor_view_t out) {
+  return guard([&]() -> int32_t {
+    CacheAttentionArgs a = cache_attention_args(operators, q, k, v, kv_lens, out);
+    if (window < 1) invalid("attention: a window of " + std::to_string(window) + " keys");
+    if (sinks < 0) invalid("attention: " + std::to_string(sinks) + " first keys that stay visible");
+    // (a window or first keys beyond the cache's length hide nothing)
+    a.window = window < a.kv_len ? window : a.kv_len;
+    a.sinks = sinks < a.kv_len ? sinks : a.kv_len;
+    return run_cache_attention(a);
+  });
+}
+
+int32_t fl_attention_shared_prefix(fl_operators_t operators, fl_tensor_view_t q, fl_tensor_view_t prefix_k_h, fl_tensor_view_t prefix_v_h,
+                                   fl_tensor_view_t k, fl_tensor_view_t v, fl_tensor_view_t kv_lens, fl_tensor_view_t out) {
+  return guard([&]() -> int32_t {
+    CacheAttentionArgs a = cache_attention_args(operators, q, k, v, kv_lens, out);
+    const fl_tensor_view_impl_t &pk = deref(prefix_k_h);
+    const fl_tensor_view_impl_t &pv = deref(prefix_v_h);
+    for (const fl_tensor_view_impl_t *t : {&pk, &pv}) {
+      if (t->shape.size() != 4 || t->shape[0] != 1) invalid("attention: the prefix's keys and values are (1, kv_heads, length, head_dim)");
+      if (device_of(*t) != FL_DEVICE_CUDA) invalid("an operand is not on the operators' device");
+      if (dtype_of(*t) != dtype_of(deref(q))) invalid("attention: the prefix is not of the operands' type");
+    }
+    if (pk.shape[1] != a.kv_heads || pk.shape[3] != a.head_dim || pv.shape != pk.shape) {
+      invalid("attention: the prefix's keys and values disagree with k or each other");
+    }
+    if (pk.shape[2] <= 0) invalid("attention: an empty prefix");
+    if (pk.shape[2] > kMaxCacheKeys) invalid("attention: more than 2^30 keys");
+    check_rows(pk, "the prefix's k");
+    check_rows(pv, "the prefix's v");
+    check_not_repeated(pk, "the prefix's k");
+    check_not_repeated(pv, "the prefix's v");
+    a.prefix_k = raw_ptr(pk);
+    a.prefix_v = raw_ptr(pv);
+    a.prefix_len = pk.shape[2];
+    for (int i = 0; i < 2; ++i) {
+      a.prefix_k_stride[i] = pk.stride[i + 1];
+      a.prefix_v_stride[i] = pv.stride[i + 1];
+    }
+    return run_cache_attention(a);
+  });
+}
+
+int32_t fl_attention_weights(fl_operators_t operators, fl_tensor_view_t q, fl_tensor_view_t k, fl_tensor_view_t v, fl_tensor_view_t kv_lens,
+                             fl_tensor_view_t weights_h, fl_tensor_view_t weights_out_h, fl_tensor_view_t out) {
+  return guard([&]() -> int32_t {
+    CacheAttentionArgs a = cache_attention_args(operators, q, k, v, kv_lens, out);
+    const fl_tensor_view_impl_t &in = deref(weights_h);
+    const fl_tensor_view_impl_t &to = deref(weights_out_h);
+    check_weights(in, a.batch, a.kv_heads, a.kv_len, "weights");
+    check_weights(to, a.batch, a.kv_heads, a.kv_len, "weights_out");
+    check_not_repeated(to, "weights_out");
+    const bool in_place = raw_ptr(in) == raw_ptr(to) && in.stride == to.stride;
+    if (!in_place && views_overlap(in, to)) invalid("attention: weights and weights_out overlap without being the same view");
+    a.weights_in = reinterpret_cast<const float *>(raw_ptr(in));
+    a.weights_out = reinterpret_cast<float *>(raw_ptr(to));
+    for (int i = 0; i < 2; ++i) {
+      a.weights_in_stride[i] = in.stride[i];
+      a.weights_out_stride[i] = to.stride[i];
+    }
+    if (a.q_len == 0 && a.batch > 0) invalid("attention: no queries whose weights could be added");
+    return run_cache_attention(a);
+  });
+}
+
+int32_t fl_cache_evict(fl_operators_t operators, fl_tensor_view_t k_h, fl_tensor_view_t v_h, fl_tensor_view_t weights_h, fl_tensor_view_t kv_lens_h,
+                       int32_t keep, int32_t recent, fl_tensor_view_t k_out_h, fl_tensor_view_t v_out_h, fl_tensor_view_t weights_out_h,
+                       fl_tensor_view_t lens_out_h, fl_tensor_view_t kept_h) {
+  return guard([&]() -> int32_t {
+    if (!operators) invalid("operators is null");
+    const fl_tensor_view_impl_t &k = deref(k_h);
+    const fl_tensor_view_impl_t &v = deref(v_h);
+    const fl_tensor_view_impl_t &k_out = deref(k_out_h);
+    const fl_tensor_view_impl_t &v_out = deref(v_out_h);
+    const fl_tensor_view_impl_t &weights = deref(weights_h);
+    const fl_tensor_view_impl_t &weights_out = deref(weights_out_h);
+    const struct { const fl_tensor_view_impl_t *view; const char *name; } all[4] = {{&k, "k"}, {&v, "v"}, {&k_out, "k_out"}, {&v_out, "v_out"}};
+    for (const auto &t : all) {
+      if (t.view->shape.size() != 4) invalid(std::string("eviction: ") + t.name + " is not four-dimensional");
+      if (device_of(*t.view) != FL_DEVICE_CUDA) invalid("an operand is not on the operators' device");
+      if (!is_half_type(dtype_of(*t.view)) || dtype_of(*t.view) != dtype_of(k)) {
+        invalid("eviction: this library takes <float16> or <bfloat16> caches of one type");
+      }
+    }
+    const int batch = k.shape[0], kv_heads = k.shape[1], kv_len = k.shape[2], d = k.shape[3], out_len = k_out.shape[2];
+    if (v.shape != k.shape) invalid("eviction: k and v disagree");
+    if (k_out.shape != std::vector<int32_t>{batch, kv_heads, out_len, d} || v_out.shape != k_out.shape) {
+      invalid("eviction: k_out and v_out disagree with k or each other");
+    }
+    if (kv_len <= 0) invalid("eviction: no keys");
+    if (kv_len > kMaxCacheKeys || out_len > kMaxCacheKeys) invalid("eviction: more than 2^30 keys");
+    if (kv_heads <= 0) invalid("eviction: no key-value heads");
+    if (d <= 0 || d % 8 != 0) invalid("eviction: head_dim is not a multiple of 8");
+    if (keep < 1 || keep > out_len) {
+      invalid("eviction: " + std::to_string(keep) + " keys to keep, in room for " + std::to_string(out_len));
+    }
+    if (recent < 0 || recent > keep) invalid("eviction: " + std::to_string(recent) + " recent keys of " + std::to_string(keep) + " to keep");
+    for (const auto &t : all) check_rows(*t.view, t.name);
+    check_not_repeated(k_out, "k_out");
+    check_not_repeated(v_out, "v_out");
+    check_weights(weights, batch, kv_heads, kv_len, "weights");
+    check_weights(weights_out, batch, kv_heads, out_len, "weights_out");
+    check_not_repeated(weights_out, "weights_out");
+    CacheEvictArgs a = {};
+    if (kv_lens_h) {
+      const fl_tensor_view_impl_t &lens = deref(kv_lens_h);
+      check_lens(lens, batch, "kv_lens");
+      a.kv_lens = reinterpret_cast<const int32_t *>(raw_ptr(lens));
+    }
+    if (lens_out_h) {
+      const fl_tensor_view_impl_t &lens = deref(lens_out_h);
+      check_lens(lens, batch, "lens_out");
+      a.lens_out = reinterpret_cast<int32_t *>(raw_ptr(lens));
+    } else if (kv_lens_h) {
+      invalid("eviction: kv_lens without lens_out, which takes the new lengths");
+    }
+    const fl_tensor_view_impl_t *kept = nullptr;
+    if (kept_h) {
+      kept = &deref(kept_h);
+      if (dtype_of(*kept) != FL_DTYPE_INT32 || kept->shape != std::vector<int32_t>{batch, kv_heads, keep} || !is_contiguous(*kept)) {
+        invalid("kept is not a contiguous <int32>" + shape_string({batch, kv_heads, keep}));
+      }
+      if (device_of(*kept) != FL_DEVICE_CUDA) invalid("kept is not on the operators' device");
+    }
+    // What is written meets nothing that is read, and nothing else that is written (only lens_out may be kv_lens).
+    const fl_tensor_view_impl_t *written[4] = {&k_out, &v_out, &weights_out, kept};
+    const fl_tensor_view_impl_t *read[3] = {&k, &v, &weights};
+    for (int i = 0; i < 4; ++i) {
+      if (!written[i]) continue;
+      for (const fl_tensor_view_impl_t *r : read) {
+        if (views_overlap(*written[i], *r)) invalid("eviction: an output overlaps k, v or weights");
+      }
+      for (int j = i + 1; j < 4; ++j) {
+        if (written[j] && views_overlap(*written[i], *written[j])) invalid("eviction: two outputs overlap");
+      }
+    }
+    require_kernels();
+    check_earlier_kernel_status();
+    if (batch == 0) return clear_error();
+    if (static_cast<int64_t>(batch) * kv_heads > INT32_MAX) invalid("eviction: more than 2^31 - 1 heads in the batch");
+    a.k = raw_ptr(k);
+    a.v = raw_ptr(v);
+    a.k_out = raw_ptr(k_out);
+    a.v_out = raw_ptr(v_out);
+    a.batch = batch;
+    a.kv_heads = kv_heads;
+    a.kv_len = kv_len;
+    a.out_len = out_len;
+    a.row_bytes = d * 2;
+    for (int i = 0; i < 3; ++i) {
+      a.k_stride[i] = static_cast<int64_t>(k.stride[i]) * 2;
+      a.v_stride[i] = static_cast<int64_t>(v.stride[i]) * 2;
+      a.k_out_stride[i] = static_cast<int64_t>(k_out.stride[i]) * 2;
+      a.v_out_stride[i] = static_cast<int64_t>(v_out.stride[i]) * 2;
+    }
+    a.weights = reinterpret_cast<const float *>(raw_ptr(weights));
+    a.weights_out = reinterpret_cast<float *>(raw_ptr(weights_out));
+    for (int i = 0; i < 2; ++i) {
+      a.weights_stride[i] = weights.stride[i];
+      a.weights_out_stride[i] = weights_out.stride[i];
+    }
+    a.keep = keep;
+    a.recent = recent;
+    a.stream = 0;
+    std::lock_guard<std::mutex> lock(g_cache_mutex);
+    a.kept = kept ? reinterpret_cast<int32_t *>(raw_ptr(*kept))
+                  : reinterpret_cast<int32_t *>(cache_workspace_locked(static_cast<size_t>(batch) * kv_heads * keep * 4));
+    cuda_check(cache_evict(a), "eviction");
+    g_block_launches += 2;
     return clear_error();
   });
 }

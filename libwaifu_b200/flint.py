@@ -143,6 +143,10 @@ def lib() -> ctypes.CDLL:
     L.fl_qk_norm_rope.restype = c_int32
     L.fl_attention.argtypes = [V, V, V, V, c_int32, c_int32, V]
     L.fl_attention.restype = c_int32
+    L.fl_attention_window.argtypes = [V, V, V, V, V, c_int32, c_int32, V]; L.fl_attention_window.restype = c_int32
+    L.fl_attention_shared_prefix.argtypes = [V, V, V, V, V, V, V, V]; L.fl_attention_shared_prefix.restype = c_int32
+    L.fl_attention_weights.argtypes = [V, V, V, V, V, V, V, V]; L.fl_attention_weights.restype = c_int32
+    L.fl_cache_evict.argtypes = [V, V, V, V, V, c_int32, c_int32, V, V, V, V, V]; L.fl_cache_evict.restype = c_int32
     L.fl_sm100_set_device.argtypes = [c_int32]
     L.fl_sm100_synchronize.argtypes = [POINTER(c_int32)]
     L.fl_sm100_launch_count.restype = c_int64
@@ -703,6 +707,68 @@ def attention(q: Tensor, k: Tensor, v: Tensor, mask_type: int = MaskType.NONE, b
         out = Tensor.empty(tuple(q.shape), q.dtype)
     check(lib().fl_attention(operators(), q.raw(), k.raw(), v.raw(), int(mask_type), int(block_size), out.raw()))
     return out
+
+
+def attention_window(q: Tensor, k: Tensor, v: Tensor, window: int, sinks: int = 0, kv_lens: Optional[Tensor] = None,
+                     out: Optional[Tensor] = None) -> Tensor:
+    """Attention over a key-value cache under a sliding window: q (N, heads, L, D), k and v (N, kv_heads, S, D)
+    of which sequence n holds kv_lens[n] keys (all S without kv_lens). Query i, at position
+    p = i + kv_lens[n] - L, sees key j <= p if j > p - window or j < sinks; where it sees none its result is 0.
+    A window of S or more is causal attention over the cache."""
+    if out is None:
+        out = Tensor.empty(tuple(q.shape), q.dtype)
+    check(lib().fl_attention_window(operators(), q.raw(), k.raw(), v.raw(), kv_lens.raw() if kv_lens else None, int(window),
+                                    int(sinks), out.raw()))
+    return out
+
+
+def attention_shared_prefix(q: Tensor, prefix_k: Tensor, prefix_v: Tensor, k: Tensor, v: Tensor,
+                            kv_lens: Optional[Tensor] = None, out: Optional[Tensor] = None) -> Tensor:
+    """Attention of a batch whose sequences share their beginning: every query sees all of prefix_k and
+    prefix_v (1, kv_heads, P, D), read once for the whole batch, and its own sequence's keys as in
+    attention_window without a window."""
+    if out is None:
+        out = Tensor.empty(tuple(q.shape), q.dtype)
+    check(lib().fl_attention_shared_prefix(operators(), q.raw(), prefix_k.raw(), prefix_v.raw(), k.raw(), v.raw(),
+                                           kv_lens.raw() if kv_lens else None, out.raw()))
+    return out
+
+
+def attention_weights(q: Tensor, k: Tensor, v: Tensor, weights: Tensor, kv_lens: Optional[Tensor] = None,
+                      weights_out: Optional[Tensor] = None, out: Optional[Tensor] = None):
+    """Causal attention over a key-value cache that also adds each key's softmax weights, summed over its query
+    heads and the queries, to `weights` <float>(N, kv_heads, S); returns (out, weights_out). Without
+    weights_out the sums are added in place."""
+    if out is None:
+        out = Tensor.empty(tuple(q.shape), q.dtype)
+    if weights_out is None:
+        weights_out = weights
+    check(lib().fl_attention_weights(operators(), q.raw(), k.raw(), v.raw(), kv_lens.raw() if kv_lens else None, weights.raw(),
+                                     weights_out.raw(), out.raw()))
+    return out, weights_out
+
+
+def cache_evict(k: Tensor, v: Tensor, weights: Tensor, keep: int, recent: int = 0, kv_lens: Optional[Tensor] = None,
+                k_out: Optional[Tensor] = None, v_out: Optional[Tensor] = None, weights_out: Optional[Tensor] = None,
+                lens_out: Optional[Tensor] = None, kept: Optional[Tensor] = None):
+    """Copies a cache's `recent` last keys and, of the others, the keep - recent of the largest weight, per
+    sequence and key-value head and in the order of their positions, to the first rows of k_out and v_out
+    (made with room for `keep` here); returns (k_out, v_out, weights_out, lens_out). lens_out takes the new
+    lengths (kv_lens may be passed for it; None without kv_lens means none is wanted), `kept`
+    <int32>(N, kv_heads, keep), if given, the kept keys' positions, -1 past the last."""
+    n, h, _, d = k.shape
+    if k_out is None:
+        k_out = Tensor.empty((n, h, int(keep), d), k.dtype)
+    if v_out is None:
+        v_out = Tensor.empty((n, h, int(k_out.shape[2]), d), v.dtype)
+    if weights_out is None:
+        weights_out = Tensor.empty((n, h, int(k_out.shape[2])), DType.FLOAT)
+    if lens_out is None and kv_lens is not None:
+        lens_out = Tensor.empty((n,), DType.INT32)
+    check(lib().fl_cache_evict(operators(), k.raw(), v.raw(), weights.raw(), kv_lens.raw() if kv_lens else None, int(keep),
+                               int(recent), k_out.raw(), v_out.raw(), weights_out.raw(), lens_out.raw() if lens_out else None,
+                               kept.raw() if kept else None))
+    return k_out, v_out, weights_out, lens_out
 
 
 def quantize_fp8_activation(a: Tensor):

@@ -1,0 +1,109 @@
+"""The entry points over a key-value cache without a GPU: what they refuse, before any device work. The views lie over
+addresses that are never touched: a call that passes every check ends at the missing device, with another code."""
+import pytest
+
+
+def at(F, shape, dtype, stride=None, address=1 << 20, room=1 << 40):
+    return F.Tensor.from_device_ptr(address, shape, dtype, stride=stride, numel=room)
+
+
+def operands(F, dt, N=2, H=4, Hk=2, L=1, S=10, D=64, P=6):
+    t = {"q": at(F, (N, H, L, D), dt), "k": at(F, (N, Hk, S, D), dt), "v": at(F, (N, Hk, S, D), dt), "out": at(F, (N, H, L, D), dt),
+         "pk": at(F, (1, Hk, P, D), dt), "pv": at(F, (1, Hk, P, D), dt), "lens": at(F, (N,), F.DType.INT32),
+         "w": at(F, (N, Hk, S), F.DType.FLOAT), "wo": at(F, (N, Hk, S), F.DType.FLOAT, address=1 << 30)}
+    return t
+
+
+class NoDevice:
+    def __init__(self, F):
+        self.F = F
+
+    def refused(self, call, *args):
+        code = call(*[a.raw() if hasattr(a, "raw") else a for a in args])
+        assert code != self.F.FL_OK
+        return code == self.F.FL_ERROR_INVALID_ARG, self.F.lib().fl_get_last_error_message().decode()
+
+
+@pytest.fixture()
+def no_device(flint):
+    import ctypes
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("a valid call would run")
+    return NoDevice(flint), ctypes.c_void_p(1)  # (operators cannot be made without a device: what is not null stands for them)
+
+
+def test_what_attention_refuses(flint, no_device):
+    F, (N, ops) = flint, no_device
+    L = F.lib()
+    bf, half = F.DType.BFLOAT16, F.DType.FLOAT16
+    t = operands(F, bf)
+    window = lambda **c: N.refused(L.fl_attention_window, ops, *[{**t, **c}[n] for n in ("q", "k", "v", "lens")], c.get("window", 5),  # noqa: E731
+                                   c.get("sinks", 0), {**t, **c}["out"])
+    assert not window()[0]      # the operands are fine: only the device is missing
+    assert not window(lens=None)[0]
+    bad = [
+        (dict(window=0), "a window of 0"), (dict(window=-3), "a window of -3"), (dict(sinks=-1), "first keys"),
+        (dict(k=at(F, (2, 3, 10, 64), bf), v=at(F, (2, 3, 10, 64), bf)), "multiple of the key-value heads"),
+        (dict(k=at(F, (2, 2, 0, 64), bf), v=at(F, (2, 2, 0, 64), bf)), "no keys"),
+        (dict(v=at(F, (2, 2, 9, 64), bf)), "disagree"), (dict(out=at(F, (2, 4, 2, 64), bf)), "out is not of q's shape"),
+        (dict(k=at(F, (2, 2, 10, 64), half)), "one type"), (dict(q=at(F, (2, 4, 64), bf)), "four-dimensional"),
+        (dict(q=at(F, (2, 4, 1, 96), bf), out=at(F, (2, 4, 1, 96), bf), k=at(F, (2, 2, 10, 96), bf), v=at(F, (2, 2, 10, 96), bf)), "64 or 128"),
+        (dict(k=at(F, (2, 2, 10, 64), bf, (1280, 640, 64, 2))), "k's last dimension"),
+        (dict(k=at(F, (2, 2, 10, 64), bf, (0, 640, 64, 1))), "stride of 0"), (dict(out=at(F, (2, 4, 1, 64), bf, (0, 64, 64, 1))), "stride of 0"),
+        (dict(v=at(F, (2, 2, 10, 64), bf, (1300, 650, 65, 1))), "multiple of 8"), (dict(q=at(F, (2, 4, 1, 64), bf, address=(1 << 20) + 2)), "16-byte"),
+        (dict(lens=at(F, (3,), F.DType.INT32)), "kv_lens"), (dict(lens=at(F, (2,), F.DType.LONG)), "kv_lens"),
+        (dict(lens=at(F, (2,), F.DType.INT32, (2,))), "kv_lens"),
+    ]
+    for change, words in bad:
+        refusal, message = window(**change)
+        assert refusal and words in message, (change.keys(), message)
+    assert window(q=at(F, (2, 4, 1, 64), bf, (0, 64, 64, 1)))[0]
+    assert N.refused(L.fl_attention_window, None, t["q"], t["k"], t["v"], None, 5, 0, t["out"])[0]
+
+    prefix = lambda **c: N.refused(L.fl_attention_shared_prefix, ops, *[{**t, **c}[n] for n in ("q", "pk", "pv", "k", "v", "lens", "out")])  # noqa: E731
+    assert not prefix()[0]
+    for change, words in [(dict(pk=at(F, (2, 2, 6, 64), bf)), "(1, kv_heads, length, head_dim)"), (dict(pv=at(F, (1, 2, 7, 64), bf)), "disagree"),
+                          (dict(pk=at(F, (1, 2, 0, 64), bf), pv=at(F, (1, 2, 0, 64), bf)), "empty prefix"), (dict(pk=at(F, (1, 2, 6, 64), half)), "type"),
+                          (dict(pk=at(F, (1, 2, 6, 64), bf, (768, 384, 0, 1))), "stride of 0"), (dict(pv=at(F, (1, 2, 6, 64), bf, address=(1 << 20) + 8)), "16-byte")]:
+        refusal, message = prefix(**change)
+        assert refusal and words in message, (change.keys(), message)
+
+    weights = lambda **c: N.refused(L.fl_attention_weights, ops, *[{**t, **c}[n] for n in ("q", "k", "v", "lens", "w", "wo", "out")])  # noqa: E731
+    assert not weights()[0]
+    assert not weights(wo=t["w"])[0]
+    for change, words in [(dict(w=at(F, (2, 2, 9), F.DType.FLOAT)), "weights"), (dict(wo=at(F, (2, 2, 10), bf)), "weights_out"),
+                          (dict(wo=at(F, (2, 2, 10), F.DType.FLOAT, (40, 20, 2), 1 << 30)), "contiguous"),
+                          (dict(wo=at(F, (2, 2, 10), F.DType.FLOAT, (0, 10, 1), 1 << 30)), "stride of 0"),
+                          (dict(wo=at(F, (2, 2, 10), F.DType.FLOAT, address=(1 << 20) + 4)), "overlap"),
+                          (dict(q=at(F, (2, 4, 0, 64), bf), out=at(F, (2, 4, 0, 64), bf)), "no queries")]:
+        refusal, message = weights(**change)
+        assert refusal and words in message, (change.keys(), message)
+
+
+def test_what_eviction_refuses(flint, no_device):
+    F, (N, ops) = flint, no_device
+    L = F.lib()
+    bf, fl = F.DType.BFLOAT16, F.DType.FLOAT
+    far = lambda i: (i + 2) << 32  # noqa: E731
+    t = {"k": at(F, (2, 2, 10, 24), bf), "v": at(F, (2, 2, 10, 24), bf), "w": at(F, (2, 2, 10), fl), "lens": at(F, (2,), F.DType.INT32),
+         "ko": at(F, (2, 2, 6, 24), bf, address=far(0)), "vo": at(F, (2, 2, 6, 24), bf, address=far(1)), "wo": at(F, (2, 2, 6), fl, address=far(2)),
+         "lo": at(F, (2,), F.DType.INT32, address=far(3)), "kept": at(F, (2, 2, 5), F.DType.INT32, address=far(4))}
+
+    def evict(keep=5, recent=2, **c):
+        u = {**t, **c}
+        return N.refused(L.fl_cache_evict, ops, u["k"], u["v"], u["w"], u["lens"], keep, recent, u["ko"], u["vo"], u["wo"], u["lo"], u["kept"])
+
+    assert not evict()[0] and not evict(kept=None)[0] and not evict(lens=None, lo=None)[0] and not evict(lo=t["lens"])[0]
+    for change, words in [
+            (dict(keep=0), "0 keys to keep"), (dict(keep=7), "room for 6"), (dict(recent=6), "recent"), (dict(recent=-1), "recent"),
+            (dict(v=at(F, (2, 2, 9, 24), bf)), "disagree"), (dict(vo=at(F, (2, 2, 7, 24), bf, address=far(1))), "disagree"),
+            (dict(ko=at(F, (2, 2, 6, 24), F.DType.FLOAT16, address=far(0))), "one type"), (dict(w=at(F, (2, 2, 6), fl)), "weights"),
+            (dict(wo=at(F, (2, 2, 10), fl, address=far(2))), "weights_out"), (dict(lo=None), "lens_out"), (dict(lens=at(F, (1,), F.DType.INT32)), "kv_lens"),
+            (dict(kept=at(F, (2, 2, 6), F.DType.INT32, address=far(4))), "kept"), (dict(ko=at(F, (2, 2, 6, 24), bf, address=(1 << 20) + 16)), "overlaps k, v or weights"),
+            (dict(vo=t["ko"]), "two outputs"), (dict(ko=at(F, (2, 2, 6, 24), bf, (0, 144, 24, 1), far(0))), "stride of 0"),
+            (dict(k=at(F, (2, 2, 10, 24), bf, (480, 240, 24, 1), (1 << 20) + 2)), "16-byte")]:
+        refusal, message = evict(**change)
+        assert refusal and words in message, (change.keys(), message)
+    assert evict(k=at(F, (2, 2, 10, 20), bf), v=at(F, (2, 2, 10, 20), bf), ko=at(F, (2, 2, 6, 20), bf, address=far(0)), vo=at(F, (2, 2, 6, 20), bf, address=far(1)))[0]
+    assert not evict(k=at(F, (2, 2, 10, 24), bf, (0, 0, 24, 1)))[0]  # read with their true strides: inputs may repeat
