@@ -33,6 +33,7 @@
 #include <cstdlib>
 #include <type_traits>
 
+#include "attention_tile_sm100.cuh"
 #include "gemm_sm100.cuh"
 #include "ptx_sm100.cuh"
 
@@ -40,11 +41,6 @@ namespace flsm100 {
 
 namespace {
 
-constexpr int kBlockQ = 128;   // queries per CTA = lanes of tensor memory
-constexpr int kBlockKv = 128;  // keys per step
-constexpr int kAtomBytes = 128;  // one swizzle atom: 64 16-bit elements of K
-constexpr int kAtomElems = 64;
-constexpr int kMmaKBytes = 32;   // one kind::f16 instruction: 16 elements of K
 constexpr int kSoftmaxWarps = 8;  // two per 32 queries
 constexpr int kProducerWarp = 8;
 constexpr int kMmaWarp = 9;
@@ -109,23 +105,6 @@ struct KernelParams {
   uint32_t *status;
 };
 
-__device__ __forceinline__ void tma_load_4d(void *smem_dst, const CUtensorMap *desc, uint64_t *bar, int32_t c0,
-                                            int32_t c1, int32_t c2, int32_t c3) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
-      ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(desc)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2),
-      "r"(c3)
-      : "memory");
-}
-
-__device__ __forceinline__ void tma_load_3d(void *smem_dst, const CUtensorMap *desc, uint64_t *bar, int32_t c0,
-                                            int32_t c1, int32_t c2) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-      ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(desc)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
-      : "memory");
-}
-
 // The first and the last key a query at `position` may see (flint/cuda/attention.cu:165-179).
 __device__ __forceinline__ int first_key_of(const KernelParams &p, int position) {
   return p.mask_type == 3 ? (position / p.block_size) * p.block_size : 0;
@@ -134,54 +113,6 @@ __device__ __forceinline__ int last_key_of(const KernelParams &p, int position) 
   if (p.mask_type == 0) return p.kv_len - 1;
   if (p.mask_type == 1) return min(p.kv_len - 1, position);
   return min(p.kv_len - 1, (position / p.block_size) * p.block_size + p.block_size - 1);
-}
-
-// 2^x for x <= 2^kRescaleStep's exponent: the hardware approximation (relative error 2^-22), -inf -> 0.
-__device__ __forceinline__ float fast_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// 2^x for a pair of exponents x <= 2^kRescaleStep's, without the special-function unit: that unit
-// delivers 16 results a cycle and SM, so the 128 x 128 exponentials of a block would hold it for
-// 1024 cycles; one pair in four of a row goes through here instead, on the multiply-add pipes
-// (with one softmax warp per scheduler at work at a time, more than that costs more issue slots
-// than it frees special-function cycles).
-// x = n + f with n = round(x) (the low mantissa bits of x + 1.5 * 2^23) and f in [-0.5, 0.5]; 2^f
-// by a cubic (relative error 7.5e-5, below the 16-bit rounding the probabilities get); n added
-// into the exponent field. Exponents below -126 (masked keys are -inf) give 2^-126 or 0.
-__device__ __forceinline__ void exp2_pair_poly(uint64_t x, float *e0, float *e1) {
-  float x0, x1;
-  f2_unpack(x, &x0, &x1);
-  x = f2_pack(fmaxf(x0, -126.0f), fmaxf(x1, -126.0f));
-  const uint64_t t = f2_add(x, f2_pack(12582912.0f, 12582912.0f));
-  const uint64_t n = f2_add(t, f2_pack(-12582912.0f, -12582912.0f));
-  const uint64_t f = f2_fma(n, f2_pack(-1.0f, -1.0f), x);
-  uint64_t q = f2_fma(f, f2_pack(0.05517162f, 0.05517162f), f2_pack(0.24261113f, 0.24261113f));
-  q = f2_fma(q, f, f2_pack(0.69326097f, 0.69326097f));
-  q = f2_fma(q, f, f2_pack(0.99992806f, 0.99992806f));
-  float q0, q1, t0, t1;
-  f2_unpack(q, &q0, &q1);
-  f2_unpack(t, &t0, &t1);
-  *e0 = __int_as_float(__float_as_int(q0) + (__float_as_int(t0) << 23));
-  *e1 = __int_as_float(__float_as_int(q1) + (__float_as_int(t1) << 23));
-}
-
-// max(a, b, c) in one instruction.
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
-
-__device__ __forceinline__ uint32_t pack16(float a, float b, int is_bf16) {
-  if (is_bf16) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
-  }
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t *>(&h);
 }
 
 // v (batch, kv_heads, kv_len, d) with strides -> vt (batch * kv_heads, d, kv_pad), zeros past kv_len.
@@ -640,8 +571,6 @@ attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
 // values and queries of the next unit then arrive, and its first scores are computed, under the last
 // products and the output of the one before, and barriers and tensor memory are set up once per SM. The
 // hardware hands the units out in the grid's order, as it starts CTAs.
-constexpr int kTiles = 2;
-constexpr int kTileWarps = 4;
 constexpr int kSoftmaxWarps2 = kTiles * kTileWarps;
 constexpr int kProducerWarp2 = kSoftmaxWarps2;
 constexpr int kMmaWarp2 = kSoftmaxWarps2 + 1;
@@ -654,12 +583,6 @@ constexpr int kUnitsIssueRegs = 96, kUnitsSoftmaxRegs = 200;
 static_assert(128 * kIssueRegs + kSoftmaxWarps2 * 32 * kSoftmaxRegs <= kThreads2 * 168 &&
                   128 * kUnitsIssueRegs + kSoftmaxWarps2 * 32 * kUnitsSoftmaxRegs <= kThreads2 * 168,
               "no more than the block was launched with");
-// A block's probabilities are handed over in so many parts of its keys. At head_dim 128 the product of
-// the first half runs under the exponentials of the second (2 x 24 x 4352: 396 -> 386 us); at 64,
-// where the products are half as long, one hand-over less is worth more (2 x 8 x 1000 x 2000: 34.6 us
-// in halves, 32.1 whole).
-template <int D>
-constexpr int kPartsOf = D == 128 ? 2 : 1;
 constexpr int kMaxSlots = 6;
 // Where a CTA goes on with another unit, by the blocks of keys of the longest walk and the number of units (microseconds
 // back to back, the kernel of one unit and this one; SMs: 148). A block takes a little longer in that form, so it pays
@@ -696,25 +619,16 @@ struct Tail2 {
 };
 
 template <int D>
-struct Layout2 {
-  static constexpr int kQAtoms = D / kAtomElems;
-  static constexpr int kQBytes = kQAtoms * kBlockQ * kAtomBytes;  // one tile's queries
-  static constexpr int kSlotBytes = kQAtoms * kBlockKv * kAtomBytes;  // a block of K: 128 keys x head_dim
-  static constexpr int kVAtoms = kBlockKv / kAtomElems;
-  static constexpr int kVAtomBytes = D * kAtomBytes;
-  static_assert(kVAtoms * kVAtomBytes == kSlotBytes, "a block of V^T fills a slot exactly as a block of K does");
-  static constexpr int kRoom = (227 * 1024 - kTiles * kQBytes - static_cast<int>(sizeof(Tail2))) / kSlotBytes;
+struct Layout2 : TileLayout<D> {
+  using T = TileLayout<D>;
+  static constexpr int kRoom = (227 * 1024 - kTiles * T::kQBytes - static_cast<int>(sizeof(Tail2))) / T::kSlotBytes;
   static constexpr int kSlots = kRoom < kMaxSlots ? kRoom : kMaxSlots;
   static_assert(kSlots >= 3, "K of the next block, V of this one and a load in flight");
   static constexpr int kQOff = 0;
-  static constexpr int kSlotOff = kQOff + kTiles * kQBytes;
-  static constexpr int kTailOff = kSlotOff + kSlots * kSlotBytes;
+  static constexpr int kSlotOff = kQOff + kTiles * T::kQBytes;
+  static constexpr int kTailOff = kSlotOff + kSlots * T::kSlotBytes;
   static_assert(kTailOff % 16 == 0, "the claim is 16-byte aligned");
   static constexpr int kSmemBytes = kTailOff + static_cast<int>(sizeof(Tail2));
-  static constexpr int kSCols = kBlockKv;           // tile t's scores at column t * kSCols, its P over their first half
-  static constexpr int kOCol = kTiles * kSCols;     // tile t's output at kOCol + t * D
-  static constexpr int kTmemCols = 512;
-  static_assert(kOCol + kTiles * D <= kTmemCols, "tensor memory holds 512 columns");
   static_assert(kSmemBytes <= 227 * 1024, "shared memory");
 };
 
@@ -753,110 +667,21 @@ struct Unit2 {
 // What the two kernels below share: a block's softmax, a row's output and the instructions of the products. They
 // differ in how they walk: one unit, or one after another.
 
-// Block j of the keys for one query (a lane's row of the tile): its scores from tensor memory, the running
-// maximum and sum, and the probabilities back into tensor memory, part by part. The row sees keys up to
-// `key_last`, every row of the tile those up to `common_last`.
-template <int D>
-__device__ __forceinline__ void softmax_block(const KernelParams &p, uint32_t t_scores, uint32_t t_out, int j, int common_last,
-                                              int key_last, uint64_t *p_full_bar, uint32_t lane, float *m_used_io,
-                                              float *l_run_io) {
-  constexpr int kPParts = kPartsOf<D>;
-  constexpr int kChunks = kBlockKv / 32;
-  static_assert(kChunks == 4, "four chunks of scores pack into the first two");
-  constexpr float kRescaleStep = 8.0f;
-  float m_used = *m_used_io, l_run = *l_run_io;
-  uint32_t sc[kChunks][32];  // the row's scores of the block, in one round trip
+// The row sees keys up to `key_last`, every row of the tile those up to `common_last`.
+struct HideBehind {
+  int block_key0, common_last, key_last;
+  __device__ __forceinline__ void operator()(uint32_t (&sc)[kBlockKv / 32][32]) const {
+    if (block_key0 + kBlockKv - 1 > common_last) {
 #pragma unroll
-  for (int c = 0; c < kChunks; ++c) tmem_ld_32x32(t_scores + c * 32, sc[c]);
+      for (int c = 0; c < kBlockKv / 32; ++c) {
 #pragma unroll
-  for (int c = 0; c < kChunks; ++c) tmem_ld_wait(sc[c]);
-  const int block_key0 = j * kBlockKv;
-  const bool edge = block_key0 + kBlockKv - 1 > common_last;
-  float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-  if (edge) {
-#pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
-#pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        if (block_key0 + c * 32 + i > key_last) sc[c][i] = __float_as_uint(-INFINITY);
-      }
-    }
-  }
-#pragma unroll
-  for (int c = 0; c < kChunks; ++c) {
-#pragma unroll
-    for (int i = 0; i < 32; i += 2) {
-      m4[(i >> 1) & 3] = max3(m4[(i >> 1) & 3], __uint_as_float(sc[c][i]), __uint_as_float(sc[c][i + 1]));
-    }
-  }
-  const float m_blk = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * p.scale_log2;
-  if (__any_sync(0xffffffffu, m_blk > m_used + kRescaleStep)) {
-    const float m_new = fmaxf(m_used, m_blk);
-    const float alpha = exp2f(m_used - ((m_new == -INFINITY) ? 0.0f : m_new));
-    l_run *= alpha;
-    if (j > 0) {
-#pragma unroll 1
-      for (int c = 0; c < D / 16; ++c) {  // sixteen columns at a time: the block's scores stay in registers
-        uint32_t v[16];
-        tmem_ld_32x16(t_out + c * 16, v);
-        tmem_ld_wait(v);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * alpha);
-        tmem_st_32x16(t_out + c * 16, v);
-      }
-    }
-    m_used = m_new;
-  }
-  const float m_sub = (m_used == -INFINITY) ? 0.0f : m_used;
-  // The probabilities, packed in place: pair i of the row's keys becomes column i of its P
-  // (a slot whose scores have been used by then).
-  const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2), neg_m2 = f2_pack(-m_sub, -m_sub);
-  uint64_t sums[2] = {0, 0};  // (pairs of float32 zeros)
-  auto emit = [&](auto bf16_tag, int part) {
-    constexpr int kBf16 = decltype(bf16_tag)::value ? 1 : 0;
-#pragma unroll
-    for (int h = 0; h < kChunks / kPParts; ++h) {
-      const int c = part * (kChunks / kPParts) + h;
-#pragma unroll
-      for (int i = 0; i < 32; i += 2) {
-        const uint64_t x = f2_fma(f2_pack(__uint_as_float(sc[c][i]), __uint_as_float(sc[c][i + 1])), scale2, neg_m2);
-        float e0, e1;
-        if ((i & 6) != 6) {  // one pair in four goes through the cubic, the others through the special-function unit
-          float x0, x1;
-          f2_unpack(x, &x0, &x1);
-          e0 = fast_exp2(x0);
-          e1 = fast_exp2(x1);
-        } else {
-          exp2_pair_poly(x, &e0, &e1);
+        for (int i = 0; i < 32; ++i) {
+          if (block_key0 + c * 32 + i > key_last) sc[c][i] = __float_as_uint(-INFINITY);
         }
-        sums[(i >> 1) & 1] = f2_add(sums[(i >> 1) & 1], f2_pack(e0, e1));
-        sc[c >> 1][(c & 1) * 16 + (i >> 1)] = pack16(e0, e1, kBf16);
       }
     }
-  };
-  // Each half of the block's keys is handed over as soon as it is there: its product runs under
-  // the exponentials of the other half.
-#pragma unroll
-  for (int part = 0; part < kPParts; ++part) {
-    if (p.is_bf16) {
-      emit(std::true_type{}, part);
-    } else {
-      emit(std::false_type{}, part);
-    }
-    tmem_st_32x32(t_scores + part * 32, sc[part]);
-    if (kPParts == 1) tmem_st_32x32(t_scores + 32, sc[1]);
-    tmem_st_wait();          // the probabilities and a rescaled output are in tensor memory
-    tc_fence_before_sync();  // before the MMAs that the hand-over starts
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&p_full_bar[part]);
   }
-  float s0, s1, s2, s3;
-  f2_unpack(sums[0], &s0, &s1);
-  f2_unpack(sums[1], &s2, &s3);
-  l_run += (s0 + s1) + (s2 + s3);
-  *m_used_io = m_used;
-  *l_run_io = l_run;
-}
+};
 
 // A finished row of a tile's output, divided by the sum of its probabilities.
 template <int D>
@@ -880,66 +705,6 @@ __device__ __forceinline__ void store_output(const KernelParams &p, uint32_t t_o
     }
   }
 }
-
-// The instructions of a tile's two products. The whole warp calls, the elected lane issues.
-template <int D>
-struct TileMmas {
-  using L = Layout2<D>;
-  static constexpr uint64_t kMmaStep = kMmaKBytes >> 4;
-  static constexpr int kMmasPerAtom = kAtomBytes / kMmaKBytes;
-  static constexpr int kScoreMmas = L::kQAtoms * kMmasPerAtom;
-  static constexpr int kOutMmas = L::kVAtoms * kMmasPerAtom;  // one per 16 keys: 8 columns of P each
-  uint32_t tmem_base, idesc_s, idesc_o, idesc_o_mn;
-  uint64_t qdesc0, mn_fields;
-  bool issuer, v_direct;
-
-  // With v as it lies, a slot's rows are keys: an instruction's 16 keys are 16 rows of 128 bytes on, the
-  // operand is MN-major (bit 16 of the instruction descriptor) and its runs of 64 head_dim positions
-  // lie a 128-key atom apart.
-  __device__ __forceinline__ TileMmas(const KernelParams &p, uint32_t tmem, uint32_t q_smem, bool elected)
-      : tmem_base(tmem), qdesc0(umma_desc_sw128(q_smem)),
-        mn_fields(umma_desc_sw128_mn(0, kBlockKv * kAtomBytes) ^ umma_desc_sw128(0)), issuer(elected), v_direct(p.v_direct != 0) {
-    const uint32_t fmt = p.is_bf16 ? 1u : 0u;
-    idesc_s = umma_idesc(kBlockQ, kBlockKv, fmt, fmt);
-    idesc_o = umma_idesc(kBlockQ, D, fmt, fmt);
-    idesc_o_mn = idesc_o | (1u << 16);
-  }
-
-  __device__ __forceinline__ void scores(int i, uint64_t kd) const {  // S_i = Q_i K^T
-    const uint32_t s_tmem = tmem_base + i * L::kSCols;
-    const uint64_t qd = qdesc0 + static_cast<uint64_t>(i * (L::kQBytes >> 4));
-#pragma unroll
-    for (int m = 0; m < kScoreMmas; ++m) {
-      const int a = m / kMmasPerAtom, s = m % kMmasPerAtom;
-      const uint64_t qa = qd + (((a * kBlockQ * kAtomBytes) >> 4) + s * kMmaStep);
-      const uint64_t ka = kd + (((a * kBlockKv * kAtomBytes) >> 4) + s * kMmaStep);
-      if (issuer) umma_ss<kKindF16>(s_tmem, qa, ka, idesc_s, m != 0 ? 1u : 0u);
-    }
-  }
-
-  // O_i += P_i V over one part of the block's keys
-  __device__ __forceinline__ void product(int i, int part, uint64_t vd, uint32_t first_block) const {
-    const uint32_t o_tmem = tmem_base + L::kOCol + i * D;
-    const uint32_t p_tmem = tmem_base + i * L::kSCols;
-    constexpr int kPartMmas = kOutMmas / kPartsOf<D>;
-    if (v_direct) {
-#pragma unroll
-      for (int k = 0; k < kPartMmas; ++k) {
-        const int m = part * kPartMmas + k;
-        const uint64_t va = (vd ^ mn_fields) + static_cast<uint64_t>(m * ((16 * kAtomBytes) >> 4));
-        if (issuer) umma_ts_f16(o_tmem, p_tmem + m * 8, va, idesc_o_mn, m != 0 ? 1u : (first_block ^ 1u));
-      }
-    } else {
-#pragma unroll
-      for (int k = 0; k < kPartMmas; ++k) {
-        const int m = part * kPartMmas + k;
-        const int a = m / kMmasPerAtom, s = m % kMmasPerAtom;
-        if (issuer) umma_ts_f16(o_tmem, p_tmem + m * 8, vd + (((a * L::kVAtomBytes) >> 4) + s * kMmaStep), idesc_o,
-                    m != 0 ? 1u : (first_block ^ 1u));
-      }
-    }
-  }
-};
 
 template <int D>
 __global__ void __launch_bounds__(kThreads2, 1)
@@ -1016,7 +781,7 @@ attention2_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       ok = __all_sync(0xffffffffu, mbar_wait(&t.s_full_bar[tile], j & 1, &abort_flag));
       if (!ok) break;
       tc_fence_after_sync();
-      softmax_block<D>(p, t_scores, t_out, j, common_last, key_last, t.p_full_bar[tile], lane, &m_used, &l_run);
+      softmax_block<D, false>(p.scale_log2, p.is_bf16, t_scores, t_out, j == 0, HideBehind{j * kBlockKv, common_last, key_last}, t.p_full_bar[tile], lane, &m_used, &l_run);
     }
     // The last product.
     if (ok && my_blocks > 0) {
@@ -1089,7 +854,7 @@ attention2_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       // measured 399, and 82 against 62 on 4 x 32 x 1000 causal.
       const bool issuer = elect_one();
       {
-        const TileMmas<D> mma(p, tmem_base, smem_u32(q_tile(0)), issuer);
+        const TileMmas<D> mma(p.is_bf16, p.v_direct != 0, tmem_base, smem_u32(q_tile(0)), issuer);
         const uint64_t sdesc0 = umma_desc_sw128(smem_u32(slot(0)));
         bool ok = true;
         auto commit = [&](uint64_t *bar) {
@@ -1292,7 +1057,7 @@ attention2_units_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
         if (!ok) break;
         s_phase ^= 1;
         tc_fence_after_sync();
-        softmax_block<D>(p, t_scores, t_out, j, common_last, key_last, t.p_full_bar[tile], lane, &m_used, &l_run);
+        softmax_block<D, false>(p.scale_log2, p.is_bf16, t_scores, t_out, j == 0, HideBehind{j * kBlockKv, common_last, key_last}, t.p_full_bar[tile], lane, &m_used, &l_run);
       }
       // The last product.
       if (ok && my_blocks > 0) {
@@ -1403,7 +1168,7 @@ attention2_units_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
       // measured 399, and 82 against 62 on 4 x 32 x 1000 causal.
       const bool issuer = elect_one();
       {
-        const TileMmas<D> mma(p, tmem_base, smem_u32(q_tile(0)), issuer);
+        const TileMmas<D> mma(p.is_bf16, p.v_direct != 0, tmem_base, smem_u32(q_tile(0)), issuer);
         const uint64_t sdesc0 = umma_desc_sw128(smem_u32(slot(0)));
         bool ok = true;
         auto commit = [&](uint64_t *bar) {
@@ -1522,41 +1287,6 @@ attention2_units_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
     tc_fence_after_sync();
     tmem_dealloc<1>(tmem_base, L::kTmemCols);
   }
-}
-
-using EncodeTiledFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
-                                   const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = [] {
-    void *ptr = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess) {
-      return reinterpret_cast<EncodeTiledFn>(ptr);
-    }
-    return static_cast<EncodeTiledFn>(nullptr);
-  }();
-  return fn;
-}
-
-// A byte tensor of `rank` dimensions, innermost contiguous, read in boxes of 128 bytes x box_rows
-// rows of the second dimension, 128-byte swizzle, zeros outside.
-bool make_tmap(CUtensorMap *map, const void *base, int rank, const uint64_t *dims, const uint64_t *strides_bytes,
-               uint32_t box_rows) {
-  EncodeTiledFn fn = encode_fn();
-  if (!fn) return false;
-  cuuint64_t d[4];
-  cuuint64_t s[3];
-  cuuint32_t box[4] = {static_cast<cuuint32_t>(kAtomBytes), box_rows, 1, 1};
-  cuuint32_t estr[4] = {1, 1, 1, 1};
-  for (int i = 0; i < rank; ++i) d[i] = dims[i];
-  for (int i = 0; i + 1 < rank; ++i) s[i] = strides_bytes[i];
-  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, static_cast<cuuint32_t>(rank), const_cast<void *>(base), d, s, box,
-                  estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS;
 }
 
 int round_up(int x, int to) { return (x + to - 1) / to * to; }

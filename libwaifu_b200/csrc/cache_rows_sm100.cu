@@ -15,7 +15,10 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
+
 #include "cache_common_sm100.cuh"
+#include "cache_tiles_sm100.cuh"
 #include "ptx_sm100.cuh"
 
 namespace flsm100 {
@@ -469,47 +472,73 @@ int splits_for(int64_t units, int keys) {
 
 size_t round_256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
 
-// The workspace and the launches of one call.
-struct RowsPlan {
-  int rows, row_tiles, splits;
+// From so many packed rows of a key-value head on a run takes the tiles of the tensor cores: up to there the tiles of 16
+// rows read the keys again from L2 at most three times.
+constexpr int kTilesFromRows = 64;
+
+// Which kernels a call takes, and its workspace.
+struct CachePlan {
+  int rows;         // packed rows of a run
+  bool tiles;       // the sequences' own keys (and a prefix before them in the same walk) on the tile kernel
+  int row_tiles;    // of 16, or pairs of 128
+  int splits;
+  bool prefix_apart;  // a kernel of its own over the prefix for the rows of the whole batch
+  bool prefix_tiles;
   int prefix_rows, prefix_row_tiles, prefix_splits;
   size_t part_out, part_sum, prefix_out, prefix_sum, scores, row_norm, bytes;
 };
 
-RowsPlan rows_plan(const CacheAttentionArgs &a) {
-  RowsPlan p = {};
+CachePlan cache_plan(const CacheAttentionArgs &a) {
+  CachePlan p = {};
   const int group = a.heads / a.kv_heads;
   const int64_t d = a.head_dim;
   p.rows = group * a.q_len;
-  p.row_tiles = (p.rows + kRows - 1) / kRows;
-  const int64_t units = static_cast<int64_t>(a.batch) * a.kv_heads * p.row_tiles;
-  int64_t most = a.kv_len;  // keys that the rows of a tile see between them
-  if (static_cast<int64_t>(a.window) + a.sinks + a.q_len < most) most = static_cast<int64_t>(a.window) + a.sinks + a.q_len;
-  p.splits = units <= kCacheCounters ? splits_for(units, static_cast<int>(most)) : 1;
+  p.tiles = p.rows >= kTilesFromRows && a.weights_out == nullptr;
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t off = at;
     at += round_256(bytes);
     return off;
   };
-  if (p.splits > 1) {
-    p.part_out = take(static_cast<size_t>(units) * p.splits * kRows * d * 4);
-    p.part_sum = take(static_cast<size_t>(units) * p.splits * kRows * 8);
+  int64_t most = a.kv_len;  // keys that the rows of a tile see between them
+  if (static_cast<int64_t>(a.window) + a.sinks + a.q_len < most) most = static_cast<int64_t>(a.window) + a.sinks + a.q_len;
+  const int64_t runs = static_cast<int64_t>(a.batch) * a.kv_heads;
+  size_t part_rows = 0;
+  if (p.tiles) {
+    p.row_tiles = cache_tiles_pairs(p.rows);
+    p.splits = cache_tiles_splits(runs * p.row_tiles, static_cast<int>(std::min<int64_t>(most + a.prefix_len, INT32_MAX)), kCacheCounters);
+    part_rows = p.splits > 1 ? cache_tiles_part_rows(runs * p.row_tiles, p.splits) : 0;
+  } else {
+    p.row_tiles = (p.rows + kRows - 1) / kRows;
+    const int64_t units = runs * p.row_tiles;
+    p.splits = units <= kCacheCounters ? splits_for(units, static_cast<int>(most)) : 1;
+    part_rows = p.splits > 1 ? static_cast<size_t>(units) * p.splits * kRows : 0;
   }
-  if (a.prefix_len > 0) {
+  if (part_rows > 0) {
+    p.part_out = take(part_rows * d * 4);
+    p.part_sum = take(part_rows * 8);
+  }
+  if (a.prefix_len > 0 && !p.tiles) {
+    p.prefix_apart = true;
     p.prefix_rows = a.batch * p.rows;
-    p.prefix_row_tiles = (p.prefix_rows + kRows - 1) / kRows;
-    // (as many as the kernel finds keys for: every part that the merge reads is written)
-    const int steps = (a.prefix_len + kStepKeys - 1) / kStepKeys;
-    const int wanted = splits_for(static_cast<int64_t>(a.kv_heads) * p.prefix_row_tiles, a.prefix_len);
-    const int per_split = (steps + wanted - 1) / wanted;
-    p.prefix_splits = (steps + per_split - 1) / per_split;
+    p.prefix_tiles = p.prefix_rows >= kTilesFromRows;
+    if (p.prefix_tiles) {
+      p.prefix_row_tiles = cache_tiles_pairs(p.prefix_rows);
+      p.prefix_splits = cache_tiles_splits(static_cast<int64_t>(a.kv_heads) * p.prefix_row_tiles, a.prefix_len, INT32_MAX);
+    } else {
+      p.prefix_row_tiles = (p.prefix_rows + kRows - 1) / kRows;
+      // (as many as the kernel finds keys for: every part that the merge reads is written)
+      const int steps = (a.prefix_len + kStepKeys - 1) / kStepKeys;
+      const int wanted = splits_for(static_cast<int64_t>(a.kv_heads) * p.prefix_row_tiles, a.prefix_len);
+      const int per_split = (steps + wanted - 1) / wanted;
+      p.prefix_splits = (steps + per_split - 1) / per_split;
+    }
     p.prefix_out = take(static_cast<size_t>(a.kv_heads) * p.prefix_splits * p.prefix_rows * d * 4);
     p.prefix_sum = take(static_cast<size_t>(a.kv_heads) * p.prefix_splits * p.prefix_rows * 8);
   }
   if (a.weights_out != nullptr) {
-    p.scores = take(static_cast<size_t>(a.batch) * a.kv_heads * p.rows * a.kv_len * 4);
-    p.row_norm = take(static_cast<size_t>(a.batch) * a.kv_heads * p.rows * 8);
+    p.scores = take(static_cast<size_t>(runs) * p.rows * a.kv_len * 4);
+    p.row_norm = take(static_cast<size_t>(runs) * p.rows * 8);
   }
   p.bytes = at;
   return p;
@@ -549,7 +578,7 @@ bool cache_attention_supported(const CacheAttentionArgs &a, const char **why) {
     *why = "more than 2^31 - 1 query rows";
     return false;
   }
-  const RowsPlan plan = rows_plan(a);
+  const CachePlan plan = cache_plan(a);
   if (static_cast<int64_t>(a.batch) * a.kv_heads * plan.row_tiles * plan.splits > most ||
       static_cast<int64_t>(a.batch) * a.kv_heads * ((static_cast<int64_t>(a.kv_len) + 255) / 256) > most) {
     *why = "more work than one launch indexes";
@@ -558,68 +587,102 @@ bool cache_attention_supported(const CacheAttentionArgs &a, const char **why) {
   return true;
 }
 
-size_t cache_attention_workspace_bytes(const CacheAttentionArgs &a) { return rows_plan(a).bytes; }
+size_t cache_attention_workspace_bytes(const CacheAttentionArgs &a) { return cache_plan(a).bytes; }
+
+// The fields that both kernels' parameters have alike.
+template <typename Params>
+void fill_params(const CacheAttentionArgs &a, Params *p) {
+  p->q = static_cast<const uint16_t *>(a.q);
+  p->k = static_cast<const uint16_t *>(a.k);
+  p->v = static_cast<const uint16_t *>(a.v);
+  p->out = static_cast<uint16_t *>(a.out);
+  for (int i = 0; i < 3; ++i) {
+    p->q_stride[i] = a.q_stride[i];
+    p->k_stride[i] = a.k_stride[i];
+    p->v_stride[i] = a.v_stride[i];
+    p->out_stride[i] = a.out_stride[i];
+  }
+  p->kv_lens = a.kv_lens;
+  p->kv_heads = a.kv_heads;
+  p->group = a.heads / a.kv_heads;
+  p->q_len = a.q_len;
+  p->kv_len = a.kv_len;
+  p->window = a.window;
+  p->sinks = a.sinks;
+  p->scale_log2 = 1.4426950408889634f / sqrtf(static_cast<float>(a.head_dim));
+  p->counters = a.counters;
+}
 
 cudaError_t cache_attention(const CacheAttentionArgs &a, const char **why, int *launches) {
   *why = "";
-  const RowsPlan plan = rows_plan(a);
-  RowsParams p = {};
-  p.q = static_cast<const uint16_t *>(a.q);
-  p.k = static_cast<const uint16_t *>(a.k);
-  p.v = static_cast<const uint16_t *>(a.v);
-  p.out = static_cast<uint16_t *>(a.out);
-  for (int i = 0; i < 3; ++i) {
-    p.q_stride[i] = a.q_stride[i];
-    p.k_stride[i] = a.k_stride[i];
-    p.v_stride[i] = a.v_stride[i];
-    p.out_stride[i] = a.out_stride[i];
+  const CachePlan plan = cache_plan(a);
+  auto floats = [&](size_t off) { return reinterpret_cast<float *>(a.workspace + off); };
+  auto pairs = [&](size_t off) { return reinterpret_cast<float2 *>(a.workspace + off); };
+  cudaError_t e;
+  TilesParams tiles = {};
+  fill_params(a, &tiles);
+  tiles.is_bf16 = a.is_bf16;
+  tiles.status = a.status;
+  tiles.prefix_len = a.prefix_len;
+  if (plan.tiles) {
+    tiles.runs = a.batch * a.kv_heads;
+    tiles.rows = plan.rows;
+    tiles.row_pairs = plan.row_tiles;
+    tiles.splits = plan.splits;
+    tiles.part_out = floats(plan.part_out);
+    tiles.part_sum = pairs(plan.part_sum);
+    e = cache_tiles(tiles, a, why);
+    *launches += e == cudaSuccess;
+    return e;
   }
-  p.kv_lens = a.kv_lens;
-  p.kv_heads = a.kv_heads;
-  p.group = a.heads / a.kv_heads;
-  p.q_len = a.q_len;
-  p.kv_len = a.kv_len;
-  p.window = a.window;
-  p.sinks = a.sinks;
-  p.scale_log2 = 1.4426950408889634f / sqrtf(static_cast<float>(a.head_dim));
+
+  RowsParams p = {};
+  fill_params(a, &p);
   p.rows = plan.rows;
   p.row_tiles = plan.row_tiles;
   p.splits = plan.splits;
-  p.counters = a.counters;
-  p.part_out = reinterpret_cast<float *>(a.workspace + plan.part_out);
-  p.part_sum = reinterpret_cast<float2 *>(a.workspace + plan.part_sum);
+  p.part_out = floats(plan.part_out);
+  p.part_sum = pairs(plan.part_sum);
   if (a.weights_out != nullptr) {
-    p.scores = reinterpret_cast<float *>(a.workspace + plan.scores);
-    p.row_norm = reinterpret_cast<float2 *>(a.workspace + plan.row_norm);
+    p.scores = floats(plan.scores);
+    p.row_norm = pairs(plan.row_norm);
   }
-  if (a.prefix_len > 0) {
-    p.prefix_out = reinterpret_cast<const float *>(a.workspace + plan.prefix_out);
-    p.prefix_sum = reinterpret_cast<const float2 *>(a.workspace + plan.prefix_sum);
+  if (plan.prefix_apart) {
+    if (plan.prefix_tiles) {
+      tiles.over_batch = true;
+      tiles.runs = a.kv_heads;
+      tiles.rows = plan.prefix_rows;
+      tiles.row_pairs = plan.prefix_row_tiles;
+      tiles.splits = plan.prefix_splits;
+      tiles.part_out = floats(plan.prefix_out);
+      tiles.part_sum = pairs(plan.prefix_sum);
+      e = cache_tiles(tiles, a, why);
+    } else {
+      RowsParams s = p;
+      s.over_batch = true;
+      s.k = static_cast<const uint16_t *>(a.prefix_k);
+      s.v = static_cast<const uint16_t *>(a.prefix_v);
+      for (int i = 0; i < 2; ++i) {
+        s.k_stride[i + 1] = a.prefix_k_stride[i];
+        s.v_stride[i + 1] = a.prefix_v_stride[i];
+      }
+      s.kv_len = a.prefix_len;
+      s.rows = plan.prefix_rows;
+      s.row_tiles = plan.prefix_row_tiles;
+      s.splits = plan.prefix_splits;
+      s.part_out = floats(plan.prefix_out);
+      s.part_sum = pairs(plan.prefix_sum);
+      *why = "launching the prefix's part";
+      e = launch_rows(a, s, static_cast<int64_t>(a.kv_heads) * s.row_tiles * s.splits, false);
+    }
+    if (e != cudaSuccess) return e;
+    ++*launches;
+    p.prefix_out = floats(plan.prefix_out);
+    p.prefix_sum = pairs(plan.prefix_sum);
     p.prefix_splits = plan.prefix_splits;
     p.prefix_rows = plan.prefix_rows;
-    RowsParams s = p;
-    s.over_batch = true;
-    s.k = static_cast<const uint16_t *>(a.prefix_k);
-    s.v = static_cast<const uint16_t *>(a.prefix_v);
-    for (int i = 0; i < 2; ++i) {
-      s.k_stride[i + 1] = a.prefix_k_stride[i];
-      s.v_stride[i + 1] = a.prefix_v_stride[i];
-    }
-    s.kv_len = a.prefix_len;
-    s.rows = plan.prefix_rows;
-    s.row_tiles = plan.prefix_row_tiles;
-    s.splits = plan.prefix_splits;
-    s.part_out = reinterpret_cast<float *>(a.workspace + plan.prefix_out);
-    s.part_sum = reinterpret_cast<float2 *>(a.workspace + plan.prefix_sum);
-    s.prefix_splits = 0;
-    const cudaError_t e = launch_rows(a, s, static_cast<int64_t>(a.kv_heads) * s.row_tiles * s.splits, false);
-    if (e != cudaSuccess) {
-      *why = "launching the prefix's part";
-      return e;
-    }
-    ++*launches;
   }
-  cudaError_t e = launch_rows(a, p, static_cast<int64_t>(a.batch) * a.kv_heads * p.row_tiles * p.splits, a.prefix_len > 0);
+  e = launch_rows(a, p, static_cast<int64_t>(a.batch) * a.kv_heads * p.row_tiles * p.splits, plan.prefix_apart);
   if (e != cudaSuccess) {
     *why = "launching the few-row kernel";
     return e;

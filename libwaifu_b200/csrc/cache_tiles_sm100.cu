@@ -1,0 +1,636 @@
+// Attention over a key-value cache for many query rows (prompts, and the rows of a whole batch over a prefix that
+// it shares): both products on tcgen05, in the way of the two-tile attention kernel.
+//
+// A CTA owns two tiles of 128 rows of one key-value head. The rows are packed: row r is query r / group of query
+// head r % group of the ones that share the head, so that a block of keys is read once for all of them and a
+// tile's rows sit close together (under a window a tile walks its 128 / group positions and the window, not 128
+// and the window). Over a prefix, which all of a batch sees, the rows of every sequence are packed one after the other.
+// The softmax warps gather the queries into shared memory themselves; K and V blocks of 128 keys arrive by TMA
+// into one ring of slots. The walk is a list of blocks: those of a prefix, those that hold sinks, those from the
+// first window's start to the last query's position.
+//
+// A block that some row does not see whole (past the sequence's end, at a window's edge, on the diagonal) passes two
+// more warps before its product: they clear the values of keys that no row sees and take infinities and NaN out of
+// the others, because a probability of zero times such a value is not zero. Rows that do see them have them added by
+// hand at the end.
+//
+// Few units are divided along the keys: each CTA leaves its rows' outputs relative to their own maxima, and the last
+// one to arrive (or, over a prefix, the kernel over the sequences' own keys) adds them in the order of the splits.
+#include "cache_tiles_sm100.cuh"
+
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+#include "attention_sm100.cuh"
+#include "attention_tile_sm100.cuh"
+#include "cache_common_sm100.cuh"
+
+namespace flsm100 {
+
+namespace {
+
+constexpr int kPairRows = kTiles * kBlockQ;
+constexpr int kSoftmaxWarps = kTiles * kTileWarps;
+constexpr int kProducerWarp = kSoftmaxWarps;
+constexpr int kMmaWarp = kSoftmaxWarps + 1;
+constexpr int kCleanWarp = kSoftmaxWarps + 2;  // and the one after it
+constexpr int kCleanWarps = 2;
+// Three warpgroups launched with 168 registers a thread; the one that loads, issues and cleans gives its own up to the
+// two of the softmax, which hold a row of 128 scores: 128 x 88 + 256 x 208 = 384 x 168.
+constexpr int kThreads = (kSoftmaxWarps + 4) * 32;
+constexpr int kIssueRegs = 88, kSoftmaxRegs = 208;
+static_assert(128 * kIssueRegs + kSoftmaxWarps * 32 * kSoftmaxRegs <= kThreads * 168, "no more than the block was launched with");
+constexpr int kMaxSlots = 6;
+
+struct Tail {
+  uint64_t q_full_bar[kTiles];
+  uint64_t slot_full_bar[kMaxSlots], slot_empty_bar[kMaxSlots], slot_clean_bar[kMaxSlots];
+  uint64_t s_full_bar[kTiles];     // MMA -> softmax: the tile's scores are in tensor memory
+  uint64_t p_full_bar[kTiles][2];  // softmax -> MMA: that part of the tile's probabilities is in tensor memory
+  uint64_t pv_done_bar[kTiles];    // MMA -> softmax: the last block is in the tile's output
+  uint32_t tmem_base_slot;
+  uint32_t abort_flag;
+  uint32_t patch_flag;  // values were taken out of a block
+  int is_last;
+};
+
+template <int D>
+struct Layout : TileLayout<D> {
+  using T = TileLayout<D>;
+  static constexpr int kRoom = (227 * 1024 - kTiles * T::kQBytes - static_cast<int>(sizeof(Tail))) / T::kSlotBytes;
+  static constexpr int kSlots = kRoom < kMaxSlots ? kRoom : kMaxSlots;
+  static_assert(kSlots >= 3, "K of the next block, V of this one and a load in flight");
+  static constexpr int kQOff = 0;
+  static constexpr int kSlotOff = kQOff + kTiles * T::kQBytes;
+  static constexpr int kTailOff = kSlotOff + kSlots * T::kSlotBytes;
+  static constexpr int kSmemBytes = kTailOff + static_cast<int>(sizeof(Tail));
+  static_assert(kSmemBytes <= 227 * 1024, "shared memory");
+};
+
+// The blocks of keys a pair of tiles walks, and what its rows see of them.
+struct Walk {
+  int prefix_blocks, prefix_len;
+  int sink_blocks, window_block;  // the blocks 0 .. sink_blocks - 1, then those from window_block on
+  int first, count;               // of this split
+  KeyRange range;                 // what the rows see between them
+  int first_pos, last_pos;        // of the pair's rows
+  int window, sinks;
+
+  __device__ __forceinline__ bool in_prefix(int j) const { return first + j < prefix_blocks; }
+  __device__ __forceinline__ int key0(int j) const {
+    const int at = first + j;
+    if (at < prefix_blocks) return at * kBlockKv;
+    const int own = at - prefix_blocks;
+    return (own < sink_blocks ? own : own - sink_blocks + window_block) * kBlockKv;
+  }
+  // Does some row not see some key of block j?
+  __device__ __forceinline__ bool differs(int j) const {
+    if (in_prefix(j)) return false;  // (keys past a prefix's end come as zeros)
+    const int k0 = key0(j), k1 = k0 + kBlockKv - 1;
+    return k1 > first_pos || (k1 >= sinks && k0 <= last_pos - window);
+  }
+  // How many blocks of the whole walk hold keys up to `position`.
+  __device__ __forceinline__ int blocks_up_to(int position) const {
+    const int own = position < 0 ? 0 : position / kBlockKv + 1;
+    return prefix_blocks + (own <= sink_blocks ? own : sink_blocks + max(0, own - window_block));
+  }
+};
+
+struct Unit {
+  int run, head, seq, pair, split, active;
+  int row0;  // of the pair
+  int len;
+  Walk walk;
+  int blocks[kTiles];  // how many of the split's blocks each tile walks
+
+  __device__ __forceinline__ Unit(const TilesParams &p, int at) {
+    // The longest walks first: the last pair of every run, then the one before it.
+    run = at % p.runs;
+    at /= p.runs;
+    split = at % p.splits;
+    pair = p.row_pairs - 1 - at / p.splits;
+    head = run % p.kv_heads;
+    seq = run / p.kv_heads;
+    row0 = pair * kPairRows;
+    const int last_row = min(row0 + kPairRows, p.rows) - 1;
+    walk.prefix_len = p.prefix_len;
+    walk.prefix_blocks = (p.prefix_len + kBlockKv - 1) / kBlockKv;
+    walk.window = p.window;
+    walk.sinks = p.sinks;
+    int total;
+    if (p.over_batch) {
+      len = 0;
+      walk.first_pos = walk.last_pos = 0;
+      walk.range = KeyRange{0, 0, 0};
+      walk.sink_blocks = walk.window_block = 0;
+      total = walk.prefix_blocks;
+    } else {
+      len = sequence_length(p.kv_lens, seq, p.kv_len);
+      walk.first_pos = row0 / p.group + len - p.q_len;
+      walk.last_pos = last_row / p.group + len - p.q_len;
+      walk.range = visible_keys(walk.first_pos, walk.last_pos, len, p.window, p.sinks);
+      walk.sink_blocks = (walk.range.sinks + kBlockKv - 1) / kBlockKv;
+      walk.window_block = walk.range.begin / kBlockKv;
+      if (walk.sink_blocks >= walk.window_block) walk.sink_blocks = walk.window_block = 0;  // they meet: one run of blocks
+      const int end_block = (walk.range.end + kBlockKv - 1) / kBlockKv;
+      total = walk.prefix_blocks + walk.sink_blocks + max(0, end_block - walk.window_block);
+    }
+    const int per_split = max(1, (total + p.splits - 1) / p.splits);
+    active = max(1, (total + per_split - 1) / per_split);
+    walk.first = split * per_split;
+    walk.count = max(0, min(per_split, total - walk.first));
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) {
+      const int first_row = row0 + i * kBlockQ, last = min(first_row + kBlockQ, p.rows) - 1;
+      const int mine = p.over_batch ? total : min(total, walk.blocks_up_to(last / p.group + len - p.q_len));
+      blocks[i] = first_row >= p.rows ? 0 : max(0, min(walk.count, mine - walk.first));
+    }
+  }
+};
+
+// Bits 0 .. n - 1.
+__device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u); }
+
+// Of the keys from key0 on, the row sees those up to `last`, behind `before` or below `sinks`.
+struct HideUnseen {
+  bool edge;
+  int key0, last, before, sinks;
+  __device__ __forceinline__ void operator()(uint32_t (&sc)[kBlockKv / 32][32]) const {
+    if (!edge) return;
+#pragma unroll
+    for (int c = 0; c < kBlockKv / 32; ++c) {
+      const int base = key0 + c * 32;
+      const uint32_t seen = bits_below(last + 1 - base) & (~bits_below(before + 1 - base) | bits_below(sinks - base));
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        if (!((seen >> i) & 1u)) sc[c][i] = __float_as_uint(-INFINITY);
+      }
+    }
+  }
+};
+
+// The address of packed row r of a head's queries (or results).
+__device__ __forceinline__ int64_t row_offset(const TilesParams &p, const int64_t (&stride)[3], int head, int seq, int r) {
+  if (p.over_batch) {
+    seq = r / (p.group * p.q_len);
+    r -= seq * p.group * p.q_len;
+  }
+  const int i = r / p.group, g = r - i * p.group;
+  return seq * stride[0] + static_cast<int64_t>(head * p.group + g) * stride[1] + i * stride[2];
+}
+
+// Adds what a row sees of the infinities and NaN that were taken out of its blocks: rare, and as slow as it is plain.
+template <int D, bool BF16>
+__device__ __noinline__ void patch_row(const TilesParams &p, int unit, int pos, const uint16_t *q, float m, float l, uint16_t *out, float *part) {
+  const Unit u(p, unit);
+  for (int j = 0; j < u.walk.count; ++j) {
+    if (!u.walk.differs(j)) continue;
+    for (int key = u.walk.key0(j); key < u.walk.key0(j) + kBlockKv; ++key) {
+      if (key > pos || key >= u.len || !(key > pos - p.window || key < p.sinks)) continue;
+      const uint16_t *v = p.v + u.seq * p.v_stride[0] + u.head * p.v_stride[1] + key * p.v_stride[2];
+      const uint16_t *k = p.k + u.seq * p.k_stride[0] + u.head * p.k_stride[1] + key * p.k_stride[2];
+      bool odd = false;
+      for (int d = 0; d < D; d += 8) odd |= has_nonfinite<BF16>(*reinterpret_cast<const uint4 *>(v + d));
+      if (!odd) continue;
+      float s = 0.0f;
+      for (int d = 0; d < D; d += 2) {
+        const float2 x = widen_pair<BF16>(*reinterpret_cast<const uint32_t *>(q + d)), y = widen_pair<BF16>(*reinterpret_cast<const uint32_t *>(k + d));
+        s = fmaf(x.x, y.x, fmaf(x.y, y.y, s));
+      }
+      const float w = exp2f(s * p.scale_log2 - m);
+      for (int d = 0; d < D; ++d) {
+        const float x = widen_pair<BF16>(v[d]).x;
+        if (fabsf(x) < INFINITY) continue;
+        if (part != nullptr) {
+          part[d] += w * x;
+        } else {
+          out[d] = static_cast<uint16_t>(pack_pair<BF16>(widen_pair<BF16>(out[d]).x + w / l * x, 0.0f));
+        }
+      }
+    }
+  }
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1)
+cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
+                   const __grid_constant__ CUtensorMap tmap_pk, const __grid_constant__ CUtensorMap tmap_pv,
+                   const __grid_constant__ TilesParams p) {
+  using L = Layout<D>;
+  constexpr int S = L::kSlots;
+  constexpr int kPParts = kPartsOf<D>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  Tail &t = *reinterpret_cast<Tail *>(smem + L::kTailOff);
+  volatile uint32_t &abort_flag = *reinterpret_cast<volatile uint32_t *>(&t.abort_flag);
+
+  const uint32_t warp = threadIdx.x >> 5;
+  const uint32_t lane = threadIdx.x & 31;
+  griddep_launch_dependents();
+  if ((smem_u32(smem) & 1023u) != 0) {
+    if (threadIdx.x == 0) atomicCAS(p.status, 0u, kStatusAttentionLayout);
+    return;
+  }
+  const Unit u(p, blockIdx.x);
+  if (u.split >= u.active) return;
+
+  if (threadIdx.x == 0) {
+    t.abort_flag = 0;
+    t.patch_flag = 0;
+    for (int i = 0; i < S; ++i) {
+      mbar_init(&t.slot_full_bar[i], 1);
+      mbar_init(&t.slot_empty_bar[i], 1);
+      mbar_init(&t.slot_clean_bar[i], kCleanWarps);
+    }
+    for (int i = 0; i < kTiles; ++i) {
+      mbar_init(&t.q_full_bar[i], kTileWarps);
+      mbar_init(&t.s_full_bar[i], 1);
+      for (int h = 0; h < kPParts; ++h) mbar_init(&t.p_full_bar[i][h], kTileWarps);
+      mbar_init(&t.pv_done_bar[i], 1);
+    }
+    fence_barrier_init();
+  }
+  if (warp == kProducerWarp && lane == 0) {
+    tma_prefetch_desc(&tmap_k);
+    tma_prefetch_desc(&tmap_v);
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc<1>(&t.tmem_base_slot, L::kTmemCols);
+    tmem_relinquish<1>();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = t.tmem_base_slot;
+
+  auto q_tile = [&](int i) { return smem + L::kQOff + i * L::kQBytes; };
+  auto slot = [&](int i) { return smem + L::kSlotOff + i * L::kSlotBytes; };
+
+  // Load n of the ring (K of block n / 2 when n is even, V of it when odd) goes to slot n % S.
+  if (warp < kSoftmaxWarps) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    // ------------------------------------------------------------------ queries, softmax and output
+    const int tile = static_cast<int>(warp >> 2);
+    const uint32_t quarter = warp & 3;
+    const int row_in_tile = static_cast<int>(quarter) * 32 + static_cast<int>(lane);
+    const int tile_row0 = u.row0 + tile * kBlockQ;
+    const int my_blocks = tile == 0 ? u.blocks[0] : u.blocks[1];
+    {
+      // This warp's 32 rows, a few at a time: piece c of row r of an atom lies at c ^ (r & 7).
+      constexpr int kPieces = D / 8, kRowsAtOnce = 32 / kPieces;
+      const int c = lane % kPieces;
+#pragma unroll 4
+      for (int i = 0; i < 32 / kRowsAtOnce; ++i) {
+        const int in_tile = static_cast<int>(quarter) * 32 + i * kRowsAtOnce + static_cast<int>(lane) / kPieces;
+        const int r = tile_row0 + in_tile;
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (r < p.rows) x = *reinterpret_cast<const uint4 *>(p.q + row_offset(p, p.q_stride, u.head, u.seq, r) + c * 8);
+        *reinterpret_cast<uint4 *>(q_tile(tile) + (c >> 3) * kBlockQ * kAtomBytes + in_tile * kAtomBytes + (((c & 7) ^ (in_tile & 7)) << 4)) = x;
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&t.q_full_bar[tile]);
+    }
+    const int row = tile_row0 + row_in_tile;
+    const bool live = row < p.rows;
+    const int pos = min(row, p.rows - 1) / p.group + u.len - p.q_len;
+    // What every row of the tile sees.
+    const int common_last = tile_row0 / p.group + u.len - p.q_len;
+    const int common_before = (min(tile_row0 + kBlockQ, p.rows) - 1) / p.group + u.len - p.q_len - p.window;
+    const uint32_t t_lane = tmem_base + ((quarter * 32u) << 16);
+    const uint32_t t_scores = t_lane + tile * L::kSCols;  // the row's 128 scores, then its 128 probabilities in 64 columns
+    const uint32_t t_out = t_lane + L::kOCol + tile * D;
+    float m_used = -INFINITY;
+    float l_run = 0.0f;
+    bool ok = true;
+    for (int j = 0; j < my_blocks && ok; ++j) {
+      // (Scores of block j are issued behind the product of block j - 1: once they are here the tile's
+      // output is complete up to that block.)
+      ok = __all_sync(0xffffffffu, mbar_wait(&t.s_full_bar[tile], j & 1, &abort_flag));
+      if (!ok) break;
+      tc_fence_after_sync();
+      HideUnseen hide;
+      hide.key0 = u.walk.key0(j);
+      if (u.walk.in_prefix(j)) {
+        hide.edge = hide.key0 + kBlockKv > p.prefix_len;
+        hide.last = p.prefix_len - 1;
+        hide.before = -1;
+        hide.sinks = 0;
+      } else {
+        hide.edge = hide.key0 + kBlockKv - 1 > common_last || (hide.key0 + kBlockKv - 1 >= p.sinks && hide.key0 <= common_before);
+        hide.last = pos;
+        hide.before = pos - p.window;
+        hide.sinks = p.sinks;
+      }
+      softmax_block<D, true>(p.scale_log2, p.is_bf16, t_scores, t_out, j == 0, hide, t.p_full_bar[tile], lane, &m_used, &l_run);
+    }
+    // The last product.
+    if (ok && my_blocks > 0) {
+      ok = __all_sync(0xffffffffu, mbar_wait(&t.pv_done_bar[tile], 0, &abort_flag));
+      tc_fence_after_sync();
+    }
+    const bool parts = p.over_batch || u.active > 1;
+    // The index of this row's part of split s: (kv_head, split, rows) over a prefix, (unit, split, 256) else.
+    const int64_t part_row0 = p.over_batch ? static_cast<int64_t>(u.head) * p.splits * p.rows + row
+                                           : (static_cast<int64_t>(u.run) * p.row_pairs + u.pair) * p.splits * kPairRows + (row - u.row0);
+    const int64_t part_step = p.over_batch ? p.rows : kPairRows;
+    const bool empty = p.prefix_len == 0 && pos < 0;  // sees no key: zeros
+    uint16_t *dst = live && !p.over_batch ? p.out + row_offset(p, p.out_stride, u.head, u.seq, row) : nullptr;
+    float *part_dst = p.part_out + (part_row0 + u.split * part_step) * D;
+    // (a row whose every score is -inf has no softmax)
+    float inv = empty ? 0.0f : (m_used == -INFINITY ? NAN : 1.0f / l_run);
+    if (ok) {
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t v[32];
+        if (my_blocks > 0) {
+          tmem_ld_32x32(t_out + c * 32, v);
+          tmem_ld_wait(v);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = 0;
+        }
+        if (live && parts) {
+#pragma unroll
+          for (int g = 0; g < 8; ++g) *reinterpret_cast<uint4 *>(part_dst + c * 32 + g * 4) = make_uint4(v[g * 4], v[g * 4 + 1], v[g * 4 + 2], v[g * 4 + 3]);
+        } else if (live) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            uint4 w;
+            w.x = pack16(__uint_as_float(v[g * 8 + 0]) * inv, __uint_as_float(v[g * 8 + 1]) * inv, p.is_bf16);
+            w.y = pack16(__uint_as_float(v[g * 8 + 2]) * inv, __uint_as_float(v[g * 8 + 3]) * inv, p.is_bf16);
+            w.z = pack16(__uint_as_float(v[g * 8 + 4]) * inv, __uint_as_float(v[g * 8 + 5]) * inv, p.is_bf16);
+            w.w = pack16(__uint_as_float(v[g * 8 + 6]) * inv, __uint_as_float(v[g * 8 + 7]) * inv, p.is_bf16);
+            *reinterpret_cast<uint4 *>(dst + c * 32 + g * 8) = empty ? make_uint4(0, 0, 0, 0) : w;
+          }
+        }
+      }
+      if (live && *reinterpret_cast<volatile uint32_t *>(&t.patch_flag) != 0 && m_used != -INFINITY && l_run == l_run) {
+        const uint16_t *q = p.q + row_offset(p, p.q_stride, u.head, u.seq, row);
+        if (p.is_bf16) {
+          patch_row<D, true>(p, blockIdx.x, pos, q, m_used, l_run, dst, parts ? part_dst : nullptr);
+        } else {
+          patch_row<D, false>(p, blockIdx.x, pos, q, m_used, l_run, dst, parts ? part_dst : nullptr);
+        }
+      }
+      // (the cubic's smallest exponentials keep a part that saw nothing from summing to zero)
+      if (live && parts) p.part_sum[part_row0 + u.split * part_step] = make_float2(m_used, m_used == -INFINITY && l_run == l_run ? 0.0f : l_run);
+      if (live && !parts && p.row_norm != nullptr) p.row_norm[static_cast<int64_t>(u.run) * p.rows + row] = make_float2(m_used, inv);
+    }
+    if (!p.over_batch && u.active > 1) {
+      __threadfence();
+      asm volatile("bar.sync 1, %0;" ::"n"(kSoftmaxWarps * 32) : "memory");
+      if (threadIdx.x == 0) {
+        uint32_t *counter = &p.counters[u.run * p.row_pairs + u.pair];
+        const uint32_t before = atomicAdd(counter, 1u);
+        t.is_last = before + 1 == static_cast<uint32_t>(u.active);
+        if (t.is_last) *counter = 0;
+      }
+      asm volatile("bar.sync 1, %0;" ::"n"(kSoftmaxWarps * 32) : "memory");
+      if (t.is_last && live) {
+        __threadfence();
+        float m = -INFINITY, l = 0.0f;
+        for (int s = 0; s < u.active; ++s) m = fmaxf(m, __ldcg(&p.part_sum[part_row0 + s * part_step]).x);
+        for (int s = 0; s < u.active; ++s) {
+          const float2 part = __ldcg(&p.part_sum[part_row0 + s * part_step]);
+          l += part.x == -INFINITY ? part.y : part.y * exp2f(part.x - m);
+        }
+        inv = empty ? 0.0f : (m == -INFINITY ? NAN : 1.0f / l);
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          float o[32] = {};
+          for (int s = 0; s < u.active; ++s) {
+            const float part_m = __ldcg(&p.part_sum[part_row0 + s * part_step]).x;
+            const float f = part_m == -INFINITY ? 0.0f : exp2f(part_m - m);
+            const float4 *src = reinterpret_cast<const float4 *>(p.part_out + (part_row0 + s * part_step) * D + c * 32);
+#pragma unroll
+            for (int g = 0; g < 8; ++g) {
+              const float4 x = __ldcg(src + g);
+              o[4 * g] = fmaf(x.x, f, o[4 * g]);
+              o[4 * g + 1] = fmaf(x.y, f, o[4 * g + 1]);
+              o[4 * g + 2] = fmaf(x.z, f, o[4 * g + 2]);
+              o[4 * g + 3] = fmaf(x.w, f, o[4 * g + 3]);
+            }
+          }
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            uint4 w;
+            w.x = pack16(o[g * 8 + 0] * inv, o[g * 8 + 1] * inv, p.is_bf16);
+            w.y = pack16(o[g * 8 + 2] * inv, o[g * 8 + 3] * inv, p.is_bf16);
+            w.z = pack16(o[g * 8 + 4] * inv, o[g * 8 + 5] * inv, p.is_bf16);
+            w.w = pack16(o[g * 8 + 6] * inv, o[g * 8 + 7] * inv, p.is_bf16);
+            *reinterpret_cast<uint4 *>(dst + c * 32 + g * 8) = empty ? make_uint4(0, 0, 0, 0) : w;
+          }
+        }
+        if (p.row_norm != nullptr) p.row_norm[static_cast<int64_t>(u.run) * p.rows + row] = make_float2(m, inv);
+      }
+    }
+    if (!ok && lane == 0) {
+      abort_flag = 1;
+      atomicCAS(p.status, 0u, kStatusAttentionTimeout);
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
+    if (warp == kProducerWarp) {
+      // ------------------------------------------------------------------ producer
+      if (elect_one()) {
+        bool ok = true;
+        for (int n = 0; n < 2 * u.walk.count && ok; ++n) {
+          const int st = n % S, j = n >> 1;
+          if (!mbar_wait(&t.slot_empty_bar[st], ((n / S) & 1) ^ 1, &abort_flag)) {
+            ok = false;
+            break;
+          }
+          mbar_arrive_expect_tx(&t.slot_full_bar[st], L::kSlotBytes);
+          const int key0 = u.walk.key0(j);
+          const bool prefix = u.walk.in_prefix(j);
+          const CUtensorMap *map = (n & 1) == 0 ? (prefix ? &tmap_pk : &tmap_k) : (prefix ? &tmap_pv : &tmap_v);
+#pragma unroll
+          for (int a = 0; a < L::kQAtoms; ++a) {
+            tma_load_4d(slot(st) + a * kBlockKv * kAtomBytes, map, &t.slot_full_bar[st], a * kAtomBytes, key0, u.head, prefix ? 0 : u.seq);
+          }
+        }
+        if (!ok) {
+          abort_flag = 1;
+          atomicCAS(p.status, 0u, kStatusAttentionTimeout);
+        }
+      }
+    } else if (warp == kMmaWarp) {
+      // ------------------------------------------------------------------ MMA issuer
+      const bool issuer = elect_one();
+      const TileMmas<D> mma(p.is_bf16, true, tmem_base, smem_u32(q_tile(0)), issuer);
+      const uint64_t sdesc0 = umma_desc_sw128(smem_u32(slot(0)));
+      bool ok = true;
+      uint32_t clean_phase = 0;  // bit i: the parity of the next values in slot i
+      auto commit = [&](uint64_t *bar) {
+        if (issuer) umma_commit(bar);
+      };
+      auto wait_full = [&](int n) -> bool { return mbar_wait(&t.slot_full_bar[n % S], (n / S) & 1, &abort_flag); };
+      auto desc_of = [&](int n) -> uint64_t { return sdesc0 + static_cast<uint64_t>((n % S) * (L::kSlotBytes >> 4)); };
+      for (int i = 0; i < kTiles && ok; ++i) ok = mbar_wait(&t.q_full_bar[i], 0, &abort_flag);
+      if (ok && u.walk.count > 0) ok = wait_full(0);
+      if (ok && u.walk.count > 0) {
+        tc_fence_after_sync();
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) {
+          if (u.blocks[i] == 0) continue;
+          mma.scores(i, desc_of(0));
+          commit(&t.s_full_bar[i]);
+        }
+        commit(&t.slot_empty_bar[0]);
+      }
+      for (int j = 0; j < u.walk.count && ok; ++j) {
+        const bool more = j + 1 < u.walk.count;
+        const int nv = 2 * j + 1, nk = 2 * j + 2;
+        if (!wait_full(nv) || !mbar_wait(&t.slot_clean_bar[nv % S], (clean_phase >> (nv % S)) & 1, &abort_flag)) ok = false;
+        clean_phase ^= 1u << (nv % S);
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) {
+          if (!ok || j >= u.blocks[i]) continue;
+          // The product reads P from the columns the next scores overwrite: the instructions of one
+          // thread run in the order they were issued.
+#pragma unroll
+          for (int part = 0; part < kPParts; ++part) {
+            if (ok) ok = mbar_wait(&t.p_full_bar[i][part], j & 1, &abort_flag);
+            if (!ok) break;
+            tc_fence_after_sync();
+            mma.product(i, part, desc_of(nv), j == 0 ? 1u : 0u);
+          }
+          if (!ok) continue;
+          if (j + 1 == u.blocks[i]) {
+            commit(&t.pv_done_bar[i]);  // (a block's scores, which the softmax waits for, follow its product)
+          } else {
+            if (!wait_full(nk)) {  // (seen by the first tile's turn, for the second's too)
+              ok = false;
+              continue;
+            }
+            tc_fence_after_sync();
+            mma.scores(i, desc_of(nk));
+            commit(&t.s_full_bar[i]);
+          }
+        }
+        if (!ok) break;
+        commit(&t.slot_empty_bar[nv % S]);  // both tiles have read the two slots
+        if (more) commit(&t.slot_empty_bar[nk % S]);
+      }
+      if (!ok && issuer) {
+        abort_flag = 1;
+        atomicCAS(p.status, 0u, kStatusAttentionTimeout);
+      }
+    } else {
+      // ------------------------------------------------------------------ values that are not seen by all
+      const int which = static_cast<int>(warp) - kCleanWarp;
+      bool ok = true;
+      // (Every block's values are waited for and passed on, so that no wait is two phases ahead of its barrier or behind it.)
+      for (int j = 0; j < u.walk.count && ok; ++j) {
+        const int nv = 2 * j + 1;
+        ok = __all_sync(0xffffffffu, mbar_wait(&t.slot_full_bar[nv % S], (nv / S) & 1, &abort_flag));
+        if (!ok) break;
+        if (!u.walk.differs(j)) {
+          if (lane == 0) mbar_arrive(&t.slot_clean_bar[nv % S]);
+          continue;
+        }
+        uint8_t *block = slot(nv % S);
+        const int key0 = u.walk.key0(j);
+        bool taken = false;
+#pragma unroll 4
+        for (int i = which; i < L::kSlotBytes / 512; i += kCleanWarps) {  // four keys' 128 bytes of an atom
+          const int key = key0 + (i % (kBlockKv / 4)) * 4 + static_cast<int>(lane >> 3);
+          uint4 *at = reinterpret_cast<uint4 *>(block + i * 512 + lane * 16);
+          const bool hidden = key >= u.walk.range.end || (key >= u.walk.range.sinks && key < u.walk.range.begin);
+          if (hidden) {
+            *at = make_uint4(0, 0, 0, 0);
+          } else {
+            const uint4 x = *at;
+            if (p.is_bf16 ? has_nonfinite<true>(x) : has_nonfinite<false>(x)) {
+              *at = p.is_bf16 ? without_nonfinite<true>(x) : without_nonfinite<false>(x);
+              taken = true;
+            }
+          }
+        }
+        if (taken) *reinterpret_cast<volatile uint32_t *>(&t.patch_flag) = 1;
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&t.slot_clean_bar[nv % S]);
+      }
+      if (!ok && lane == 0) {
+        abort_flag = 1;
+        atomicCAS(p.status, 0u, kStatusAttentionTimeout);
+      }
+    }
+  }
+
+  // ---------------------------------------------------------------------- teardown
+  tc_fence_before_sync();
+  __syncthreads();
+  if (abort_flag != 0) {
+    // A wait gave up: copies that may still be in flight land before the shared memory they target is released.
+    for (int i = 0; i < 64; ++i) __nanosleep(2000);
+    __syncthreads();
+  }
+  if (warp == kMmaWarp) {
+    tc_fence_after_sync();
+    tmem_dealloc<1>(tmem_base, L::kTmemCols);
+  }
+}
+
+template <int D>
+cudaError_t launch(const CUtensorMap (&maps)[4], const TilesParams &p, int64_t ctas, bool dependent, cudaStream_t stream) {
+  using L = Layout<D>;
+  auto kernel = cache_tiles_kernel<D>;
+  static const cudaError_t attr_set = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmemBytes);
+  if (attr_set != cudaSuccess) return attr_set;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas), 1, 1);
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.dynamicSmemBytes = L::kSmemBytes;
+  cfg.stream = stream;
+  return cudaLaunchKernelEx(&cfg, kernel, maps[0], maps[1], maps[2], maps[3], p);
+}
+
+// Keys or values as (head_dim bytes, positions, heads, batch), strides in elements (batch, head, position).
+bool key_map(CUtensorMap *map, const void *base, int head_dim, int len, int heads, int batch, int64_t batch_stride, int64_t head_stride,
+             int64_t position_stride) {
+  const uint64_t dims[4] = {static_cast<uint64_t>(head_dim) * 2, static_cast<uint64_t>(len), static_cast<uint64_t>(heads), static_cast<uint64_t>(batch)};
+  // (the stride of a dimension of extent 1 is never used, but has to pass the encoder's checks)
+  auto bytes = [&](int64_t s) { return static_cast<uint64_t>(s > 0 ? s : head_dim) * 2; };
+  const uint64_t strides[3] = {bytes(len > 1 ? position_stride : 0), bytes(heads > 1 ? head_stride : 0), bytes(batch > 1 ? batch_stride : 0)};
+  return make_tmap(map, base, 4, dims, strides, kBlockKv);
+}
+
+}  // namespace
+
+int cache_tiles_pairs(int rows) { return (rows + kPairRows - 1) / kPairRows; }
+
+int cache_tiles_splits(int64_t units, int keys, int most_units) {
+  const int blocks = (keys + kBlockKv - 1) / kBlockKv;
+  if (units >= sm_count() || units > most_units) return 1;
+  // One CTA an SM, no more of them than SMs, four blocks each at least.
+  const int wanted = static_cast<int>(std::min<int64_t>(sm_count() / units, std::max(1, blocks / 4)));
+  const int per_split = (blocks + wanted - 1) / wanted;
+  return (blocks + per_split - 1) / per_split;
+}
+
+size_t cache_tiles_part_rows(int64_t units, int splits) { return static_cast<size_t>(units) * splits * kPairRows; }
+
+cudaError_t cache_tiles(const TilesParams &p, const CacheAttentionArgs &a, const char **why) {
+  CUtensorMap maps[4];
+  const bool own = !p.over_batch, prefix = p.prefix_len > 0;
+  if (own && (!key_map(&maps[0], a.k, a.head_dim, a.kv_len, a.kv_heads, a.batch, a.k_stride[0], a.k_stride[1], a.k_stride[2]) ||
+              !key_map(&maps[1], a.v, a.head_dim, a.kv_len, a.kv_heads, a.batch, a.v_stride[0], a.v_stride[1], a.v_stride[2]))) {
+    *why = "cuTensorMapEncodeTiled refused k or v";
+    return cudaErrorInvalidValue;
+  }
+  if (prefix && (!key_map(&maps[2], a.prefix_k, a.head_dim, a.prefix_len, a.kv_heads, 1, 0, a.prefix_k_stride[0], a.prefix_k_stride[1]) ||
+                 !key_map(&maps[3], a.prefix_v, a.head_dim, a.prefix_len, a.kv_heads, 1, 0, a.prefix_v_stride[0], a.prefix_v_stride[1]))) {
+    *why = "cuTensorMapEncodeTiled refused the prefix";
+    return cudaErrorInvalidValue;
+  }
+  if (!own) maps[0] = maps[2], maps[1] = maps[3];
+  if (!prefix) maps[2] = maps[0], maps[3] = maps[1];
+  const int64_t ctas = static_cast<int64_t>(p.runs) * p.row_pairs * p.splits;
+  *why = "launching the tile kernel";
+  return a.head_dim == 64 ? launch<64>(maps, p, ctas, false, a.stream) : launch<128>(maps, p, ctas, false, a.stream);
+}
+
+}  // namespace flsm100

@@ -1,0 +1,39 @@
+// The kernel over a key-value cache for many query rows (cache_tiles_sm100.cu), as cache_rows_sm100.cu plans and launches it.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "cache_attention_sm100.cuh"
+
+namespace flsm100 {
+
+struct TilesParams {
+  const uint16_t *q, *k, *v;
+  uint16_t *out;
+  int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3];
+  const int32_t *kv_lens;
+  int is_bf16;
+  int kv_heads, group, q_len, kv_len;
+  int window, sinks;
+  int prefix_len;   // keys that every row sees, walked first; 0 without
+  bool over_batch;  // the rows of the whole batch over the prefix alone: parts only
+  int runs;         // (sequence, key-value head), or the heads alone
+  int rows;         // packed rows of a run
+  int row_pairs;    // pairs of tiles of 128 of them
+  int splits;       // CTAs that divide a pair's blocks of keys
+  float scale_log2;
+  float *part_out;   // (kv_head, split, rows, D) over a prefix, (run, pair, split, 256, D) else
+  float2 *part_sum;  // the same without D: maximum in log2 units, sum
+  uint32_t *counters;
+  float2 *row_norm;  // (run, rows): maximum and 1 / sum, or null
+  uint32_t *status;
+};
+
+int cache_tiles_pairs(int rows);
+// `keys`: the most that a pair's rows see between them. At most `most_units` units may be divided.
+int cache_tiles_splits(int64_t units, int keys, int most_units);
+size_t cache_tiles_part_rows(int64_t units, int splits);
+cudaError_t cache_tiles(const TilesParams &p, const CacheAttentionArgs &a, const char **why);
+
+}  // namespace flsm100
