@@ -19,6 +19,7 @@
 
 #include "cache_common_sm100.cuh"
 #include "cache_tiles_sm100.cuh"
+#include "cache_weights_sm100.cuh"
 #include "ptx_sm100.cuh"
 
 namespace flsm100 {
@@ -485,7 +486,8 @@ struct CachePlan {
   bool prefix_apart;  // a kernel of its own over the prefix for the rows of the whole batch
   bool prefix_tiles;
   int prefix_rows, prefix_row_tiles, prefix_splits;
-  size_t part_out, part_sum, prefix_out, prefix_sum, scores, row_norm, bytes;
+  WeightsPlan weights;  // with `tiles`
+  size_t part_out, part_sum, prefix_out, prefix_sum, scores, row_norm, bytes;  // (scores: or the sums of their parts)
 };
 
 CachePlan cache_plan(const CacheAttentionArgs &a) {
@@ -493,7 +495,7 @@ CachePlan cache_plan(const CacheAttentionArgs &a) {
   const int group = a.heads / a.kv_heads;
   const int64_t d = a.head_dim;
   p.rows = group * a.q_len;
-  p.tiles = p.rows >= kTilesFromRows && a.weights_out == nullptr;
+  p.tiles = p.rows >= kTilesFromRows;
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t off = at;
@@ -536,7 +538,11 @@ CachePlan cache_plan(const CacheAttentionArgs &a) {
     p.prefix_out = take(static_cast<size_t>(a.kv_heads) * p.prefix_splits * p.prefix_rows * d * 4);
     p.prefix_sum = take(static_cast<size_t>(a.kv_heads) * p.prefix_splits * p.prefix_rows * 8);
   }
-  if (a.weights_out != nullptr) {
+  if (a.weights_out != nullptr && p.tiles) {
+    p.weights = cache_weights_plan(a, kCacheCounters);
+    p.row_norm = take(static_cast<size_t>(runs) * group * cache_weights_norm_pitch(a.q_len) * 8);
+    p.scores = take(p.weights.part_bytes);
+  } else if (a.weights_out != nullptr) {
     p.scores = take(static_cast<size_t>(runs) * p.rows * a.kv_len * 4);
     p.row_norm = take(static_cast<size_t>(runs) * p.rows * 8);
   }
@@ -579,7 +585,7 @@ bool cache_attention_supported(const CacheAttentionArgs &a, const char **why) {
     return false;
   }
   const CachePlan plan = cache_plan(a);
-  if (static_cast<int64_t>(a.batch) * a.kv_heads * plan.row_tiles * plan.splits > most ||
+  if (static_cast<int64_t>(a.batch) * a.kv_heads * plan.row_tiles * plan.splits > most || plan.weights.ctas > most ||
       static_cast<int64_t>(a.batch) * a.kv_heads * ((static_cast<int64_t>(a.kv_len) + 255) / 256) > most) {
     *why = "more work than one launch indexes";
     return false;
@@ -631,7 +637,37 @@ cudaError_t cache_attention(const CacheAttentionArgs &a, const char **why, int *
     tiles.splits = plan.splits;
     tiles.part_out = floats(plan.part_out);
     tiles.part_sum = pairs(plan.part_sum);
+    if (a.weights_out != nullptr) {
+      tiles.row_norm = pairs(plan.row_norm);
+      tiles.norm_pitch = cache_weights_norm_pitch(a.q_len);
+    }
     e = cache_tiles(tiles, a, why);
+    *launches += e == cudaSuccess;
+    if (e != cudaSuccess || a.weights_out == nullptr) return e;
+    WeightsParams w = {};
+    w.kv_lens = a.kv_lens;
+    w.is_bf16 = a.is_bf16;
+    w.kv_heads = a.kv_heads;
+    w.group = tiles.group;
+    w.q_len = a.q_len;
+    w.kv_len = a.kv_len;
+    w.runs = tiles.runs;
+    w.pairs = plan.weights.pairs;
+    w.parts = plan.weights.parts;
+    w.part_blocks = plan.weights.part_blocks;
+    w.scale_log2 = tiles.scale_log2;
+    w.row_norm = tiles.row_norm;
+    w.norm_pitch = tiles.norm_pitch;
+    w.part_sums = floats(plan.scores);
+    w.counters = a.counters;
+    w.weights_in = a.weights_in;
+    w.weights_out = a.weights_out;
+    for (int i = 0; i < 2; ++i) {
+      w.in_stride[i] = a.weights_in_stride[i];
+      w.out_stride[i] = a.weights_out_stride[i];
+    }
+    w.status = a.status;
+    e = cache_weights(w, a, why);
     *launches += e == cudaSuccess;
     return e;
   }

@@ -337,6 +337,7 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
     const bool empty = p.prefix_len == 0 && pos < 0;  // sees no key: zeros
     uint16_t *dst = live && !p.over_batch ? p.out + row_offset(p, p.out_stride, u.head, u.seq, row) : nullptr;
     float *part_dst = p.part_out + (part_row0 + u.split * part_step) * D;
+    const int64_t norm_at = (static_cast<int64_t>(u.run) * p.group + row % p.group) * p.norm_pitch + row / p.group;
     // (a row whose every score is -inf has no softmax)
     float inv = empty ? 0.0f : (m_used == -INFINITY ? NAN : 1.0f / l_run);
     if (ok) {
@@ -375,7 +376,7 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
       }
       // (the cubic's smallest exponentials keep a part that saw nothing from summing to zero)
       if (live && parts) p.part_sum[part_row0 + u.split * part_step] = make_float2(m_used, m_used == -INFINITY && l_run == l_run ? 0.0f : l_run);
-      if (live && !parts && p.row_norm != nullptr) p.row_norm[static_cast<int64_t>(u.run) * p.rows + row] = make_float2(m_used, inv);
+      if (live && !parts && p.row_norm != nullptr) p.row_norm[norm_at] = make_float2(m_used, inv);
     }
     if (!p.over_batch && u.active > 1) {
       __threadfence();
@@ -422,7 +423,7 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
             *reinterpret_cast<uint4 *>(dst + c * 32 + g * 8) = empty ? make_uint4(0, 0, 0, 0) : w;
           }
         }
-        if (p.row_norm != nullptr) p.row_norm[static_cast<int64_t>(u.run) * p.rows + row] = make_float2(m, inv);
+        if (p.row_norm != nullptr) p.row_norm[norm_at] = make_float2(m, inv);
       }
     }
     if (!ok && lane == 0) {
@@ -588,16 +589,6 @@ cudaError_t launch(const CUtensorMap (&maps)[4], const TilesParams &p, int64_t c
   return cudaLaunchKernelEx(&cfg, kernel, maps[0], maps[1], maps[2], maps[3], p);
 }
 
-// Keys or values as (head_dim bytes, positions, heads, batch), strides in elements (batch, head, position).
-bool key_map(CUtensorMap *map, const void *base, int head_dim, int len, int heads, int batch, int64_t batch_stride, int64_t head_stride,
-             int64_t position_stride) {
-  const uint64_t dims[4] = {static_cast<uint64_t>(head_dim) * 2, static_cast<uint64_t>(len), static_cast<uint64_t>(heads), static_cast<uint64_t>(batch)};
-  // (the stride of a dimension of extent 1 is never used, but has to pass the encoder's checks)
-  auto bytes = [&](int64_t s) { return static_cast<uint64_t>(s > 0 ? s : head_dim) * 2; };
-  const uint64_t strides[3] = {bytes(len > 1 ? position_stride : 0), bytes(heads > 1 ? head_stride : 0), bytes(batch > 1 ? batch_stride : 0)};
-  return make_tmap(map, base, 4, dims, strides, kBlockKv);
-}
-
 }  // namespace
 
 int cache_tiles_pairs(int rows) { return (rows + kPairRows - 1) / kPairRows; }
@@ -616,13 +607,13 @@ size_t cache_tiles_part_rows(int64_t units, int splits) { return static_cast<siz
 cudaError_t cache_tiles(const TilesParams &p, const CacheAttentionArgs &a, const char **why) {
   CUtensorMap maps[4];
   const bool own = !p.over_batch, prefix = p.prefix_len > 0;
-  if (own && (!key_map(&maps[0], a.k, a.head_dim, a.kv_len, a.kv_heads, a.batch, a.k_stride[0], a.k_stride[1], a.k_stride[2]) ||
-              !key_map(&maps[1], a.v, a.head_dim, a.kv_len, a.kv_heads, a.batch, a.v_stride[0], a.v_stride[1], a.v_stride[2]))) {
+  if (own && (!row_map(&maps[0], a.k, a.head_dim, a.kv_len, a.kv_heads, a.batch, a.k_stride[0], a.k_stride[1], a.k_stride[2]) ||
+              !row_map(&maps[1], a.v, a.head_dim, a.kv_len, a.kv_heads, a.batch, a.v_stride[0], a.v_stride[1], a.v_stride[2]))) {
     *why = "cuTensorMapEncodeTiled refused k or v";
     return cudaErrorInvalidValue;
   }
-  if (prefix && (!key_map(&maps[2], a.prefix_k, a.head_dim, a.prefix_len, a.kv_heads, 1, 0, a.prefix_k_stride[0], a.prefix_k_stride[1]) ||
-                 !key_map(&maps[3], a.prefix_v, a.head_dim, a.prefix_len, a.kv_heads, 1, 0, a.prefix_v_stride[0], a.prefix_v_stride[1]))) {
+  if (prefix && (!row_map(&maps[2], a.prefix_k, a.head_dim, a.prefix_len, a.kv_heads, 1, 0, a.prefix_k_stride[0], a.prefix_k_stride[1]) ||
+                 !row_map(&maps[3], a.prefix_v, a.head_dim, a.prefix_len, a.kv_heads, 1, 0, a.prefix_v_stride[0], a.prefix_v_stride[1]))) {
     *why = "cuTensorMapEncodeTiled refused the prefix";
     return cudaErrorInvalidValue;
   }

@@ -26,7 +26,8 @@ struct TilesParams {
   float *part_out;   // (kv_head, split, rows, D) over a prefix, (run, pair, split, 256, D) else
   float2 *part_sum;  // the same without D: maximum in log2 units, sum
   uint32_t *counters;
-  float2 *row_norm;  // (run, rows): maximum and 1 / sum, or null
+  float2 *row_norm;  // (run, query head of the group, norm_pitch): maximum and 1 / sum, or null
+  int norm_pitch;
   uint32_t *status;
 };
 
