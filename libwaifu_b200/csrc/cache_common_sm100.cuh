@@ -32,6 +32,13 @@ __device__ __forceinline__ KeyRange visible_keys(int first, int last, int len, i
   return r;
 }
 
+// 2^x by the hardware's function (relative error 2^-22), -inf -> 0.
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack_pair(float a, float b) {
   if constexpr (BF16) {

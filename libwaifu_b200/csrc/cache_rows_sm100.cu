@@ -2,12 +2,14 @@
 // the GPU, and a key's row is read once for all the query heads that share it.
 //
 // The rows of one key-value head, its group of query heads times the queries, are packed into tiles of 16, the M
-// of mma.sync m16n8k16. A unit is such a tile with its keys; its keys are divided over `splits` CTAs of four
-// warps, and a warp walks 16 keys at a time on its own: its own ring of shared-memory stages filled by 16-byte
-// asynchronous copies (a key's address is computed by itself, so sinks, window and any strides need no tile of
-// their own), its own running maximum, sum and output. No barrier stands in the loop. The four meet in
-// shared memory at the end, the CTAs of a unit in the workspace, where the last one to arrive adds the parts in
-// the order of the splits: the result does not depend on which came last.
+// of mma.sync m16n8k16. A unit is such a tile with the keys its sequence's queries see, in steps of 64. The steps of
+// all units, one after the other, are dealt out in equal runs over two CTAs an SM, whatever the sequences'
+// lengths: a CTA takes the end of one unit, whole units, the beginning of another. Its four warps walk 16 keys
+// of a step each on their own: a ring of shared-memory stages per warp, filled by 16-byte asynchronous copies that run
+// on into the next unit (a key's address is computed by itself, so sinks, window and any strides need no tile of
+// their own), and a running maximum, sum and output per warp. No barrier stands in the loop. At a unit's end the four
+// meet over the stages they have just read; a unit that several CTAs share meets in the workspace, where the last one to
+// arrive adds the parts in their order: the result does not depend on which came last.
 //
 // What bounds it is the keys' way from HBM: 2 head_dim bytes twice per key, against 16 x head_dim x 4 operations.
 #include "cache_attention_sm100.cuh"
@@ -32,6 +34,7 @@ constexpr int kTileKeys = 16;  // keys a warp takes at a time
 constexpr int kStages = 3;
 constexpr int kStepKeys = kWarps * kTileKeys;
 constexpr int kRows = kFewRowsTile;
+constexpr int kLeastSteps = 4;  // that are worth a CTA of their own
 
 template <int D>
 struct RowsLayout {
@@ -41,7 +44,7 @@ struct RowsLayout {
   static constexpr int kQOff = 0;
   static constexpr int kRingOff = kRows * kRowBytes;
   static constexpr int kSmemBytes = kRingOff + kWarps * kStages * kStageBytes;
-  static_assert(kWarps * kRows * D * 4 <= kWarps * kStages * kStageBytes, "the warps' outputs fit the ring");
+  static_assert(kRows * D * 4 == kStageBytes, "a warp's outputs fit the stage that it has read");
   static_assert(2 * (kSmemBytes + 2048) <= 227 * 1024, "two CTAs an SM");
 };
 
@@ -97,12 +100,13 @@ struct RowsParams {
   float scale_log2;
   // Rows of the whole batch over keys that all of them see (a shared prefix): parts only.
   bool over_batch;
+  int batch;
   int rows;       // packed rows of a key-value head: group * q_len, times the batch over a prefix
   int row_tiles;  // of 16
-  int splits;
-  float *part_out;   // (unit, split, 16, D), or (kv_head, split, rows, D) over a prefix
+  int splits;     // over a prefix: CTAs that divide a unit
+  float *part_out;   // (CTA, 2, 16, D): a unit's end, and a unit's beginning; (kv_head, split, rows, D) over a prefix
   float2 *part_sum;  // the same without D: maximum in log2 units, sum
-  uint32_t *counters;
+  uint32_t *counters;  // of the unit that the CTA's last run of steps begins
   // The parts over the prefix that an earlier kernel left, as above; 0 splits without.
   const float *prefix_out;
   const float2 *prefix_sum;
@@ -112,331 +116,457 @@ struct RowsParams {
   float2 *row_norm;
 };
 
+// Where a CTA's walk over the units' steps stands. Units lie in the order of their sequences, heads and tiles; those of a
+// sequence walk the same keys, what its first to its last query sees.
+struct Cursor {
+  int seq, head, tile, step, steps, len;
+  KeyRange range;
+
+  __device__ __forceinline__ void enter_sequence(const RowsParams &p) {
+    if (p.over_batch) {
+      len = 0;
+      range = KeyRange{0, 0, p.kv_len};
+    } else {
+      len = sequence_length(p.kv_lens, seq, p.kv_len);
+      range = visible_keys(len - p.q_len, len - 1, len, p.window, p.sinks);
+    }
+    steps = max(1, (range.count() + kStepKeys - 1) / kStepKeys);  // (a unit without keys still has its result to write)
+  }
+  // True where the step begins another unit.
+  __device__ __forceinline__ bool advance(const RowsParams &p) {
+    if (++step < steps) return false;
+    step = 0;
+    if (++tile == p.row_tiles) {
+      tile = 0;
+      if (++head == p.kv_heads) {
+        head = 0;
+        if (++seq < p.batch) enter_sequence(p);
+      }
+    }
+    return true;
+  }
+};
+
 template <int D, bool BF16>
-__global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const RowsParams p) {
+__global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_constant__ RowsParams p) {
   using L = RowsLayout<D>;
-  constexpr int kPieces = D / 8;       // of a row
-  constexpr int kColTiles = D / 8;     // of the output, eight columns each
-  constexpr int kMyCols = D / 8;       // columns a thread finishes: eight threads a row
+  constexpr int kPieces = D / 8;    // of a row
+  constexpr int kColTiles = D / 8;  // of the output, eight columns each
+  constexpr int kQuads = D / 4;     // of a row: a thread finishes four columns at a time
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float2 warp_sum[kWarps][kRows];
-  __shared__ int is_last;
+  __shared__ int64_t scan[kWarps];
+  __shared__ int64_t found_before;
+  __shared__ int found_seq, is_last, longest[kWarps];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int at = blockIdx.x;
-  const int tile = at % p.row_tiles;
-  at /= p.row_tiles;
-  const int split = at % p.splits;
-  at /= p.splits;  // the run: (sequence, key-value head), or the head alone over a prefix
-  const int run = at;
-  const int head = at % p.kv_heads, seq = at / p.kv_heads;
-  const int row0 = tile * kRows;
-  const int live = min(kRows, p.rows - row0);
-
   griddep_launch_dependents();
 
-  KeyRange range;
-  int len = p.kv_len, first_pos = 0, last_pos = 0;
+  // ---- this CTA's run of steps
+  Cursor load;
+  int64_t begin, per_cta;
+  int count;
   if (p.over_batch) {
-    range = KeyRange{0, 0, p.kv_len};
+    load.seq = 0;
+    load.enter_sequence(p);
+    int at = blockIdx.x;
+    load.tile = at % p.row_tiles;
+    at /= p.row_tiles;
+    load.head = at % p.kv_heads;
+    per_cta = (load.steps + p.splits - 1) / p.splits;
+    begin = load.step = static_cast<int>(at / p.kv_heads * per_cta);
+    count = min(static_cast<int>(per_cta), load.steps - load.step);
   } else {
-    len = sequence_length(p.kv_lens, seq, p.kv_len);
-    first_pos = row0 / p.group + len - p.q_len;
-    last_pos = (row0 + live - 1) / p.group + len - p.q_len;
-    range = visible_keys(first_pos, last_pos, len, p.window, p.sinks);
-  }
-  const int total = range.count();
-  const int steps = (total + kStepKeys - 1) / kStepKeys;
-  const int per_split = max(1, (steps + p.splits - 1) / p.splits);
-  const int active = max(1, (steps + per_split - 1) / per_split);  // splits that have keys (one where there are none)
-  if (split >= active) return;
-  const int tile_begin = split * per_split * kWarps;
-  const int tile_end = min((split + 1) * per_split * kWarps, (total + kTileKeys - 1) / kTileKeys);
-
-  const uint16_t *k_base = p.k + head * p.k_stride[1] + (p.over_batch ? 0 : seq * p.k_stride[0]);
-  const uint16_t *v_base = p.v + head * p.v_stride[1] + (p.over_batch ? 0 : seq * p.v_stride[0]);
-  uint8_t *ring = smem + L::kRingOff + warp * kStages * L::kStageBytes;
-
-  auto load_tile = [&](int t, int stage) {
-    uint8_t *dst = ring + stage * L::kStageBytes;
-    constexpr int kRowsAtOnce = 32 / kPieces;
-    const int c = lane % kPieces;
-#pragma unroll
-    for (int i = 0; i < kTileKeys / kRowsAtOnce; ++i) {
-      const int r = i * kRowsAtOnce + lane / kPieces;
-      const int at = t * kTileKeys + r;
-      const bool there = at < total;
-      const int64_t key = there ? range.key(at) : 0;
-      const int off = piece_offset<D>(r, c);
-      cp_async_16(dst + off, k_base + key * p.k_stride[2] + c * 8, there ? 16 : 0);
-      cp_async_16(dst + L::kTileBytes + off, v_base + key * p.v_stride[2] + c * 8, there ? 16 : 0);
+    // The steps of the whole batch, and the sequence in which this CTA's begin. Each thread has some sequences.
+    const int mine = (p.batch + kThreads - 1) / kThreads;
+    const int first = threadIdx.x * mine, last = min(first + mine, p.batch);
+    const int units = p.kv_heads * p.row_tiles;
+    int64_t sum = 0;
+    int most = 1;
+    for (load.seq = first; load.seq < last; ++load.seq) {
+      load.enter_sequence(p);
+      sum += static_cast<int64_t>(load.steps) * units;
+      most = max(most, load.steps);
     }
+    int64_t upto = sum;
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, upto, x);
+      if (lane >= x) upto += y;
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, x));
+    }
+    if (lane == 31) scan[warp] = upto;
+    if (lane == 0) longest[warp] = most;
+    __syncthreads();
+    int64_t before = upto - sum, total = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) before += scan[w];
+      total += scan[w];
+      most = max(most, longest[w]);
+    }
+    // Four steps each at least, or one unit where they are shorter.
+    per_cta = max((total + gridDim.x - 1) / gridDim.x, static_cast<int64_t>(min(kLeastSteps, most)));
+    begin = blockIdx.x * per_cta;
+    if (begin >= total) return;
+    count = static_cast<int>(min(per_cta, total - begin));
+    if (before <= begin && begin < before + sum) {
+      for (load.seq = first;; ++load.seq) {
+        load.enter_sequence(p);
+        const int64_t here = static_cast<int64_t>(load.steps) * units;
+        if (begin < before + here) break;
+        before += here;
+      }
+      found_seq = load.seq;
+      found_before = before;
+    }
+    __syncthreads();
+    load.seq = found_seq;
+    load.enter_sequence(p);
+    const int64_t in_seq = begin - found_before;
+    const int unit = static_cast<int>(in_seq / load.steps);
+    load.step = static_cast<int>(in_seq - static_cast<int64_t>(unit) * load.steps);
+    load.tile = unit % p.row_tiles;
+    load.head = unit / p.row_tiles;
+  }
+  Cursor at = load;
+
+  // ---- the ring
+  uint8_t *ring = smem + L::kRingOff + warp * kStages * L::kStageBytes;
+  constexpr int kRowsAtOnce = 32 / kPieces;
+  const int lane_row = lane / kPieces, lane_piece = lane % kPieces;
+  int loaded = 0, load_stage = 0;
+  auto load_tile = [&]() {
+    if (loaded < count) {
+      uint8_t *dst = ring + load_stage * L::kStageBytes;
+      const int at0 = (load.step * kWarps + warp) * kTileKeys, total = load.range.count();
+      const uint16_t *k = p.k + load.head * p.k_stride[1] + (p.over_batch ? 0 : load.seq * p.k_stride[0]) + lane_piece * 8;
+      const uint16_t *v = p.v + load.head * p.v_stride[1] + (p.over_batch ? 0 : load.seq * p.v_stride[0]) + lane_piece * 8;
+      if (at0 + kTileKeys <= total && (at0 >= load.range.sinks || at0 + kTileKeys <= load.range.sinks)) {  // one run of keys
+        const int key = load.range.key(at0) + lane_row;
+        k += key * p.k_stride[2];
+        v += key * p.v_stride[2];
+#pragma unroll
+        for (int i = 0; i < kTileKeys / kRowsAtOnce; ++i) {
+          const int off = piece_offset<D>(i * kRowsAtOnce + lane_row, lane_piece);
+          cp_async_16(dst + off, k + i * kRowsAtOnce * p.k_stride[2], 16);
+          cp_async_16(dst + L::kTileBytes + off, v + i * kRowsAtOnce * p.v_stride[2], 16);
+        }
+      } else {
+#pragma unroll 1
+        for (int i = 0; i < kTileKeys / kRowsAtOnce; ++i) {
+          const int r = i * kRowsAtOnce + lane_row;
+          const bool there = at0 + r < total;
+          const int64_t key = there ? load.range.key(at0 + r) : 0;
+          const int off = piece_offset<D>(r, lane_piece);
+          cp_async_16(dst + off, k + key * p.k_stride[2], there ? 16 : 0);
+          cp_async_16(dst + L::kTileBytes + off, v + key * p.v_stride[2], there ? 16 : 0);
+        }
+      }
+      ++loaded;
+      load_stage = load_stage + 1 == kStages ? 0 : load_stage + 1;
+      if (loaded < count) load.advance(p);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
   };
 #pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) {
-    const int t = tile_begin + warp + s * kWarps;
-    if (t < tile_end) load_tile(t, s);
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  }
+  for (int s = 0; s < kStages - 1; ++s) load_tile();
 
-  // The queries: eight threads a row, then each warp's A operand.
-  {
-    const int r = threadIdx.x >> 3;
-    const uint16_t *src = nullptr;
-    if (r < live) {
-      int n = seq, in_seq = row0 + r;
+  // ---- the queries of a unit: eight threads a row
+  constexpr int kMyPieces = kPieces / 8;
+  auto fetch_queries = [&](const Cursor &u, uint4 (&x)[kMyPieces]) {
+    const int r = u.tile * kRows + (threadIdx.x >> 3);
+#pragma unroll
+    for (int c = 0; c < kMyPieces; ++c) x[c] = make_uint4(0, 0, 0, 0);
+    if (r < p.rows) {
+      int n = u.seq, in_seq = r;
       if (p.over_batch) {
         n = in_seq / (p.group * p.q_len);
         in_seq -= n * p.group * p.q_len;
       }
       const int i = in_seq / p.group, g = in_seq - i * p.group;
-      src = p.q + n * p.q_stride[0] + static_cast<int64_t>(head * p.group + g) * p.q_stride[1] + i * p.q_stride[2];
-    }
+      const uint16_t *src = p.q + n * p.q_stride[0] + static_cast<int64_t>(u.head * p.group + g) * p.q_stride[1] + i * p.q_stride[2];
 #pragma unroll
-    for (int c = threadIdx.x & 7; c < kPieces; c += 8) {
-      *reinterpret_cast<uint4 *>(smem + L::kQOff + piece_offset<D>(r, c)) =
-          src ? *reinterpret_cast<const uint4 *>(src + c * 8) : make_uint4(0, 0, 0, 0);
+      for (int c = 0; c < kMyPieces; ++c) x[c] = *reinterpret_cast<const uint4 *>(src + ((threadIdx.x & 7) + 8 * c) * 8);
     }
+  };
+  auto stage_queries = [&](const uint4 (&x)[kMyPieces]) {
+#pragma unroll
+    for (int c = 0; c < kMyPieces; ++c) *reinterpret_cast<uint4 *>(smem + L::kQOff + piece_offset<D>(threadIdx.x >> 3, (threadIdx.x & 7) + 8 * c)) = x[c];
+  };
+  {
+    uint4 x[kMyPieces];
+    fetch_queries(at, x);
+    stage_queries(x);
   }
   __syncthreads();
+
+  const int my_row = lane >> 2;  // this thread's rows of the tile: my_row and my_row + 8
   uint32_t qf[D / 16][4];
+  float o[kColTiles][4];
+  float m0, m1, l0, l1;
+  int first_pos, last_pos, pos0, pos1;  // of the tile's rows, and of this thread's
+  int unit_step;                        // the first step that this CTA takes of the unit
+  auto begin_unit = [&]() {
 #pragma unroll
-  for (int s = 0; s < D / 16; ++s) {
-    ldmatrix_x4(qf[s], smem_u32(smem + L::kQOff + piece_offset<D>(lane & 15, 2 * s + (lane >> 4))));
-  }
-
-  // This thread's two rows of the tile (fragment rows lane / 4 and + 8), and where they sit.
-  const int my_row = lane >> 2;
-  const int pos0 = (row0 + my_row) / p.group + len - p.q_len, pos1 = (row0 + my_row + 8) / p.group + len - p.q_len;
+    for (int s = 0; s < D / 16; ++s) {
+      ldmatrix_x4(qf[s], smem_u32(smem + L::kQOff + piece_offset<D>(lane & 15, 2 * s + (lane >> 4))));
+    }
+#pragma unroll
+    for (int c = 0; c < kColTiles; ++c) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[c][i] = 0.0f;
+    }
+    m0 = m1 = -INFINITY;
+    l0 = l1 = 0.0f;
+    const int row0 = at.tile * kRows, offset = at.len - p.q_len;
+    first_pos = row0 / p.group + offset;
+    last_pos = (min(row0 + kRows, p.rows) - 1) / p.group + offset;
+    pos0 = (row0 + my_row) / p.group + offset;
+    pos1 = (row0 + my_row + 8) / p.group + offset;
+    unit_step = at.step;
+  };
   auto sees = [&](int key, int pos) { return p.over_batch || (key <= pos && (key > pos - p.window || key < p.sinks)); };
+  begin_unit();
+  __syncthreads();  // the queries have been read
 
-  float o[kColTiles][4] = {};
-  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
   int stage = 0;
-  for (int t = tile_begin + warp; t < tile_end; t += kWarps) {
+  for (int done = 0; done < count; ++done) {
     cp_async_wait_group<kStages - 2>();
     __syncwarp();
-    {
-      const int ahead = t + (kStages - 1) * kWarps;
-      if (ahead < tile_end) load_tile(ahead, stage == 0 ? kStages - 1 : stage - 1);
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    }
+    load_tile();
     uint8_t *k_tile = ring + stage * L::kStageBytes;
     uint8_t *v_tile = k_tile + L::kTileBytes;
     stage = stage + 1 == kStages ? 0 : stage + 1;
 
-    float sc[2][4] = {};  // keys 0 .. 7 and 8 .. 15 of the tile: (row, key), (row, key + 1), (row + 8, key), ...
+    const int at0 = (at.step * kWarps + warp) * kTileKeys, total = at.range.count();
+    if (at0 < total) {
+      float sc[2][4] = {};  // keys 0 .. 7 and 8 .. 15 of the tile: (row, key), (row, key + 1), (row + 8, key), ...
 #pragma unroll
-    for (int s = 0; s < D / 16; ++s) {
-      uint32_t b[4];
-      ldmatrix_x4(b, smem_u32(k_tile + piece_offset<D>((lane & 7) + ((lane >> 4) << 3), 2 * s + ((lane >> 3) & 1))));
-      mma_16<BF16>(sc[0], qf[s], b[0], b[1]);
-      mma_16<BF16>(sc[1], qf[s], b[2], b[3]);
-    }
-    const int at0 = t * kTileKeys;
-    const int key_lo = range.key(at0), key_hi = range.key(min(at0 + kTileKeys, total) - 1);
-    // Does some row not see some key here? (The keys between key_lo and key_hi may jump from the sinks to the window.)
-    const bool differ = !p.over_batch && (key_hi > first_pos || (key_hi >= p.sinks && key_lo <= last_pos - p.window));
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) sc[h][i] *= p.scale_log2;
-    }
-    if (differ || at0 + kTileKeys > total) {
+      for (int s = 0; s < D / 16; ++s) {
+        uint32_t b[4];
+        ldmatrix_x4(b, smem_u32(k_tile + piece_offset<D>((lane & 7) + ((lane >> 4) << 3), 2 * s + ((lane >> 3) & 1))));
+        mma_16<BF16>(sc[0], qf[s], b[0], b[1]);
+        mma_16<BF16>(sc[1], qf[s], b[2], b[3]);
+      }
+      const int key_lo = at.range.key(at0), key_hi = at.range.key(min(at0 + kTileKeys, total) - 1);
+      // Does some row not see some key here? (The keys between key_lo and key_hi may jump from the sinks to the window.)
+      const bool differ = !p.over_batch && (key_hi > first_pos || (key_hi >= p.sinks && key_lo <= last_pos - p.window));
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int at = at0 + h * 8 + (lane & 3) * 2 + (i & 1);
-          if (at >= total || !sees(range.key(at), i < 2 ? pos0 : pos1)) sc[h][i] = -INFINITY;
-        }
+        for (int i = 0; i < 4; ++i) sc[h][i] *= p.scale_log2;
       }
-    }
-    if (p.scores != nullptr) {  // (no window there: a key's place is the key)
-      float *dst = p.scores + (static_cast<int64_t>(run) * p.rows + row0 + my_row) * p.kv_len;
+      if (differ || at0 + kTileKeys > total) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < 2; ++h) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int key = at0 + h * 8 + (lane & 3) * 2 + (i & 1);
-          if (key < total && my_row + (i < 2 ? 0 : 8) < live) dst[(i < 2 ? 0 : 8) * static_cast<int64_t>(p.kv_len) + key] = sc[h][i];
-        }
-      }
-    }
-    float b0 = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[1][0], sc[1][1]));
-    float b1 = fmaxf(fmaxf(sc[0][2], sc[0][3]), fmaxf(sc[1][2], sc[1][3]));
-#pragma unroll
-    for (int x = 1; x <= 2; x <<= 1) {
-      b0 = fmaxf(b0, __shfl_xor_sync(0xffffffffu, b0, x));
-      b1 = fmaxf(b1, __shfl_xor_sync(0xffffffffu, b1, x));
-    }
-    // The output and the sum are relative to a maximum that follows the rows' own only when one has grown by more
-    // than 2^8: until then the exponentials stay below what every type here holds.
-    if (__any_sync(0xffffffffu, b0 > m0 + 8.0f || b1 > m1 + 8.0f)) {
-      const float n0 = fmaxf(m0, b0), n1 = fmaxf(m1, b1);
-      const float f0 = n0 == -INFINITY ? 1.0f : exp2f(m0 - n0), f1 = n1 == -INFINITY ? 1.0f : exp2f(m1 - n1);
-      l0 *= f0;
-      l1 *= f1;
-#pragma unroll
-      for (int c = 0; c < kColTiles; ++c) {
-        o[c][0] *= f0;
-        o[c][1] *= f0;
-        o[c][2] *= f1;
-        o[c][3] *= f1;
-      }
-      m0 = n0;
-      m1 = n1;
-    }
-    const float s0 = m0 == -INFINITY ? 0.0f : m0, s1 = m1 == -INFINITY ? 0.0f : m1;
-    // The probabilities enter the second product as two 16-bit values each, the rounded one and what it lost: the
-    // product is not what bounds the walk (see above), and the result keeps the precision of its own rounding.
-    uint32_t hi[4], lo[4];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) sc[h][i] = exp2f(sc[h][i] - (i < 2 ? s0 : s1));
-      l0 += sc[h][0] + sc[h][1];
-      l1 += sc[h][2] + sc[h][3];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) split_pair<BF16>(sc[h][2 * i], sc[h][2 * i + 1], &hi[2 * h + i], &lo[2 * h + i]);
-    }
-    // Infinities and NaN in the values of a key that one row sees and another does not: zero times such a value is
-    // not zero, so they leave the tile, and the rows that see them get their products by hand.
-    if (differ) {
-      bool odd = false;
-#pragma unroll
-      for (int i = 0; i < L::kTileBytes / 512; ++i) {
-        odd |= has_nonfinite<BF16>(*reinterpret_cast<const uint4 *>(v_tile + (i * 32 + lane) * 16));
-      }
-      if (__any_sync(0xffffffffu, odd)) {
-        for (int kk = 0; kk < kTileKeys; ++kk) {
-          const int from = (lane & ~3) | ((kk & 7) >> 1);
-          const float e0 = __shfl_sync(0xffffffffu, kk < 8 ? ((kk & 1) ? sc[0][1] : sc[0][0]) : ((kk & 1) ? sc[1][1] : sc[1][0]), from);
-          const float e1 = __shfl_sync(0xffffffffu, kk < 8 ? ((kk & 1) ? sc[0][3] : sc[0][2]) : ((kk & 1) ? sc[1][3] : sc[1][2]), from);
-          const int key = at0 + kk < total ? range.key(at0 + kk) : 0;
-          const bool see0 = at0 + kk < total && sees(key, pos0), see1 = at0 + kk < total && sees(key, pos1);
-#pragma unroll
-          for (int c = 0; c < kColTiles; ++c) {
-            const uint32_t w = *reinterpret_cast<const uint32_t *>(v_tile + piece_offset<D>(kk, c) + (lane & 3) * 4);
-            const float2 x = widen_pair<BF16>(w);
-            const bool odd0 = !(fabsf(x.x) < INFINITY), odd1 = !(fabsf(x.y) < INFINITY);
-            if (odd0 && see0) o[c][0] += e0 * x.x;
-            if (odd1 && see0) o[c][1] += e0 * x.y;
-            if (odd0 && see1) o[c][2] += e1 * x.x;
-            if (odd1 && see1) o[c][3] += e1 * x.y;
+          for (int i = 0; i < 4; ++i) {
+            const int place = at0 + h * 8 + (lane & 3) * 2 + (i & 1);
+            if (place >= total || !sees(at.range.key(place), i < 2 ? pos0 : pos1)) sc[h][i] = -INFINITY;
           }
         }
-        __syncwarp();
-#pragma unroll 1
-        for (int i = 0; i < L::kTileBytes / 512; ++i) {
-          uint4 *w = reinterpret_cast<uint4 *>(v_tile + (i * 32 + lane) * 16);
-          *w = without_nonfinite<BF16>(*w);
+      }
+      if (p.scores != nullptr) {  // (no window there: a key's place is the key)
+        const int row0 = at.tile * kRows;
+        float *dst = p.scores + ((static_cast<int64_t>(at.seq) * p.kv_heads + at.head) * p.rows + row0 + my_row) * p.kv_len;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int key = at0 + h * 8 + (lane & 3) * 2 + (i & 1);
+            if (key < total && row0 + my_row + (i < 2 ? 0 : 8) < p.rows) dst[(i < 2 ? 0 : 8) * static_cast<int64_t>(p.kv_len) + key] = sc[h][i];
+          }
         }
-        __syncwarp();
+      }
+      float b0 = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[1][0], sc[1][1]));
+      float b1 = fmaxf(fmaxf(sc[0][2], sc[0][3]), fmaxf(sc[1][2], sc[1][3]));
+#pragma unroll
+      for (int x = 1; x <= 2; x <<= 1) {
+        b0 = fmaxf(b0, __shfl_xor_sync(0xffffffffu, b0, x));
+        b1 = fmaxf(b1, __shfl_xor_sync(0xffffffffu, b1, x));
+      }
+      // The output and the sum are relative to a maximum that follows the rows' own only when one has grown by more
+      // than 2^8: until then the exponentials stay below what every type here holds.
+      if (__any_sync(0xffffffffu, b0 > m0 + 8.0f || b1 > m1 + 8.0f)) {
+        const float n0 = fmaxf(m0, b0), n1 = fmaxf(m1, b1);
+        const float f0 = n0 == -INFINITY ? 1.0f : exp2f(m0 - n0), f1 = n1 == -INFINITY ? 1.0f : exp2f(m1 - n1);
+        l0 *= f0;
+        l1 *= f1;
+#pragma unroll
+        for (int c = 0; c < kColTiles; ++c) {
+          o[c][0] *= f0;
+          o[c][1] *= f0;
+          o[c][2] *= f1;
+          o[c][3] *= f1;
+        }
+        m0 = n0;
+        m1 = n1;
+      }
+      const float s0 = m0 == -INFINITY ? 0.0f : m0, s1 = m1 == -INFINITY ? 0.0f : m1;
+      // The probabilities enter the second product as two 16-bit values each, the rounded one and what it lost: the
+      // product is not what bounds the walk (see above), and the result keeps the precision of its own rounding.
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sc[h][i] = exp2_approx(sc[h][i] - (i < 2 ? s0 : s1));
+        l0 += sc[h][0] + sc[h][1];
+        l1 += sc[h][2] + sc[h][3];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) split_pair<BF16>(sc[h][2 * i], sc[h][2 * i + 1], &hi[2 * h + i], &lo[2 * h + i]);
+      }
+      // Infinities and NaN in the values of a key that one row sees and another does not: zero times such a value is
+      // not zero, so they leave the tile, and the rows that see them get their products by hand.
+      if (differ) {
+        bool odd = false;
+#pragma unroll
+        for (int i = 0; i < L::kTileBytes / 512; ++i) {
+          odd |= has_nonfinite<BF16>(*reinterpret_cast<const uint4 *>(v_tile + (i * 32 + lane) * 16));
+        }
+        if (__any_sync(0xffffffffu, odd)) {
+          for (int kk = 0; kk < kTileKeys; ++kk) {
+            const int from = (lane & ~3) | ((kk & 7) >> 1);
+            const float e0 = __shfl_sync(0xffffffffu, kk < 8 ? ((kk & 1) ? sc[0][1] : sc[0][0]) : ((kk & 1) ? sc[1][1] : sc[1][0]), from);
+            const float e1 = __shfl_sync(0xffffffffu, kk < 8 ? ((kk & 1) ? sc[0][3] : sc[0][2]) : ((kk & 1) ? sc[1][3] : sc[1][2]), from);
+            const int key = at0 + kk < total ? at.range.key(at0 + kk) : 0;
+            const bool see0 = at0 + kk < total && sees(key, pos0), see1 = at0 + kk < total && sees(key, pos1);
+#pragma unroll
+            for (int c = 0; c < kColTiles; ++c) {
+              const uint32_t w = *reinterpret_cast<const uint32_t *>(v_tile + piece_offset<D>(kk, c) + (lane & 3) * 4);
+              const float2 x = widen_pair<BF16>(w);
+              const bool odd0 = !(fabsf(x.x) < INFINITY), odd1 = !(fabsf(x.y) < INFINITY);
+              if (odd0 && see0) o[c][0] += e0 * x.x;
+              if (odd1 && see0) o[c][1] += e0 * x.y;
+              if (odd0 && see1) o[c][2] += e1 * x.x;
+              if (odd1 && see1) o[c][3] += e1 * x.y;
+            }
+          }
+          __syncwarp();
+#pragma unroll 1
+          for (int i = 0; i < L::kTileBytes / 512; ++i) {
+            uint4 *w = reinterpret_cast<uint4 *>(v_tile + (i * 32 + lane) * 16);
+            *w = without_nonfinite<BF16>(*w);
+          }
+          __syncwarp();
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < kColTiles; c += 2) {
+        uint32_t b[4];
+        ldmatrix_x4_trans(b, smem_u32(v_tile + piece_offset<D>(lane & 15, c + (lane >> 4))));
+        mma_16<BF16>(o[c], hi, b[0], b[1]);
+        mma_16<BF16>(o[c + 1], hi, b[2], b[3]);
+        mma_16<BF16>(o[c], lo, b[0], b[1]);
+        mma_16<BF16>(o[c + 1], lo, b[2], b[3]);
       }
     }
-#pragma unroll
-    for (int c = 0; c < kColTiles; c += 2) {
-      uint32_t b[4];
-      ldmatrix_x4_trans(b, smem_u32(v_tile + piece_offset<D>(lane & 15, c + (lane >> 4))));
-      mma_16<BF16>(o[c], hi, b[0], b[1]);
-      mma_16<BF16>(o[c + 1], hi, b[2], b[3]);
-      mma_16<BF16>(o[c], lo, b[0], b[1]);
-      mma_16<BF16>(o[c + 1], lo, b[2], b[3]);
-    }
-  }
 
-  // The four warps' outputs meet over the ring.
-  cp_async_wait_all();
-  __syncthreads();
-#pragma unroll
-  for (int x = 1; x <= 2; x <<= 1) {
-    l0 += __shfl_xor_sync(0xffffffffu, l0, x);
-    l1 += __shfl_xor_sync(0xffffffffu, l1, x);
-  }
-  if ((lane & 3) == 0) {
-    warp_sum[warp][my_row] = make_float2(m0, l0);
-    warp_sum[warp][my_row + 8] = make_float2(m1, l1);
-  }
-  float *warp_out = reinterpret_cast<float *>(smem + L::kRingOff);
-#pragma unroll
-  for (int c = 0; c < kColTiles; ++c) {
-    float *dst = warp_out + (warp * kRows + my_row) * D + c * 8 + (lane & 3) * 2;
-    *reinterpret_cast<float2 *>(dst) = make_float2(o[c][0], o[c][1]);
-    *reinterpret_cast<float2 *>(dst + 8 * D) = make_float2(o[c][2], o[c][3]);
-  }
-  __syncthreads();
+    const Cursor unit = at;
+    if (done + 1 < count && !at.advance(p)) continue;
 
-  const int r = threadIdx.x >> 3, col = (threadIdx.x & 7) * kMyCols;
-  RowSum<kMyCols> sum;
-  sum.clear();
+    // ---- the end of the unit, or of this CTA's part of it. The four warps' outputs meet over the stages that they
+    // have just read, which no load fills before the next step's turn.
+    uint4 next_queries[kMyPieces];
+    if (done + 1 < count) fetch_queries(at, next_queries);
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) sum.raise(warp_sum[w][r].x);
+    for (int x = 1; x <= 2; x <<= 1) {
+      l0 += __shfl_xor_sync(0xffffffffu, l0, x);
+      l1 += __shfl_xor_sync(0xffffffffu, l1, x);
+    }
+    if ((lane & 3) == 0) {
+      warp_sum[warp][my_row] = make_float2(m0, l0);
+      warp_sum[warp][my_row + 8] = make_float2(m1, l1);
+    }
+    __syncwarp();  // (every lane has read its stage)
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) sum.add(warp_sum[w][r], warp_out + (w * kRows + r) * D + col);
-
-  if (p.over_batch) {
-    if (r < live) {
-      const int64_t part = (static_cast<int64_t>(head) * p.splits + split) * p.rows + row0 + r;
-      sum.store(p.part_out + part * D + col);
-      if ((threadIdx.x & 7) == 0) p.part_sum[part] = sum.max_and_sum();
+    for (int c = 0; c < kColTiles; ++c) {
+      float *dst = reinterpret_cast<float *>(k_tile) + my_row * D + c * 8 + (lane & 3) * 2;
+      *reinterpret_cast<float2 *>(dst) = make_float2(o[c][0], o[c][1]);
+      *reinterpret_cast<float2 *>(dst + 8 * D) = make_float2(o[c][2], o[c][3]);
     }
-    return;
-  }
-  if (active > 1) {
-    const int64_t unit = static_cast<int64_t>(run) * p.row_tiles + tile;
-    const int64_t part = (unit * p.splits + split) * kRows + r;
-    if (r < live) {
-      sum.store(p.part_out + part * D + col);
-      if ((threadIdx.x & 7) == 0) p.part_sum[part] = sum.max_and_sum();
-    }
-    __threadfence();
+    if (done + 1 < count) stage_queries(next_queries);
     __syncthreads();
-    if (threadIdx.x == 0) {
-      const uint32_t before = atomicAdd(&p.counters[unit], 1u);
-      is_last = before + 1 == static_cast<uint32_t>(active);
-      if (is_last) p.counters[unit] = 0;
-    }
-    __syncthreads();
-    if (!is_last) return;
-    __threadfence();
-    if (r < live) {
-      sum.clear();
-      const int64_t first = unit * p.splits * kRows + r;
-      for (int s = 0; s < active; ++s) sum.raise(__ldcg(&p.part_sum[first + s * kRows]).x);
-#pragma unroll 4
-      for (int s = 0; s < active; ++s) sum.add_parts(__ldcg(&p.part_sum[first + s * kRows]), p.part_out + (first + s * kRows) * D + col);
-    }
-  }
-  if (p.prefix_splits > 0) {
-    griddep_wait();  // the parts over the prefix
-    if (r < live) {
-      const int64_t first = static_cast<int64_t>(head) * p.prefix_splits * p.prefix_rows + static_cast<int64_t>(seq) * p.rows + row0 + r;
-      for (int s = 0; s < p.prefix_splits; ++s) sum.raise(__ldcg(&p.prefix_sum[first + static_cast<int64_t>(s) * p.prefix_rows]).x);
-#pragma unroll 4
-      for (int s = 0; s < p.prefix_splits; ++s) {
-        const int64_t part = first + static_cast<int64_t>(s) * p.prefix_rows;
-        sum.add_parts(__ldcg(&p.prefix_sum[part]), p.prefix_out + part * D + col);
+
+    const int row0 = unit.tile * kRows, live = min(kRows, p.rows - row0);
+    const int64_t unit_begin = begin + done - unit.step;  // the unit's first step among all
+    const int first_cta = static_cast<int>(unit_begin / per_cta), last_cta = static_cast<int>((unit_begin + unit.steps - 1) / per_cta);
+    const bool shared = !p.over_batch && last_cta > first_cta;
+    const uint8_t *stages = smem + L::kRingOff + (k_tile - ring);  // the first warp's
+    auto own_part = [&](int r, int col, RowSum<4> *sum) {
+      sum->clear();
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) sum->raise(warp_sum[w][r].x);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        sum->add(warp_sum[w][r], reinterpret_cast<const float *>(stages + w * kStages * L::kStageBytes) + r * D + col);
+      }
+    };
+    if (p.over_batch || shared) {
+      const int64_t part = p.over_batch ? (static_cast<int64_t>(unit.head) * p.splits + unit_step / per_cta) * p.rows + row0
+                                        : (static_cast<int64_t>(blockIdx.x) * 2 + (unit_step == 0 ? 1 : 0)) * kRows;
+      for (int i = threadIdx.x; i < live * kQuads; i += kThreads) {
+        const int r = i / kQuads, col = i % kQuads * 4;
+        RowSum<4> sum;
+        own_part(r, col, &sum);
+        sum.store(p.part_out + (part + r) * D + col);
+        if (col == 0) p.part_sum[part + r] = sum.max_and_sum();
       }
     }
-  }
-  if (r >= live) return;
-  const int i = (row0 + r) / p.group, g = (row0 + r) - i * p.group;
-  // A query that sees no key: zeros. (Where it sees some and their exponentials sum to zero or to NaN, that is its result.)
-  const bool empty = p.prefix_splits == 0 && i + len - p.q_len < 0;
-  const float inv = empty ? 0.0f : 1.0f / sum.l;
-  uint16_t *dst = p.out + seq * p.out_stride[0] + static_cast<int64_t>(head * p.group + g) * p.out_stride[1] + i * p.out_stride[2] + col;
-#pragma unroll
-  for (int c = 0; c < kMyCols; c += 8) {
-    uint4 w;
-    w.x = pack_pair<BF16>(sum.o[c] * inv, sum.o[c + 1] * inv);
-    w.y = pack_pair<BF16>(sum.o[c + 2] * inv, sum.o[c + 3] * inv);
-    w.z = pack_pair<BF16>(sum.o[c + 4] * inv, sum.o[c + 5] * inv);
-    w.w = pack_pair<BF16>(sum.o[c + 6] * inv, sum.o[c + 7] * inv);
-    *reinterpret_cast<uint4 *>(dst + c) = empty ? make_uint4(0, 0, 0, 0) : w;
-  }
-  if (p.row_norm != nullptr && (threadIdx.x & 7) == 0) {
-    p.row_norm[static_cast<int64_t>(run) * p.rows + row0 + r] = make_float2(sum.m, inv);
+    bool finish = !p.over_batch;
+    if (shared) {
+      __threadfence();
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        const uint32_t before = atomicAdd(&p.counters[first_cta], 1u);
+        is_last = before == static_cast<uint32_t>(last_cta - first_cta);
+        if (is_last) p.counters[first_cta] = 0;
+      }
+      __syncthreads();
+      finish = is_last;
+      __threadfence();
+    }
+    if (finish) {
+      if (p.prefix_splits > 0) griddep_wait();  // the parts over the prefix
+      for (int i = threadIdx.x; i < live * kQuads; i += kThreads) {
+        const int r = i / kQuads, col = i % kQuads * 4;
+        RowSum<4> sum;
+        if (shared) {
+          sum.clear();
+          auto part_of = [&](int cta) { return (static_cast<int64_t>(cta) * 2 + (cta == first_cta ? 1 : 0)) * kRows + r; };
+#pragma unroll 8
+          for (int c = first_cta; c <= last_cta; ++c) sum.raise(__ldcg(&p.part_sum[part_of(c)]).x);
+#pragma unroll 8
+          for (int c = first_cta; c <= last_cta; ++c) sum.add_parts(__ldcg(&p.part_sum[part_of(c)]), p.part_out + part_of(c) * D + col);
+        } else {
+          own_part(r, col, &sum);
+        }
+        if (p.prefix_splits > 0) {
+          const int64_t first = static_cast<int64_t>(unit.head) * p.prefix_splits * p.prefix_rows + static_cast<int64_t>(unit.seq) * p.rows + row0 + r;
+#pragma unroll 8
+          for (int s = 0; s < p.prefix_splits; ++s) sum.raise(__ldcg(&p.prefix_sum[first + static_cast<int64_t>(s) * p.prefix_rows]).x);
+#pragma unroll 8
+          for (int s = 0; s < p.prefix_splits; ++s) {
+            const int64_t part = first + static_cast<int64_t>(s) * p.prefix_rows;
+            sum.add_parts(__ldcg(&p.prefix_sum[part]), p.prefix_out + part * D + col);
+          }
+        }
+        const int q = (row0 + r) / p.group, g = (row0 + r) - q * p.group;
+        // A query that sees no key: zeros. (Where it sees some and their exponentials sum to zero or to NaN, that is its result.)
+        const bool empty = p.prefix_splits == 0 && q + unit.len - p.q_len < 0;
+        const float inv = empty ? 0.0f : 1.0f / sum.l;
+        const uint2 w = make_uint2(pack_pair<BF16>(sum.o[0] * inv, sum.o[1] * inv), pack_pair<BF16>(sum.o[2] * inv, sum.o[3] * inv));
+        *reinterpret_cast<uint2 *>(p.out + unit.seq * p.out_stride[0] + static_cast<int64_t>(unit.head * p.group + g) * p.out_stride[1] +
+                                   q * p.out_stride[2] + col) = empty ? make_uint2(0, 0) : w;
+        if (p.row_norm != nullptr && col == 0) {
+          p.row_norm[(static_cast<int64_t>(unit.seq) * p.kv_heads + unit.head) * p.rows + row0 + r] = make_float2(sum.m, inv);
+        }
+      }
+    }
+    if (done + 1 < count) {
+      begin_unit();
+      __syncthreads();  // the stages have been read, and the queries
+    }
   }
 }
 
@@ -463,10 +593,11 @@ __global__ void __launch_bounds__(256) add_weights_kernel(const float *__restric
   weights_out[seq * out_seq + head * out_head + key] = weights_in[seq * in_seq + head * in_head + key] + sum;
 }
 
-// How many CTAs divide a unit's keys: enough for about four waves of two CTAs an SM, so that sequences of different
-// lengths even out, but no fewer than 256 keys each.
-int splits_for(int64_t units, int keys) {
-  const int64_t wanted = units > 0 ? (8ll * sm_count() + units - 1) / units : 1;
+constexpr int kCtasPerSm = 2;
+
+// How many CTAs divide a prefix for one of `units` tiles of rows: together two an SM, but no fewer than 256 keys each.
+int prefix_splits(int64_t units, int keys) {
+  const int64_t wanted = kCtasPerSm * static_cast<int64_t>(sm_count()) / units;
   const int most = keys / 256;
   return static_cast<int>(wanted < 1 || most < 1 ? 1 : (wanted < most ? wanted : most));
 }
@@ -482,7 +613,8 @@ struct CachePlan {
   int rows;         // packed rows of a run
   bool tiles;       // the sequences' own keys (and a prefix before them in the same walk) on the tile kernel
   int row_tiles;    // of 16, or pairs of 128
-  int splits;
+  int splits;       // of a pair of tiles
+  int ctas;         // of the few-row kernel
   bool prefix_apart;  // a kernel of its own over the prefix for the rows of the whole batch
   bool prefix_tiles;
   int prefix_rows, prefix_row_tiles, prefix_splits;
@@ -512,9 +644,9 @@ CachePlan cache_plan(const CacheAttentionArgs &a) {
     part_rows = p.splits > 1 ? cache_tiles_part_rows(runs * p.row_tiles, p.splits) : 0;
   } else {
     p.row_tiles = (p.rows + kRows - 1) / kRows;
-    const int64_t units = runs * p.row_tiles;
-    p.splits = units <= kCacheCounters ? splits_for(units, static_cast<int>(most)) : 1;
-    part_rows = p.splits > 1 ? static_cast<size_t>(units) * p.splits * kRows : 0;
+    const int64_t steps = (most + kStepKeys - 1) / kStepKeys, least = std::min<int64_t>(kLeastSteps, steps);  // of a unit, and of a CTA
+    p.ctas = static_cast<int>(std::min<int64_t>(kCtasPerSm * sm_count(), (runs * p.row_tiles * steps + least - 1) / least));
+    part_rows = static_cast<size_t>(p.ctas) * 2 * kRows;
   }
   if (part_rows > 0) {
     p.part_out = take(part_rows * d * 4);
@@ -531,7 +663,7 @@ CachePlan cache_plan(const CacheAttentionArgs &a) {
       p.prefix_row_tiles = (p.prefix_rows + kRows - 1) / kRows;
       // (as many as the kernel finds keys for: every part that the merge reads is written)
       const int steps = (a.prefix_len + kStepKeys - 1) / kStepKeys;
-      const int wanted = splits_for(static_cast<int64_t>(a.kv_heads) * p.prefix_row_tiles, a.prefix_len);
+      const int wanted = prefix_splits(static_cast<int64_t>(a.kv_heads) * p.prefix_row_tiles, a.prefix_len);
       const int per_split = (steps + wanted - 1) / wanted;
       p.prefix_splits = (steps + per_split - 1) / per_split;
     }
@@ -585,7 +717,7 @@ bool cache_attention_supported(const CacheAttentionArgs &a, const char **why) {
     return false;
   }
   const CachePlan plan = cache_plan(a);
-  if (static_cast<int64_t>(a.batch) * a.kv_heads * plan.row_tiles * plan.splits > most || plan.weights.ctas > most ||
+  if ((plan.tiles && static_cast<int64_t>(a.batch) * a.kv_heads * plan.row_tiles * plan.splits > most) || plan.weights.ctas > most ||
       static_cast<int64_t>(a.batch) * a.kv_heads * ((static_cast<int64_t>(a.kv_len) + 255) / 256) > most) {
     *why = "more work than one launch indexes";
     return false;
@@ -676,7 +808,7 @@ cudaError_t cache_attention(const CacheAttentionArgs &a, const char **why, int *
   fill_params(a, &p);
   p.rows = plan.rows;
   p.row_tiles = plan.row_tiles;
-  p.splits = plan.splits;
+  p.batch = a.batch;
   p.part_out = floats(plan.part_out);
   p.part_sum = pairs(plan.part_sum);
   if (a.weights_out != nullptr) {
@@ -718,7 +850,7 @@ cudaError_t cache_attention(const CacheAttentionArgs &a, const char **why, int *
     p.prefix_splits = plan.prefix_splits;
     p.prefix_rows = plan.prefix_rows;
   }
-  e = launch_rows(a, p, static_cast<int64_t>(a.batch) * a.kv_heads * p.row_tiles * p.splits, plan.prefix_apart);
+  e = launch_rows(a, p, plan.ctas, plan.prefix_apart);
   if (e != cudaSuccess) {
     *why = "launching the few-row kernel";
     return e;
