@@ -10,7 +10,6 @@
 
 namespace flsm100 {
 
-constexpr int kFewRowsTile = 16;
 
 __device__ __forceinline__ int sequence_length(const int32_t *kv_lens, int seq, int kv_len) {
   return kv_lens == nullptr ? kv_len : min(max(kv_lens[seq], 0), kv_len);
@@ -83,59 +82,30 @@ __device__ __forceinline__ uint4 without_nonfinite(uint4 w) {
                     w.w & ~nonfinite_halves<BF16>(w.w));
 }
 
-// C columns of a row's output and its sum, relative to the maximum m (log2 units), from parts that have their own:
-// the maxima are seen first (raise), then the parts added, which scales them down to m once. What was there before is
-// scaled when a later maximum raises m.
-template <int C>
+// Four columns of a row's output and its sum, relative to the maximum m (log2 units), from parts that have their own:
+// a part's maximum is seen (raise) before the part is added, which scales it down to m; what was there is scaled when m rises.
 struct RowSum {
-  float m, l, o[C];
+  float m, l;
+  float4 o;
   __device__ __forceinline__ void clear() {
     m = -INFINITY;
     l = 0.0f;
-#pragma unroll
-    for (int i = 0; i < C; ++i) o[i] = 0.0f;
+    o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   }
   __device__ __forceinline__ void raise(float part_max) {
     if (part_max > m) {
       const float f = exp2f(m - part_max);
       m = part_max;
       l *= f;
-#pragma unroll
-      for (int i = 0; i < C; ++i) o[i] *= f;
+      o = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
     }
   }
   // (A part whose rows saw no finite score has the maximum -inf: its sum is 0 or NaN, taken as it is.)
-  __device__ __forceinline__ float factor(float part_max) const { return part_max == -INFINITY ? 1.0f : exp2f(part_max - m); }
-  __device__ __forceinline__ void add(float2 part, const float *part_out) {
-    const float f = factor(part.x);
+  __device__ __forceinline__ void add(float2 part, float4 x) {
+    const float f = part.x == -INFINITY ? 1.0f : exp2f(part.x - m);
     l = fmaf(part.y, f, l);
-#pragma unroll
-    for (int i = 0; i < C; i += 4) {
-      const float4 x = *reinterpret_cast<const float4 *>(part_out + i);
-      o[i] = fmaf(x.x, f, o[i]);
-      o[i + 1] = fmaf(x.y, f, o[i + 1]);
-      o[i + 2] = fmaf(x.z, f, o[i + 2]);
-      o[i + 3] = fmaf(x.w, f, o[i + 3]);
-    }
+    o = make_float4(fmaf(x.x, f, o.x), fmaf(x.y, f, o.y), fmaf(x.z, f, o.z), fmaf(x.w, f, o.w));
   }
-  // The same from global memory that another CTA wrote.
-  __device__ __forceinline__ void add_parts(float2 part, const float *part_out) {
-    const float f = factor(part.x);
-    l = fmaf(part.y, f, l);
-#pragma unroll
-    for (int i = 0; i < C; i += 4) {
-      const float4 x = __ldcg(reinterpret_cast<const float4 *>(part_out + i));
-      o[i] = fmaf(x.x, f, o[i]);
-      o[i + 1] = fmaf(x.y, f, o[i + 1]);
-      o[i + 2] = fmaf(x.z, f, o[i + 2]);
-      o[i + 3] = fmaf(x.w, f, o[i + 3]);
-    }
-  }
-  __device__ __forceinline__ void store(float *dst) const {
-#pragma unroll
-    for (int i = 0; i < C; i += 4) *reinterpret_cast<float4 *>(dst + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-  }
-  __device__ __forceinline__ float2 max_and_sum() const { return make_float2(m, l); }
 };
 
 }  // namespace flsm100

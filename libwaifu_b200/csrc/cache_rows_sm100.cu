@@ -1,8 +1,9 @@
 // Attention over a key-value cache for few query rows (single tokens): the keys of a sequence are split over
 // the GPU, and a key's row is read once for all the query heads that share it.
 //
-// The rows of one key-value head, its group of query heads times the queries, are packed into tiles of 16, the M
-// of mma.sync m16n8k16. A unit is such a tile with the keys its sequence's queries see, in steps of 64. The steps of
+// The rows of one key-value head, its group of query heads times the queries, are packed into tiles of 8 or 16, the N of
+// mma.sync m16n8k16, once or twice; the keys of a tile are its M (S^T = K Q^T), and so are the columns of the output
+// (O^T = V^T P^T): a decode step has a few rows to a head, and would leave most of an M of 16 empty. A unit is such a tile with the keys its sequence's queries see, in steps of 64. The steps of
 // all units, one after the other, are dealt out in equal runs over two CTAs an SM, whatever the sequences'
 // lengths: a CTA takes the end of one unit, whole units, the beginning of another. Its four warps walk 16 keys
 // of a step each on their own: a ring of shared-memory stages per warp, filled by 16-byte asynchronous copies that run
@@ -11,7 +12,8 @@
 // meet over the stages they have just read; a unit that several CTAs share meets in the workspace, where the last one to
 // arrive adds the parts in their order: the result does not depend on which came last.
 //
-// What bounds it is the keys' way from HBM: 2 head_dim bytes twice per key, against 16 x head_dim x 4 operations.
+// What bounds it is the keys' way from HBM: 2 head_dim bytes twice per key, against 8 or 16 x head_dim x 4 operations. A warp
+// has about 350 cycles of it per 16 keys at head_dim 128, times the eight warps of an SM, for its own instructions.
 #include "cache_attention_sm100.cuh"
 
 #include <cuda_bf16.h>
@@ -33,7 +35,7 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kTileKeys = 16;  // keys a warp takes at a time
 constexpr int kStages = 3;
 constexpr int kStepKeys = kWarps * kTileKeys;
-constexpr int kRows = kFewRowsTile;
+constexpr int kMaxRows = 16;
 constexpr int kLeastSteps = 4;  // that are worth a CTA of their own
 
 template <int D>
@@ -42,9 +44,9 @@ struct RowsLayout {
   static constexpr int kTileBytes = kTileKeys * kRowBytes;
   static constexpr int kStageBytes = 2 * kTileBytes;  // K and V of 16 keys
   static constexpr int kQOff = 0;
-  static constexpr int kRingOff = kRows * kRowBytes;
+  static constexpr int kRingOff = kMaxRows * kRowBytes;
   static constexpr int kSmemBytes = kRingOff + kWarps * kStages * kStageBytes;
-  static_assert(kRows * D * 4 == kStageBytes, "a warp's outputs fit the stage that it has read");
+  static_assert(kMaxRows * D * 4 == kStageBytes, "a warp's outputs fit the stage that it has read");
   static_assert(2 * (kSmemBytes + 2048) <= 227 * 1024, "two CTAs an SM");
 };
 
@@ -52,6 +54,12 @@ struct RowsLayout {
 template <int D>
 __device__ __forceinline__ int piece_offset(int r, int c) {
   return r * (D * 2) + ((c ^ (r & 7)) << 4);
+}
+
+// Where column `col` of row r of a warp's output lies, in floats: lanes that hold two rows each apart write to different banks.
+template <int D>
+__device__ __forceinline__ int out_offset(int r, int col) {
+  return r * D + (col ^ ((r & 6) << 2));
 }
 
 __device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
@@ -85,6 +93,13 @@ __device__ __forceinline__ void mma_16(float (&d)[4], const uint32_t (&a)[4], ui
   }
 }
 
+// An 8 x 8 matrix of 16-bit values, a pair of one row per lane, transposed.
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
 template <int N>
 __device__ __forceinline__ void cp_async_wait_group() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
@@ -102,9 +117,9 @@ struct RowsParams {
   bool over_batch;
   int batch;
   int rows;       // packed rows of a key-value head: group * q_len, times the batch over a prefix
-  int row_tiles;  // of 16
+  int row_tiles;  // of 8 or 16
   int splits;     // over a prefix: CTAs that divide a unit
-  float *part_out;   // (CTA, 2, 16, D): a unit's end, and a unit's beginning; (kv_head, split, rows, D) over a prefix
+  float *part_out;   // (CTA, 2, rows of a tile, D): a unit's end, and a unit's beginning; (kv_head, split, rows, D) over a prefix
   float2 *part_sum;  // the same without D: maximum in log2 units, sum
   uint32_t *counters;  // of the unit that the CTA's last run of steps begins
   // The parts over the prefix that an earlier kernel left, as above; 0 splits without.
@@ -147,14 +162,40 @@ struct Cursor {
   }
 };
 
-template <int D, bool BF16>
+// Adds four columns of `count` parts that other CTAs wrote, part c at row place(c), in their order, eight of them on their way
+// at a time.
+template <int D, typename Place>
+__device__ __forceinline__ void add_parts(int count, const float2 *sums, const float *outs, int col, RowSum *sum, Place &&place) {
+  constexpr int kAtOnce = 8;
+  for (int c0 = 0; c0 < count; c0 += kAtOnce) {
+    float2 part[kAtOnce];
+    float4 out[kAtOnce];
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int64_t at = place(min(c0 + i, count - 1));
+      part[i] = __ldcg(&sums[at]);
+      out[i] = __ldcg(reinterpret_cast<const float4 *>(outs + at * D + col));
+    }
+    float top = part[0].x;
+#pragma unroll
+    for (int i = 1; i < kAtOnce; ++i) top = fmaxf(top, part[i].x);
+    sum->raise(top);
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      if (c0 + i < count) sum->add(part[i], out[i]);
+    }
+  }
+}
+
+template <int D, bool BF16, int NB>
 __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_constant__ RowsParams p) {
   using L = RowsLayout<D>;
-  constexpr int kPieces = D / 8;    // of a row
-  constexpr int kColTiles = D / 8;  // of the output, eight columns each
-  constexpr int kQuads = D / 4;     // of a row: a thread finishes four columns at a time
+  constexpr int kRows = NB * 8;
+  constexpr int kPieces = D / 8;     // of a row
+  constexpr int kColTiles = D / 16;  // of the output, sixteen columns each
+  constexpr int kQuads = D / 4;      // of a row: a thread finishes four columns at a time
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float2 warp_sum[kWarps][kRows];
+  __shared__ float2 warp_sum[kWarps][NB * 8];
   __shared__ int64_t scan[kWarps];
   __shared__ int64_t found_before;
   __shared__ int found_seq, is_last, longest[kWarps];
@@ -177,53 +218,69 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
     begin = load.step = static_cast<int>(at / p.kv_heads * per_cta);
     count = min(static_cast<int>(per_cta), load.steps - load.step);
   } else {
-    // The steps of the whole batch, and the sequence in which this CTA's begin. Each thread has some sequences.
-    const int mine = (p.batch + kThreads - 1) / kThreads;
-    const int first = threadIdx.x * mine, last = min(first + mine, p.batch);
     const int units = p.kv_heads * p.row_tiles;
-    int64_t sum = 0;
-    int most = 1;
-    for (load.seq = first; load.seq < last; ++load.seq) {
-      load.enter_sequence(p);
-      sum += static_cast<int64_t>(load.steps) * units;
-      most = max(most, load.steps);
-    }
-    int64_t upto = sum;
-#pragma unroll
-    for (int x = 1; x < 32; x <<= 1) {
-      const int64_t y = __shfl_up_sync(0xffffffffu, upto, x);
-      if (lane >= x) upto += y;
-      most = max(most, __shfl_xor_sync(0xffffffffu, most, x));
-    }
-    if (lane == 31) scan[warp] = upto;
-    if (lane == 0) longest[warp] = most;
-    __syncthreads();
-    int64_t before = upto - sum, total = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) before += scan[w];
-      total += scan[w];
-      most = max(most, longest[w]);
-    }
     // Four steps each at least, or one unit where they are shorter.
-    per_cta = max((total + gridDim.x - 1) / gridDim.x, static_cast<int64_t>(min(kLeastSteps, most)));
-    begin = blockIdx.x * per_cta;
-    if (begin >= total) return;
-    count = static_cast<int>(min(per_cta, total - begin));
-    if (before <= begin && begin < before + sum) {
-      for (load.seq = first;; ++load.seq) {
+    auto deal_out = [&](int64_t total, int most) {
+      per_cta = max((total + gridDim.x - 1) / gridDim.x, static_cast<int64_t>(min(kLeastSteps, most)));
+      begin = blockIdx.x * per_cta;
+      count = static_cast<int>(max(static_cast<int64_t>(0), min(per_cta, total - begin)));
+    };
+    int64_t before = 0;
+    if (p.kv_lens == nullptr || p.batch == 1) {  // all alike
+      load.seq = 0;
+      load.enter_sequence(p);
+      const int64_t each = static_cast<int64_t>(load.steps) * units;
+      deal_out(each * p.batch, load.steps);
+      if (count == 0) return;
+      load.seq = static_cast<int>(begin / each);
+      before = load.seq * each;
+    } else {
+      // The steps of the whole batch, and the sequence in which this CTA's begin. Each thread has some sequences.
+      const int mine = (p.batch + kThreads - 1) / kThreads;
+      const int first = threadIdx.x * mine, last = min(first + mine, p.batch);
+      int64_t sum = 0;
+      int most = 1;
+      for (load.seq = first; load.seq < last; ++load.seq) {
         load.enter_sequence(p);
-        const int64_t here = static_cast<int64_t>(load.steps) * units;
-        if (begin < before + here) break;
-        before += here;
+        sum += static_cast<int64_t>(load.steps) * units;
+        most = max(most, load.steps);
       }
-      found_seq = load.seq;
-      found_before = before;
+      int64_t upto = sum;
+#pragma unroll
+      for (int x = 1; x < 32; x <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, upto, x);
+        if (lane >= x) upto += y;
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, x));
+      }
+      if (lane == 31) scan[warp] = upto;
+      if (lane == 0) longest[warp] = most;
+      __syncthreads();
+      before = upto - sum;
+      int64_t total = 0;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) before += scan[w];
+        total += scan[w];
+        most = max(most, longest[w]);
+      }
+      deal_out(total, most);
+      if (count == 0) return;
+      if (before <= begin && begin < before + sum) {
+        for (load.seq = first;; ++load.seq) {
+          load.enter_sequence(p);
+          const int64_t here = static_cast<int64_t>(load.steps) * units;
+          if (begin < before + here) break;
+          before += here;
+        }
+        found_seq = load.seq;
+        found_before = before;
+      }
+      __syncthreads();
+      load.seq = found_seq;
+      before = found_before;
     }
-    __syncthreads();
-    load.seq = found_seq;
     load.enter_sequence(p);
-    const int64_t in_seq = begin - found_before;
+    const int64_t in_seq = begin - before;
     const int unit = static_cast<int>(in_seq / load.steps);
     load.step = static_cast<int>(in_seq - static_cast<int64_t>(unit) * load.steps);
     load.tile = unit % p.row_tiles;
@@ -236,21 +293,26 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
   constexpr int kRowsAtOnce = 32 / kPieces;
   const int lane_row = lane / kPieces, lane_piece = lane % kPieces;
   int loaded = 0, load_stage = 0;
+  const uint16_t *k_base, *v_base;  // of the unit that is loaded, and this lane's piece
+  auto find_unit = [&]() {
+    k_base = p.k + load.head * p.k_stride[1] + (p.over_batch ? 0 : load.seq * p.k_stride[0]) + lane_piece * 8;
+    v_base = p.v + load.head * p.v_stride[1] + (p.over_batch ? 0 : load.seq * p.v_stride[0]) + lane_piece * 8;
+  };
+  find_unit();
   auto load_tile = [&]() {
     if (loaded < count) {
       uint8_t *dst = ring + load_stage * L::kStageBytes;
       const int at0 = (load.step * kWarps + warp) * kTileKeys, total = load.range.count();
-      const uint16_t *k = p.k + load.head * p.k_stride[1] + (p.over_batch ? 0 : load.seq * p.k_stride[0]) + lane_piece * 8;
-      const uint16_t *v = p.v + load.head * p.v_stride[1] + (p.over_batch ? 0 : load.seq * p.v_stride[0]) + lane_piece * 8;
       if (at0 + kTileKeys <= total && (at0 >= load.range.sinks || at0 + kTileKeys <= load.range.sinks)) {  // one run of keys
         const int key = load.range.key(at0) + lane_row;
-        k += key * p.k_stride[2];
-        v += key * p.v_stride[2];
+        const uint16_t *k = k_base + key * p.k_stride[2], *v = v_base + key * p.v_stride[2];
 #pragma unroll
         for (int i = 0; i < kTileKeys / kRowsAtOnce; ++i) {
           const int off = piece_offset<D>(i * kRowsAtOnce + lane_row, lane_piece);
-          cp_async_16(dst + off, k + i * kRowsAtOnce * p.k_stride[2], 16);
-          cp_async_16(dst + L::kTileBytes + off, v + i * kRowsAtOnce * p.v_stride[2], 16);
+          cp_async_16(dst + off, k, 16);
+          cp_async_16(dst + L::kTileBytes + off, v, 16);
+          k += kRowsAtOnce * p.k_stride[2];
+          v += kRowsAtOnce * p.v_stride[2];
         }
       } else {
 #pragma unroll 1
@@ -259,13 +321,13 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
           const bool there = at0 + r < total;
           const int64_t key = there ? load.range.key(at0 + r) : 0;
           const int off = piece_offset<D>(r, lane_piece);
-          cp_async_16(dst + off, k + key * p.k_stride[2], there ? 16 : 0);
-          cp_async_16(dst + L::kTileBytes + off, v + key * p.v_stride[2], there ? 16 : 0);
+          cp_async_16(dst + off, k_base + key * p.k_stride[2], there ? 16 : 0);
+          cp_async_16(dst + L::kTileBytes + off, v_base + key * p.v_stride[2], there ? 16 : 0);
         }
       }
       ++loaded;
       load_stage = load_stage + 1 == kStages ? 0 : load_stage + 1;
-      if (loaded < count) load.advance(p);
+      if (loaded < count && load.advance(p)) find_unit();
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -278,7 +340,7 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
     const int r = u.tile * kRows + (threadIdx.x >> 3);
 #pragma unroll
     for (int c = 0; c < kMyPieces; ++c) x[c] = make_uint4(0, 0, 0, 0);
-    if (r < p.rows) {
+    if ((threadIdx.x >> 3) < kRows && r < p.rows) {
       int n = u.seq, in_seq = r;
       if (p.over_batch) {
         n = in_seq / (p.group * p.q_len);
@@ -301,29 +363,47 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
   }
   __syncthreads();
 
-  const int my_row = lane >> 2;  // this thread's rows of the tile: my_row and my_row + 8
-  uint32_t qf[D / 16][4];
-  float o[kColTiles][4];
-  float m0, m1, l0, l1;
-  int first_pos, last_pos, pos0, pos1;  // of the tile's rows, and of this thread's
+  // Of the fragments of S^T and O^T this lane has the rows (keys, columns) lane / 4 and + 8, and of every eight query rows
+  // the two from my_row on.
+  const int my_key = lane >> 2, my_row = (lane & 3) * 2;
+  uint32_t qf[D / 16][NB][2];
+  float o[kColTiles][NB][4];
+  float m[NB][2], l[NB][2];
+  int first_pos, last_pos, pos[NB][2];  // of the tile's rows, and of this thread's
   int unit_step;                        // the first step that this CTA takes of the unit
   auto begin_unit = [&]() {
 #pragma unroll
     for (int s = 0; s < D / 16; ++s) {
-      ldmatrix_x4(qf[s], smem_u32(smem + L::kQOff + piece_offset<D>(lane & 15, 2 * s + (lane >> 4))));
+      if constexpr (NB == 2) {
+        uint32_t b[4];
+        ldmatrix_x4(b, smem_u32(smem + L::kQOff + piece_offset<D>((lane & 7) + ((lane >> 4) << 3), 2 * s + ((lane >> 3) & 1))));
+        qf[s][0][0] = b[0], qf[s][0][1] = b[1], qf[s][NB - 1][0] = b[2], qf[s][NB - 1][1] = b[3];
+      } else if ((s & 1) == 0) {
+        uint32_t b[4];
+        ldmatrix_x4(b, smem_u32(smem + L::kQOff + piece_offset<D>(lane & 7, 2 * s + (lane >> 3))));
+        qf[s][0][0] = b[0], qf[s][0][1] = b[1], qf[s + 1][0][0] = b[2], qf[s + 1][0][1] = b[3];
+      }
     }
 #pragma unroll
     for (int c = 0; c < kColTiles; ++c) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[c][i] = 0.0f;
+      for (int n = 0; n < NB; ++n) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[c][n][i] = 0.0f;
+      }
     }
-    m0 = m1 = -INFINITY;
-    l0 = l1 = 0.0f;
     const int row0 = at.tile * kRows, offset = at.len - p.q_len;
     first_pos = row0 / p.group + offset;
     last_pos = (min(row0 + kRows, p.rows) - 1) / p.group + offset;
-    pos0 = (row0 + my_row) / p.group + offset;
-    pos1 = (row0 + my_row + 8) / p.group + offset;
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        m[n][i] = -INFINITY;
+        l[n][i] = 0.0f;
+        pos[n][i] = (row0 + n * 8 + my_row + i) / p.group + offset;
+      }
+    }
     unit_step = at.step;
   };
   auto sees = [&](int key, int pos) { return p.over_batch || (key <= pos && (key > pos - p.window || key < p.sinks)); };
@@ -341,80 +421,90 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
 
     const int at0 = (at.step * kWarps + warp) * kTileKeys, total = at.range.count();
     if (at0 < total) {
-      float sc[2][4] = {};  // keys 0 .. 7 and 8 .. 15 of the tile: (row, key), (row, key + 1), (row + 8, key), ...
+      float sc[NB][4] = {};  // (key, row), (key, row + 1), (key + 8, row), (key + 8, row + 1)
 #pragma unroll
       for (int s = 0; s < D / 16; ++s) {
-        uint32_t b[4];
-        ldmatrix_x4(b, smem_u32(k_tile + piece_offset<D>((lane & 7) + ((lane >> 4) << 3), 2 * s + ((lane >> 3) & 1))));
-        mma_16<BF16>(sc[0], qf[s], b[0], b[1]);
-        mma_16<BF16>(sc[1], qf[s], b[2], b[3]);
+        uint32_t a[4];
+        ldmatrix_x4(a, smem_u32(k_tile + piece_offset<D>(lane & 15, 2 * s + (lane >> 4))));
+#pragma unroll
+        for (int n = 0; n < NB; ++n) mma_16<BF16>(sc[n], a, qf[s][n][0], qf[s][n][1]);
       }
       const int key_lo = at.range.key(at0), key_hi = at.range.key(min(at0 + kTileKeys, total) - 1);
       // Does some row not see some key here? (The keys between key_lo and key_hi may jump from the sinks to the window.)
       const bool differ = !p.over_batch && (key_hi > first_pos || (key_hi >= p.sinks && key_lo <= last_pos - p.window));
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      for (int n = 0; n < NB; ++n) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sc[h][i] *= p.scale_log2;
+        for (int i = 0; i < 4; ++i) sc[n][i] *= p.scale_log2;
       }
       if (differ || at0 + kTileKeys > total) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
+          const int place = at0 + h * 8 + my_key, key = place < total ? at.range.key(place) : 0;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int place = at0 + h * 8 + (lane & 3) * 2 + (i & 1);
-            if (place >= total || !sees(at.range.key(place), i < 2 ? pos0 : pos1)) sc[h][i] = -INFINITY;
+          for (int n = 0; n < NB; ++n) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              if (place >= total || !sees(key, pos[n][i])) sc[n][2 * h + i] = -INFINITY;
+            }
           }
         }
       }
       if (p.scores != nullptr) {  // (no window there: a key's place is the key)
         const int row0 = at.tile * kRows;
-        float *dst = p.scores + ((static_cast<int64_t>(at.seq) * p.kv_heads + at.head) * p.rows + row0 + my_row) * p.kv_len;
+        float *dst = p.scores + ((static_cast<int64_t>(at.seq) * p.kv_heads + at.head) * p.rows + row0) * p.kv_len + at0 + my_key;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int n = 0; n < NB; ++n) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int key = at0 + h * 8 + (lane & 3) * 2 + (i & 1);
-            if (key < total && row0 + my_row + (i < 2 ? 0 : 8) < p.rows) dst[(i < 2 ? 0 : 8) * static_cast<int64_t>(p.kv_len) + key] = sc[h][i];
+            const int row = n * 8 + my_row + (i & 1);
+            if (at0 + (i >> 1) * 8 + my_key < total && row0 + row < p.rows) dst[row * static_cast<int64_t>(p.kv_len) + (i >> 1) * 8] = sc[n][i];
           }
         }
       }
-      float b0 = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[1][0], sc[1][1]));
-      float b1 = fmaxf(fmaxf(sc[0][2], sc[0][3]), fmaxf(sc[1][2], sc[1][3]));
-#pragma unroll
-      for (int x = 1; x <= 2; x <<= 1) {
-        b0 = fmaxf(b0, __shfl_xor_sync(0xffffffffu, b0, x));
-        b1 = fmaxf(b1, __shfl_xor_sync(0xffffffffu, b1, x));
-      }
       // The output and the sum are relative to a maximum that follows the rows' own only when one has grown by more
-      // than 2^8: until then the exponentials stay below what every type here holds.
-      if (__any_sync(0xffffffffu, b0 > m0 + 8.0f || b1 > m1 + 8.0f)) {
-        const float n0 = fmaxf(m0, b0), n1 = fmaxf(m1, b1);
-        const float f0 = n0 == -INFINITY ? 1.0f : exp2f(m0 - n0), f1 = n1 == -INFINITY ? 1.0f : exp2f(m1 - n1);
-        l0 *= f0;
-        l1 *= f1;
+      // than 2^8: until then the exponentials stay below what every type here holds, and no lane has to know another's.
+      bool grown = false;
 #pragma unroll
-        for (int c = 0; c < kColTiles; ++c) {
-          o[c][0] *= f0;
-          o[c][1] *= f0;
-          o[c][2] *= f1;
-          o[c][3] *= f1;
-        }
-        m0 = n0;
-        m1 = n1;
+      for (int n = 0; n < NB; ++n) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) grown |= sc[n][i] > m[n][i & 1] + 8.0f;
       }
-      const float s0 = m0 == -INFINITY ? 0.0f : m0, s1 = m1 == -INFINITY ? 0.0f : m1;
+      if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float top = fmaxf(m[n][i], fmaxf(sc[n][i], sc[n][2 + i]));
+#pragma unroll
+            for (int x = 4; x <= 16; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+            const float f = top == -INFINITY ? 1.0f : exp2f(m[n][i] - top);
+            m[n][i] = top;
+            l[n][i] *= f;
+#pragma unroll
+            for (int c = 0; c < kColTiles; ++c) {
+              o[c][n][i] *= f;
+              o[c][n][2 + i] *= f;
+            }
+          }
+        }
+      }
       // The probabilities enter the second product as two 16-bit values each, the rounded one and what it lost: the
       // product is not what bounds the walk (see above), and the result keeps the precision of its own rounding.
-      uint32_t hi[4], lo[4];
+      uint32_t hi[NB][2], lo[NB][2];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      for (int n = 0; n < NB; ++n) {
+        const float s0 = m[n][0] == -INFINITY ? 0.0f : m[n][0], s1 = m[n][1] == -INFINITY ? 0.0f : m[n][1];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sc[h][i] = exp2_approx(sc[h][i] - (i < 2 ? s0 : s1));
-        l0 += sc[h][0] + sc[h][1];
-        l1 += sc[h][2] + sc[h][3];
+        for (int i = 0; i < 4; ++i) sc[n][i] = exp2_approx(sc[n][i] - ((i & 1) ? s1 : s0));
+        l[n][0] += sc[n][0] + sc[n][2];
+        l[n][1] += sc[n][1] + sc[n][3];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) split_pair<BF16>(sc[h][2 * i], sc[h][2 * i + 1], &hi[2 * h + i], &lo[2 * h + i]);
+        for (int h = 0; h < 2; ++h) {
+          split_pair<BF16>(sc[n][2 * h], sc[n][2 * h + 1], &hi[n][h], &lo[n][h]);
+          hi[n][h] = transpose_8x8(hi[n][h]);
+          lo[n][h] = transpose_8x8(lo[n][h]);
+        }
       }
       // Infinities and NaN in the values of a key that one row sees and another does not: zero times such a value is
       // not zero, so they leave the tile, and the rows that see them get their products by hand.
@@ -426,20 +516,21 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
         }
         if (__any_sync(0xffffffffu, odd)) {
           for (int kk = 0; kk < kTileKeys; ++kk) {
-            const int from = (lane & ~3) | ((kk & 7) >> 1);
-            const float e0 = __shfl_sync(0xffffffffu, kk < 8 ? ((kk & 1) ? sc[0][1] : sc[0][0]) : ((kk & 1) ? sc[1][1] : sc[1][0]), from);
-            const float e1 = __shfl_sync(0xffffffffu, kk < 8 ? ((kk & 1) ? sc[0][3] : sc[0][2]) : ((kk & 1) ? sc[1][3] : sc[1][2]), from);
+            const int from = ((kk & 7) << 2) | (lane & 3);
             const int key = at0 + kk < total ? at.range.key(at0 + kk) : 0;
-            const bool see0 = at0 + kk < total && sees(key, pos0), see1 = at0 + kk < total && sees(key, pos1);
 #pragma unroll
-            for (int c = 0; c < kColTiles; ++c) {
-              const uint32_t w = *reinterpret_cast<const uint32_t *>(v_tile + piece_offset<D>(kk, c) + (lane & 3) * 4);
-              const float2 x = widen_pair<BF16>(w);
-              const bool odd0 = !(fabsf(x.x) < INFINITY), odd1 = !(fabsf(x.y) < INFINITY);
-              if (odd0 && see0) o[c][0] += e0 * x.x;
-              if (odd1 && see0) o[c][1] += e0 * x.y;
-              if (odd0 && see1) o[c][2] += e1 * x.x;
-              if (odd1 && see1) o[c][3] += e1 * x.y;
+            for (int n = 0; n < NB; ++n) {
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const float e = __shfl_sync(0xffffffffu, kk < 8 ? sc[n][i] : sc[n][2 + i], from);
+                if (at0 + kk >= total || !sees(key, pos[n][i])) continue;
+#pragma unroll
+                for (int c = 0; c < 2 * kColTiles; ++c) {
+                  const uint16_t w = *reinterpret_cast<const uint16_t *>(v_tile + piece_offset<D>(kk, c) + my_key * 2);
+                  const float x = widen_pair<BF16>(w).x;
+                  if (!(fabsf(x) < INFINITY)) o[c >> 1][n][(c & 1) * 2 + i] += e * x;
+                }
+              }
             }
           }
           __syncwarp();
@@ -452,13 +543,14 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
         }
       }
 #pragma unroll
-      for (int c = 0; c < kColTiles; c += 2) {
-        uint32_t b[4];
-        ldmatrix_x4_trans(b, smem_u32(v_tile + piece_offset<D>(lane & 15, c + (lane >> 4))));
-        mma_16<BF16>(o[c], hi, b[0], b[1]);
-        mma_16<BF16>(o[c + 1], hi, b[2], b[3]);
-        mma_16<BF16>(o[c], lo, b[0], b[1]);
-        mma_16<BF16>(o[c + 1], lo, b[2], b[3]);
+      for (int c = 0; c < kColTiles; ++c) {
+        uint32_t a[4];  // columns by keys
+        ldmatrix_x4_trans(a, smem_u32(v_tile + piece_offset<D>((lane & 7) + ((lane >> 4) << 3), 2 * c + ((lane >> 3) & 1))));
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          mma_16<BF16>(o[c][n], a, hi[n][0], hi[n][1]);
+          mma_16<BF16>(o[c][n], a, lo[n][0], lo[n][1]);
+        }
       }
     }
 
@@ -470,20 +562,25 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
     uint4 next_queries[kMyPieces];
     if (done + 1 < count) fetch_queries(at, next_queries);
 #pragma unroll
-    for (int x = 1; x <= 2; x <<= 1) {
-      l0 += __shfl_xor_sync(0xffffffffu, l0, x);
-      l1 += __shfl_xor_sync(0xffffffffu, l1, x);
-    }
-    if ((lane & 3) == 0) {
-      warp_sum[warp][my_row] = make_float2(m0, l0);
-      warp_sum[warp][my_row + 8] = make_float2(m1, l1);
+    for (int n = 0; n < NB; ++n) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int x = 4; x <= 16; x <<= 1) l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], x);
+        if (lane < 4) warp_sum[warp][n * 8 + my_row + i] = make_float2(m[n][i], l[n][i]);
+      }
     }
     __syncwarp();  // (every lane has read its stage)
 #pragma unroll
     for (int c = 0; c < kColTiles; ++c) {
-      float *dst = reinterpret_cast<float *>(k_tile) + my_row * D + c * 8 + (lane & 3) * 2;
-      *reinterpret_cast<float2 *>(dst) = make_float2(o[c][0], o[c][1]);
-      *reinterpret_cast<float2 *>(dst + 8 * D) = make_float2(o[c][2], o[c][3]);
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int row = n * 8 + my_row + (i & 1);
+          reinterpret_cast<float *>(k_tile)[out_offset<D>(row, c * 16 + (i >> 1) * 8 + my_key)] = o[c][n][i];
+        }
+      }
     }
     if (done + 1 < count) stage_queries(next_queries);
     __syncthreads();
@@ -493,13 +590,14 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
     const int first_cta = static_cast<int>(unit_begin / per_cta), last_cta = static_cast<int>((unit_begin + unit.steps - 1) / per_cta);
     const bool shared = !p.over_batch && last_cta > first_cta;
     const uint8_t *stages = smem + L::kRingOff + (k_tile - ring);  // the first warp's
-    auto own_part = [&](int r, int col, RowSum<4> *sum) {
+    auto own_part = [&](int r, int col, RowSum *sum) {
       sum->clear();
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) sum->raise(warp_sum[w][r].x);
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        sum->add(warp_sum[w][r], reinterpret_cast<const float *>(stages + w * kStages * L::kStageBytes) + r * D + col);
+        sum->add(warp_sum[w][r], *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(stages + w * kStages * L::kStageBytes) +
+                                                                   out_offset<D>(r, col)));
       }
     };
     if (p.over_batch || shared) {
@@ -507,10 +605,10 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
                                         : (static_cast<int64_t>(blockIdx.x) * 2 + (unit_step == 0 ? 1 : 0)) * kRows;
       for (int i = threadIdx.x; i < live * kQuads; i += kThreads) {
         const int r = i / kQuads, col = i % kQuads * 4;
-        RowSum<4> sum;
+        RowSum sum;
         own_part(r, col, &sum);
-        sum.store(p.part_out + (part + r) * D + col);
-        if (col == 0) p.part_sum[part + r] = sum.max_and_sum();
+        *reinterpret_cast<float4 *>(p.part_out + (part + r) * D + col) = sum.o;
+        if (col == 0) p.part_sum[part + r] = make_float2(sum.m, sum.l);
       }
     }
     bool finish = !p.over_batch;
@@ -530,32 +628,24 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
       if (p.prefix_splits > 0) griddep_wait();  // the parts over the prefix
       for (int i = threadIdx.x; i < live * kQuads; i += kThreads) {
         const int r = i / kQuads, col = i % kQuads * 4;
-        RowSum<4> sum;
+        RowSum sum;
         if (shared) {
           sum.clear();
-          auto part_of = [&](int cta) { return (static_cast<int64_t>(cta) * 2 + (cta == first_cta ? 1 : 0)) * kRows + r; };
-#pragma unroll 8
-          for (int c = first_cta; c <= last_cta; ++c) sum.raise(__ldcg(&p.part_sum[part_of(c)]).x);
-#pragma unroll 8
-          for (int c = first_cta; c <= last_cta; ++c) sum.add_parts(__ldcg(&p.part_sum[part_of(c)]), p.part_out + part_of(c) * D + col);
+          add_parts<D>(last_cta - first_cta + 1, p.part_sum, p.part_out, col, &sum,
+                       [&](int c) { return (static_cast<int64_t>(first_cta + c) * 2 + (c == 0 ? 1 : 0)) * kRows + r; });
         } else {
           own_part(r, col, &sum);
         }
         if (p.prefix_splits > 0) {
           const int64_t first = static_cast<int64_t>(unit.head) * p.prefix_splits * p.prefix_rows + static_cast<int64_t>(unit.seq) * p.rows + row0 + r;
-#pragma unroll 8
-          for (int s = 0; s < p.prefix_splits; ++s) sum.raise(__ldcg(&p.prefix_sum[first + static_cast<int64_t>(s) * p.prefix_rows]).x);
-#pragma unroll 8
-          for (int s = 0; s < p.prefix_splits; ++s) {
-            const int64_t part = first + static_cast<int64_t>(s) * p.prefix_rows;
-            sum.add_parts(__ldcg(&p.prefix_sum[part]), p.prefix_out + part * D + col);
-          }
+          add_parts<D>(p.prefix_splits, p.prefix_sum, p.prefix_out, col, &sum,
+                       [&](int c) { return first + static_cast<int64_t>(c) * p.prefix_rows; });
         }
         const int q = (row0 + r) / p.group, g = (row0 + r) - q * p.group;
         // A query that sees no key: zeros. (Where it sees some and their exponentials sum to zero or to NaN, that is its result.)
         const bool empty = p.prefix_splits == 0 && q + unit.len - p.q_len < 0;
         const float inv = empty ? 0.0f : 1.0f / sum.l;
-        const uint2 w = make_uint2(pack_pair<BF16>(sum.o[0] * inv, sum.o[1] * inv), pack_pair<BF16>(sum.o[2] * inv, sum.o[3] * inv));
+        const uint2 w = make_uint2(pack_pair<BF16>(sum.o.x * inv, sum.o.y * inv), pack_pair<BF16>(sum.o.z * inv, sum.o.w * inv));
         *reinterpret_cast<uint2 *>(p.out + unit.seq * p.out_stride[0] + static_cast<int64_t>(unit.head * p.group + g) * p.out_stride[1] +
                                    q * p.out_stride[2] + col) = empty ? make_uint2(0, 0) : w;
         if (p.row_norm != nullptr && col == 0) {
@@ -608,16 +698,19 @@ size_t round_256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
 // rows read the keys again from L2 at most three times.
 constexpr int kTilesFromRows = 64;
 
+int tile_rows_of(int rows) { return rows <= 8 ? 8 : 16; }
+
 // Which kernels a call takes, and its workspace.
 struct CachePlan {
   int rows;         // packed rows of a run
   bool tiles;       // the sequences' own keys (and a prefix before them in the same walk) on the tile kernel
-  int row_tiles;    // of 16, or pairs of 128
+  int tile_rows;    // of the few-row kernel: 8 or 16
+  int row_tiles;    // of so many, or pairs of 128
   int splits;       // of a pair of tiles
   int ctas;         // of the few-row kernel
   bool prefix_apart;  // a kernel of its own over the prefix for the rows of the whole batch
   bool prefix_tiles;
-  int prefix_rows, prefix_row_tiles, prefix_splits;
+  int prefix_rows, prefix_tile_rows, prefix_row_tiles, prefix_splits;
   WeightsPlan weights;  // with `tiles`
   size_t part_out, part_sum, prefix_out, prefix_sum, scores, row_norm, bytes;  // (scores: or the sums of their parts)
 };
@@ -643,10 +736,11 @@ CachePlan cache_plan(const CacheAttentionArgs &a) {
     p.splits = cache_tiles_splits(runs * p.row_tiles, static_cast<int>(std::min<int64_t>(most + a.prefix_len, INT32_MAX)), kCacheCounters);
     part_rows = p.splits > 1 ? cache_tiles_part_rows(runs * p.row_tiles, p.splits) : 0;
   } else {
-    p.row_tiles = (p.rows + kRows - 1) / kRows;
+    p.tile_rows = tile_rows_of(p.rows);
+    p.row_tiles = (p.rows + p.tile_rows - 1) / p.tile_rows;
     const int64_t steps = (most + kStepKeys - 1) / kStepKeys, least = std::min<int64_t>(kLeastSteps, steps);  // of a unit, and of a CTA
     p.ctas = static_cast<int>(std::min<int64_t>(kCtasPerSm * sm_count(), (runs * p.row_tiles * steps + least - 1) / least));
-    part_rows = static_cast<size_t>(p.ctas) * 2 * kRows;
+    part_rows = static_cast<size_t>(p.ctas) * 2 * p.tile_rows;
   }
   if (part_rows > 0) {
     p.part_out = take(part_rows * d * 4);
@@ -660,7 +754,8 @@ CachePlan cache_plan(const CacheAttentionArgs &a) {
       p.prefix_row_tiles = cache_tiles_pairs(p.prefix_rows);
       p.prefix_splits = cache_tiles_splits(static_cast<int64_t>(a.kv_heads) * p.prefix_row_tiles, a.prefix_len, INT32_MAX);
     } else {
-      p.prefix_row_tiles = (p.prefix_rows + kRows - 1) / kRows;
+      p.prefix_tile_rows = tile_rows_of(p.prefix_rows);
+      p.prefix_row_tiles = (p.prefix_rows + p.prefix_tile_rows - 1) / p.prefix_tile_rows;
       // (as many as the kernel finds keys for: every part that the merge reads is written)
       const int steps = (a.prefix_len + kStepKeys - 1) / kStepKeys;
       const int wanted = prefix_splits(static_cast<int64_t>(a.kv_heads) * p.prefix_row_tiles, a.prefix_len);
@@ -682,10 +777,10 @@ CachePlan cache_plan(const CacheAttentionArgs &a) {
   return p;
 }
 
-template <int D, bool BF16>
+template <int D, bool BF16, int NB>
 cudaError_t launch_rows(const RowsParams &p, int64_t ctas, bool dependent, cudaStream_t stream) {
   using L = RowsLayout<D>;
-  auto kernel = few_rows_kernel<D, BF16>;
+  auto kernel = few_rows_kernel<D, BF16, NB>;
   static const cudaError_t attr_set = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmemBytes);
   if (attr_set != cudaSuccess) return attr_set;
   cudaLaunchConfig_t cfg = {};
@@ -701,11 +796,16 @@ cudaError_t launch_rows(const RowsParams &p, int64_t ctas, bool dependent, cudaS
   return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
-cudaError_t launch_rows(const CacheAttentionArgs &a, const RowsParams &p, int64_t ctas, bool dependent) {
+template <int D, bool BF16>
+cudaError_t launch_rows(const RowsParams &p, int tile_rows, int64_t ctas, bool dependent, cudaStream_t stream) {
+  return tile_rows == 8 ? launch_rows<D, BF16, 1>(p, ctas, dependent, stream) : launch_rows<D, BF16, 2>(p, ctas, dependent, stream);
+}
+
+cudaError_t launch_rows(const CacheAttentionArgs &a, const RowsParams &p, int tile_rows, int64_t ctas, bool dependent) {
   if (a.head_dim == 64) {
-    return a.is_bf16 ? launch_rows<64, true>(p, ctas, dependent, a.stream) : launch_rows<64, false>(p, ctas, dependent, a.stream);
+    return a.is_bf16 ? launch_rows<64, true>(p, tile_rows, ctas, dependent, a.stream) : launch_rows<64, false>(p, tile_rows, ctas, dependent, a.stream);
   }
-  return a.is_bf16 ? launch_rows<128, true>(p, ctas, dependent, a.stream) : launch_rows<128, false>(p, ctas, dependent, a.stream);
+  return a.is_bf16 ? launch_rows<128, true>(p, tile_rows, ctas, dependent, a.stream) : launch_rows<128, false>(p, tile_rows, ctas, dependent, a.stream);
 }
 
 }  // namespace
@@ -841,7 +941,7 @@ cudaError_t cache_attention(const CacheAttentionArgs &a, const char **why, int *
       s.part_out = floats(plan.prefix_out);
       s.part_sum = pairs(plan.prefix_sum);
       *why = "launching the prefix's part";
-      e = launch_rows(a, s, static_cast<int64_t>(a.kv_heads) * s.row_tiles * s.splits, false);
+      e = launch_rows(a, s, plan.prefix_tile_rows, static_cast<int64_t>(a.kv_heads) * s.row_tiles * s.splits, false);
     }
     if (e != cudaSuccess) return e;
     ++*launches;
@@ -850,7 +950,7 @@ cudaError_t cache_attention(const CacheAttentionArgs &a, const char **why, int *
     p.prefix_splits = plan.prefix_splits;
     p.prefix_rows = plan.prefix_rows;
   }
-  e = launch_rows(a, p, plan.ctas, plan.prefix_apart);
+  e = launch_rows(a, p, plan.tile_rows, plan.ctas, plan.prefix_apart);
   if (e != cudaSuccess) {
     *why = "launching the few-row kernel";
     return e;
