@@ -3,9 +3,13 @@
 // One CTA per sequence and key-value head finds the weight of the last key that stays by its bits, eight at a time
 // from the top (a histogram of the keys that agree so far, then the bin in which the wanted rank falls), and
 // lists the keys above it and the first of those equal to it in the order of their positions (a scan over the CTA).
+// The weights are read once, into shared memory as far as they fit. Lanes of a warp whose keys fall into one bin count
+// them together: accumulated weights crowd into a few exponents, and equal ones into a single bin.
 // The rows are then copied by a kernel over the whole GPU, sixteen bytes a thread. Both are bound by memory: a weight is
 // read once and a kept row once, and written once.
 #include "cache_attention_sm100.cuh"
+
+#include <algorithm>
 
 #include "cache_common_sm100.cuh"
 #include "ptx_sm100.cuh"
@@ -32,92 +36,122 @@ struct SelectParams {
   const int32_t *kv_lens;
   int32_t *kept;
   int kv_heads, kv_len, out_len, keep, recent;
+  int cached_keys;  // room for so many in shared memory
 };
 
-// The exclusive sum of `mine` over the CTA's threads in order, and the total.
-__device__ __forceinline__ int scan_cta(int mine, int *warp_sums, int *total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int sum = mine;
-#pragma unroll
-  for (int x = 1; x < 32; x <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, sum, x);
-    if (lane >= x) sum += y;
-  }
-  __syncthreads();  // (an earlier scan's sums have been read)
-  if (lane == 31) warp_sums[warp] = sum;
-  __syncthreads();
-  int before = 0, all = 0;
-#pragma unroll
-  for (int w = 0; w < kSelectThreads / 32; ++w) {
-    if (w < warp) before += warp_sums[w];
-    all += warp_sums[w];
-  }
-  *total = all;
-  return before + sum - mine;
-}
+constexpr int kKeysPerThread = 4;  // of the scan
+constexpr int kMaxCachedKeys = 48 * 1024;
 
-__global__ void __launch_bounds__(kSelectThreads) select_kept_kernel(const SelectParams p) {
+__global__ void __launch_bounds__(kSelectThreads) select_kept_kernel(const __grid_constant__ SelectParams p) {
+  extern __shared__ __align__(16) uint32_t cache[];
   __shared__ uint32_t bins[256];
-  __shared__ int warp_sums[kSelectThreads / 32];
+  __shared__ uint32_t warp_counts[kSelectThreads / 32];
   __shared__ uint32_t found_bin;
   __shared__ int found_rank;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  griddep_wait();
+  griddep_launch_dependents();
   const int run = blockIdx.x, seq = run / p.kv_heads, head = run % p.kv_heads;
   const int len = sequence_length(p.kv_lens, seq, p.kv_len);
   const float *weights = p.weights + seq * p.weights_stride[0] + head * p.weights_stride[1];
   float *weights_out = p.weights_out + seq * p.weights_out_stride[0] + head * p.weights_out_stride[1];
   int32_t *kept = p.kept + static_cast<int64_t>(run) * p.keep;
-  griddep_launch_dependents();
 
   const int old = len <= p.keep ? 0 : len - p.recent;  // the keys that have to earn their place
-  int wanted = p.keep - p.recent;                       // how many of them stay
-  uint32_t prefix = 0, mask = 0;
-  if (old > 0 && wanted > 0) {
+  const bool choose = old > 0 && p.keep > p.recent;
+  int wanted = p.keep - p.recent;  // how many of them stay
+  uint32_t last = 0;               // the order of the lightest that does
+  const int cached = choose ? min(old, p.cached_keys) : 0;
+  auto order_at = [&](int i) -> uint32_t { return i < cached ? cache[i] : order_of(weights[i]); };
+  if (choose) {
+#pragma unroll 4
+    for (int i = threadIdx.x; i < cached; i += kSelectThreads) cache[i] = order_of(weights[i]);
+    uint32_t mask = 0;
     for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = threadIdx.x; i < 256; i += kSelectThreads) bins[i] = 0;
+      if (threadIdx.x < 256) bins[threadIdx.x] = 0;
       __syncthreads();
-      for (int i = threadIdx.x; i < old; i += kSelectThreads) {
-        const uint32_t o = order_of(weights[i]);
-        if ((o & mask) == prefix) atomicAdd(&bins[(o >> shift) & 255], 1u);
+      for (int base = 0; base < old; base += kSelectThreads) {
+        const int i = base + threadIdx.x;
+        const uint32_t o = i < old ? order_at(i) : 0u;
+        const uint32_t bin = i < old && (o & mask) == last ? (o >> shift) & 255u : 256u;
+        const uint32_t same = __match_any_sync(0xffffffffu, bin);
+        if (bin < 256u && lane == __ffs(static_cast<int>(same)) - 1) atomicAdd(&bins[bin], static_cast<uint32_t>(__popc(same)));
       }
       __syncthreads();
-      if (threadIdx.x == 0) {
-        int rank = wanted;
-        int b = 255;
-        for (; b > 0; --b) {
-          const int here = static_cast<int>(bins[b]);
-          if (rank <= here) break;
-          rank -= here;
+      if (warp == 0) {
+        // Eight bins a lane, the highest first: the bin in which the rank falls, and what is left of the rank there.
+        int here[8], sum = 0;
+#pragma unroll
+        for (int b = 0; b < 8; ++b) {
+          here[b] = static_cast<int>(bins[255 - lane * 8 - b]);
+          sum += here[b];
         }
-        found_bin = static_cast<uint32_t>(b);
-        found_rank = rank;
+        int upto = sum;
+#pragma unroll
+        for (int x = 1; x < 32; x <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, upto, x);
+          if (lane >= x) upto += y;
+        }
+        int rank = wanted - (upto - sum);
+        if (rank > 0 && rank <= sum) {
+          int b = 0;
+          while (rank > here[b]) rank -= here[b++];
+          found_bin = static_cast<uint32_t>(255 - lane * 8 - b);
+          found_rank = rank;
+        }
       }
       __syncthreads();
-      prefix |= found_bin << shift;
+      last |= found_bin << shift;
       mask |= 255u << shift;
       wanted = found_rank;
     }
   }
-  // Of the old keys those above `prefix` stay, and the first `wanted` that equal it.
-  const bool choose = old > 0 && p.keep > p.recent;
-  int placed = 0, equal_before = 0;
-  for (int base = 0; base < len; base += kSelectThreads) {
-    const int i = base + threadIdx.x;
-    const float w = i < len ? weights[i] : 0.0f;
-    const uint32_t o = order_of(w);
-    const bool is_old = i < old;
-    const bool equal = choose && is_old && o == prefix;
-    int total = 0;
-    const int equal_here = equal_before + scan_cta(equal ? 1 : 0, warp_sums, &total);
-    equal_before += total;
-    const bool stays = i < len && (!is_old || (choose && (o > prefix || (equal && equal_here < wanted))));
-    const int to = placed + scan_cta(stays ? 1 : 0, warp_sums, &total);
-    placed += total;
-    if (stays) {
-      kept[to] = i;
-      weights_out[to] = w;
+  // Of the old keys those above `last` stay, and the first `wanted` that equal it; of the others all.
+  int sure = 0, equal = 0;  // before this thread's keys
+  for (int base = 0; base < len; base += kSelectThreads * kKeysPerThread) {
+    const int first = base + static_cast<int>(threadIdx.x) * kKeysPerThread;
+    uint32_t mine = 0;  // how many stay for sure (upper half) and how many equal the last (lower half): 4096 a round at most
+    bool is_sure[kKeysPerThread], is_equal[kKeysPerThread];
+#pragma unroll
+    for (int k = 0; k < kKeysPerThread; ++k) {
+      const int i = first + k;
+      const uint32_t o = choose && i < old ? order_at(i) : 0u;
+      is_sure[k] = i < len && (i >= old || (choose && o > last));
+      is_equal[k] = choose && i < old && o == last;
+      mine += (is_sure[k] ? 0x10000u : 0u) + (is_equal[k] ? 1u : 0u);
     }
+    uint32_t upto = mine;
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+      const uint32_t y = __shfl_up_sync(0xffffffffu, upto, x);
+      if (lane >= x) upto += y;
+    }
+    if (lane == 31) warp_counts[warp] = upto;
+    __syncthreads();
+    uint32_t of_warps = warp_counts[lane];
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+      const uint32_t y = __shfl_up_sync(0xffffffffu, of_warps, x);
+      if (lane >= x) of_warps += y;
+    }
+    const uint32_t total = __shfl_sync(0xffffffffu, of_warps, 31);
+    const uint32_t before = (warp == 0 ? 0u : __shfl_sync(0xffffffffu, of_warps, max(warp - 1, 0))) + upto - mine;
+    int my_sure = sure + static_cast<int>(before >> 16), my_equal = equal + static_cast<int>(before & 0xffffu);
+#pragma unroll
+    for (int k = 0; k < kKeysPerThread; ++k) {
+      if (is_sure[k] || (is_equal[k] && my_equal < wanted)) {
+        const int to = my_sure + min(my_equal, wanted);
+        kept[to] = first + k;
+        weights_out[to] = weights[first + k];
+      }
+      my_sure += is_sure[k];
+      my_equal += is_equal[k];
+    }
+    sure += static_cast<int>(total >> 16);
+    equal += static_cast<int>(total & 0xffffu);
+    __syncthreads();  // (the warps' counts have been read)
   }
-  for (int i = placed + threadIdx.x; i < p.out_len; i += kSelectThreads) {
+  for (int i = min(len, p.keep) + threadIdx.x; i < p.out_len; i += kSelectThreads) {
     if (i < p.keep) kept[i] = -1;
     weights_out[i] = 0.0f;
   }
@@ -135,6 +169,7 @@ struct GatherParams {
 
 __global__ void __launch_bounds__(256) gather_kept_kernel(const GatherParams p) {
   griddep_wait();
+  griddep_launch_dependents();
   const int64_t step = static_cast<int64_t>(gridDim.x) * 256;
   for (int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; at < p.total; at += step) {
     const int piece = static_cast<int>(at % p.pieces);
@@ -168,8 +203,12 @@ cudaError_t cache_evict(const CacheEvictArgs &a) {
   s.out_len = a.out_len;
   s.keep = a.keep;
   s.recent = a.recent;
-  select_kept_kernel<<<static_cast<unsigned>(a.batch * a.kv_heads), kSelectThreads, 0, a.stream>>>(s);
-  cudaError_t e = cudaGetLastError();
+  static const cudaError_t attr_set = cudaFuncSetAttribute(select_kept_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxCachedKeys * 4);
+  if (attr_set != cudaSuccess) return attr_set;
+  // (a cache that holds no more than stays has nothing to choose from)
+  s.cached_keys = a.kv_len <= a.keep ? 0 : std::min(a.kv_len, kMaxCachedKeys);
+  cudaError_t e = launch_overlapped(select_kept_kernel, static_cast<int64_t>(a.batch) * a.kv_heads, kSelectThreads,
+                                    static_cast<size_t>(s.cached_keys) * 4, a.stream, s);
   if (e != cudaSuccess) return e;
 
   GatherParams g = {};
@@ -191,17 +230,8 @@ cudaError_t cache_evict(const CacheEvictArgs &a) {
   g.keep = a.keep;
   g.pieces = a.row_bytes / 16;
   g.total = static_cast<int64_t>(a.batch) * a.kv_heads * a.keep * g.pieces;
-  cudaLaunchConfig_t cfg = {};
   const int64_t ctas = (g.total + 255) / 256, most = static_cast<int64_t>(sm_count()) * 32;
-  cfg.gridDim = dim3(static_cast<unsigned>(ctas < most ? ctas : most), 1, 1);
-  cfg.blockDim = dim3(256, 1, 1);
-  cfg.stream = a.stream;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, gather_kept_kernel, g);
+  return launch_overlapped(gather_kept_kernel, ctas < most ? ctas : most, 256, 0, a.stream, g);
 }
 
 }  // namespace flsm100

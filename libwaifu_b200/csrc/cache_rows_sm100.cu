@@ -201,6 +201,7 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
   __shared__ int found_seq, is_last, longest[kWarps];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (p.prefix_splits == 0) griddep_wait();  // (behind a prefix's kernel the inputs are complete, and only its parts are waited for)
   griddep_launch_dependents();
 
   // ---- this CTA's run of steps
@@ -613,16 +614,16 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
     }
     bool finish = !p.over_batch;
     if (shared) {
-      __threadfence();
       __syncthreads();
       if (threadIdx.x == 0) {
+        __threadfence();
         const uint32_t before = atomicAdd(&p.counters[first_cta], 1u);
         is_last = before == static_cast<uint32_t>(last_cta - first_cta);
         if (is_last) p.counters[first_cta] = 0;
+        __threadfence();
       }
       __syncthreads();
       finish = is_last;
-      __threadfence();
     }
     if (finish) {
       if (p.prefix_splits > 0) griddep_wait();  // the parts over the prefix
@@ -666,6 +667,7 @@ __global__ void __launch_bounds__(256) add_weights_kernel(const float *__restric
                                                           const float *weights_in, int64_t in_seq, int64_t in_head, float *weights_out,
                                                           int64_t out_seq, int64_t out_head) {
   griddep_wait();
+  griddep_launch_dependents();
   const int chunks = (kv_len + 255) / 256;
   const int run = blockIdx.x / chunks, seq = run / kv_heads, head = run % kv_heads;
   const int key = (blockIdx.x % chunks) * 256 + threadIdx.x;
@@ -778,34 +780,24 @@ CachePlan cache_plan(const CacheAttentionArgs &a) {
 }
 
 template <int D, bool BF16, int NB>
-cudaError_t launch_rows(const RowsParams &p, int64_t ctas, bool dependent, cudaStream_t stream) {
+cudaError_t launch_rows(const RowsParams &p, int64_t ctas, cudaStream_t stream) {
   using L = RowsLayout<D>;
   auto kernel = few_rows_kernel<D, BF16, NB>;
   static const cudaError_t attr_set = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmemBytes);
   if (attr_set != cudaSuccess) return attr_set;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(ctas), 1, 1);
-  cfg.blockDim = dim3(kThreads, 1, 1);
-  cfg.dynamicSmemBytes = L::kSmemBytes;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = dependent ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kernel, p);
+  return launch_overlapped(kernel, ctas, kThreads, L::kSmemBytes, stream, p);
 }
 
 template <int D, bool BF16>
-cudaError_t launch_rows(const RowsParams &p, int tile_rows, int64_t ctas, bool dependent, cudaStream_t stream) {
-  return tile_rows == 8 ? launch_rows<D, BF16, 1>(p, ctas, dependent, stream) : launch_rows<D, BF16, 2>(p, ctas, dependent, stream);
+cudaError_t launch_rows(const RowsParams &p, int tile_rows, int64_t ctas, cudaStream_t stream) {
+  return tile_rows == 8 ? launch_rows<D, BF16, 1>(p, ctas, stream) : launch_rows<D, BF16, 2>(p, ctas, stream);
 }
 
-cudaError_t launch_rows(const CacheAttentionArgs &a, const RowsParams &p, int tile_rows, int64_t ctas, bool dependent) {
+cudaError_t launch_rows(const CacheAttentionArgs &a, const RowsParams &p, int tile_rows, int64_t ctas) {
   if (a.head_dim == 64) {
-    return a.is_bf16 ? launch_rows<64, true>(p, tile_rows, ctas, dependent, a.stream) : launch_rows<64, false>(p, tile_rows, ctas, dependent, a.stream);
+    return a.is_bf16 ? launch_rows<64, true>(p, tile_rows, ctas, a.stream) : launch_rows<64, false>(p, tile_rows, ctas, a.stream);
   }
-  return a.is_bf16 ? launch_rows<128, true>(p, tile_rows, ctas, dependent, a.stream) : launch_rows<128, false>(p, tile_rows, ctas, dependent, a.stream);
+  return a.is_bf16 ? launch_rows<128, true>(p, tile_rows, ctas, a.stream) : launch_rows<128, false>(p, tile_rows, ctas, a.stream);
 }
 
 }  // namespace
@@ -941,7 +933,7 @@ cudaError_t cache_attention(const CacheAttentionArgs &a, const char **why, int *
       s.part_out = floats(plan.prefix_out);
       s.part_sum = pairs(plan.prefix_sum);
       *why = "launching the prefix's part";
-      e = launch_rows(a, s, plan.prefix_tile_rows, static_cast<int64_t>(a.kv_heads) * s.row_tiles * s.splits, false);
+      e = launch_rows(a, s, plan.prefix_tile_rows, static_cast<int64_t>(a.kv_heads) * s.row_tiles * s.splits);
     }
     if (e != cudaSuccess) return e;
     ++*launches;
@@ -950,25 +942,17 @@ cudaError_t cache_attention(const CacheAttentionArgs &a, const char **why, int *
     p.prefix_splits = plan.prefix_splits;
     p.prefix_rows = plan.prefix_rows;
   }
-  e = launch_rows(a, p, plan.tile_rows, plan.ctas, plan.prefix_apart);
+  e = launch_rows(a, p, plan.tile_rows, plan.ctas);
   if (e != cudaSuccess) {
     *why = "launching the few-row kernel";
     return e;
   }
   ++*launches;
   if (a.weights_out != nullptr) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>((a.kv_len + 255) / 256) * static_cast<unsigned>(a.batch * a.kv_heads), 1, 1);
-    cfg.blockDim = dim3(256, 1, 1);
-    cfg.stream = a.stream;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, add_weights_kernel, static_cast<const float *>(p.scores), static_cast<const float2 *>(p.row_norm), p.rows, p.group,
-                           a.q_len, a.kv_len, a.kv_heads, a.kv_lens, a.weights_in, a.weights_in_stride[0], a.weights_in_stride[1], a.weights_out,
-                           a.weights_out_stride[0], a.weights_out_stride[1]);
+    const int64_t ctas = (static_cast<int64_t>(a.kv_len) + 255) / 256 * a.batch * a.kv_heads;
+    e = launch_overlapped(add_weights_kernel, ctas, 256, 0, a.stream, p.scores, p.row_norm, p.rows, p.group, a.q_len, a.kv_len, a.kv_heads, a.kv_lens,
+                          a.weights_in, a.weights_in_stride[0], a.weights_in_stride[1], a.weights_out, a.weights_out_stride[0],
+                          a.weights_out_stride[1]);
     if (e != cudaSuccess) {
       *why = "launching the keys' weights";
       return e;

@@ -226,14 +226,10 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
 
   const uint32_t warp = threadIdx.x >> 5;
   const uint32_t lane = threadIdx.x & 31;
-  griddep_launch_dependents();
   if ((smem_u32(smem) & 1023u) != 0) {
     if (threadIdx.x == 0) atomicCAS(p.status, 0u, kStatusAttentionLayout);
     return;
   }
-  const Unit u(p, blockIdx.x);
-  if (u.split >= u.active) return;
-
   if (threadIdx.x == 0) {
     t.abort_flag = 0;
     t.patch_flag = 0;
@@ -262,12 +258,17 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem_base = t.tmem_base_slot;
+  griddep_wait();
+  griddep_launch_dependents();
+  const Unit u(p, blockIdx.x);
 
   auto q_tile = [&](int i) { return smem + L::kQOff + i * L::kQBytes; };
   auto slot = [&](int i) { return smem + L::kSlotOff + i * L::kSlotBytes; };
 
   // Load n of the ring (K of block n / 2 when n is even, V of it when odd) goes to slot n % S.
-  if (warp < kSoftmaxWarps) {
+  if (u.split >= u.active) {
+    // (fewer parts than CTAs: nothing to do)
+  } else if (warp < kSoftmaxWarps) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     // ------------------------------------------------------------------ queries, softmax and output
     const int tile = static_cast<int>(warp >> 2);
@@ -379,17 +380,17 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
       if (live && !parts && p.row_norm != nullptr) p.row_norm[norm_at] = make_float2(m_used, inv);
     }
     if (!p.over_batch && u.active > 1) {
-      __threadfence();
       asm volatile("bar.sync 1, %0;" ::"n"(kSoftmaxWarps * 32) : "memory");
       if (threadIdx.x == 0) {
+        __threadfence();
         uint32_t *counter = &p.counters[u.run * p.row_pairs + u.pair];
         const uint32_t before = atomicAdd(counter, 1u);
         t.is_last = before + 1 == static_cast<uint32_t>(u.active);
         if (t.is_last) *counter = 0;
+        __threadfence();
       }
       asm volatile("bar.sync 1, %0;" ::"n"(kSoftmaxWarps * 32) : "memory");
       if (t.is_last && live) {
-        __threadfence();
         float m = -INFINITY, l = 0.0f;
         for (int s = 0; s < u.active; ++s) m = fmaxf(m, __ldcg(&p.part_sum[part_row0 + s * part_step]).x);
         for (int s = 0; s < u.active; ++s) {
@@ -576,17 +577,12 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
 }
 
 template <int D>
-cudaError_t launch(const CUtensorMap (&maps)[4], const TilesParams &p, int64_t ctas, bool dependent, cudaStream_t stream) {
+cudaError_t launch(const CUtensorMap (&maps)[4], const TilesParams &p, int64_t ctas, cudaStream_t stream) {
   using L = Layout<D>;
   auto kernel = cache_tiles_kernel<D>;
   static const cudaError_t attr_set = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmemBytes);
   if (attr_set != cudaSuccess) return attr_set;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(ctas), 1, 1);
-  cfg.blockDim = dim3(kThreads, 1, 1);
-  cfg.dynamicSmemBytes = L::kSmemBytes;
-  cfg.stream = stream;
-  return cudaLaunchKernelEx(&cfg, kernel, maps[0], maps[1], maps[2], maps[3], p);
+  return launch_overlapped(kernel, ctas, kThreads, L::kSmemBytes, stream, maps[0], maps[1], maps[2], maps[3], p);
 }
 
 }  // namespace
@@ -621,7 +617,7 @@ cudaError_t cache_tiles(const TilesParams &p, const CacheAttentionArgs &a, const
   if (!prefix) maps[2] = maps[0], maps[3] = maps[1];
   const int64_t ctas = static_cast<int64_t>(p.runs) * p.row_pairs * p.splits;
   *why = "launching the tile kernel";
-  return a.head_dim == 64 ? launch<64>(maps, p, ctas, false, a.stream) : launch<128>(maps, p, ctas, false, a.stream);
+  return a.head_dim == 64 ? launch<64>(maps, p, ctas, a.stream) : launch<128>(maps, p, ctas, a.stream);
 }
 
 }  // namespace flsm100

@@ -198,17 +198,17 @@ cache_weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     if (u.active > 1) {
       float *parts = p.part_sums + (static_cast<int64_t>(u.run) * p.pairs + u.pair) * p.parts * kKeysPerCta + in_cta;
       parts[u.part * kKeysPerCta] = sum;
-      __threadfence();
       asm volatile("bar.sync 1, %0;" ::"n"(kSumWarps * 32) : "memory");
       if (threadIdx.x == 0) {
+        __threadfence();
         uint32_t *counter = &p.counters[u.run * p.pairs + u.pair];
         const uint32_t before = atomicAdd(counter, 1u);
         t.is_last = before + 1 == static_cast<uint32_t>(u.active);
         if (t.is_last) *counter = 0;
+        __threadfence();
       }
       asm volatile("bar.sync 1, %0;" ::"n"(kSumWarps * 32) : "memory");
       if (t.is_last) {
-        __threadfence();
         sum = 0.0f;
         for (int s = 0; s < u.active; ++s) sum += __ldcg(parts + s * kKeysPerCta);
       }
@@ -310,17 +310,7 @@ cudaError_t launch(const CUtensorMap &tq, const CUtensorMap &tk, const WeightsPa
   auto kernel = cache_weights_kernel<D>;
   static const cudaError_t attr_set = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmemBytes);
   if (attr_set != cudaSuccess) return attr_set;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(ctas), 1, 1);
-  cfg.blockDim = dim3(kThreads, 1, 1);
-  cfg.dynamicSmemBytes = L::kSmemBytes;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, tq, tk, p);
+  return launch_overlapped(kernel, ctas, kThreads, L::kSmemBytes, stream, tq, tk, p);
 }
 
 }  // namespace
