@@ -930,38 +930,6 @@ attention2_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
 
 // ---- the same, going on from unit to unit ------------------------------------------------------
 
-// Asks for a CTA of this grid that has not started: sixteen bytes of answer, counted on `bar`.
-__device__ __forceinline__ void claim_next_cta(uint4 *answer, uint64_t *bar) {
-  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];"
-               ::"r"(smem_u32(answer)), "r"(smem_u32(bar))
-               : "memory");
-}
-
-// The block indices of the CTA that was taken over, w = 1; w = 0 where none was left.
-__device__ __forceinline__ int4 claimed_cta(const uint4 *answer) {
-  int4 c;
-  asm volatile(
-      "{\n\t"
-      ".reg .b128 r;\n\t"
-      ".reg .pred p;\n\t"
-      ".reg .b32 x, y, z, u;\n\t"
-      "ld.shared.b128 r, [%4];\n\t"
-      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
-      "selp.b32 %3, 1, 0, p;\n\t"
-      "mov.b32 x, 0;\n\t"
-      "mov.b32 y, 0;\n\t"
-      "mov.b32 z, 0;\n\t"
-      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {x, y, z, u}, r;\n\t"
-      "mov.b32 %0, x;\n\t"
-      "mov.b32 %1, y;\n\t"
-      "mov.b32 %2, z;\n\t"
-      "}"
-      : "=r"(c.x), "=r"(c.y), "=r"(c.z), "=r"(c.w)
-      : "r"(smem_u32(answer))
-      : "memory");
-  return c;
-}
-
 template <int D>
 __global__ void __launch_bounds__(kThreads2, 1)
 attention2_units_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,

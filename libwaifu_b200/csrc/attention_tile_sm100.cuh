@@ -103,6 +103,38 @@ __device__ __forceinline__ uint32_t pack16(float a, float b, int is_bf16) {
   return *reinterpret_cast<const uint32_t *>(&h);
 }
 
+// Asks for a CTA of this grid that has not started: sixteen bytes of answer, counted on `bar`.
+__device__ __forceinline__ void claim_next_cta(uint4 *answer, uint64_t *bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];"
+               ::"r"(smem_u32(answer)), "r"(smem_u32(bar))
+               : "memory");
+}
+
+// The block indices of the CTA that was taken over, w = 1; w = 0 where none was left.
+__device__ __forceinline__ int4 claimed_cta(const uint4 *answer) {
+  int4 c;
+  asm volatile(
+      "{\n\t"
+      ".reg .b128 r;\n\t"
+      ".reg .pred p;\n\t"
+      ".reg .b32 x, y, z, u;\n\t"
+      "ld.shared.b128 r, [%4];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+      "selp.b32 %3, 1, 0, p;\n\t"
+      "mov.b32 x, 0;\n\t"
+      "mov.b32 y, 0;\n\t"
+      "mov.b32 z, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {x, y, z, u}, r;\n\t"
+      "mov.b32 %0, x;\n\t"
+      "mov.b32 %1, y;\n\t"
+      "mov.b32 %2, z;\n\t"
+      "}"
+      : "=r"(c.x), "=r"(c.y), "=r"(c.z), "=r"(c.w)
+      : "r"(smem_u32(answer))
+      : "memory");
+  return c;
+}
+
 // The tiles in shared and tensor memory.
 template <int D>
 struct TileLayout {
@@ -280,7 +312,7 @@ using EncodeTiledFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_
                                    const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
                                    CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-EncodeTiledFn encode_fn() {
+inline EncodeTiledFn encode_fn() {
   static EncodeTiledFn fn = [] {
     void *ptr = nullptr;
     cudaDriverEntryPointQueryResult q;
@@ -293,15 +325,15 @@ EncodeTiledFn encode_fn() {
   return fn;
 }
 
-// A byte tensor of `rank` dimensions, innermost contiguous, read in boxes of 128 bytes x box_rows
-// rows of the second dimension, 128-byte swizzle, zeros outside.
-bool make_tmap(CUtensorMap *map, const void *base, int rank, const uint64_t *dims, const uint64_t *strides_bytes,
-               uint32_t box_rows) {
+// A byte tensor of `rank` dimensions, innermost contiguous, read in boxes of 128 bytes x box[0] x box[1] x box[2] of
+// the others, 128-byte swizzle, zeros outside.
+inline bool make_tmap(CUtensorMap *map, const void *base, int rank, const uint64_t *dims, const uint64_t *strides_bytes,
+                      const uint32_t (&rows)[3]) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return false;
   cuuint64_t d[4];
   cuuint64_t s[3];
-  cuuint32_t box[4] = {static_cast<cuuint32_t>(kAtomBytes), box_rows, 1, 1};
+  cuuint32_t box[4] = {static_cast<cuuint32_t>(kAtomBytes), rows[0], rows[1], rows[2]};
   cuuint32_t estr[4] = {1, 1, 1, 1};
   for (int i = 0; i < rank; ++i) d[i] = dims[i];
   for (int i = 0; i + 1 < rank; ++i) s[i] = strides_bytes[i];
@@ -309,6 +341,13 @@ bool make_tmap(CUtensorMap *map, const void *base, int rank, const uint64_t *dim
                   estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS;
+}
+
+// The same in boxes of 128 bytes x box_rows of the second dimension.
+inline bool make_tmap(CUtensorMap *map, const void *base, int rank, const uint64_t *dims, const uint64_t *strides_bytes,
+                      uint32_t box_rows) {
+  const uint32_t rows[3] = {box_rows, 1, 1};
+  return make_tmap(map, base, rank, dims, strides_bytes, rows);
 }
 
 // Queries, keys or values as (head_dim bytes, positions, heads, batch), strides in elements, in boxes of 128 positions.

@@ -5,14 +5,18 @@
 // head r % group of the ones that share the head, so that a block of keys is read once for all of them and a
 // tile's rows sit close together (under a window a tile walks its 128 / group positions and the window, not 128
 // and the window). Over a prefix, which all of a batch sees, the rows of every sequence are packed one after the other.
-// The softmax warps gather the queries into shared memory themselves; K and V blocks of 128 keys arrive by TMA
-// into one ring of slots. The walk is a list of blocks: those of a prefix, those that hold sinks, those from the
-// first window's start to the last query's position.
+// K and V blocks of 128 keys arrive by TMA into one ring of slots; the walk is a list of blocks: those of a prefix, those that
+// hold sinks, those from the first window's start to the last query's position.
 //
-// A block that some row does not see whole (past the sequence's end, at a window's edge, on the diagonal) passes two
-// more warps before its product: they clear the values of keys that no row sees and take infinities and NaN out of
-// the others, because a probability of zero times such a value is not zero. Rows that do see them have them added by
-// hand at the end.
+// So do the queries where a tile is a box of the tensor (a group, or a group and its queries, that divides 128); otherwise two
+// helping warps gather them. A block that some row does not see whole (past the sequence's end, at a window's edge, on
+// the diagonal) passes those warps before its product: they clear the values of keys that no
+// row sees and take infinities and NaN out of the others, because a probability of zero times such a value is not
+// zero. Rows that do see them have them added by hand at the end.
+//
+// A running CTA takes over units whose own CTA has not started (clusterlaunchcontrol.try_cancel): the next unit's keys,
+// queries and first scores come under the last products and the output of the one before. Walks are short here (a window's,
+// a chunk's), and a unit's own start and end would be a third of them.
 //
 // Few units are divided along the keys: each CTA leaves its rows' outputs relative to their own maxima, and the last
 // one to arrive (or, over a prefix, the kernel over the sequences' own keys) adds them in the order of the splits.
@@ -34,24 +38,28 @@ constexpr int kPairRows = kTiles * kBlockQ;
 constexpr int kSoftmaxWarps = kTiles * kTileWarps;
 constexpr int kProducerWarp = kSoftmaxWarps;
 constexpr int kMmaWarp = kSoftmaxWarps + 1;
-constexpr int kCleanWarp = kSoftmaxWarps + 2;  // and the one after it
-constexpr int kCleanWarps = 2;
-// Three warpgroups launched with 168 registers a thread; the one that loads, issues and cleans gives its own up to the
-// two of the softmax, which hold a row of 128 scores: 128 x 88 + 256 x 208 = 384 x 168.
+constexpr int kHelpWarp = kSoftmaxWarps + 2;  // and the one after it
+constexpr int kHelpWarps = 2;
+// Three warpgroups launched with 168 registers a thread; the one that loads, issues and helps gives its own up to the
+// two of the softmax, which hold a row of 128 scores: 128 x 96 + 256 x 200 < 384 x 168.
 constexpr int kThreads = (kSoftmaxWarps + 4) * 32;
-constexpr int kIssueRegs = 88, kSoftmaxRegs = 208;
+constexpr int kIssueRegs = 96, kSoftmaxRegs = 200;
 static_assert(128 * kIssueRegs + kSoftmaxWarps * 32 * kSoftmaxRegs <= kThreads * 168, "no more than the block was launched with");
 constexpr int kMaxSlots = 6;
 
 struct Tail {
-  uint64_t q_full_bar[kTiles];
+  uint4 claim;         // the answer to the last try_cancel
+  uint64_t claim_bar;  // ... which has arrived
+  uint64_t unit_full_bar[2], unit_empty_bar[2];  // producer -> all: the next unit is in next_unit[slot]; all -> producer
+  int next_unit[2];                              // -1 when there is none left
+  uint64_t q_full_bar[kTiles], q_empty_bar[kTiles];
   uint64_t slot_full_bar[kMaxSlots], slot_empty_bar[kMaxSlots], slot_clean_bar[kMaxSlots];
   uint64_t s_full_bar[kTiles];     // MMA -> softmax: the tile's scores are in tensor memory
   uint64_t p_full_bar[kTiles][2];  // softmax -> MMA: that part of the tile's probabilities is in tensor memory
   uint64_t pv_done_bar[kTiles];    // MMA -> softmax: the last block is in the tile's output
   uint32_t tmem_base_slot;
   uint32_t abort_flag;
-  uint32_t patch_flag;  // values were taken out of a block
+  uint32_t patch_flag[2];  // the last unit of an even and of an odd count that had values taken out of a block
   int is_last;
 };
 
@@ -98,13 +106,13 @@ struct Walk {
 };
 
 struct Unit {
-  int run, head, seq, pair, split, active;
+  int index, run, head, seq, pair, split, active;
   int row0;  // of the pair
   int len;
   Walk walk;
   int blocks[kTiles];  // how many of the split's blocks each tile walks
 
-  __device__ __forceinline__ Unit(const TilesParams &p, int at) {
+  __device__ __forceinline__ Unit(const TilesParams &p, int at) : index(at) {
     // The longest walks first: the last pair of every run, then the one before it.
     run = at % p.runs;
     at /= p.runs;
@@ -139,7 +147,7 @@ struct Unit {
     const int per_split = max(1, (total + p.splits - 1) / p.splits);
     active = max(1, (total + per_split - 1) / per_split);
     walk.first = split * per_split;
-    walk.count = max(0, min(per_split, total - walk.first));
+    walk.count = max(0, min(per_split, total - walk.first));  // (0 past the active splits)
 #pragma unroll
     for (int i = 0; i < kTiles; ++i) {
       const int first_row = row0 + i * kBlockQ, last = min(first_row + kBlockQ, p.rows) - 1;
@@ -212,9 +220,111 @@ __device__ __noinline__ void patch_row(const TilesParams &p, int unit, int pos, 
   }
 }
 
+// A row's result, or its part of it, and what becomes of the parts of a unit that several CTAs share.
+template <int D>
+__device__ __forceinline__ void finish_row(const TilesParams &p, const Unit &u, Tail &t, uint32_t t_out, int row, int pos, int my_blocks, bool ok,
+                                           bool patch, float m_used, float l_run) {
+  const bool live = row < p.rows;
+  const bool parts = p.over_batch || u.active > 1;
+  // The index of this row's part of split s: (kv_head, split, rows) over a prefix, (unit, split, 256) else.
+  const int64_t part_row0 = p.over_batch ? static_cast<int64_t>(u.head) * p.splits * p.rows + row
+                                         : (static_cast<int64_t>(u.run) * p.row_pairs + u.pair) * p.splits * kPairRows + (row - u.row0);
+  const int64_t part_step = p.over_batch ? p.rows : kPairRows;
+  const bool empty = p.prefix_len == 0 && pos < 0;  // sees no key: zeros
+  uint16_t *dst = live && !p.over_batch ? p.out + row_offset(p, p.out_stride, u.head, u.seq, row) : nullptr;
+  float *part_dst = p.part_out + (part_row0 + u.split * part_step) * D;
+  const int64_t norm_at = (static_cast<int64_t>(u.run) * p.group + row % p.group) * p.norm_pitch + row / p.group;
+  // (a row whose every score is -inf has no softmax)
+  float inv = empty ? 0.0f : (m_used == -INFINITY ? NAN : 1.0f / l_run);
+  if (ok) {
+#pragma unroll 1
+    for (int c = 0; c < D / 32; ++c) {
+      uint32_t v[32];
+      if (my_blocks > 0) {
+        tmem_ld_32x32(t_out + c * 32, v);
+        tmem_ld_wait(v);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = 0;
+      }
+      if (live && parts) {
+#pragma unroll
+        for (int g = 0; g < 8; ++g) *reinterpret_cast<uint4 *>(part_dst + c * 32 + g * 4) = make_uint4(v[g * 4], v[g * 4 + 1], v[g * 4 + 2], v[g * 4 + 3]);
+      } else if (live) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          uint4 w;
+          w.x = pack16(__uint_as_float(v[g * 8 + 0]) * inv, __uint_as_float(v[g * 8 + 1]) * inv, p.is_bf16);
+          w.y = pack16(__uint_as_float(v[g * 8 + 2]) * inv, __uint_as_float(v[g * 8 + 3]) * inv, p.is_bf16);
+          w.z = pack16(__uint_as_float(v[g * 8 + 4]) * inv, __uint_as_float(v[g * 8 + 5]) * inv, p.is_bf16);
+          w.w = pack16(__uint_as_float(v[g * 8 + 6]) * inv, __uint_as_float(v[g * 8 + 7]) * inv, p.is_bf16);
+          *reinterpret_cast<uint4 *>(dst + c * 32 + g * 8) = empty ? make_uint4(0, 0, 0, 0) : w;
+        }
+      }
+    }
+    if (live && patch && m_used != -INFINITY && l_run == l_run) {
+      const uint16_t *q = p.q + row_offset(p, p.q_stride, u.head, u.seq, row);
+      if (p.is_bf16) {
+        patch_row<D, true>(p, u.index, pos, q, m_used, l_run, dst, parts ? part_dst : nullptr);
+      } else {
+        patch_row<D, false>(p, u.index, pos, q, m_used, l_run, dst, parts ? part_dst : nullptr);
+      }
+    }
+    // (the cubic's smallest exponentials keep a part that saw nothing from summing to zero)
+    if (live && parts) p.part_sum[part_row0 + u.split * part_step] = make_float2(m_used, m_used == -INFINITY && l_run == l_run ? 0.0f : l_run);
+    if (live && !parts && p.row_norm != nullptr) p.row_norm[norm_at] = make_float2(m_used, inv);
+  }
+  if (p.over_batch || u.active == 1) return;
+  asm volatile("bar.sync 1, %0;" ::"n"(kSoftmaxWarps * 32) : "memory");
+  if (threadIdx.x == 0) {
+    __threadfence();
+    uint32_t *counter = &p.counters[u.run * p.row_pairs + u.pair];
+    const uint32_t before = atomicAdd(counter, 1u);
+    t.is_last = before + 1 == static_cast<uint32_t>(u.active);
+    if (t.is_last) *counter = 0;
+    __threadfence();
+  }
+  asm volatile("bar.sync 1, %0;" ::"n"(kSoftmaxWarps * 32) : "memory");
+  if (!t.is_last || !live) return;
+  float m = -INFINITY, l = 0.0f;
+  for (int s = 0; s < u.active; ++s) m = fmaxf(m, __ldcg(&p.part_sum[part_row0 + s * part_step]).x);
+  for (int s = 0; s < u.active; ++s) {
+    const float2 part = __ldcg(&p.part_sum[part_row0 + s * part_step]);
+    l += part.x == -INFINITY ? part.y : part.y * exp2f(part.x - m);
+  }
+  inv = empty ? 0.0f : (m == -INFINITY ? NAN : 1.0f / l);
+#pragma unroll 1
+  for (int c = 0; c < D / 32; ++c) {
+    float o[32] = {};
+    for (int s = 0; s < u.active; ++s) {
+      const float part_m = __ldcg(&p.part_sum[part_row0 + s * part_step]).x;
+      const float f = part_m == -INFINITY ? 0.0f : exp2f(part_m - m);
+      const float4 *src = reinterpret_cast<const float4 *>(p.part_out + (part_row0 + s * part_step) * D + c * 32);
+#pragma unroll
+      for (int g = 0; g < 8; ++g) {
+        const float4 x = __ldcg(src + g);
+        o[4 * g] = fmaf(x.x, f, o[4 * g]);
+        o[4 * g + 1] = fmaf(x.y, f, o[4 * g + 1]);
+        o[4 * g + 2] = fmaf(x.z, f, o[4 * g + 2]);
+        o[4 * g + 3] = fmaf(x.w, f, o[4 * g + 3]);
+      }
+    }
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      uint4 w;
+      w.x = pack16(o[g * 8 + 0] * inv, o[g * 8 + 1] * inv, p.is_bf16);
+      w.y = pack16(o[g * 8 + 2] * inv, o[g * 8 + 3] * inv, p.is_bf16);
+      w.z = pack16(o[g * 8 + 4] * inv, o[g * 8 + 5] * inv, p.is_bf16);
+      w.w = pack16(o[g * 8 + 6] * inv, o[g * 8 + 7] * inv, p.is_bf16);
+      *reinterpret_cast<uint4 *>(dst + c * 32 + g * 8) = empty ? make_uint4(0, 0, 0, 0) : w;
+    }
+  }
+  if (p.row_norm != nullptr) p.row_norm[norm_at] = make_float2(m, inv);
+}
+
 template <int D>
 __global__ void __launch_bounds__(kThreads, 1)
-cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
+cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
                    const __grid_constant__ CUtensorMap tmap_pk, const __grid_constant__ CUtensorMap tmap_pv,
                    const __grid_constant__ TilesParams p) {
   using L = Layout<D>;
@@ -232,14 +342,20 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
   }
   if (threadIdx.x == 0) {
     t.abort_flag = 0;
-    t.patch_flag = 0;
+    t.patch_flag[0] = t.patch_flag[1] = 0;
+    mbar_init(&t.claim_bar, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&t.unit_full_bar[i], 1);
+      mbar_init(&t.unit_empty_bar[i], kSoftmaxWarps + 1 + kHelpWarps);
+    }
     for (int i = 0; i < S; ++i) {
       mbar_init(&t.slot_full_bar[i], 1);
       mbar_init(&t.slot_empty_bar[i], 1);
-      mbar_init(&t.slot_clean_bar[i], kCleanWarps);
+      mbar_init(&t.slot_clean_bar[i], kHelpWarps);
     }
     for (int i = 0; i < kTiles; ++i) {
-      mbar_init(&t.q_full_bar[i], kTileWarps);
+      mbar_init(&t.q_full_bar[i], p.q_by_tma ? 1 : kHelpWarps);
+      mbar_init(&t.q_empty_bar[i], 1);
       mbar_init(&t.s_full_bar[i], 1);
       for (int h = 0; h < kPParts; ++h) mbar_init(&t.p_full_bar[i][h], kTileWarps);
       mbar_init(&t.pv_done_bar[i], 1);
@@ -247,6 +363,7 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
     fence_barrier_init();
   }
   if (warp == kProducerWarp && lane == 0) {
+    if (p.q_by_tma) tma_prefetch_desc(&tmap_q);
     tma_prefetch_desc(&tmap_k);
     tma_prefetch_desc(&tmap_v);
   }
@@ -260,172 +377,78 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
   const uint32_t tmem_base = t.tmem_base_slot;
   griddep_wait();
   griddep_launch_dependents();
-  const Unit u(p, blockIdx.x);
 
   auto q_tile = [&](int i) { return smem + L::kQOff + i * L::kQBytes; };
   auto slot = [&](int i) { return smem + L::kSlotOff + i * L::kSlotBytes; };
+  // Unit number `count` of this CTA (from 1 on), once the producer has put it there; -1: none left. The warp's lanes call together.
+  auto next_unit = [&](int count, int *unit) -> bool {
+    if (!__all_sync(0xffffffffu, mbar_wait(&t.unit_full_bar[count & 1], ((count - 1) >> 1) & 1, &abort_flag))) return false;
+    *unit = *reinterpret_cast<volatile int *>(&t.next_unit[count & 1]);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&t.unit_empty_bar[count & 1]);
+    return true;
+  };
 
-  // Load n of the ring (K of block n / 2 when n is even, V of it when odd) goes to slot n % S.
-  if (u.split >= u.active) {
-    // (fewer parts than CTAs: nothing to do)
-  } else if (warp < kSoftmaxWarps) {
+  // Load n of the ring, counted over all of the CTA's units (K of a block, V of it, K of the next), goes to slot n % S.
+  if (warp < kSoftmaxWarps) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
-    // ------------------------------------------------------------------ queries, softmax and output
+    // ------------------------------------------------------------------ softmax and output
     const int tile = static_cast<int>(warp >> 2);
     const uint32_t quarter = warp & 3;
-    const int row_in_tile = static_cast<int>(quarter) * 32 + static_cast<int>(lane);
-    const int tile_row0 = u.row0 + tile * kBlockQ;
-    const int my_blocks = tile == 0 ? u.blocks[0] : u.blocks[1];
-    {
-      // This warp's 32 rows, a few at a time: piece c of row r of an atom lies at c ^ (r & 7).
-      constexpr int kPieces = D / 8, kRowsAtOnce = 32 / kPieces;
-      const int c = lane % kPieces;
-#pragma unroll 4
-      for (int i = 0; i < 32 / kRowsAtOnce; ++i) {
-        const int in_tile = static_cast<int>(quarter) * 32 + i * kRowsAtOnce + static_cast<int>(lane) / kPieces;
-        const int r = tile_row0 + in_tile;
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (r < p.rows) x = *reinterpret_cast<const uint4 *>(p.q + row_offset(p, p.q_stride, u.head, u.seq, r) + c * 8);
-        *reinterpret_cast<uint4 *>(q_tile(tile) + (c >> 3) * kBlockQ * kAtomBytes + in_tile * kAtomBytes + (((c & 7) ^ (in_tile & 7)) << 4)) = x;
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&t.q_full_bar[tile]);
-    }
-    const int row = tile_row0 + row_in_tile;
-    const bool live = row < p.rows;
-    const int pos = min(row, p.rows - 1) / p.group + u.len - p.q_len;
-    // What every row of the tile sees.
-    const int common_last = tile_row0 / p.group + u.len - p.q_len;
-    const int common_before = (min(tile_row0 + kBlockQ, p.rows) - 1) / p.group + u.len - p.q_len - p.window;
     const uint32_t t_lane = tmem_base + ((quarter * 32u) << 16);
     const uint32_t t_scores = t_lane + tile * L::kSCols;  // the row's 128 scores, then its 128 probabilities in 64 columns
     const uint32_t t_out = t_lane + L::kOCol + tile * D;
-    float m_used = -INFINITY;
-    float l_run = 0.0f;
     bool ok = true;
-    for (int j = 0; j < my_blocks && ok; ++j) {
-      // (Scores of block j are issued behind the product of block j - 1: once they are here the tile's
-      // output is complete up to that block.)
-      ok = __all_sync(0xffffffffu, mbar_wait(&t.s_full_bar[tile], j & 1, &abort_flag));
-      if (!ok) break;
-      tc_fence_after_sync();
-      HideUnseen hide;
-      hide.key0 = u.walk.key0(j);
-      if (u.walk.in_prefix(j)) {
-        hide.edge = hide.key0 + kBlockKv > p.prefix_len;
-        hide.last = p.prefix_len - 1;
-        hide.before = -1;
-        hide.sinks = 0;
-      } else {
-        hide.edge = hide.key0 + kBlockKv - 1 > common_last || (hide.key0 + kBlockKv - 1 >= p.sinks && hide.key0 <= common_before);
-        hide.last = pos;
-        hide.before = pos - p.window;
-        hide.sinks = p.sinks;
-      }
-      softmax_block<D, true>(p.scale_log2, p.is_bf16, t_scores, t_out, j == 0, hide, t.p_full_bar[tile], lane, &m_used, &l_run);
-    }
-    // The last product.
-    if (ok && my_blocks > 0) {
-      ok = __all_sync(0xffffffffu, mbar_wait(&t.pv_done_bar[tile], 0, &abort_flag));
-      tc_fence_after_sync();
-    }
-    const bool parts = p.over_batch || u.active > 1;
-    // The index of this row's part of split s: (kv_head, split, rows) over a prefix, (unit, split, 256) else.
-    const int64_t part_row0 = p.over_batch ? static_cast<int64_t>(u.head) * p.splits * p.rows + row
-                                           : (static_cast<int64_t>(u.run) * p.row_pairs + u.pair) * p.splits * kPairRows + (row - u.row0);
-    const int64_t part_step = p.over_batch ? p.rows : kPairRows;
-    const bool empty = p.prefix_len == 0 && pos < 0;  // sees no key: zeros
-    uint16_t *dst = live && !p.over_batch ? p.out + row_offset(p, p.out_stride, u.head, u.seq, row) : nullptr;
-    float *part_dst = p.part_out + (part_row0 + u.split * part_step) * D;
-    const int64_t norm_at = (static_cast<int64_t>(u.run) * p.group + row % p.group) * p.norm_pitch + row / p.group;
-    // (a row whose every score is -inf has no softmax)
-    float inv = empty ? 0.0f : (m_used == -INFINITY ? NAN : 1.0f / l_run);
-    if (ok) {
+    uint32_t s_phase = 0, pv_phase = 0;  // of the tile's scores and of its finished outputs
+    int unit = blockIdx.x;
 #pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t v[32];
-        if (my_blocks > 0) {
-          tmem_ld_32x32(t_out + c * 32, v);
-          tmem_ld_wait(v);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = 0;
-        }
-        if (live && parts) {
-#pragma unroll
-          for (int g = 0; g < 8; ++g) *reinterpret_cast<uint4 *>(part_dst + c * 32 + g * 4) = make_uint4(v[g * 4], v[g * 4 + 1], v[g * 4 + 2], v[g * 4 + 3]);
-        } else if (live) {
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            uint4 w;
-            w.x = pack16(__uint_as_float(v[g * 8 + 0]) * inv, __uint_as_float(v[g * 8 + 1]) * inv, p.is_bf16);
-            w.y = pack16(__uint_as_float(v[g * 8 + 2]) * inv, __uint_as_float(v[g * 8 + 3]) * inv, p.is_bf16);
-            w.z = pack16(__uint_as_float(v[g * 8 + 4]) * inv, __uint_as_float(v[g * 8 + 5]) * inv, p.is_bf16);
-            w.w = pack16(__uint_as_float(v[g * 8 + 6]) * inv, __uint_as_float(v[g * 8 + 7]) * inv, p.is_bf16);
-            *reinterpret_cast<uint4 *>(dst + c * 32 + g * 8) = empty ? make_uint4(0, 0, 0, 0) : w;
+    for (int count = 1; ok && unit >= 0; ++count) {
+      const Unit u(p, unit);
+      if (u.split < u.active) {
+        const int tile_row0 = u.row0 + tile * kBlockQ;
+        const int my_blocks = tile == 0 ? u.blocks[0] : u.blocks[1];
+        const int row = tile_row0 + static_cast<int>(quarter) * 32 + static_cast<int>(lane);
+        const int pos = min(row, p.rows - 1) / p.group + u.len - p.q_len;
+        // What every row of the tile sees.
+        const int common_last = tile_row0 / p.group + u.len - p.q_len;
+        const int common_before = (min(tile_row0 + kBlockQ, p.rows) - 1) / p.group + u.len - p.q_len - p.window;
+        float m_used = -INFINITY;
+        float l_run = 0.0f;
+        for (int j = 0; j < my_blocks && ok; ++j) {
+          // (Scores of block j are issued behind the product of block j - 1: once they are here the tile's
+          // output is complete up to that block.)
+          ok = __all_sync(0xffffffffu, mbar_wait(&t.s_full_bar[tile], s_phase, &abort_flag));
+          if (!ok) break;
+          s_phase ^= 1;
+          tc_fence_after_sync();
+          HideUnseen hide;
+          hide.key0 = u.walk.key0(j);
+          if (u.walk.in_prefix(j)) {
+            hide.edge = hide.key0 + kBlockKv > p.prefix_len;
+            hide.last = p.prefix_len - 1;
+            hide.before = -1;
+            hide.sinks = 0;
+          } else {
+            hide.edge = hide.key0 + kBlockKv - 1 > common_last || (hide.key0 + kBlockKv - 1 >= p.sinks && hide.key0 <= common_before);
+            hide.last = pos;
+            hide.before = pos - p.window;
+            hide.sinks = p.sinks;
           }
+          softmax_block<D, true>(p.scale_log2, p.is_bf16, t_scores, t_out, j == 0, hide, t.p_full_bar[tile], lane, &m_used, &l_run);
         }
-      }
-      if (live && *reinterpret_cast<volatile uint32_t *>(&t.patch_flag) != 0 && m_used != -INFINITY && l_run == l_run) {
-        const uint16_t *q = p.q + row_offset(p, p.q_stride, u.head, u.seq, row);
-        if (p.is_bf16) {
-          patch_row<D, true>(p, blockIdx.x, pos, q, m_used, l_run, dst, parts ? part_dst : nullptr);
-        } else {
-          patch_row<D, false>(p, blockIdx.x, pos, q, m_used, l_run, dst, parts ? part_dst : nullptr);
+        // The last product.
+        if (ok && my_blocks > 0) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&t.pv_done_bar[tile], pv_phase, &abort_flag));
+          pv_phase ^= 1;
+          tc_fence_after_sync();
         }
+        const bool patch = *reinterpret_cast<volatile uint32_t *>(&t.patch_flag[count & 1]) == static_cast<uint32_t>(count);
+        finish_row<D>(p, u, t, t_out, row, pos, my_blocks, ok, patch, m_used, l_run);
+        // The next unit's first product overwrites this output: it waits for probabilities that the tile's
+        // four warps hand over only after these reads.
+        tc_fence_before_sync();
       }
-      // (the cubic's smallest exponentials keep a part that saw nothing from summing to zero)
-      if (live && parts) p.part_sum[part_row0 + u.split * part_step] = make_float2(m_used, m_used == -INFINITY && l_run == l_run ? 0.0f : l_run);
-      if (live && !parts && p.row_norm != nullptr) p.row_norm[norm_at] = make_float2(m_used, inv);
-    }
-    if (!p.over_batch && u.active > 1) {
-      asm volatile("bar.sync 1, %0;" ::"n"(kSoftmaxWarps * 32) : "memory");
-      if (threadIdx.x == 0) {
-        __threadfence();
-        uint32_t *counter = &p.counters[u.run * p.row_pairs + u.pair];
-        const uint32_t before = atomicAdd(counter, 1u);
-        t.is_last = before + 1 == static_cast<uint32_t>(u.active);
-        if (t.is_last) *counter = 0;
-        __threadfence();
-      }
-      asm volatile("bar.sync 1, %0;" ::"n"(kSoftmaxWarps * 32) : "memory");
-      if (t.is_last && live) {
-        float m = -INFINITY, l = 0.0f;
-        for (int s = 0; s < u.active; ++s) m = fmaxf(m, __ldcg(&p.part_sum[part_row0 + s * part_step]).x);
-        for (int s = 0; s < u.active; ++s) {
-          const float2 part = __ldcg(&p.part_sum[part_row0 + s * part_step]);
-          l += part.x == -INFINITY ? part.y : part.y * exp2f(part.x - m);
-        }
-        inv = empty ? 0.0f : (m == -INFINITY ? NAN : 1.0f / l);
-#pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
-          float o[32] = {};
-          for (int s = 0; s < u.active; ++s) {
-            const float part_m = __ldcg(&p.part_sum[part_row0 + s * part_step]).x;
-            const float f = part_m == -INFINITY ? 0.0f : exp2f(part_m - m);
-            const float4 *src = reinterpret_cast<const float4 *>(p.part_out + (part_row0 + s * part_step) * D + c * 32);
-#pragma unroll
-            for (int g = 0; g < 8; ++g) {
-              const float4 x = __ldcg(src + g);
-              o[4 * g] = fmaf(x.x, f, o[4 * g]);
-              o[4 * g + 1] = fmaf(x.y, f, o[4 * g + 1]);
-              o[4 * g + 2] = fmaf(x.z, f, o[4 * g + 2]);
-              o[4 * g + 3] = fmaf(x.w, f, o[4 * g + 3]);
-            }
-          }
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            uint4 w;
-            w.x = pack16(o[g * 8 + 0] * inv, o[g * 8 + 1] * inv, p.is_bf16);
-            w.y = pack16(o[g * 8 + 2] * inv, o[g * 8 + 3] * inv, p.is_bf16);
-            w.z = pack16(o[g * 8 + 4] * inv, o[g * 8 + 5] * inv, p.is_bf16);
-            w.w = pack16(o[g * 8 + 6] * inv, o[g * 8 + 7] * inv, p.is_bf16);
-            *reinterpret_cast<uint4 *>(dst + c * 32 + g * 8) = empty ? make_uint4(0, 0, 0, 0) : w;
-          }
-        }
-        if (p.row_norm != nullptr) p.row_norm[norm_at] = make_float2(m, inv);
-      }
+      if (ok) ok = next_unit(count, &unit);
     }
     if (!ok && lane == 0) {
       abort_flag = 1;
@@ -437,20 +460,57 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
       // ------------------------------------------------------------------ producer
       if (elect_one()) {
         bool ok = true;
-        for (int n = 0; n < 2 * u.walk.count && ok; ++n) {
-          const int st = n % S, j = n >> 1;
-          if (!mbar_wait(&t.slot_empty_bar[st], ((n / S) & 1) ^ 1, &abort_flag)) {
+        int n = 0;  // loads of the ring so far
+        uint32_t q_phase[kTiles] = {0, 0};
+        int unit = blockIdx.x;
+        for (int count = 1; ok && unit >= 0; ++count) {
+          const Unit u(p, unit);
+          for (int i = 0; i < 2 * u.walk.count && ok; ++i, ++n) {
+            const int st = n % S, j = i >> 1;
+            if (!mbar_wait(&t.slot_empty_bar[st], ((n / S) & 1) ^ 1, &abort_flag)) {
+              ok = false;
+              break;
+            }
+            mbar_arrive_expect_tx(&t.slot_full_bar[st], L::kSlotBytes);
+            const int key0 = u.walk.key0(j);
+            const bool prefix = u.walk.in_prefix(j);
+            const CUtensorMap *map = (i & 1) == 0 ? (prefix ? &tmap_pk : &tmap_k) : (prefix ? &tmap_pv : &tmap_v);
+#pragma unroll
+            for (int a = 0; a < L::kQAtoms; ++a) {
+              tma_load_4d(slot(st) + a * kBlockKv * kAtomBytes, map, &t.slot_full_bar[st], a * kAtomBytes, key0, u.head, prefix ? 0 : u.seq);
+            }
+            // The queries behind the first block of keys, once the last scores of the unit before have been computed.
+            for (int q = 0; i == 0 && p.q_by_tma && q < kTiles && ok; ++q) {
+              if (u.blocks[q] == 0) continue;
+              if (!mbar_wait(&t.q_empty_bar[q], q_phase[q] ^ 1, &abort_flag)) {
+                ok = false;
+                break;
+              }
+              q_phase[q] ^= 1;
+              mbar_arrive_expect_tx(&t.q_full_bar[q], L::kQBytes);
+              const int row = u.row0 + q * kBlockQ;
+              const int seq = p.over_batch ? row / (p.group * p.q_len) : u.seq, query = p.over_batch ? 0 : row / p.group;
+#pragma unroll
+              for (int a = 0; a < L::kQAtoms; ++a) {
+                tma_load_4d(q_tile(q) + a * kBlockQ * kAtomBytes, &tmap_q, &t.q_full_bar[q], a * kAtomBytes, u.head * p.group, query, seq);
+              }
+            }
+          }
+          if (!ok) break;
+          // The next unit is claimed once the last block of this one is on its way: as late as its own
+          // loads allow, so that the CTA that is ahead takes it.
+          mbar_arrive_expect_tx(&t.claim_bar, sizeof(t.claim));
+          claim_next_cta(&t.claim, &t.claim_bar);
+          if (!mbar_wait(&t.claim_bar, (count - 1) & 1, &abort_flag) ||
+              !mbar_wait(&t.unit_empty_bar[count & 1], (((count - 1) >> 1) & 1) ^ 1, &abort_flag)) {
             ok = false;
             break;
           }
-          mbar_arrive_expect_tx(&t.slot_full_bar[st], L::kSlotBytes);
-          const int key0 = u.walk.key0(j);
-          const bool prefix = u.walk.in_prefix(j);
-          const CUtensorMap *map = (n & 1) == 0 ? (prefix ? &tmap_pk : &tmap_k) : (prefix ? &tmap_pv : &tmap_v);
-#pragma unroll
-          for (int a = 0; a < L::kQAtoms; ++a) {
-            tma_load_4d(slot(st) + a * kBlockKv * kAtomBytes, map, &t.slot_full_bar[st], a * kAtomBytes, key0, u.head, prefix ? 0 : u.seq);
-          }
+          const int4 at = claimed_cta(&t.claim);
+          unit = at.w != 0 ? at.x : -1;
+          fence_proxy_async_smem();  // the answer has been read before the next one overwrites it
+          *reinterpret_cast<volatile int *>(&t.next_unit[count & 1]) = unit;
+          mbar_arrive(&t.unit_full_bar[count & 1]);
         }
         if (!ok) {
           abort_flag = 1;
@@ -459,101 +519,157 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
       }
     } else if (warp == kMmaWarp) {
       // ------------------------------------------------------------------ MMA issuer
+      // The whole warp walks the loop and an elected lane issues.
       const bool issuer = elect_one();
       const TileMmas<D> mma(p.is_bf16, true, tmem_base, smem_u32(q_tile(0)), issuer);
       const uint64_t sdesc0 = umma_desc_sw128(smem_u32(slot(0)));
       bool ok = true;
       uint32_t clean_phase = 0;  // bit i: the parity of the next values in slot i
+      uint32_t q_phase[kTiles] = {0, 0}, p_phase[kTiles] = {0, 0};
       auto commit = [&](uint64_t *bar) {
         if (issuer) umma_commit(bar);
       };
       auto wait_full = [&](int n) -> bool { return mbar_wait(&t.slot_full_bar[n % S], (n / S) & 1, &abort_flag); };
       auto desc_of = [&](int n) -> uint64_t { return sdesc0 + static_cast<uint64_t>((n % S) * (L::kSlotBytes >> 4)); };
-      for (int i = 0; i < kTiles && ok; ++i) ok = mbar_wait(&t.q_full_bar[i], 0, &abort_flag);
-      if (ok && u.walk.count > 0) ok = wait_full(0);
-      if (ok && u.walk.count > 0) {
-        tc_fence_after_sync();
-#pragma unroll
-        for (int i = 0; i < kTiles; ++i) {
-          if (u.blocks[i] == 0) continue;
-          mma.scores(i, desc_of(0));
+      int n = 0;  // the ring's load that holds K of the unit's first block
+      int unit = blockIdx.x;
+      for (int count = 1; ok && unit >= 0; ++count) {
+        int blocks[kTiles], total;
+        {
+          const Unit u(p, unit);
+          blocks[0] = u.blocks[0], blocks[1] = u.blocks[1], total = u.walk.count;
+        }
+        // Tile i's scores with the keys in load nk; after the last of them its queries may be replaced.
+        auto issue_scores = [&](int i, int nk, bool last) {
+          tc_fence_after_sync();
+          mma.scores(i, desc_of(nk));
           commit(&t.s_full_bar[i]);
-        }
-        commit(&t.slot_empty_bar[0]);
-      }
-      for (int j = 0; j < u.walk.count && ok; ++j) {
-        const bool more = j + 1 < u.walk.count;
-        const int nv = 2 * j + 1, nk = 2 * j + 2;
-        if (!wait_full(nv) || !mbar_wait(&t.slot_clean_bar[nv % S], (clean_phase >> (nv % S)) & 1, &abort_flag)) ok = false;
-        clean_phase ^= 1u << (nv % S);
+          if (last) commit(&t.q_empty_bar[i]);
+        };
+        if (total > 0) {
 #pragma unroll
-        for (int i = 0; i < kTiles; ++i) {
-          if (!ok || j >= u.blocks[i]) continue;
-          // The product reads P from the columns the next scores overwrite: the instructions of one
-          // thread run in the order they were issued.
-#pragma unroll
-          for (int part = 0; part < kPParts; ++part) {
-            if (ok) ok = mbar_wait(&t.p_full_bar[i][part], j & 1, &abort_flag);
-            if (!ok) break;
-            tc_fence_after_sync();
-            mma.product(i, part, desc_of(nv), j == 0 ? 1u : 0u);
+          for (int i = 0; i < kTiles; ++i) {
+            if (!ok || blocks[i] == 0) continue;
+            ok = mbar_wait(&t.q_full_bar[i], q_phase[i], &abort_flag) && wait_full(n);
+            q_phase[i] ^= 1;
+            if (ok) issue_scores(i, n, blocks[i] == 1);
           }
-          if (!ok) continue;
-          if (j + 1 == u.blocks[i]) {
-            commit(&t.pv_done_bar[i]);  // (a block's scores, which the softmax waits for, follow its product)
-          } else {
-            if (!wait_full(nk)) {  // (seen by the first tile's turn, for the second's too)
-              ok = false;
-              continue;
+          if (!ok) break;
+          commit(&t.slot_empty_bar[n % S]);
+        }
+        for (int j = 0; j < total && ok; ++j) {
+          const bool more = j + 1 < total;
+          const int nv = n + 2 * j + 1, nk = nv + 1;
+          if (!wait_full(nv) || !mbar_wait(&t.slot_clean_bar[nv % S], (clean_phase >> (nv % S)) & 1, &abort_flag)) ok = false;
+          clean_phase ^= 1u << (nv % S);
+#pragma unroll
+          for (int i = 0; i < kTiles; ++i) {
+            if (!ok || j >= blocks[i]) continue;
+            // The product reads P from the columns the next scores overwrite: the instructions of one
+            // thread run in the order they were issued.
+#pragma unroll
+            for (int part = 0; part < kPParts; ++part) {
+              if (ok) ok = mbar_wait(&t.p_full_bar[i][part], p_phase[i], &abort_flag);
+              if (!ok) break;
+              tc_fence_after_sync();
+              mma.product(i, part, desc_of(nv), j == 0 ? 1u : 0u);
             }
-            tc_fence_after_sync();
-            mma.scores(i, desc_of(nk));
-            commit(&t.s_full_bar[i]);
+            if (!ok) continue;
+            p_phase[i] ^= 1;
+            if (j + 1 == blocks[i]) {
+              commit(&t.pv_done_bar[i]);  // (a block's scores, which the softmax waits for, follow its product)
+            } else if (!wait_full(nk)) {  // (seen by the first tile's turn, for the second's too)
+              ok = false;
+            } else {
+              issue_scores(i, nk, j + 2 == blocks[i]);
+            }
           }
+          if (!ok) break;
+          commit(&t.slot_empty_bar[nv % S]);  // both tiles have read the two slots
+          if (more) commit(&t.slot_empty_bar[nk % S]);
         }
-        if (!ok) break;
-        commit(&t.slot_empty_bar[nv % S]);  // both tiles have read the two slots
-        if (more) commit(&t.slot_empty_bar[nk % S]);
+        n += 2 * total;
+        if (ok) ok = next_unit(count, &unit);
       }
       if (!ok && issuer) {
         abort_flag = 1;
         atomicCAS(p.status, 0u, kStatusAttentionTimeout);
       }
     } else {
-      // ------------------------------------------------------------------ values that are not seen by all
-      const int which = static_cast<int>(warp) - kCleanWarp;
+      // ------------------------------------------------------------------ queries, and values that are not seen by all
+      const int which = static_cast<int>(warp) - kHelpWarp;
       bool ok = true;
-      // (Every block's values are waited for and passed on, so that no wait is two phases ahead of its barrier or behind it.)
-      for (int j = 0; j < u.walk.count && ok; ++j) {
-        const int nv = 2 * j + 1;
-        ok = __all_sync(0xffffffffu, mbar_wait(&t.slot_full_bar[nv % S], (nv / S) & 1, &abort_flag));
-        if (!ok) break;
-        if (!u.walk.differs(j)) {
-          if (lane == 0) mbar_arrive(&t.slot_clean_bar[nv % S]);
-          continue;
-        }
-        uint8_t *block = slot(nv % S);
-        const int key0 = u.walk.key0(j);
-        bool taken = false;
+      uint32_t q_phase = 0;  // bit i: of tile i's queries
+      int n = 0;
+      int unit = blockIdx.x;
+      for (int count = 1; ok && unit >= 0; ++count) {
+        const Unit u(p, unit);
+        if (!p.q_by_tma) {
+          // Half of each tile's rows, a few at a time: piece c of row r of an atom lies at c ^ (r & 7).
+          constexpr int kPieces = D / 8, kRowsAtOnce = 32 / kPieces;
+          const int c = static_cast<int>(lane) % kPieces;
+#pragma unroll 1
+          for (int i = 0; i < kTiles; ++i) {
+            if (ok && u.blocks[i] > 0) {
+              ok = __all_sync(0xffffffffu, mbar_wait(&t.q_empty_bar[i], ((q_phase >> i) & 1) ^ 1, &abort_flag));
+              q_phase ^= 1u << i;
 #pragma unroll 4
-        for (int i = which; i < L::kSlotBytes / 512; i += kCleanWarps) {  // four keys' 128 bytes of an atom
-          const int key = key0 + (i % (kBlockKv / 4)) * 4 + static_cast<int>(lane >> 3);
-          uint4 *at = reinterpret_cast<uint4 *>(block + i * 512 + lane * 16);
-          const bool hidden = key >= u.walk.range.end || (key >= u.walk.range.sinks && key < u.walk.range.begin);
-          if (hidden) {
-            *at = make_uint4(0, 0, 0, 0);
-          } else {
-            const uint4 x = *at;
-            if (p.is_bf16 ? has_nonfinite<true>(x) : has_nonfinite<false>(x)) {
-              *at = p.is_bf16 ? without_nonfinite<true>(x) : without_nonfinite<false>(x);
-              taken = true;
+              for (int k = 0; ok && k < kBlockQ / kHelpWarps / kRowsAtOnce; ++k) {
+                const int in_tile = which * (kBlockQ / kHelpWarps) + k * kRowsAtOnce + static_cast<int>(lane) / kPieces;
+                const int r = u.row0 + i * kBlockQ + in_tile;
+                cp_async_16(q_tile(i) + (c >> 3) * kBlockQ * kAtomBytes + in_tile * kAtomBytes + (((c & 7) ^ (in_tile & 7)) << 4),
+                            p.q + row_offset(p, p.q_stride, u.head, u.seq, min(r, p.rows - 1)) + c * 8, r < p.rows ? 16 : 0);
+              }
             }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+          }
+#pragma unroll
+          for (int i = 0; i < kTiles; ++i) {
+            if (i == 0) {
+              asm volatile("cp.async.wait_group 1;" ::: "memory");
+            } else {
+              asm volatile("cp.async.wait_group 0;" ::: "memory");
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (ok && u.blocks[i] > 0 && lane == 0) mbar_arrive(&t.q_full_bar[i]);
           }
         }
-        if (taken) *reinterpret_cast<volatile uint32_t *>(&t.patch_flag) = 1;
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&t.slot_clean_bar[nv % S]);
+        // (Every load is waited for and all values are passed on, so that no wait is a phase ahead of its barrier or behind it.)
+        for (int j = 0; j < u.walk.count && ok; ++j) {
+          const int nv = n + 2 * j + 1;
+          ok = __all_sync(0xffffffffu, mbar_wait(&t.slot_full_bar[(nv - 1) % S], ((nv - 1) / S) & 1, &abort_flag) &&
+                                           mbar_wait(&t.slot_full_bar[nv % S], (nv / S) & 1, &abort_flag));
+          if (!ok) break;
+          if (!u.walk.differs(j)) {
+            if (lane == 0) mbar_arrive(&t.slot_clean_bar[nv % S]);
+            continue;
+          }
+          uint8_t *block = slot(nv % S);
+          const int key0 = u.walk.key0(j);
+          bool taken = false;
+#pragma unroll 4
+          for (int i = which; i < L::kSlotBytes / 512; i += kHelpWarps) {  // four keys' 128 bytes of an atom
+            const int key = key0 + (i % (kBlockKv / 4)) * 4 + static_cast<int>(lane >> 3);
+            uint4 *at = reinterpret_cast<uint4 *>(block + i * 512 + lane * 16);
+            const bool hidden = key >= u.walk.range.end || (key >= u.walk.range.sinks && key < u.walk.range.begin);
+            if (hidden) {
+              *at = make_uint4(0, 0, 0, 0);
+            } else {
+              const uint4 x = *at;
+              if (p.is_bf16 ? has_nonfinite<true>(x) : has_nonfinite<false>(x)) {
+                *at = p.is_bf16 ? without_nonfinite<true>(x) : without_nonfinite<false>(x);
+                taken = true;
+              }
+            }
+          }
+          if (taken) *reinterpret_cast<volatile uint32_t *>(&t.patch_flag[count & 1]) = static_cast<uint32_t>(count);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&t.slot_clean_bar[nv % S]);
+        }
+        n += 2 * u.walk.count;
+        if (ok) ok = next_unit(count, &unit);
       }
       if (!ok && lane == 0) {
         abort_flag = 1;
@@ -577,12 +693,12 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
 }
 
 template <int D>
-cudaError_t launch(const CUtensorMap (&maps)[4], const TilesParams &p, int64_t ctas, cudaStream_t stream) {
+cudaError_t launch(const CUtensorMap &tq, const CUtensorMap (&maps)[4], const TilesParams &p, int64_t ctas, cudaStream_t stream) {
   using L = Layout<D>;
   auto kernel = cache_tiles_kernel<D>;
   static const cudaError_t attr_set = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmemBytes);
   if (attr_set != cudaSuccess) return attr_set;
-  return launch_overlapped(kernel, ctas, kThreads, L::kSmemBytes, stream, maps[0], maps[1], maps[2], maps[3], p);
+  return launch_overlapped(kernel, ctas, kThreads, L::kSmemBytes, stream, tq, maps[0], maps[1], maps[2], maps[3], p);
 }
 
 }  // namespace
@@ -600,8 +716,25 @@ int cache_tiles_splits(int64_t units, int keys, int most_units) {
 
 size_t cache_tiles_part_rows(int64_t units, int splits) { return static_cast<size_t>(units) * splits * kPairRows; }
 
-cudaError_t cache_tiles(const TilesParams &p, const CacheAttentionArgs &a, const char **why) {
-  CUtensorMap maps[4];
+cudaError_t cache_tiles(TilesParams p, const CacheAttentionArgs &a, const char **why) {
+  CUtensorMap tq, maps[4];
+  // A tile's rows as a box: the heads of a group, a run of queries, and over a prefix a run of sequences.
+  const int per_query = p.group, per_sequence = p.group * p.q_len;
+  const bool whole_queries = !p.over_batch && per_query <= kBlockQ && kBlockQ % per_query == 0;
+  const bool whole_sequences = p.over_batch && per_sequence <= kBlockQ && kBlockQ % per_sequence == 0;
+  p.q_by_tma = whole_queries || whole_sequences;
+  if (p.q_by_tma) {
+    const uint64_t dims[4] = {static_cast<uint64_t>(a.head_dim) * 2, static_cast<uint64_t>(a.heads), static_cast<uint64_t>(a.q_len),
+                              static_cast<uint64_t>(a.batch)};
+    auto bytes = [&](int64_t s, int extent) { return static_cast<uint64_t>(extent > 1 ? s : a.head_dim) * 2; };
+    const uint64_t strides[3] = {bytes(a.q_stride[1], a.heads), bytes(a.q_stride[2], a.q_len), bytes(a.q_stride[0], a.batch)};
+    const uint32_t box[3] = {static_cast<uint32_t>(p.group), static_cast<uint32_t>(whole_sequences ? p.q_len : kBlockQ / per_query),
+                             static_cast<uint32_t>(whole_sequences ? kBlockQ / per_sequence : 1)};
+    if (!make_tmap(&tq, a.q, 4, dims, strides, box)) {
+      *why = "cuTensorMapEncodeTiled refused q";
+      return cudaErrorInvalidValue;
+    }
+  }
   const bool own = !p.over_batch, prefix = p.prefix_len > 0;
   if (own && (!row_map(&maps[0], a.k, a.head_dim, a.kv_len, a.kv_heads, a.batch, a.k_stride[0], a.k_stride[1], a.k_stride[2]) ||
               !row_map(&maps[1], a.v, a.head_dim, a.kv_len, a.kv_heads, a.batch, a.v_stride[0], a.v_stride[1], a.v_stride[2]))) {
@@ -613,11 +746,12 @@ cudaError_t cache_tiles(const TilesParams &p, const CacheAttentionArgs &a, const
     *why = "cuTensorMapEncodeTiled refused the prefix";
     return cudaErrorInvalidValue;
   }
+  if (!p.q_by_tma) tq = own ? maps[0] : maps[2];  // (not used)
   if (!own) maps[0] = maps[2], maps[1] = maps[3];
   if (!prefix) maps[2] = maps[0], maps[3] = maps[1];
   const int64_t ctas = static_cast<int64_t>(p.runs) * p.row_pairs * p.splits;
   *why = "launching the tile kernel";
-  return a.head_dim == 64 ? launch<64>(maps, p, ctas, a.stream) : launch<128>(maps, p, ctas, a.stream);
+  return a.head_dim == 64 ? launch<64>(tq, maps, p, ctas, a.stream) : launch<128>(tq, maps, p, ctas, a.stream);
 }
 
 }  // namespace flsm100

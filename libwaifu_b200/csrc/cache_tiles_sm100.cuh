@@ -22,6 +22,7 @@ struct TilesParams {
   int rows;         // packed rows of a run
   int row_pairs;    // pairs of tiles of 128 of them
   int splits;       // CTAs that divide a pair's blocks of keys
+  bool q_by_tma;    // set by cache_tiles()
   float scale_log2;
   float *part_out;   // (kv_head, split, rows, D) over a prefix, (run, pair, split, 256, D) else
   float2 *part_sum;  // the same without D: maximum in log2 units, sum
@@ -35,6 +36,6 @@ int cache_tiles_pairs(int rows);
 // `keys`: the most that a pair's rows see between them. At most `most_units` units may be divided.
 int cache_tiles_splits(int64_t units, int keys, int most_units);
 size_t cache_tiles_part_rows(int64_t units, int splits);
-cudaError_t cache_tiles(const TilesParams &p, const CacheAttentionArgs &a, const char **why);
+cudaError_t cache_tiles(TilesParams p, const CacheAttentionArgs &a, const char **why);
 
 }  // namespace flsm100

@@ -147,9 +147,10 @@ cache_weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     int met = 0;
     for (int b = 0; b < u.count && ok; ++b) {
       const int st = b % S;
+      ok = __all_sync(0xffffffffu, mbar_wait(&t.slot_full_bar[st], (b / S) & 1, &abort_flag));
+      if (!ok) break;
       if (u.meets(b, tile)) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&t.slot_full_bar[st], (b / S) & 1, &abort_flag) &&
-                                         mbar_wait(&t.s_full_bar[tile][met & 1], (met >> 1) & 1, &abort_flag));
+        ok = __all_sync(0xffffffffu, mbar_wait(&t.s_full_bar[tile][met & 1], (met >> 1) & 1, &abort_flag));
         if (!ok) break;
         tc_fence_after_sync();
         uint32_t sc[4][32];
