@@ -350,14 +350,14 @@ inline bool make_tmap(CUtensorMap *map, const void *base, int rank, const uint64
   return make_tmap(map, base, rank, dims, strides_bytes, rows);
 }
 
-// Queries, keys or values as (head_dim bytes, positions, heads, batch), strides in elements, in boxes of 128 positions.
+// Queries, keys or values as (head_dim bytes, positions, heads, batch), strides in elements, in boxes of box_rows positions.
 inline bool row_map(CUtensorMap *map, const void *base, int head_dim, int len, int heads, int batch, int64_t batch_stride, int64_t head_stride,
-             int64_t position_stride) {
+             int64_t position_stride, uint32_t box_rows) {
   const uint64_t dims[4] = {static_cast<uint64_t>(head_dim) * 2, static_cast<uint64_t>(len), static_cast<uint64_t>(heads), static_cast<uint64_t>(batch)};
   // (the stride of a dimension of extent 1 is never used, but has to pass the encoder's checks)
   auto bytes = [&](int64_t s) { return static_cast<uint64_t>(s > 0 ? s : head_dim) * 2; };
   const uint64_t strides[3] = {bytes(len > 1 ? position_stride : 0), bytes(heads > 1 ? head_stride : 0), bytes(batch > 1 ? batch_stride : 0)};
-  return make_tmap(map, base, 4, dims, strides, kBlockKv);
+  return make_tmap(map, base, 4, dims, strides, box_rows);
 }
 
 }  // namespace

@@ -5,8 +5,10 @@
 // head r % group of the ones that share the head, so that a block of keys is read once for all of them and a
 // tile's rows sit close together (under a window a tile walks its 128 / group positions and the window, not 128
 // and the window). Over a prefix, which all of a batch sees, the rows of every sequence are packed one after the other.
-// K and V blocks of 128 keys arrive by TMA into one ring of slots; the walk is a list of blocks: those of a prefix, those that
-// hold sinks, those from the first window's start to the last query's position.
+// K and V blocks of 128 keys arrive by TMA into one ring of slots. The walk is a list of blocks: those of a prefix, then the
+// sinks and the keys from the first window's start to the last query's position, one after the other and cut every 128
+// keys (a block that holds both comes in boxes of 16 rows, the sinks filled up to whole ones): 8192 tokens under a window of
+// 1024 keys and 16 sinks walk 9 blocks a unit so, and 10.4 in blocks at multiples of 128.
 //
 // So do the queries where a tile is a box of the tensor (a group, or a group and its queries, that divides 128); otherwise two
 // helping warps gather them. A block that some row does not see whole (past the sequence's end, at a window's edge, on
@@ -76,32 +78,38 @@ struct Layout : TileLayout<D> {
   static_assert(kSmemBytes <= 227 * 1024, "shared memory");
 };
 
-// The blocks of keys a pair of tiles walks, and what its rows see of them.
+constexpr int kBoxRows = 16;  // of the boxes in which a block of sinks and window keys comes
+
+// The blocks of keys a pair of tiles walks, and what its rows see of them. The own keys have places 0 .. total - 1: the sinks
+// from 0 on, hidden keys up to `pad`, then the keys from `begin` on. (pad is 0 where sinks and window meet, and without sinks.)
 struct Walk {
   int prefix_blocks, prefix_len;
-  int sink_blocks, window_block;  // the blocks 0 .. sink_blocks - 1, then those from window_block on
-  int first, count;               // of this split
-  KeyRange range;                 // what the rows see between them
-  int first_pos, last_pos;        // of the pair's rows
+  int pad, begin, total;
+  int first, count;         // blocks of this split
+  int first_pos, last_pos;  // of the pair's rows
   int window, sinks;
 
   __device__ __forceinline__ bool in_prefix(int j) const { return first + j < prefix_blocks; }
-  __device__ __forceinline__ int key0(int j) const {
-    const int at = first + j;
-    if (at < prefix_blocks) return at * kBlockKv;
-    const int own = at - prefix_blocks;
-    return (own < sink_blocks ? own : own - sink_blocks + window_block) * kBlockKv;
-  }
+  __device__ __forceinline__ int place0(int j) const { return (first + j - prefix_blocks) * kBlockKv; }
+  __device__ __forceinline__ int key_at(int place) const { return place < pad ? place : place - pad + begin; }
   // Does some row not see some key of block j?
   __device__ __forceinline__ bool differs(int j) const {
     if (in_prefix(j)) return false;  // (keys past a prefix's end come as zeros)
-    const int k0 = key0(j), k1 = k0 + kBlockKv - 1;
+    const int x0 = place0(j);
+    if (x0 < pad) return x0 + kBlockKv > sinks;
+    const int k0 = x0 - pad + begin, k1 = k0 + kBlockKv - 1;
     return k1 > first_pos || (k1 >= sinks && k0 <= last_pos - window);
+  }
+  // No row sees the key at this place (of its own keys).
+  __device__ __forceinline__ bool hidden(int place) const { return place >= total || (place >= sinks && place < pad); }
+  // Some rows see it and others do not.
+  __device__ __forceinline__ bool mixed(int place) const {
+    const int key = key_at(place);
+    return key > first_pos || (key <= last_pos - window && key >= sinks);
   }
   // How many blocks of the whole walk hold keys up to `position`.
   __device__ __forceinline__ int blocks_up_to(int position) const {
-    const int own = position < 0 ? 0 : position / kBlockKv + 1;
-    return prefix_blocks + (own <= sink_blocks ? own : sink_blocks + max(0, own - window_block));
+    return prefix_blocks + (position < 0 ? 0 : (position - begin + pad) / kBlockKv + 1);
   }
 };
 
@@ -126,24 +134,19 @@ struct Unit {
     walk.prefix_blocks = (p.prefix_len + kBlockKv - 1) / kBlockKv;
     walk.window = p.window;
     walk.sinks = p.sinks;
-    int total;
-    if (p.over_batch) {
-      len = 0;
-      walk.first_pos = walk.last_pos = 0;
-      walk.range = KeyRange{0, 0, 0};
-      walk.sink_blocks = walk.window_block = 0;
-      total = walk.prefix_blocks;
-    } else {
+    len = 0;
+    walk.first_pos = walk.last_pos = walk.pad = walk.begin = walk.total = 0;
+    if (!p.over_batch) {
       len = sequence_length(p.kv_lens, seq, p.kv_len);
       walk.first_pos = row0 / p.group + len - p.q_len;
       walk.last_pos = last_row / p.group + len - p.q_len;
-      walk.range = visible_keys(walk.first_pos, walk.last_pos, len, p.window, p.sinks);
-      walk.sink_blocks = (walk.range.sinks + kBlockKv - 1) / kBlockKv;
-      walk.window_block = walk.range.begin / kBlockKv;
-      if (walk.sink_blocks >= walk.window_block) walk.sink_blocks = walk.window_block = 0;  // they meet: one run of blocks
-      const int end_block = (walk.range.end + kBlockKv - 1) / kBlockKv;
-      total = walk.prefix_blocks + walk.sink_blocks + max(0, end_block - walk.window_block);
+      const KeyRange range = visible_keys(walk.first_pos, walk.last_pos, len, p.window, p.sinks);
+      const bool apart = range.sinks > 0 && range.sinks < range.begin;
+      walk.pad = apart ? (range.sinks + kBoxRows - 1) / kBoxRows * kBoxRows : 0;
+      walk.begin = apart || range.sinks == 0 ? range.begin : 0;
+      walk.total = walk.pad + range.end - walk.begin;
     }
+    const int total = walk.prefix_blocks + (walk.total + kBlockKv - 1) / kBlockKv;
     const int per_split = max(1, (total + p.splits - 1) / p.splits);
     active = max(1, (total + per_split - 1) / per_split);
     walk.first = split * per_split;
@@ -160,7 +163,7 @@ struct Unit {
 // Bits 0 .. n - 1.
 __device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u); }
 
-// Of the keys from key0 on, the row sees those up to `last`, behind `before` or below `sinks`.
+// Of a block's keys, the first of which is key0, the row sees those up to `last` that are behind `before`, and the first `sinks`.
 struct HideUnseen {
   bool edge;
   int key0, last, before, sinks;
@@ -169,7 +172,7 @@ struct HideUnseen {
 #pragma unroll
     for (int c = 0; c < kBlockKv / 32; ++c) {
       const int base = key0 + c * 32;
-      const uint32_t seen = bits_below(last + 1 - base) & (~bits_below(before + 1 - base) | bits_below(sinks - base));
+      const uint32_t seen = bits_below(last + 1 - base) & (~bits_below(before + 1 - base) | bits_below(sinks - c * 32));
 #pragma unroll
       for (int i = 0; i < 32; ++i) {
         if (!((seen >> i) & 1u)) sc[c][i] = __float_as_uint(-INFINITY);
@@ -194,8 +197,9 @@ __device__ __noinline__ void patch_row(const TilesParams &p, int unit, int pos, 
   const Unit u(p, unit);
   for (int j = 0; j < u.walk.count; ++j) {
     if (!u.walk.differs(j)) continue;
-    for (int key = u.walk.key0(j); key < u.walk.key0(j) + kBlockKv; ++key) {
-      if (key > pos || key >= u.len || !(key > pos - p.window || key < p.sinks)) continue;
+    for (int x = u.walk.place0(j); x < u.walk.place0(j) + kBlockKv; ++x) {
+      const int key = u.walk.key_at(x);
+      if (u.walk.hidden(x) || key > pos || !(key > pos - p.window || key < p.sinks)) continue;
       const uint16_t *v = p.v + u.seq * p.v_stride[0] + u.head * p.v_stride[1] + key * p.v_stride[2];
       const uint16_t *k = p.k + u.seq * p.k_stride[0] + u.head * p.k_stride[1] + key * p.k_stride[2];
       bool odd = false;
@@ -325,6 +329,7 @@ __device__ __forceinline__ void finish_row(const TilesParams &p, const Unit &u, 
 template <int D>
 __global__ void __launch_bounds__(kThreads, 1)
 cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
+                   const __grid_constant__ CUtensorMap tmap_k16, const __grid_constant__ CUtensorMap tmap_v16,
                    const __grid_constant__ CUtensorMap tmap_pk, const __grid_constant__ CUtensorMap tmap_pv,
                    const __grid_constant__ TilesParams p) {
   using L = Layout<D>;
@@ -422,17 +427,25 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
           s_phase ^= 1;
           tc_fence_after_sync();
           HideUnseen hide;
-          hide.key0 = u.walk.key0(j);
           if (u.walk.in_prefix(j)) {
+            hide.key0 = (u.walk.first + j) * kBlockKv;
             hide.edge = hide.key0 + kBlockKv > p.prefix_len;
             hide.last = p.prefix_len - 1;
             hide.before = -1;
             hide.sinks = 0;
           } else {
-            hide.edge = hide.key0 + kBlockKv - 1 > common_last || (hide.key0 + kBlockKv - 1 >= p.sinks && hide.key0 <= common_before);
+            const int x0 = u.walk.place0(j);
+            hide.key0 = x0 - u.walk.pad + u.walk.begin;
             hide.last = pos;
-            hide.before = pos - p.window;
-            hide.sinks = p.sinks;
+            if (x0 < u.walk.pad) {  // sinks, and what follows them
+              hide.edge = x0 + kBlockKv > p.sinks;
+              hide.before = max(pos - p.window, u.walk.begin - 1);
+              hide.sinks = p.sinks - x0;
+            } else {
+              hide.edge = hide.key0 + kBlockKv - 1 > common_last || (hide.key0 + kBlockKv - 1 >= p.sinks && hide.key0 <= common_before);
+              hide.before = pos - p.window;
+              hide.sinks = p.sinks - hide.key0;
+            }
           }
           softmax_block<D, true>(p.scale_log2, p.is_bf16, t_scores, t_out, j == 0, hide, t.p_full_bar[tile], lane, &m_used, &l_run);
         }
@@ -472,12 +485,24 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
               break;
             }
             mbar_arrive_expect_tx(&t.slot_full_bar[st], L::kSlotBytes);
-            const int key0 = u.walk.key0(j);
-            const bool prefix = u.walk.in_prefix(j);
-            const CUtensorMap *map = (i & 1) == 0 ? (prefix ? &tmap_pk : &tmap_k) : (prefix ? &tmap_pv : &tmap_v);
+            const bool prefix = u.walk.in_prefix(j), keys = (i & 1) == 0;
+            const int x0 = u.walk.place0(j);
+            if (!prefix && x0 < u.walk.pad && x0 + kBlockKv > u.walk.pad) {
+              const CUtensorMap *map = keys ? &tmap_k16 : &tmap_v16;
+              for (int r = 0; r < kBlockKv; r += kBoxRows) {
 #pragma unroll
-            for (int a = 0; a < L::kQAtoms; ++a) {
-              tma_load_4d(slot(st) + a * kBlockKv * kAtomBytes, map, &t.slot_full_bar[st], a * kAtomBytes, key0, u.head, prefix ? 0 : u.seq);
+                for (int a = 0; a < L::kQAtoms; ++a) {
+                  tma_load_4d(slot(st) + a * kBlockKv * kAtomBytes + r * kAtomBytes, map, &t.slot_full_bar[st], a * kAtomBytes, u.walk.key_at(x0 + r),
+                              u.head, u.seq);
+                }
+              }
+            } else {
+              const CUtensorMap *map = keys ? (prefix ? &tmap_pk : &tmap_k) : (prefix ? &tmap_pv : &tmap_v);
+              const int key0 = prefix ? (u.walk.first + j) * kBlockKv : u.walk.key_at(x0);
+#pragma unroll
+              for (int a = 0; a < L::kQAtoms; ++a) {
+                tma_load_4d(slot(st) + a * kBlockKv * kAtomBytes, map, &t.slot_full_bar[st], a * kAtomBytes, key0, u.head, prefix ? 0 : u.seq);
+              }
             }
             // The queries behind the first block of keys, once the last scores of the unit before have been computed.
             for (int q = 0; i == 0 && p.q_by_tma && q < kTiles && ok; ++q) {
@@ -645,21 +670,23 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             if (lane == 0) mbar_arrive(&t.slot_clean_bar[nv % S]);
             continue;
           }
-          uint8_t *block = slot(nv % S);
-          const int key0 = u.walk.key0(j);
+          uint8_t *block = slot(nv % S) + lane * 16;
+          const int x0 = u.walk.place0(j);
           bool taken = false;
-#pragma unroll 4
-          for (int i = which; i < L::kSlotBytes / 512; i += kHelpWarps) {  // four keys' 128 bytes of an atom
-            const int key = key0 + (i % (kBlockKv / 4)) * 4 + static_cast<int>(lane >> 3);
-            uint4 *at = reinterpret_cast<uint4 *>(block + i * 512 + lane * 16);
-            const bool hidden = key >= u.walk.range.end || (key >= u.walk.range.sinks && key < u.walk.range.begin);
-            if (hidden) {
-              *at = make_uint4(0, 0, 0, 0);
-            } else {
-              const uint4 x = *at;
-              if (p.is_bf16 ? has_nonfinite<true>(x) : has_nonfinite<false>(x)) {
-                *at = p.is_bf16 ? without_nonfinite<true>(x) : without_nonfinite<false>(x);
-                taken = true;
+          for (int r = which * 4; r < kBlockKv; r += kHelpWarps * 4) {  // four keys' 128 bytes of an atom
+            const int x = x0 + r + static_cast<int>(lane >> 3);
+            const bool hidden = u.walk.hidden(x), mixed = !hidden && u.walk.mixed(x);
+            if (!__any_sync(0xffffffffu, hidden || mixed)) continue;
+#pragma unroll
+            for (int a = 0; a < L::kQAtoms; ++a) {
+              uint4 *at = reinterpret_cast<uint4 *>(block + a * kBlockKv * kAtomBytes + r * kAtomBytes);
+              if (hidden) *at = make_uint4(0, 0, 0, 0);
+              if (mixed) {
+                const uint4 w = *at;
+                if (p.is_bf16 ? has_nonfinite<true>(w) : has_nonfinite<false>(w)) {
+                  *at = p.is_bf16 ? without_nonfinite<true>(w) : without_nonfinite<false>(w);
+                  taken = true;
+                }
               }
             }
           }
@@ -693,12 +720,12 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
 }
 
 template <int D>
-cudaError_t launch(const CUtensorMap &tq, const CUtensorMap (&maps)[4], const TilesParams &p, int64_t ctas, cudaStream_t stream) {
+cudaError_t launch(const CUtensorMap &tq, const CUtensorMap (&maps)[6], const TilesParams &p, int64_t ctas, cudaStream_t stream) {
   using L = Layout<D>;
   auto kernel = cache_tiles_kernel<D>;
   static const cudaError_t attr_set = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmemBytes);
   if (attr_set != cudaSuccess) return attr_set;
-  return launch_overlapped(kernel, ctas, kThreads, L::kSmemBytes, stream, tq, maps[0], maps[1], maps[2], maps[3], p);
+  return launch_overlapped(kernel, ctas, kThreads, L::kSmemBytes, stream, tq, maps[0], maps[1], maps[2], maps[3], maps[4], maps[5], p);
 }
 
 }  // namespace
@@ -717,7 +744,7 @@ int cache_tiles_splits(int64_t units, int keys, int most_units) {
 size_t cache_tiles_part_rows(int64_t units, int splits) { return static_cast<size_t>(units) * splits * kPairRows; }
 
 cudaError_t cache_tiles(TilesParams p, const CacheAttentionArgs &a, const char **why) {
-  CUtensorMap tq, maps[4];
+  CUtensorMap tq, maps[6];  // of q; of k and v, the same in boxes of 16 positions, of the prefix
   // A tile's rows as a box: the heads of a group, a run of queries, and over a prefix a run of sequences.
   const int per_query = p.group, per_sequence = p.group * p.q_len;
   const bool whole_queries = !p.over_batch && per_query <= kBlockQ && kBlockQ % per_query == 0;
@@ -736,19 +763,22 @@ cudaError_t cache_tiles(TilesParams p, const CacheAttentionArgs &a, const char *
     }
   }
   const bool own = !p.over_batch, prefix = p.prefix_len > 0;
-  if (own && (!row_map(&maps[0], a.k, a.head_dim, a.kv_len, a.kv_heads, a.batch, a.k_stride[0], a.k_stride[1], a.k_stride[2]) ||
-              !row_map(&maps[1], a.v, a.head_dim, a.kv_len, a.kv_heads, a.batch, a.v_stride[0], a.v_stride[1], a.v_stride[2]))) {
-    *why = "cuTensorMapEncodeTiled refused k or v";
-    return cudaErrorInvalidValue;
+  for (int i = 0; own && i < 4; ++i) {
+    const int64_t *stride = i % 2 == 0 ? a.k_stride : a.v_stride;
+    if (!row_map(&maps[i], i % 2 == 0 ? a.k : a.v, a.head_dim, a.kv_len, a.kv_heads, a.batch, stride[0], stride[1], stride[2], i < 2 ? kBlockKv : kBoxRows)) {
+      *why = "cuTensorMapEncodeTiled refused k or v";
+      return cudaErrorInvalidValue;
+    }
   }
-  if (prefix && (!row_map(&maps[2], a.prefix_k, a.head_dim, a.prefix_len, a.kv_heads, 1, 0, a.prefix_k_stride[0], a.prefix_k_stride[1]) ||
-                 !row_map(&maps[3], a.prefix_v, a.head_dim, a.prefix_len, a.kv_heads, 1, 0, a.prefix_v_stride[0], a.prefix_v_stride[1]))) {
+  if (prefix && (!row_map(&maps[4], a.prefix_k, a.head_dim, a.prefix_len, a.kv_heads, 1, 0, a.prefix_k_stride[0], a.prefix_k_stride[1], kBlockKv) ||
+                 !row_map(&maps[5], a.prefix_v, a.head_dim, a.prefix_len, a.kv_heads, 1, 0, a.prefix_v_stride[0], a.prefix_v_stride[1], kBlockKv))) {
     *why = "cuTensorMapEncodeTiled refused the prefix";
     return cudaErrorInvalidValue;
   }
-  if (!p.q_by_tma) tq = own ? maps[0] : maps[2];  // (not used)
-  if (!own) maps[0] = maps[2], maps[1] = maps[3];
-  if (!prefix) maps[2] = maps[0], maps[3] = maps[1];
+  // (the others are not used)
+  if (!own) maps[0] = maps[2] = maps[4], maps[1] = maps[3] = maps[5];
+  if (!prefix) maps[4] = maps[0], maps[5] = maps[1];
+  if (!p.q_by_tma) tq = maps[0];
   const int64_t ctas = static_cast<int64_t>(p.runs) * p.row_pairs * p.splits;
   *why = "launching the tile kernel";
   return a.head_dim == 64 ? launch<64>(tq, maps, p, ctas, a.stream) : launch<128>(tq, maps, p, ctas, a.stream);

@@ -337,8 +337,8 @@ WeightsPlan cache_weights_plan(const CacheAttentionArgs &a, int most_units) {
 
 cudaError_t cache_weights(const WeightsParams &p, const CacheAttentionArgs &a, const char **why) {
   CUtensorMap tq, tk;
-  if (!row_map(&tq, a.q, a.head_dim, a.q_len, a.heads, a.batch, a.q_stride[0], a.q_stride[1], a.q_stride[2]) ||
-      !row_map(&tk, a.k, a.head_dim, a.kv_len, a.kv_heads, a.batch, a.k_stride[0], a.k_stride[1], a.k_stride[2])) {
+  if (!row_map(&tq, a.q, a.head_dim, a.q_len, a.heads, a.batch, a.q_stride[0], a.q_stride[1], a.q_stride[2], kBlockQ) ||
+      !row_map(&tk, a.k, a.head_dim, a.kv_len, a.kv_heads, a.batch, a.k_stride[0], a.k_stride[1], a.k_stride[2], kBlockKv)) {
     *why = "cuTensorMapEncodeTiled refused q or k";
     return cudaErrorInvalidValue;
   }
