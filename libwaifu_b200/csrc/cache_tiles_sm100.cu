@@ -78,6 +78,13 @@ struct Layout : TileLayout<D> {
   static_assert(kSmemBytes <= 227 * 1024, "shared memory");
 };
 
+// The blocks of a walk that hold keys some row does not see: from one up to another (sinks, the windows' starts), and from one
+// on (the rows' own positions, the end).
+struct Dirty {
+  int begin, end, from;
+  __device__ __forceinline__ bool has(int j) const { return (j >= begin && j < end) || j >= from; }
+};
+
 constexpr int kBoxRows = 16;  // of the boxes in which a block of sinks and window keys comes
 
 // The blocks of keys a pair of tiles walks, and what its rows see of them. The own keys have places 0 .. total - 1: the sinks
@@ -88,21 +95,21 @@ struct Walk {
   int first, count;         // blocks of this split
   int first_pos, last_pos;  // of the pair's rows
   int window, sinks;
+  Dirty dirty;              // (keys past a prefix's end come as zeros: its blocks never are)
 
+  __device__ __forceinline__ void find_dirty() {
+    const int own = prefix_blocks - first;  // the walk's first own block, in this split
+    auto block_of = [](int place) { return place < 0 ? 0 : place / kBlockKv; };
+    dirty.begin = own + block_of(pad > 0 ? sinks : sinks - begin);
+    dirty.end = own + (last_pos - window - begin + pad < 0 ? 0 : block_of(last_pos - window - begin + pad) + 1);
+    dirty.from = own + block_of(first_pos + 1 + pad - begin);
+  }
   __device__ __forceinline__ bool in_prefix(int j) const { return first + j < prefix_blocks; }
   __device__ __forceinline__ int place0(int j) const { return (first + j - prefix_blocks) * kBlockKv; }
   __device__ __forceinline__ int key_at(int place) const { return place < pad ? place : place - pad + begin; }
-  // Does some row not see some key of block j?
-  __device__ __forceinline__ bool differs(int j) const {
-    if (in_prefix(j)) return false;  // (keys past a prefix's end come as zeros)
-    const int x0 = place0(j);
-    if (x0 < pad) return x0 + kBlockKv > sinks;
-    const int k0 = x0 - pad + begin, k1 = k0 + kBlockKv - 1;
-    return k1 > first_pos || (k1 >= sinks && k0 <= last_pos - window);
-  }
   // No row sees the key at this place (of its own keys).
   __device__ __forceinline__ bool hidden(int place) const { return place >= total || (place >= sinks && place < pad); }
-  // Some rows see it and others do not.
+  // Some rows see it and others do not (of keys that are not hidden).
   __device__ __forceinline__ bool mixed(int place) const {
     const int key = key_at(place);
     return key > first_pos || (key <= last_pos - window && key >= sinks);
@@ -151,6 +158,8 @@ struct Unit {
     active = max(1, (total + per_split - 1) / per_split);
     walk.first = split * per_split;
     walk.count = max(0, min(per_split, total - walk.first));  // (0 past the active splits)
+    walk.find_dirty();
+    if (p.over_batch) walk.dirty = Dirty{0, 0, INT32_MAX};
 #pragma unroll
     for (int i = 0; i < kTiles; ++i) {
       const int first_row = row0 + i * kBlockQ, last = min(first_row + kBlockQ, p.rows) - 1;
@@ -158,6 +167,14 @@ struct Unit {
       blocks[i] = first_row >= p.rows ? 0 : max(0, min(walk.count, mine - walk.first));
     }
   }
+};
+
+// What the issuing warp has to know of a unit.
+struct Todo {
+  int blocks[kTiles], total;
+  Dirty dirty;
+  __device__ __forceinline__ Todo() : blocks{0, 0}, total(0) {}
+  __device__ __forceinline__ explicit Todo(const Unit &u) : blocks{u.blocks[0], u.blocks[1]}, total(u.walk.count), dirty(u.walk.dirty) {}
 };
 
 // Bits 0 .. n - 1.
@@ -196,7 +213,7 @@ template <int D, bool BF16>
 __device__ __noinline__ void patch_row(const TilesParams &p, int unit, int pos, const uint16_t *q, float m, float l, uint16_t *out, float *part) {
   const Unit u(p, unit);
   for (int j = 0; j < u.walk.count; ++j) {
-    if (!u.walk.differs(j)) continue;
+    if (!u.walk.dirty.has(j)) continue;
     for (int x = u.walk.place0(j); x < u.walk.place0(j) + kBlockKv; ++x) {
       const int key = u.walk.key_at(x);
       if (u.walk.hidden(x) || key > pos || !(key > pos - p.window || key < p.sinks)) continue;
@@ -355,7 +372,7 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     }
     for (int i = 0; i < S; ++i) {
       mbar_init(&t.slot_full_bar[i], 1);
-      mbar_init(&t.slot_empty_bar[i], 1);
+      mbar_init(&t.slot_empty_bar[i], 1 + kHelpWarps);
       mbar_init(&t.slot_clean_bar[i], kHelpWarps);
     }
     for (int i = 0; i < kTiles; ++i) {
@@ -474,7 +491,7 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       if (elect_one()) {
         bool ok = true;
         int n = 0;  // loads of the ring so far
-        uint32_t q_phase[kTiles] = {0, 0};
+        uint32_t q_phase = 0;  // bit i: of tile i's queries
         int unit = blockIdx.x;
         for (int count = 1; ok && unit >= 0; ++count) {
           const Unit u(p, unit);
@@ -506,12 +523,12 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             }
             // The queries behind the first block of keys, once the last scores of the unit before have been computed.
             for (int q = 0; i == 0 && p.q_by_tma && q < kTiles && ok; ++q) {
-              if (u.blocks[q] == 0) continue;
-              if (!mbar_wait(&t.q_empty_bar[q], q_phase[q] ^ 1, &abort_flag)) {
+              if ((q == 0 ? u.blocks[0] : u.blocks[1]) == 0) continue;
+              if (!mbar_wait(&t.q_empty_bar[q], ((q_phase >> q) & 1) ^ 1, &abort_flag)) {
                 ok = false;
                 break;
               }
-              q_phase[q] ^= 1;
+              q_phase ^= 1u << q;
               mbar_arrive_expect_tx(&t.q_full_bar[q], L::kQBytes);
               const int row = u.row0 + q * kBlockQ;
               const int seq = p.over_batch ? row / (p.group * p.q_len) : u.seq, query = p.over_batch ? 0 : row / p.group;
@@ -549,7 +566,7 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       const TileMmas<D> mma(p.is_bf16, true, tmem_base, smem_u32(q_tile(0)), issuer);
       const uint64_t sdesc0 = umma_desc_sw128(smem_u32(slot(0)));
       bool ok = true;
-      uint32_t clean_phase = 0;  // bit i: the parity of the next values in slot i
+      uint32_t clean_phase = 0;  // bit i: the parity of the next unclean values in slot i
       uint32_t q_phase[kTiles] = {0, 0}, p_phase[kTiles] = {0, 0};
       auto commit = [&](uint64_t *bar) {
         if (issuer) umma_commit(bar);
@@ -558,42 +575,56 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       auto desc_of = [&](int n) -> uint64_t { return sdesc0 + static_cast<uint64_t>((n % S) * (L::kSlotBytes >> 4)); };
       int n = 0;  // the ring's load that holds K of the unit's first block
       int unit = blockIdx.x;
+      Todo now(Unit(p, unit));
+      // Tile i's scores with the keys in load nk; after the last of them its queries may be replaced.
+      auto issue_scores = [&](int i, int nk, bool last) {
+        tc_fence_after_sync();
+        mma.scores(i, desc_of(nk));
+        commit(&t.s_full_bar[i]);
+        if (last) commit(&t.q_empty_bar[i]);
+      };
+      auto first_scores = [&](int i, int nk, bool last) -> bool {
+        const bool there = mbar_wait(&t.q_full_bar[i], q_phase[i], &abort_flag) && wait_full(nk);
+        q_phase[i] ^= 1;
+        if (there) issue_scores(i, nk, last);
+        return there;
+      };
+      bool started[kTiles] = {false, false};  // the tile's first scores of the unit are under way
       for (int count = 1; ok && unit >= 0; ++count) {
-        int blocks[kTiles], total;
-        {
-          const Unit u(p, unit);
-          blocks[0] = u.blocks[0], blocks[1] = u.blocks[1], total = u.walk.count;
-        }
-        // Tile i's scores with the keys in load nk; after the last of them its queries may be replaced.
-        auto issue_scores = [&](int i, int nk, bool last) {
-          tc_fence_after_sync();
-          mma.scores(i, desc_of(nk));
-          commit(&t.s_full_bar[i]);
-          if (last) commit(&t.q_empty_bar[i]);
-        };
-        if (total > 0) {
+        if (now.total > 0) {
 #pragma unroll
           for (int i = 0; i < kTiles; ++i) {
-            if (!ok || blocks[i] == 0) continue;
-            ok = mbar_wait(&t.q_full_bar[i], q_phase[i], &abort_flag) && wait_full(n);
-            q_phase[i] ^= 1;
-            if (ok) issue_scores(i, n, blocks[i] == 1);
+            if (ok && !started[i] && now.blocks[i] > 0) ok = first_scores(i, n, now.blocks[i] == 1);
           }
           if (!ok) break;
           commit(&t.slot_empty_bar[n % S]);
         }
-        for (int j = 0; j < total && ok; ++j) {
-          const bool more = j + 1 < total;
-          const int nv = n + 2 * j + 1, nk = nv + 1;
-          if (!wait_full(nv) || !mbar_wait(&t.slot_clean_bar[nv % S], (clean_phase >> (nv % S)) & 1, &abort_flag)) ok = false;
-          clean_phase ^= 1u << (nv % S);
+        started[0] = started[1] = false;
+        bool known = false;
+        Todo next;
+        auto find_next = [&]() -> bool {
+          known = true;
+          if (!next_unit(count, &unit)) return false;
+          if (unit >= 0) next = Todo(Unit(p, unit));
+          return true;
+        };
+        for (int j = 0; j < now.total && ok; ++j) {
+          const bool more = j + 1 < now.total;
+          const int nv = n + 2 * j + 1, nk = nv + 1;  // (nk: of this unit's next block or the next unit's first)
+          if (!wait_full(nv)) ok = false;
+          bool unclean = now.dirty.has(j);
 #pragma unroll
           for (int i = 0; i < kTiles; ++i) {
-            if (!ok || j >= blocks[i]) continue;
+            if (!ok || j >= now.blocks[i]) continue;
             // The product reads P from the columns the next scores overwrite: the instructions of one
             // thread run in the order they were issued.
 #pragma unroll
             for (int part = 0; part < kPParts; ++part) {
+              if (unclean) {
+                ok = mbar_wait(&t.slot_clean_bar[nv % S], (clean_phase >> (nv % S)) & 1, &abort_flag);
+                clean_phase ^= 1u << (nv % S);
+                unclean = false;
+              }
               if (ok) ok = mbar_wait(&t.p_full_bar[i][part], p_phase[i], &abort_flag);
               if (!ok) break;
               tc_fence_after_sync();
@@ -601,20 +632,31 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             }
             if (!ok) continue;
             p_phase[i] ^= 1;
-            if (j + 1 == blocks[i]) {
-              commit(&t.pv_done_bar[i]);  // (a block's scores, which the softmax waits for, follow its product)
-            } else if (!wait_full(nk)) {  // (seen by the first tile's turn, for the second's too)
-              ok = false;
-            } else {
-              issue_scores(i, nk, j + 2 == blocks[i]);
+            if (j + 1 < now.blocks[i]) {
+              if (!wait_full(nk)) {  // (seen by the first tile's turn, for the second's too)
+                ok = false;
+              } else {
+                issue_scores(i, nk, j + 2 == now.blocks[i]);
+              }
+              continue;
+            }
+            commit(&t.pv_done_bar[i]);  // (a block's scores, which the softmax waits for, follow its product)
+            if (more) continue;
+            // Through with the unit: on with the first scores of the next one, which run under the
+            // other tile's last product and this one's output.
+            if (!known) ok = find_next();
+            if (ok && next.blocks[i] > 0) {
+              started[i] = true;
+              ok = first_scores(i, nk, next.blocks[i] == 1);
             }
           }
           if (!ok) break;
           commit(&t.slot_empty_bar[nv % S]);  // both tiles have read the two slots
           if (more) commit(&t.slot_empty_bar[nk % S]);
         }
-        n += 2 * total;
-        if (ok) ok = next_unit(count, &unit);
+        n += 2 * now.total;
+        if (ok && !known) ok = find_next();
+        now = next;
       }
       if (!ok && issuer) {
         abort_flag = 1;
@@ -623,6 +665,8 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     } else {
       // ------------------------------------------------------------------ queries, and values that are not seen by all
       const int which = static_cast<int>(warp) - kHelpWarp;
+      // A half whose exponent is all ones carries into its sign bit.
+      const uint32_t exponent = p.is_bf16 ? 0x7F807F80u : 0x7C007C00u, carry = p.is_bf16 ? 0x00800080u : 0x04000400u;
       bool ok = true;
       uint32_t q_phase = 0;  // bit i: of tile i's queries
       int n = 0;
@@ -635,7 +679,7 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
           const int c = static_cast<int>(lane) % kPieces;
 #pragma unroll 1
           for (int i = 0; i < kTiles; ++i) {
-            if (ok && u.blocks[i] > 0) {
+            if (ok && (i == 0 ? u.blocks[0] : u.blocks[1]) > 0) {
               ok = __all_sync(0xffffffffu, mbar_wait(&t.q_empty_bar[i], ((q_phase >> i) & 1) ^ 1, &abort_flag));
               q_phase ^= 1u << i;
 #pragma unroll 4
@@ -660,40 +704,54 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             if (ok && u.blocks[i] > 0 && lane == 0) mbar_arrive(&t.q_full_bar[i]);
           }
         }
-        // (Every load is waited for and all values are passed on, so that no wait is a phase ahead of its barrier or behind it.)
+        // (Every load is waited for and its slot given back, so that none is filled again before its turn here.)
         for (int j = 0; j < u.walk.count && ok; ++j) {
-          const int nv = n + 2 * j + 1;
-          ok = __all_sync(0xffffffffu, mbar_wait(&t.slot_full_bar[(nv - 1) % S], ((nv - 1) / S) & 1, &abort_flag) &&
-                                           mbar_wait(&t.slot_full_bar[nv % S], (nv / S) & 1, &abort_flag));
+          const int nk = n + 2 * j, nv = nk + 1;
+          ok = __all_sync(0xffffffffu, mbar_wait(&t.slot_full_bar[nk % S], (nk / S) & 1, &abort_flag));
+          if (ok && lane == 0) mbar_arrive(&t.slot_empty_bar[nk % S]);
+          ok = ok && __all_sync(0xffffffffu, mbar_wait(&t.slot_full_bar[nv % S], (nv / S) & 1, &abort_flag));
           if (!ok) break;
-          if (!u.walk.differs(j)) {
-            if (lane == 0) mbar_arrive(&t.slot_clean_bar[nv % S]);
+          if (!u.walk.dirty.has(j)) {
+            if (lane == 0) mbar_arrive(&t.slot_empty_bar[nv % S]);
             continue;
           }
           uint8_t *block = slot(nv % S) + lane * 16;
           const int x0 = u.walk.place0(j);
-          bool taken = false;
+          uint32_t odd = 0;  // the sign bits of halves whose exponent is all ones
+#pragma unroll 4
           for (int r = which * 4; r < kBlockKv; r += kHelpWarps * 4) {  // four keys' 128 bytes of an atom
             const int x = x0 + r + static_cast<int>(lane >> 3);
             const bool hidden = u.walk.hidden(x), mixed = !hidden && u.walk.mixed(x);
-            if (!__any_sync(0xffffffffu, hidden || mixed)) continue;
 #pragma unroll
             for (int a = 0; a < L::kQAtoms; ++a) {
               uint4 *at = reinterpret_cast<uint4 *>(block + a * kBlockKv * kAtomBytes + r * kAtomBytes);
               if (hidden) *at = make_uint4(0, 0, 0, 0);
               if (mixed) {
                 const uint4 w = *at;
-                if (p.is_bf16 ? has_nonfinite<true>(w) : has_nonfinite<false>(w)) {
-                  *at = p.is_bf16 ? without_nonfinite<true>(w) : without_nonfinite<false>(w);
-                  taken = true;
-                }
+                odd |= ((w.x & exponent) + carry) | ((w.y & exponent) + carry) | ((w.z & exponent) + carry) | ((w.w & exponent) + carry);
+              }
+            }
+          }
+          bool taken = false;
+          if (__any_sync(0xffffffffu, (odd & 0x80008000u) != 0)) {
+#pragma unroll 1
+            for (int r = which * 4; r < kBlockKv; r += kHelpWarps * 4) {
+              if (u.walk.hidden(x0 + r + static_cast<int>(lane >> 3)) || !u.walk.mixed(x0 + r + static_cast<int>(lane >> 3))) continue;
+              for (int a = 0; a < L::kQAtoms; ++a) {
+                uint4 *at = reinterpret_cast<uint4 *>(block + a * kBlockKv * kAtomBytes + r * kAtomBytes);
+                const uint4 w = *at;
+                *at = p.is_bf16 ? without_nonfinite<true>(w) : without_nonfinite<false>(w);
+                taken = taken || (p.is_bf16 ? has_nonfinite<true>(w) : has_nonfinite<false>(w));
               }
             }
           }
           if (taken) *reinterpret_cast<volatile uint32_t *>(&t.patch_flag[count & 1]) = static_cast<uint32_t>(count);
           fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&t.slot_clean_bar[nv % S]);
+          if (lane == 0) {
+            mbar_arrive(&t.slot_clean_bar[nv % S]);
+            mbar_arrive(&t.slot_empty_bar[nv % S]);
+          }
         }
         n += 2 * u.walk.count;
         if (ok) ok = next_unit(count, &unit);
