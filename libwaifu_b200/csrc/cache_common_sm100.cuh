@@ -14,6 +14,36 @@
 namespace flsm100 {
 
 
+// Division by a number that the host knows, of numbers below 2^31: with 2^s >= d > 2^(s - 1) and m = ceil(2^(32 + s) / d) - 2^32 the
+// quotient is (n m / 2^32 + n) / 2^s, rounded down twice. A unit's place takes a dozen divisions, which at some 40
+// instructions each were a microsecond and more at the beginning of a kernel.
+struct Divisor {
+  uint32_t d, m;
+  int s;
+  static Divisor of(uint32_t d) {
+    Divisor r = {d, 0, 0};
+    while ((uint64_t{1} << r.s) < d) ++r.s;
+    r.m = static_cast<uint32_t>(((uint64_t{1} << (32 + r.s)) + d - 1) / d - (uint64_t{1} << 32));
+    return r;
+  }
+  __device__ __forceinline__ int quotient(int n) const {
+    return static_cast<int>((__umulhi(static_cast<uint32_t>(n), m) + static_cast<uint32_t>(n)) >> s);
+  }
+  // n becomes the quotient, and the remainder is returned.
+  __device__ __forceinline__ int take(int *n) const {
+    const int q = quotient(*n), r = *n - q * static_cast<int>(d);
+    *n = q;
+    return r;
+  }
+};
+
+// Eight 32-bit values to 32-byte aligned memory: a whole sector from one lane.
+__device__ __forceinline__ void store_32_bytes(void *dst, uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t e, uint32_t f, uint32_t g,
+                                               uint32_t h) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(a), "r"(b), "r"(c), "r"(d), "r"(e), "r"(f), "r"(g), "r"(h)
+               : "memory");
+}
+
 __device__ __forceinline__ int sequence_length(const int32_t *kv_lens, int seq, int kv_len) {
   return kv_lens == nullptr ? kv_len : min(max(kv_lens[seq], 0), kv_len);
 }

@@ -111,6 +111,7 @@ struct RowsParams {
   int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3];
   const int32_t *kv_lens;
   int kv_heads, group, q_len, kv_len;
+  Divisor by_kv_heads, by_group, by_row_tiles, by_sequence_rows;  // (the last: group * q_len)
   int window, sinks;
   float scale_log2;
   // Rows of the whole batch over keys that all of them see (a shared prefix): parts only.
@@ -212,11 +213,10 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
     load.seq = 0;
     load.enter_sequence(p);
     int at = blockIdx.x;
-    load.tile = at % p.row_tiles;
-    at /= p.row_tiles;
-    load.head = at % p.kv_heads;
+    load.tile = p.by_row_tiles.take(&at);
+    load.head = p.by_kv_heads.take(&at);
     per_cta = (load.steps + p.splits - 1) / p.splits;
-    begin = load.step = static_cast<int>(at / p.kv_heads * per_cta);
+    begin = load.step = at * static_cast<int>(per_cta);
     count = min(static_cast<int>(per_cta), load.steps - load.step);
   } else {
     const int units = p.kv_heads * p.row_tiles;
@@ -282,10 +282,9 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
     }
     load.enter_sequence(p);
     const int64_t in_seq = begin - before;
-    const int unit = static_cast<int>(in_seq / load.steps);
-    load.step = static_cast<int>(in_seq - static_cast<int64_t>(unit) * load.steps);
-    load.tile = unit % p.row_tiles;
-    load.head = unit / p.row_tiles;
+    load.head = static_cast<int>(in_seq / load.steps);
+    load.step = static_cast<int>(in_seq - static_cast<int64_t>(load.head) * load.steps);
+    load.tile = p.by_row_tiles.take(&load.head);
   }
   Cursor at = load;
 
@@ -344,10 +343,11 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
     if ((threadIdx.x >> 3) < kRows && r < p.rows) {
       int n = u.seq, in_seq = r;
       if (p.over_batch) {
-        n = in_seq / (p.group * p.q_len);
-        in_seq -= n * p.group * p.q_len;
+        n = in_seq;
+        in_seq = p.by_sequence_rows.take(&n);
       }
-      const int i = in_seq / p.group, g = in_seq - i * p.group;
+      int i = in_seq;
+      const int g = p.by_group.take(&i);
       const uint16_t *src = p.q + n * p.q_stride[0] + static_cast<int64_t>(u.head * p.group + g) * p.q_stride[1] + i * p.q_stride[2];
 #pragma unroll
       for (int c = 0; c < kMyPieces; ++c) x[c] = *reinterpret_cast<const uint4 *>(src + ((threadIdx.x & 7) + 8 * c) * 8);
@@ -394,15 +394,15 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
       }
     }
     const int row0 = at.tile * kRows, offset = at.len - p.q_len;
-    first_pos = row0 / p.group + offset;
-    last_pos = (min(row0 + kRows, p.rows) - 1) / p.group + offset;
+    first_pos = p.by_group.quotient(row0) + offset;
+    last_pos = p.by_group.quotient(min(row0 + kRows, p.rows) - 1) + offset;
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         m[n][i] = -INFINITY;
         l[n][i] = 0.0f;
-        pos[n][i] = (row0 + n * 8 + my_row + i) / p.group + offset;
+        pos[n][i] = p.by_group.quotient(row0 + n * 8 + my_row + i) + offset;
       }
     }
     unit_step = at.step;
@@ -587,8 +587,10 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
     __syncthreads();
 
     const int row0 = unit.tile * kRows, live = min(kRows, p.rows - row0);
-    const int64_t unit_begin = begin + done - unit.step;  // the unit's first step among all
-    const int first_cta = static_cast<int>(unit_begin / per_cta), last_cta = static_cast<int>((unit_begin + unit.steps - 1) / per_cta);
+    // The CTAs that share it: so many runs of steps before this one's, and so many behind.
+    const int run = static_cast<int>(per_cta), before = unit.step - done, behind = done + unit.steps - unit.step - run;
+    const int here = static_cast<int>(blockIdx.x);
+    const int first_cta = before > 0 ? here - (before + run - 1) / run : here, last_cta = behind > 0 ? here + (behind + run - 1) / run : here;
     const bool shared = !p.over_batch && last_cta > first_cta;
     const uint8_t *stages = smem + L::kRingOff + (k_tile - ring);  // the first warp's
     auto own_part = [&](int r, int col, RowSum *sum) {
@@ -642,7 +644,8 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
           add_parts<D>(p.prefix_splits, p.prefix_sum, p.prefix_out, col, &sum,
                        [&](int c) { return first + static_cast<int64_t>(c) * p.prefix_rows; });
         }
-        const int q = (row0 + r) / p.group, g = (row0 + r) - q * p.group;
+        int q = row0 + r;
+        const int g = p.by_group.take(&q);
         // A query that sees no key: zeros. (Where it sees some and their exponentials sum to zero or to NaN, that is its result.)
         const bool empty = p.prefix_splits == 0 && q + unit.len - p.q_len < 0;
         const float inv = empty ? 0.0f : 1.0f / sum.l;
@@ -835,6 +838,9 @@ void fill_params(const CacheAttentionArgs &a, Params *p) {
   p->kv_lens = a.kv_lens;
   p->kv_heads = a.kv_heads;
   p->group = a.heads / a.kv_heads;
+  p->by_kv_heads = Divisor::of(static_cast<uint32_t>(p->kv_heads));
+  p->by_group = Divisor::of(static_cast<uint32_t>(p->group));
+  p->by_sequence_rows = Divisor::of(static_cast<uint32_t>(p->group * a.q_len));
   p->q_len = a.q_len;
   p->kv_len = a.kv_len;
   p->window = a.window;
@@ -900,6 +906,7 @@ cudaError_t cache_attention(const CacheAttentionArgs &a, const char **why, int *
   fill_params(a, &p);
   p.rows = plan.rows;
   p.row_tiles = plan.row_tiles;
+  p.by_row_tiles = Divisor::of(static_cast<uint32_t>(p.row_tiles));
   p.batch = a.batch;
   p.part_out = floats(plan.part_out);
   p.part_sum = pairs(plan.part_sum);
@@ -929,6 +936,7 @@ cudaError_t cache_attention(const CacheAttentionArgs &a, const char **why, int *
       s.kv_len = a.prefix_len;
       s.rows = plan.prefix_rows;
       s.row_tiles = plan.prefix_row_tiles;
+      s.by_row_tiles = Divisor::of(static_cast<uint32_t>(s.row_tiles));
       s.splits = plan.prefix_splits;
       s.part_out = floats(plan.prefix_out);
       s.part_sum = pairs(plan.prefix_sum);

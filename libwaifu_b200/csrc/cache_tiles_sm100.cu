@@ -129,12 +129,11 @@ struct Unit {
 
   __device__ __forceinline__ Unit(const TilesParams &p, int at) : index(at) {
     // The longest walks first: the last pair of every run, then the one before it.
-    run = at % p.runs;
-    at /= p.runs;
-    split = at % p.splits;
-    pair = p.row_pairs - 1 - at / p.splits;
-    head = run % p.kv_heads;
-    seq = run / p.kv_heads;
+    run = p.by_runs.take(&at);
+    split = p.by_splits.take(&at);
+    pair = p.row_pairs - 1 - at;
+    seq = run;
+    head = p.by_kv_heads.take(&seq);
     row0 = pair * kPairRows;
     const int last_row = min(row0 + kPairRows, p.rows) - 1;
     walk.prefix_len = p.prefix_len;
@@ -145,8 +144,8 @@ struct Unit {
     walk.first_pos = walk.last_pos = walk.pad = walk.begin = walk.total = 0;
     if (!p.over_batch) {
       len = sequence_length(p.kv_lens, seq, p.kv_len);
-      walk.first_pos = row0 / p.group + len - p.q_len;
-      walk.last_pos = last_row / p.group + len - p.q_len;
+      walk.first_pos = p.by_group.quotient(row0) + len - p.q_len;
+      walk.last_pos = p.by_group.quotient(last_row) + len - p.q_len;
       const KeyRange range = visible_keys(walk.first_pos, walk.last_pos, len, p.window, p.sinks);
       const bool apart = range.sinks > 0 && range.sinks < range.begin;
       walk.pad = apart ? (range.sinks + kBoxRows - 1) / kBoxRows * kBoxRows : 0;
@@ -154,8 +153,8 @@ struct Unit {
       walk.total = walk.pad + range.end - walk.begin;
     }
     const int total = walk.prefix_blocks + (walk.total + kBlockKv - 1) / kBlockKv;
-    const int per_split = max(1, (total + p.splits - 1) / p.splits);
-    active = max(1, (total + per_split - 1) / per_split);
+    const int per_split = max(1, p.by_splits.quotient(total + p.splits - 1));
+    active = p.splits == 1 ? 1 : max(1, (total + per_split - 1) / per_split);
     walk.first = split * per_split;
     walk.count = max(0, min(per_split, total - walk.first));  // (0 past the active splits)
     walk.find_dirty();
@@ -163,7 +162,7 @@ struct Unit {
 #pragma unroll
     for (int i = 0; i < kTiles; ++i) {
       const int first_row = row0 + i * kBlockQ, last = min(first_row + kBlockQ, p.rows) - 1;
-      const int mine = p.over_batch ? total : min(total, walk.blocks_up_to(last / p.group + len - p.q_len));
+      const int mine = p.over_batch ? total : min(total, walk.blocks_up_to(p.by_group.quotient(last) + len - p.q_len));
       blocks[i] = first_row >= p.rows ? 0 : max(0, min(walk.count, mine - walk.first));
     }
   }
@@ -201,10 +200,11 @@ struct HideUnseen {
 // The address of packed row r of a head's queries (or results).
 __device__ __forceinline__ int64_t row_offset(const TilesParams &p, const int64_t (&stride)[3], int head, int seq, int r) {
   if (p.over_batch) {
-    seq = r / (p.group * p.q_len);
-    r -= seq * p.group * p.q_len;
+    seq = r;
+    r = p.by_sequence_rows.take(&seq);
   }
-  const int i = r / p.group, g = r - i * p.group;
+  int i = r;
+  const int g = p.by_group.take(&i);
   return seq * stride[0] + static_cast<int64_t>(head * p.group + g) * stride[1] + i * stride[2];
 }
 
@@ -254,7 +254,9 @@ __device__ __forceinline__ void finish_row(const TilesParams &p, const Unit &u, 
   const bool empty = p.prefix_len == 0 && pos < 0;  // sees no key: zeros
   uint16_t *dst = live && !p.over_batch ? p.out + row_offset(p, p.out_stride, u.head, u.seq, row) : nullptr;
   float *part_dst = p.part_out + (part_row0 + u.split * part_step) * D;
-  const int64_t norm_at = (static_cast<int64_t>(u.run) * p.group + row % p.group) * p.norm_pitch + row / p.group;
+  int query = row;
+  const int in_group = p.by_group.take(&query);
+  const int64_t norm_at = (static_cast<int64_t>(u.run) * p.group + in_group) * p.norm_pitch + query;
   // (a row whose every score is -inf has no softmax)
   float inv = empty ? 0.0f : (m_used == -INFINITY ? NAN : 1.0f / l_run);
   if (ok) {
@@ -270,7 +272,9 @@ __device__ __forceinline__ void finish_row(const TilesParams &p, const Unit &u, 
       }
       if (live && parts) {
 #pragma unroll
-        for (int g = 0; g < 8; ++g) *reinterpret_cast<uint4 *>(part_dst + c * 32 + g * 4) = make_uint4(v[g * 4], v[g * 4 + 1], v[g * 4 + 2], v[g * 4 + 3]);
+        for (int g = 0; g < 32; g += 8) {
+          store_32_bytes(part_dst + c * 32 + g, v[g], v[g + 1], v[g + 2], v[g + 3], v[g + 4], v[g + 5], v[g + 6], v[g + 7]);
+        }
       } else if (live) {
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
@@ -430,10 +434,10 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         const int tile_row0 = u.row0 + tile * kBlockQ;
         const int my_blocks = tile == 0 ? u.blocks[0] : u.blocks[1];
         const int row = tile_row0 + static_cast<int>(quarter) * 32 + static_cast<int>(lane);
-        const int pos = min(row, p.rows - 1) / p.group + u.len - p.q_len;
+        const int pos = p.by_group.quotient(min(row, p.rows - 1)) + u.len - p.q_len;
         // What every row of the tile sees.
-        const int common_last = tile_row0 / p.group + u.len - p.q_len;
-        const int common_before = (min(tile_row0 + kBlockQ, p.rows) - 1) / p.group + u.len - p.q_len - p.window;
+        const int common_last = p.by_group.quotient(tile_row0) + u.len - p.q_len;
+        const int common_before = p.by_group.quotient(min(tile_row0 + kBlockQ, p.rows) - 1) + u.len - p.q_len - p.window;
         float m_used = -INFINITY;
         float l_run = 0.0f;
         for (int j = 0; j < my_blocks && ok; ++j) {
@@ -531,7 +535,7 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
               q_phase ^= 1u << q;
               mbar_arrive_expect_tx(&t.q_full_bar[q], L::kQBytes);
               const int row = u.row0 + q * kBlockQ;
-              const int seq = p.over_batch ? row / (p.group * p.q_len) : u.seq, query = p.over_batch ? 0 : row / p.group;
+              const int seq = p.over_batch ? p.by_sequence_rows.quotient(row) : u.seq, query = p.over_batch ? 0 : p.by_group.quotient(row);
 #pragma unroll
               for (int a = 0; a < L::kQAtoms; ++a) {
                 tma_load_4d(q_tile(q) + a * kBlockQ * kAtomBytes, &tmap_q, &t.q_full_bar[q], a * kAtomBytes, u.head * p.group, query, seq);
@@ -803,6 +807,8 @@ size_t cache_tiles_part_rows(int64_t units, int splits) { return static_cast<siz
 
 cudaError_t cache_tiles(TilesParams p, const CacheAttentionArgs &a, const char **why) {
   CUtensorMap tq, maps[6];  // of q; of k and v, the same in boxes of 16 positions, of the prefix
+  p.by_runs = Divisor::of(static_cast<uint32_t>(p.runs));
+  p.by_splits = Divisor::of(static_cast<uint32_t>(p.splits));
   // A tile's rows as a box: the heads of a group, a run of queries, and over a prefix a run of sequences.
   const int per_query = p.group, per_sequence = p.group * p.q_len;
   const bool whole_queries = !p.over_batch && per_query <= kBlockQ && kBlockQ % per_query == 0;

@@ -5,6 +5,7 @@
 #include <stdint.h>
 
 #include "cache_attention_sm100.cuh"
+#include "cache_common_sm100.cuh"
 
 namespace flsm100 {
 
@@ -22,7 +23,10 @@ struct TilesParams {
   int rows;         // packed rows of a run
   int row_pairs;    // pairs of tiles of 128 of them
   int splits;       // CTAs that divide a pair's blocks of keys
-  bool q_by_tma;    // set by cache_tiles()
+  Divisor by_kv_heads, by_group, by_sequence_rows;  // (the last: group * q_len)
+  // Set by cache_tiles():
+  bool q_by_tma;
+  Divisor by_runs, by_splits;
   float scale_log2;
   float *part_out;   // (kv_head, split, rows, D) over a prefix, (run, pair, split, 256, D) else
   float2 *part_sum;  // the same without D: maximum in log2 units, sum
