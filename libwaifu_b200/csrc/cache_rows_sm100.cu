@@ -44,7 +44,8 @@ struct RowsLayout {
   static constexpr int kTileBytes = kTileKeys * kRowBytes;
   static constexpr int kStageBytes = 2 * kTileBytes;  // K and V of 16 keys
   static constexpr int kQOff = 0;
-  static constexpr int kRingOff = kMaxRows * kRowBytes;
+  static constexpr int kQBytes = kMaxRows * kRowBytes;
+  static constexpr int kRingOff = 2 * kQBytes;  // the queries of the unit that comes, and of the one behind it
   static constexpr int kSmemBytes = kRingOff + kWarps * kStages * kStageBytes;
   static_assert(kMaxRows * D * 4 == kStageBytes, "a warp's outputs fit the stage that it has read");
   static_assert(2 * (kSmemBytes + 2048) <= 227 * 1024, "two CTAs an SM");
@@ -197,9 +198,7 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
   constexpr int kQuads = D / 4;      // of a row: a thread finishes four columns at a time
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float2 warp_sum[kWarps][NB * 8];
-  __shared__ int64_t scan[kWarps];
-  __shared__ int64_t found_before;
-  __shared__ int found_seq, is_last, longest[kWarps];
+  __shared__ int is_last;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (p.prefix_splits == 0) griddep_wait();  // (behind a prefix's kernel the inputs are complete, and only its parts are waited for)
@@ -236,49 +235,43 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
       load.seq = static_cast<int>(begin / each);
       before = load.seq * each;
     } else {
-      // The steps of the whole batch, and the sequence in which this CTA's begin. Each thread has some sequences.
-      const int mine = (p.batch + kThreads - 1) / kThreads;
-      const int first = threadIdx.x * mine, last = min(first + mine, p.batch);
-      int64_t sum = 0;
+      // The steps of the whole batch, and then the sequence in which this CTA's begin: every warp for itself, a lane a sequence.
+      int64_t total = 0;
       int most = 1;
-      for (load.seq = first; load.seq < last; ++load.seq) {
+      for (load.seq = lane; load.seq < p.batch; load.seq += 32) {
         load.enter_sequence(p);
-        sum += static_cast<int64_t>(load.steps) * units;
+        total += static_cast<int64_t>(load.steps) * units;
         most = max(most, load.steps);
       }
-      int64_t upto = sum;
 #pragma unroll
       for (int x = 1; x < 32; x <<= 1) {
-        const int64_t y = __shfl_up_sync(0xffffffffu, upto, x);
-        if (lane >= x) upto += y;
+        total += __shfl_xor_sync(0xffffffffu, total, x);
         most = max(most, __shfl_xor_sync(0xffffffffu, most, x));
-      }
-      if (lane == 31) scan[warp] = upto;
-      if (lane == 0) longest[warp] = most;
-      __syncthreads();
-      before = upto - sum;
-      int64_t total = 0;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) before += scan[w];
-        total += scan[w];
-        most = max(most, longest[w]);
       }
       deal_out(total, most);
       if (count == 0) return;
-      if (before <= begin && begin < before + sum) {
-        for (load.seq = first;; ++load.seq) {
+      for (int first = 0;; first += 32) {
+        load.seq = first + lane;
+        int64_t here = 0;
+        if (load.seq < p.batch) {
           load.enter_sequence(p);
-          const int64_t here = static_cast<int64_t>(load.steps) * units;
-          if (begin < before + here) break;
-          before += here;
+          here = static_cast<int64_t>(load.steps) * units;
         }
-        found_seq = load.seq;
-        found_before = before;
+        int64_t upto = here;
+#pragma unroll
+        for (int x = 1; x < 32; x <<= 1) {
+          const int64_t y = __shfl_up_sync(0xffffffffu, upto, x);
+          if (lane >= x) upto += y;
+        }
+        const uint32_t past = __ballot_sync(0xffffffffu, before + upto > begin);
+        if (past != 0) {
+          const int at = __ffs(static_cast<int>(past)) - 1;
+          before += __shfl_sync(0xffffffffu, upto - here, at);
+          load.seq = first + at;
+          break;
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
       }
-      __syncthreads();
-      load.seq = found_seq;
-      before = found_before;
     }
     load.enter_sequence(p);
     const int64_t in_seq = begin - before;
@@ -299,8 +292,32 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
     v_base = p.v + load.head * p.v_stride[1] + (p.over_batch ? 0 : load.seq * p.v_stride[0]) + lane_piece * 8;
   };
   find_unit();
+  // The queries of the unit that is loaded come with its first tile, eight rows or sixteen by all threads.
+  int load_unit = 0;
+  auto load_queries = [&]() {
+    constexpr int kCopies = kRows * kPieces;
+#pragma unroll
+    for (int i = 0; i < (kCopies + kThreads - 1) / kThreads; ++i) {
+      const int c = i * kThreads + threadIdx.x, in_tile = c / kPieces, piece = c % kPieces;
+      if (kCopies % kThreads != 0 && c >= kCopies) break;
+      const int r = load.tile * kRows + in_tile;
+      int n = load.seq, q = min(r, p.rows - 1);
+      if (p.over_batch) {
+        n = q;
+        q = p.by_sequence_rows.take(&n);
+      }
+      const int g = p.by_group.take(&q);
+      cp_async_16(smem + L::kQOff + (load_unit & 1) * L::kQBytes + piece_offset<D>(in_tile, piece),
+                  p.q + n * p.q_stride[0] + static_cast<int64_t>(load.head * p.group + g) * p.q_stride[1] + q * p.q_stride[2] + piece * 8,
+                  r < p.rows ? 16 : 0);
+    }
+    ++load_unit;
+  };
+  bool load_begins = true;
   auto load_tile = [&]() {
     if (loaded < count) {
+      if (load_begins) load_queries();
+      load_begins = false;
       uint8_t *dst = ring + load_stage * L::kStageBytes;
       const int at0 = (load.step * kWarps + warp) * kTileKeys, total = load.range.count();
       if (at0 + kTileKeys <= total && (at0 >= load.range.sinks || at0 + kTileKeys <= load.range.sinks)) {  // one run of keys
@@ -327,42 +344,15 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
       }
       ++loaded;
       load_stage = load_stage + 1 == kStages ? 0 : load_stage + 1;
-      if (loaded < count && load.advance(p)) find_unit();
+      if (loaded < count && load.advance(p)) {
+        find_unit();
+        load_begins = true;
+      }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 #pragma unroll
   for (int s = 0; s < kStages - 1; ++s) load_tile();
-
-  // ---- the queries of a unit: eight threads a row
-  constexpr int kMyPieces = kPieces / 8;
-  auto fetch_queries = [&](const Cursor &u, uint4 (&x)[kMyPieces]) {
-    const int r = u.tile * kRows + (threadIdx.x >> 3);
-#pragma unroll
-    for (int c = 0; c < kMyPieces; ++c) x[c] = make_uint4(0, 0, 0, 0);
-    if ((threadIdx.x >> 3) < kRows && r < p.rows) {
-      int n = u.seq, in_seq = r;
-      if (p.over_batch) {
-        n = in_seq;
-        in_seq = p.by_sequence_rows.take(&n);
-      }
-      int i = in_seq;
-      const int g = p.by_group.take(&i);
-      const uint16_t *src = p.q + n * p.q_stride[0] + static_cast<int64_t>(u.head * p.group + g) * p.q_stride[1] + i * p.q_stride[2];
-#pragma unroll
-      for (int c = 0; c < kMyPieces; ++c) x[c] = *reinterpret_cast<const uint4 *>(src + ((threadIdx.x & 7) + 8 * c) * 8);
-    }
-  };
-  auto stage_queries = [&](const uint4 (&x)[kMyPieces]) {
-#pragma unroll
-    for (int c = 0; c < kMyPieces; ++c) *reinterpret_cast<uint4 *>(smem + L::kQOff + piece_offset<D>(threadIdx.x >> 3, (threadIdx.x & 7) + 8 * c)) = x[c];
-  };
-  {
-    uint4 x[kMyPieces];
-    fetch_queries(at, x);
-    stage_queries(x);
-  }
-  __syncthreads();
 
   // Of the fragments of S^T and O^T this lane has the rows (keys, columns) lane / 4 and + 8, and of every eight query rows
   // the two from my_row on.
@@ -372,16 +362,19 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
   float m[NB][2], l[NB][2];
   int first_pos, last_pos, pos[NB][2];  // of the tile's rows, and of this thread's
   int unit_step;                        // the first step that this CTA takes of the unit
+  int begun = 0;
   auto begin_unit = [&]() {
+    const uint8_t *queries = smem + L::kQOff + (begun & 1) * L::kQBytes;
+    ++begun;
 #pragma unroll
     for (int s = 0; s < D / 16; ++s) {
       if constexpr (NB == 2) {
         uint32_t b[4];
-        ldmatrix_x4(b, smem_u32(smem + L::kQOff + piece_offset<D>((lane & 7) + ((lane >> 4) << 3), 2 * s + ((lane >> 3) & 1))));
+        ldmatrix_x4(b, smem_u32(queries + piece_offset<D>((lane & 7) + ((lane >> 4) << 3), 2 * s + ((lane >> 3) & 1))));
         qf[s][0][0] = b[0], qf[s][0][1] = b[1], qf[s][NB - 1][0] = b[2], qf[s][NB - 1][1] = b[3];
       } else if ((s & 1) == 0) {
         uint32_t b[4];
-        ldmatrix_x4(b, smem_u32(smem + L::kQOff + piece_offset<D>(lane & 7, 2 * s + (lane >> 3))));
+        ldmatrix_x4(b, smem_u32(queries + piece_offset<D>(lane & 7, 2 * s + (lane >> 3))));
         qf[s][0][0] = b[0], qf[s][0][1] = b[1], qf[s + 1][0][0] = b[2], qf[s + 1][0][1] = b[3];
       }
     }
@@ -408,8 +401,9 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
     unit_step = at.step;
   };
   auto sees = [&](int key, int pos) { return p.over_batch || (key <= pos && (key > pos - p.window || key < p.sinks)); };
+  cp_async_wait_group<kStages - 2>();
+  __syncthreads();  // the first unit's queries are there
   begin_unit();
-  __syncthreads();  // the queries have been read
 
   int stage = 0;
   for (int done = 0; done < count; ++done) {
@@ -560,8 +554,6 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
 
     // ---- the end of the unit, or of this CTA's part of it. The four warps' outputs meet over the stages that they
     // have just read, which no load fills before the next step's turn.
-    uint4 next_queries[kMyPieces];
-    if (done + 1 < count) fetch_queries(at, next_queries);
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
 #pragma unroll
@@ -583,7 +575,7 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
         }
       }
     }
-    if (done + 1 < count) stage_queries(next_queries);
+    cp_async_wait_group<kStages - 2>();  // the next unit's queries, with its first tile
     __syncthreads();
 
     const int row0 = unit.tile * kRows, live = min(kRows, p.rows - row0);
@@ -659,7 +651,7 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
     }
     if (done + 1 < count) {
       begin_unit();
-      __syncthreads();  // the stages have been read, and the queries
+      __syncthreads();  // the stages have been read
     }
   }
 }
