@@ -128,8 +128,9 @@ struct RowsParams {
   const float *prefix_out;
   const float2 *prefix_sum;
   int prefix_splits, prefix_rows;
-  // For the keys' weights: the scores (batch * kv_heads, rows, kv_len) in log2 units and each row's maximum and 1 / sum.
+  // For the keys' weights: the scores (batch * kv_heads, rows, score_pitch) in log2 units and each row's maximum and 1 / sum.
   float *scores;
+  int64_t score_pitch;
   float2 *row_norm;
 };
 
@@ -447,13 +448,13 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
       }
       if (p.scores != nullptr) {  // (no window there: a key's place is the key)
         const int row0 = at.tile * kRows;
-        float *dst = p.scores + ((static_cast<int64_t>(at.seq) * p.kv_heads + at.head) * p.rows + row0) * p.kv_len + at0 + my_key;
+        float *dst = p.scores + ((static_cast<int64_t>(at.seq) * p.kv_heads + at.head) * p.rows + row0) * p.score_pitch + at0 + my_key;
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int row = n * 8 + my_row + (i & 1);
-            if (at0 + (i >> 1) * 8 + my_key < total && row0 + row < p.rows) dst[row * static_cast<int64_t>(p.kv_len) + (i >> 1) * 8] = sc[n][i];
+            if (at0 + (i >> 1) * 8 + my_key < total && row0 + row < p.rows) dst[row * p.score_pitch + (i >> 1) * 8] = sc[n][i];
           }
         }
       }
@@ -656,28 +657,51 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
   }
 }
 
-// weights_out = weights_in + the sum over the rows of a key-value head of exp2(score - maximum) / sum.
-__global__ void __launch_bounds__(256) add_weights_kernel(const float *__restrict__ scores, const float2 *__restrict__ row_norm, int rows,
-                                                          int group, int q_len, int kv_len, int kv_heads, const int32_t *kv_lens,
-                                                          const float *weights_in, int64_t in_seq, int64_t in_head, float *weights_out,
-                                                          int64_t out_seq, int64_t out_head) {
+constexpr int kKeysAtOnce = 4;  // of a thread
+constexpr int kAddThreads = 128;
+
+// weights_out = weights_in + the sum over the rows of a key-value head of exp2(score - maximum) / sum, in the order of the rows.
+__global__ void __launch_bounds__(kAddThreads) add_weights_kernel(const float *scores, int64_t score_pitch, const float2 *row_norm, int rows,
+                                                                  Divisor by_chunks, Divisor by_kv_heads, int group, int q_len, int kv_len,
+                                                                  const int32_t *kv_lens, const float *weights_in, int64_t in_seq,
+                                                                  int64_t in_head, float *weights_out, int64_t out_seq, int64_t out_head) {
   griddep_wait();
   griddep_launch_dependents();
-  const int chunks = (kv_len + 255) / 256;
-  const int run = blockIdx.x / chunks, seq = run / kv_heads, head = run % kv_heads;
-  const int key = (blockIdx.x % chunks) * 256 + threadIdx.x;
+  int run = blockIdx.x;
+  const int key = (by_chunks.take(&run) * kAddThreads + threadIdx.x) * kKeysAtOnce;
   if (key >= kv_len) return;
+  int seq = run;
+  const int head = by_kv_heads.take(&seq);
+  const float *in = weights_in + seq * in_seq + head * in_head + key;
+  float *out = weights_out + seq * out_seq + head * out_head + key;
+  float before[kKeysAtOnce], sum[kKeysAtOnce] = {};
+#pragma unroll
+  for (int k = 0; k < kKeysAtOnce; ++k) before[k] = key + k < kv_len ? in[k] : 0.0f;
   const int len = sequence_length(kv_lens, seq, kv_len);
-  float sum = 0.0f;
   if (key < len) {
-    // The first query at or behind the key's own position.
-    const int first = max(0, key - len + q_len) * group;
+    // Query i sees the keys up to i + len - q_len; the rows' scores of others were not written.
+    const float *score = scores + static_cast<int64_t>(run) * rows * score_pitch + key;
+    const int offset = len - q_len, first = max(0, key - offset) * group;
+    int query = max(0, key - offset), in_query = 0;
+#pragma unroll 4
     for (int r = first; r < rows; ++r) {
       const float2 norm = row_norm[static_cast<int64_t>(run) * rows + r];
-      sum += exp2f(scores[(static_cast<int64_t>(run) * rows + r) * kv_len + key] - norm.x) * norm.y;
+      const float4 s = *reinterpret_cast<const float4 *>(score + r * score_pitch);
+      const float each[kKeysAtOnce] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+      for (int k = 0; k < kKeysAtOnce; ++k) {
+        if (key + k <= query + offset) sum[k] += exp2f(each[k] - norm.x) * norm.y;
+      }
+      if (++in_query == group) {
+        in_query = 0;
+        ++query;
+      }
     }
   }
-  weights_out[seq * out_seq + head * out_head + key] = weights_in[seq * in_seq + head * in_head + key] + sum;
+#pragma unroll
+  for (int k = 0; k < kKeysAtOnce; ++k) {
+    if (key + k < kv_len) out[k] = before[k] + sum[k];
+  }
 }
 
 constexpr int kCtasPerSm = 2;
@@ -694,6 +718,8 @@ size_t round_256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
 // From so many packed rows of a key-value head on a run takes the tiles of the tensor cores: up to there the tiles of 16
 // rows read the keys again from L2 at most three times.
 constexpr int kTilesFromRows = 64;
+
+int64_t score_pitch_of(int kv_len) { return (static_cast<int64_t>(kv_len) + kKeysAtOnce - 1) / kKeysAtOnce * kKeysAtOnce; }
 
 int tile_rows_of(int rows) { return rows <= 8 ? 8 : 16; }
 
@@ -767,7 +793,7 @@ CachePlan cache_plan(const CacheAttentionArgs &a) {
     p.row_norm = take(static_cast<size_t>(runs) * group * cache_weights_norm_pitch(a.q_len) * 8);
     p.scores = take(p.weights.part_bytes);
   } else if (a.weights_out != nullptr) {
-    p.scores = take(static_cast<size_t>(runs) * p.rows * a.kv_len * 4);
+    p.scores = take(static_cast<size_t>(runs) * p.rows * score_pitch_of(a.kv_len) * 4);
     p.row_norm = take(static_cast<size_t>(runs) * p.rows * 8);
   }
   p.bytes = at;
@@ -904,6 +930,7 @@ cudaError_t cache_attention(const CacheAttentionArgs &a, const char **why, int *
   p.part_sum = pairs(plan.part_sum);
   if (a.weights_out != nullptr) {
     p.scores = floats(plan.scores);
+    p.score_pitch = score_pitch_of(a.kv_len);
     p.row_norm = pairs(plan.row_norm);
   }
   if (plan.prefix_apart) {
@@ -949,8 +976,10 @@ cudaError_t cache_attention(const CacheAttentionArgs &a, const char **why, int *
   }
   ++*launches;
   if (a.weights_out != nullptr) {
-    const int64_t ctas = (static_cast<int64_t>(a.kv_len) + 255) / 256 * a.batch * a.kv_heads;
-    e = launch_overlapped(add_weights_kernel, ctas, 256, 0, a.stream, p.scores, p.row_norm, p.rows, p.group, a.q_len, a.kv_len, a.kv_heads, a.kv_lens,
+    constexpr int kPerCta = kAddThreads * kKeysAtOnce;
+    const int chunks = (a.kv_len + kPerCta - 1) / kPerCta;
+    e = launch_overlapped(add_weights_kernel, static_cast<int64_t>(chunks) * a.batch * a.kv_heads, kAddThreads, 0, a.stream, p.scores, p.score_pitch,
+                          p.row_norm, p.rows, Divisor::of(static_cast<uint32_t>(chunks)), p.by_kv_heads, p.group, a.q_len, a.kv_len, a.kv_lens,
                           a.weights_in, a.weights_in_stride[0], a.weights_in_stride[1], a.weights_out, a.weights_out_stride[0],
                           a.weights_out_stride[1]);
     if (e != cudaSuccess) {

@@ -78,11 +78,26 @@ struct Unit {
     first = part * p.part_blocks;
     count = max(0, min(p.part_blocks, total - first));
   }
-  __device__ __forceinline__ int query0(int b) const { return (first_block + (first + b) % per_head) * kBlockQ; }
-  __device__ __forceinline__ int group_head(int b) const { return (first + b) / per_head; }
-  // Does a query of block b see a key of tile i?
-  __device__ __forceinline__ bool meets(int b, int i) const {
-    return key0 + i * kBlockKv < len && query0(b) + kBlockQ - 1 + offset >= key0 + i * kBlockKv;
+  // Does a query of the block from query0 on see a key of tile i?
+  __device__ __forceinline__ bool meets(int query0, int i) const {
+    return key0 + i * kBlockKv < len && query0 + kBlockQ - 1 + offset >= key0 + i * kBlockKv;
+  }
+};
+
+// Where a role's walk over a part's blocks stands.
+struct Place {
+  int head, query0, end;
+  __device__ __forceinline__ explicit Place(const Unit &u) {
+    head = u.per_head > 0 ? u.first / u.per_head : 0;
+    query0 = (u.first_block + u.first - head * u.per_head) * kBlockQ;
+    end = (u.first_block + u.per_head) * kBlockQ;
+  }
+  __device__ __forceinline__ void advance(const Unit &u) {
+    query0 += kBlockQ;
+    if (query0 == end) {
+      query0 = u.first_block * kBlockQ;
+      ++head;
+    }
   }
 };
 
@@ -145,11 +160,12 @@ cache_weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     float sum = 0.0f;
     bool ok = true;
     int met = 0;
-    for (int b = 0; b < u.count && ok; ++b) {
+    Place at(u);
+    for (int b = 0; b < u.count && ok; ++b, at.advance(u)) {
       const int st = b % S;
       ok = __all_sync(0xffffffffu, mbar_wait(&t.slot_full_bar[st], (b / S) & 1, &abort_flag));
       if (!ok) break;
-      if (u.meets(b, tile)) {
+      if (u.meets(at.query0, tile)) {
         ok = __all_sync(0xffffffffu, mbar_wait(&t.s_full_bar[tile][met & 1], (met >> 1) & 1, &abort_flag));
         if (!ok) break;
         tc_fence_after_sync();
@@ -164,7 +180,7 @@ cache_weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         if (lane == 0) mbar_arrive(&t.s_empty_bar[tile][met & 1]);
         ++met;
         const float4 *norm = reinterpret_cast<const float4 *>(smem + L::kNormsOff + st * kNormBytes);  // two queries each
-        const int query0 = u.query0(b);
+        const int query0 = at.query0;
         float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         if (query0 + u.offset >= tile_last && query0 + kBlockQ <= p.q_len) {  // every query of the block sees every key of the tile
 #pragma unroll
@@ -237,13 +253,14 @@ cache_weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
           }
         }
       }
-      for (int b = 0; b < u.count && ok; ++b) {
+      Place at(u);
+      for (int b = 0; b < u.count && ok; ++b, at.advance(u)) {
         const int st = b % S;
         if (!mbar_wait(&t.slot_empty_bar[st], ((b / S) & 1) ^ 1, &abort_flag)) {
           ok = false;
           break;
         }
-        const int g = u.group_head(b), query0 = u.query0(b);
+        const int g = at.head, query0 = at.query0;
         mbar_arrive_expect_tx(&t.slot_full_bar[st], L::kSlotBytes);
 #pragma unroll
         for (int a = 0; a < L::kQAtoms; ++a) {
@@ -266,13 +283,14 @@ cache_weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     const uint64_t qdesc0 = umma_desc_sw128(smem_u32(smem + L::kQueriesOff));
     bool ok = u.count == 0 || mbar_wait(&t.k_full_bar, 0, &abort_flag);
     int met[kTiles] = {0, 0};
-    for (int b = 0; b < u.count && ok; ++b) {
+    Place at(u);
+    for (int b = 0; b < u.count && ok; ++b, at.advance(u)) {
       const int st = b % S;
       ok = mbar_wait(&t.slot_full_bar[st], (b / S) & 1, &abort_flag);
       const uint64_t qd = qdesc0 + static_cast<uint64_t>(st * (L::kQBytes >> 4));
 #pragma unroll
       for (int i = 0; i < kTiles; ++i) {
-        if (!ok || !u.meets(b, i)) continue;
+        if (!ok || !u.meets(at.query0, i)) continue;
         ok = mbar_wait(&t.s_empty_bar[i][met[i] & 1], ((met[i] >> 1) & 1) ^ 1, &abort_flag);
         if (!ok) continue;
         tc_fence_after_sync();
@@ -322,12 +340,30 @@ WeightsPlan cache_weights_plan(const CacheAttentionArgs &a, int most_units) {
   WeightsPlan plan;
   const int64_t runs = static_cast<int64_t>(a.batch) * a.kv_heads;
   plan.pairs = (a.kv_len + kKeysPerCta - 1) / kKeysPerCta;
-  const int64_t longest = static_cast<int64_t>(a.heads / a.kv_heads) * ((a.q_len + kBlockQ - 1) / kBlockQ);  // blocks of the first keys' walk
+  const int query_blocks = (a.q_len + kBlockQ - 1) / kBlockQ, group = a.heads / a.kv_heads;
+  const int64_t longest = static_cast<int64_t>(group) * query_blocks;  // blocks of the first keys' walk
   plan.part_blocks = static_cast<int>(longest);
   if (runs * plan.pairs <= most_units) {
-    // About two CTAs an SM over all walks, were they as long as the longest; eight blocks each at least.
-    const int64_t blocks = (runs * plan.pairs * longest + 2 * sm_count() - 1) / (2 * sm_count());
-    plan.part_blocks = static_cast<int>(std::min<int64_t>(longest, std::max<int64_t>(8, blocks)));
+    // The shortest parts (eight blocks at least) of which there are no more than SMs, for sequences that fill the cache: one
+    // round of CTAs (2 x 4 runs of 2048 keys and queries: parts of 14 blocks in three rounds 53 us, of 20 in one 31).
+    auto parts_of = [&](int64_t part) {
+      int64_t sum = 0;
+      for (int pair = 0; pair < plan.pairs; ++pair) {
+        const int64_t first = std::max<int64_t>(0, static_cast<int64_t>(pair) * kKeysPerCta - (a.kv_len - a.q_len)) / kBlockQ;
+        sum += (group * std::max<int64_t>(0, query_blocks - first) + part - 1) / part;
+      }
+      return sum * runs;
+    };
+    int64_t low = std::min<int64_t>(8, longest), high = longest;
+    while (low < high) {
+      const int64_t middle = (low + high) / 2;
+      if (parts_of(middle) <= sm_count()) {
+        high = middle;
+      } else {
+        low = middle + 1;
+      }
+    }
+    plan.part_blocks = static_cast<int>(low);
   }
   plan.parts = static_cast<int>((longest + plan.part_blocks - 1) / plan.part_blocks);
   plan.part_bytes = plan.parts > 1 ? static_cast<size_t>(runs) * plan.pairs * plan.parts * kKeysPerCta * 4 : 0;
