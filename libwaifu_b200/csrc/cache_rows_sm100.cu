@@ -121,10 +121,14 @@ struct RowsParams {
   int rows;       // packed rows of a key-value head: group * q_len, times the batch over a prefix
   int row_tiles;  // of 8 or 16
   int splits;     // over a prefix: CTAs that divide a unit
+  int ctas;       // else: CTAs that the steps are dealt out to
   float *part_out;   // (CTA, 2, rows of a tile, D): a unit's end, and a unit's beginning; (kv_head, split, rows, D) over a prefix
   float2 *part_sum;  // the same without D: maximum in log2 units, sum
   uint32_t *counters;  // of the unit that the CTA's last run of steps begins
-  // The parts over the prefix that an earlier kernel left, as above; 0 splits without.
+  // Behind a prefix's tile kernel, which a third kernel joins with this one: a row's output and sum, (batch * kv_heads, rows, D).
+  float *own_out;
+  float2 *own_sum;
+  // The parts over the prefix that an earlier kernel of few rows left, as above; 0 splits without.
   const float *prefix_out;
   const float2 *prefix_sum;
   int prefix_splits, prefix_rows;
@@ -202,8 +206,13 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
   __shared__ int is_last;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (p.prefix_splits == 0) griddep_wait();  // (behind a prefix's kernel the inputs are complete, and only its parts are waited for)
+  // (Behind a prefix's kernel the inputs are complete: only its parts are waited for.)
+  if (p.prefix_splits == 0 && p.own_out == nullptr) griddep_wait();
   griddep_launch_dependents();
+  if (static_cast<int>(blockIdx.x) == p.ctas) {  // the kernel that joins the two waits for this one: so this one ends behind the prefix's
+    griddep_wait();
+    return;
+  }
 
   // ---- this CTA's run of steps
   Cursor load;
@@ -222,7 +231,7 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
     const int units = p.kv_heads * p.row_tiles;
     // Four steps each at least, or one unit where they are shorter.
     auto deal_out = [&](int64_t total, int most) {
-      per_cta = max((total + gridDim.x - 1) / gridDim.x, static_cast<int64_t>(min(kLeastSteps, most)));
+      per_cta = max((total + p.ctas - 1) / p.ctas, static_cast<int64_t>(min(kLeastSteps, most)));
       begin = blockIdx.x * per_cta;
       count = static_cast<int>(max(static_cast<int64_t>(0), min(per_cta, total - begin)));
     };
@@ -637,6 +646,12 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
           add_parts<D>(p.prefix_splits, p.prefix_sum, p.prefix_out, col, &sum,
                        [&](int c) { return first + static_cast<int64_t>(c) * p.prefix_rows; });
         }
+        if (p.own_out != nullptr) {
+          const int64_t row = (static_cast<int64_t>(unit.seq) * p.kv_heads + unit.head) * p.rows + row0 + r;
+          *reinterpret_cast<float4 *>(p.own_out + row * D + col) = sum.o;
+          if (col == 0) p.own_sum[row] = make_float2(sum.m, sum.l);
+          continue;
+        }
         int q = row0 + r;
         const int g = p.by_group.take(&q);
         // A query that sees no key: zeros. (Where it sees some and their exponentials sum to zero or to NaN, that is its result.)
@@ -655,6 +670,44 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
       __syncthreads();  // the stages have been read
     }
   }
+}
+
+struct JoinParams {
+  const float *own_out, *prefix_out;
+  const float2 *own_sum, *prefix_sum;
+  uint16_t *out;
+  int64_t out_stride[3];
+  Divisor by_rows, by_kv_heads, by_group;
+  int rows, prefix_rows, prefix_splits, group;
+  int64_t total;  // rows of all runs times the fours of a row's columns
+};
+
+// A row's own part and its parts over the prefix, in their order: four columns a thread.
+template <int D, bool BF16>
+__global__ void __launch_bounds__(128) join_prefix_kernel(const __grid_constant__ JoinParams p) {
+  griddep_wait();
+  griddep_launch_dependents();
+  constexpr int kQuads = D / 4;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 128 + threadIdx.x;
+  if (at >= p.total) return;
+  const int col = static_cast<int>(at % kQuads) * 4;
+  const int row = static_cast<int>(at / kQuads);
+  int run = row;
+  const int r = p.by_rows.take(&run);
+  int seq = run;
+  const int head = p.by_kv_heads.take(&seq);
+  RowSum sum;
+  sum.clear();
+  const float2 own = p.own_sum[row];
+  sum.raise(own.x);
+  sum.add(own, *reinterpret_cast<const float4 *>(p.own_out + static_cast<int64_t>(row) * D + col));
+  const int64_t first = static_cast<int64_t>(head) * p.prefix_splits * p.prefix_rows + static_cast<int64_t>(seq) * p.rows + r;
+  add_parts<D>(p.prefix_splits, p.prefix_sum, p.prefix_out, col, &sum, [&](int c) { return first + static_cast<int64_t>(c) * p.prefix_rows; });
+  const float inv = 1.0f / sum.l;
+  int q = r;
+  const int g = p.by_group.take(&q);
+  *reinterpret_cast<uint2 *>(p.out + seq * p.out_stride[0] + static_cast<int64_t>(head * p.group + g) * p.out_stride[1] + q * p.out_stride[2] + col) =
+      make_uint2(pack_pair<BF16>(sum.o.x * inv, sum.o.y * inv), pack_pair<BF16>(sum.o.z * inv, sum.o.w * inv));
 }
 
 constexpr int kKeysAtOnce = 4;  // of a thread
@@ -721,6 +774,11 @@ constexpr int kTilesFromRows = 64;
 
 int64_t score_pitch_of(int kv_len) { return (static_cast<int64_t>(kv_len) + kKeysAtOnce - 1) / kKeysAtOnce * kKeysAtOnce; }
 
+// The least blocks of 128 keys of a prefix that are worth a CTA of the tile kernel: a CTA of four takes some 11 us to begin and
+// to write its parts, and 2.3 us a block, while the kernel over the own keys has the other SMs (64 sequences behind 8192
+// keys: parts of four blocks 60 us, of eight 50; of sixteen 72 before the two overlapped).
+constexpr int kPrefixBlocks = 8;
+
 int tile_rows_of(int rows) { return rows <= 8 ? 8 : 16; }
 
 // Which kernels a call takes, and its workspace.
@@ -735,6 +793,7 @@ struct CachePlan {
   bool prefix_tiles;
   int prefix_rows, prefix_tile_rows, prefix_row_tiles, prefix_splits;
   WeightsPlan weights;  // with `tiles`
+  size_t own_out, own_sum;  // with `prefix_tiles`
   size_t part_out, part_sum, prefix_out, prefix_sum, scores, row_norm, bytes;  // (scores: or the sums of their parts)
 };
 
@@ -756,13 +815,15 @@ CachePlan cache_plan(const CacheAttentionArgs &a) {
   size_t part_rows = 0;
   if (p.tiles) {
     p.row_tiles = cache_tiles_pairs(p.rows);
-    p.splits = cache_tiles_splits(runs * p.row_tiles, static_cast<int>(std::min<int64_t>(most + a.prefix_len, INT32_MAX)), kCacheCounters);
+    p.splits = cache_tiles_splits(runs * p.row_tiles, static_cast<int>(std::min<int64_t>(most + a.prefix_len, INT32_MAX)), kCacheCounters, 4);
     part_rows = p.splits > 1 ? cache_tiles_part_rows(runs * p.row_tiles, p.splits) : 0;
   } else {
     p.tile_rows = tile_rows_of(p.rows);
     p.row_tiles = (p.rows + p.tile_rows - 1) / p.tile_rows;
     const int64_t steps = (most + kStepKeys - 1) / kStepKeys, least = std::min<int64_t>(kLeastSteps, steps);  // of a unit, and of a CTA
-    p.ctas = static_cast<int>(std::min<int64_t>(kCtasPerSm * sm_count(), (runs * p.row_tiles * steps + least - 1) / least));
+    // (beside a prefix's tile kernel, whose CTAs hold their SMs for a while, in two rounds: the SMs it leaves free take more of them)
+    const bool beside_tiles = a.prefix_len > 0 && static_cast<int64_t>(a.batch) * p.rows >= kTilesFromRows;
+    p.ctas = static_cast<int>(std::min<int64_t>((beside_tiles ? 2 : 1) * kCtasPerSm * sm_count(), (runs * p.row_tiles * steps + least - 1) / least));
     part_rows = static_cast<size_t>(p.ctas) * 2 * p.tile_rows;
   }
   if (part_rows > 0) {
@@ -774,8 +835,10 @@ CachePlan cache_plan(const CacheAttentionArgs &a) {
     p.prefix_rows = a.batch * p.rows;
     p.prefix_tiles = p.prefix_rows >= kTilesFromRows;
     if (p.prefix_tiles) {
+      p.own_out = take(static_cast<size_t>(runs) * p.rows * d * 4);
+      p.own_sum = take(static_cast<size_t>(runs) * p.rows * 8);
       p.prefix_row_tiles = cache_tiles_pairs(p.prefix_rows);
-      p.prefix_splits = cache_tiles_splits(static_cast<int64_t>(a.kv_heads) * p.prefix_row_tiles, a.prefix_len, INT32_MAX);
+      p.prefix_splits = cache_tiles_splits(static_cast<int64_t>(a.kv_heads) * p.prefix_row_tiles, a.prefix_len, INT32_MAX, kPrefixBlocks);
     } else {
       p.prefix_tile_rows = tile_rows_of(p.prefix_rows);
       p.prefix_row_tiles = (p.prefix_rows + p.prefix_tile_rows - 1) / p.prefix_tile_rows;
@@ -926,6 +989,7 @@ cudaError_t cache_attention(const CacheAttentionArgs &a, const char **why, int *
   p.row_tiles = plan.row_tiles;
   p.by_row_tiles = Divisor::of(static_cast<uint32_t>(p.row_tiles));
   p.batch = a.batch;
+  p.ctas = plan.ctas;
   p.part_out = floats(plan.part_out);
   p.part_sum = pairs(plan.part_sum);
   if (a.weights_out != nullptr) {
@@ -957,6 +1021,7 @@ cudaError_t cache_attention(const CacheAttentionArgs &a, const char **why, int *
       s.row_tiles = plan.prefix_row_tiles;
       s.by_row_tiles = Divisor::of(static_cast<uint32_t>(s.row_tiles));
       s.splits = plan.prefix_splits;
+      s.ctas = INT32_MAX;
       s.part_out = floats(plan.prefix_out);
       s.part_sum = pairs(plan.prefix_sum);
       *why = "launching the prefix's part";
@@ -964,17 +1029,47 @@ cudaError_t cache_attention(const CacheAttentionArgs &a, const char **why, int *
     }
     if (e != cudaSuccess) return e;
     ++*launches;
-    p.prefix_out = floats(plan.prefix_out);
-    p.prefix_sum = pairs(plan.prefix_sum);
-    p.prefix_splits = plan.prefix_splits;
-    p.prefix_rows = plan.prefix_rows;
+    if (plan.prefix_tiles) {
+      p.own_out = floats(plan.own_out);
+      p.own_sum = pairs(plan.own_sum);
+    } else {
+      p.prefix_out = floats(plan.prefix_out);
+      p.prefix_sum = pairs(plan.prefix_sum);
+      p.prefix_splits = plan.prefix_splits;
+      p.prefix_rows = plan.prefix_rows;
+    }
   }
-  e = launch_rows(a, p, plan.tile_rows, plan.ctas);
+  e = launch_rows(a, p, plan.tile_rows, plan.ctas + (p.own_out != nullptr ? 1 : 0));
   if (e != cudaSuccess) {
     *why = "launching the few-row kernel";
     return e;
   }
   ++*launches;
+  if (plan.prefix_apart && plan.prefix_tiles) {
+    JoinParams j = {};
+    j.own_out = p.own_out;
+    j.own_sum = p.own_sum;
+    j.prefix_out = floats(plan.prefix_out);
+    j.prefix_sum = pairs(plan.prefix_sum);
+    j.out = p.out;
+    for (int i = 0; i < 3; ++i) j.out_stride[i] = p.out_stride[i];
+    j.by_rows = Divisor::of(static_cast<uint32_t>(p.rows));
+    j.by_kv_heads = p.by_kv_heads;
+    j.by_group = p.by_group;
+    j.rows = p.rows;
+    j.prefix_rows = plan.prefix_rows;
+    j.prefix_splits = plan.prefix_splits;
+    j.group = p.group;
+    j.total = static_cast<int64_t>(a.batch) * a.kv_heads * p.rows * (a.head_dim / 4);
+    auto join = a.head_dim == 64 ? (a.is_bf16 ? join_prefix_kernel<64, true> : join_prefix_kernel<64, false>)
+                                 : (a.is_bf16 ? join_prefix_kernel<128, true> : join_prefix_kernel<128, false>);
+    e = launch_overlapped(join, (j.total + 127) / 128, 128, 0, a.stream, j);
+    if (e != cudaSuccess) {
+      *why = "launching the kernel that joins the prefix's part";
+      return e;
+    }
+    ++*launches;
+  }
   if (a.weights_out != nullptr) {
     constexpr int kPerCta = kAddThreads * kKeysAtOnce;
     const int chunks = (a.kv_len + kPerCta - 1) / kPerCta;

@@ -794,11 +794,11 @@ cudaError_t launch(const CUtensorMap &tq, const CUtensorMap (&maps)[6], const Ti
 
 int cache_tiles_pairs(int rows) { return (rows + kPairRows - 1) / kPairRows; }
 
-int cache_tiles_splits(int64_t units, int keys, int most_units) {
+int cache_tiles_splits(int64_t units, int keys, int most_units, int least_blocks) {
   const int blocks = (keys + kBlockKv - 1) / kBlockKv;
   if (units >= sm_count() || units > most_units) return 1;
-  // One CTA an SM, no more of them than SMs, four blocks each at least.
-  const int wanted = static_cast<int>(std::min<int64_t>(sm_count() / units, std::max(1, blocks / 4)));
+  // One CTA an SM, and no more of them than SMs.
+  const int wanted = static_cast<int>(std::min<int64_t>(sm_count() / units, std::max(1, blocks / least_blocks)));
   const int per_split = (blocks + wanted - 1) / wanted;
   return (blocks + per_split - 1) / per_split;
 }

@@ -37,8 +37,9 @@ struct TilesParams {
 };
 
 int cache_tiles_pairs(int rows);
-// `keys`: the most that a pair's rows see between them. At most `most_units` units may be divided.
-int cache_tiles_splits(int64_t units, int keys, int most_units);
+// `keys`: the most that a pair's rows see between them. At most `most_units` units may be divided, into parts of
+// `least_blocks` blocks of 128 keys at least.
+int cache_tiles_splits(int64_t units, int keys, int most_units, int least_blocks);
 size_t cache_tiles_part_rows(int64_t units, int splits);
 cudaError_t cache_tiles(TilesParams p, const CacheAttentionArgs &a, const char **why);
 
