@@ -141,6 +141,31 @@ struct RowSum {
   }
 };
 
+// Adds four columns of `count` parts that other CTAs wrote, part c at row place(c), in their order, eight of them on their way
+// at a time.
+template <int D, typename Place>
+__device__ __forceinline__ void add_parts(int count, const float2 *sums, const float *outs, int col, RowSum *sum, Place &&place) {
+  constexpr int kAtOnce = 8;
+  for (int c0 = 0; c0 < count; c0 += kAtOnce) {
+    float2 part[kAtOnce];
+    float4 out[kAtOnce];
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int64_t at = place(min(c0 + i, count - 1));
+      part[i] = __ldcg(&sums[at]);
+      out[i] = __ldcg(reinterpret_cast<const float4 *>(outs + at * D + col));
+    }
+    float top = part[0].x;
+#pragma unroll
+    for (int i = 1; i < kAtOnce; ++i) top = fmaxf(top, part[i].x);
+    sum->raise(top);
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      if (c0 + i < count) sum->add(part[i], out[i]);
+    }
+  }
+}
+
 // Launches a kernel that may start under the end of the one before it in the stream. Every kernel here waits for that one
 // (griddep_wait) before it reads or writes global memory, and only then lets the next one start: so whatever starts
 // early finds the inputs of the call complete. The kernels that follow another one of the same call wait where

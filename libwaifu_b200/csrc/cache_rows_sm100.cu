@@ -169,31 +169,6 @@ struct Cursor {
   }
 };
 
-// Adds four columns of `count` parts that other CTAs wrote, part c at row place(c), in their order, eight of them on their way
-// at a time.
-template <int D, typename Place>
-__device__ __forceinline__ void add_parts(int count, const float2 *sums, const float *outs, int col, RowSum *sum, Place &&place) {
-  constexpr int kAtOnce = 8;
-  for (int c0 = 0; c0 < count; c0 += kAtOnce) {
-    float2 part[kAtOnce];
-    float4 out[kAtOnce];
-#pragma unroll
-    for (int i = 0; i < kAtOnce; ++i) {
-      const int64_t at = place(min(c0 + i, count - 1));
-      part[i] = __ldcg(&sums[at]);
-      out[i] = __ldcg(reinterpret_cast<const float4 *>(outs + at * D + col));
-    }
-    float top = part[0].x;
-#pragma unroll
-    for (int i = 1; i < kAtOnce; ++i) top = fmaxf(top, part[i].x);
-    sum->raise(top);
-#pragma unroll
-    for (int i = 0; i < kAtOnce; ++i) {
-      if (c0 + i < count) sum->add(part[i], out[i]);
-    }
-  }
-}
-
 template <int D, bool BF16, int NB>
 __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_constant__ RowsParams p) {
   using L = RowsLayout<D>;
@@ -703,7 +678,7 @@ __global__ void __launch_bounds__(128) join_prefix_kernel(const __grid_constant_
   sum.add(own, *reinterpret_cast<const float4 *>(p.own_out + static_cast<int64_t>(row) * D + col));
   const int64_t first = static_cast<int64_t>(head) * p.prefix_splits * p.prefix_rows + static_cast<int64_t>(seq) * p.rows + r;
   add_parts<D>(p.prefix_splits, p.prefix_sum, p.prefix_out, col, &sum, [&](int c) { return first + static_cast<int64_t>(c) * p.prefix_rows; });
-  const float inv = 1.0f / sum.l;
+  const float inv = sum.m == -INFINITY ? NAN : 1.0f / sum.l;  // (a row whose every score is -inf has no softmax)
   int q = r;
   const int g = p.by_group.take(&q);
   *reinterpret_cast<uint2 *>(p.out + seq * p.out_stride[0] + static_cast<int64_t>(head * p.group + g) * p.out_stride[1] + q * p.out_stride[2] + col) =
@@ -814,8 +789,9 @@ CachePlan cache_plan(const CacheAttentionArgs &a) {
   const int64_t runs = static_cast<int64_t>(a.batch) * a.kv_heads;
   size_t part_rows = 0;
   if (p.tiles) {
+    most = std::min<int64_t>(a.kv_len, static_cast<int64_t>(a.window) + a.sinks + std::min(a.q_len, cache_tiles_positions(group)));
     p.row_tiles = cache_tiles_pairs(p.rows);
-    p.splits = cache_tiles_splits(runs * p.row_tiles, static_cast<int>(std::min<int64_t>(most + a.prefix_len, INT32_MAX)), kCacheCounters, 4);
+    p.splits = cache_tiles_splits(runs * p.row_tiles, static_cast<int>(std::min<int64_t>(most + a.prefix_len, INT32_MAX)), 4);
     part_rows = p.splits > 1 ? cache_tiles_part_rows(runs * p.row_tiles, p.splits) : 0;
   } else {
     p.tile_rows = tile_rows_of(p.rows);
@@ -838,7 +814,7 @@ CachePlan cache_plan(const CacheAttentionArgs &a) {
       p.own_out = take(static_cast<size_t>(runs) * p.rows * d * 4);
       p.own_sum = take(static_cast<size_t>(runs) * p.rows * 8);
       p.prefix_row_tiles = cache_tiles_pairs(p.prefix_rows);
-      p.prefix_splits = cache_tiles_splits(static_cast<int64_t>(a.kv_heads) * p.prefix_row_tiles, a.prefix_len, INT32_MAX, kPrefixBlocks);
+      p.prefix_splits = cache_tiles_splits(static_cast<int64_t>(a.kv_heads) * p.prefix_row_tiles, a.prefix_len, kPrefixBlocks);
     } else {
       p.prefix_tile_rows = tile_rows_of(p.prefix_rows);
       p.prefix_row_tiles = (p.prefix_rows + p.prefix_tile_rows - 1) / p.prefix_tile_rows;
@@ -927,7 +903,6 @@ void fill_params(const CacheAttentionArgs &a, Params *p) {
   p->window = a.window;
   p->sinks = a.sinks;
   p->scale_log2 = 1.4426950408889634f / sqrtf(static_cast<float>(a.head_dim));
-  p->counters = a.counters;
 }
 
 cudaError_t cache_attention(const CacheAttentionArgs &a, const char **why, int *launches) {
@@ -953,7 +928,7 @@ cudaError_t cache_attention(const CacheAttentionArgs &a, const char **why, int *
       tiles.norm_pitch = cache_weights_norm_pitch(a.q_len);
     }
     e = cache_tiles(tiles, a, why);
-    *launches += e == cudaSuccess;
+    *launches += e == cudaSuccess ? (plan.splits > 1 ? 2 : 1) : 0;
     if (e != cudaSuccess || a.weights_out == nullptr) return e;
     WeightsParams w = {};
     w.kv_lens = a.kv_lens;
@@ -988,6 +963,7 @@ cudaError_t cache_attention(const CacheAttentionArgs &a, const char **why, int *
   p.rows = plan.rows;
   p.row_tiles = plan.row_tiles;
   p.by_row_tiles = Divisor::of(static_cast<uint32_t>(p.row_tiles));
+  p.counters = a.counters;
   p.batch = a.batch;
   p.ctas = plan.ctas;
   p.part_out = floats(plan.part_out);

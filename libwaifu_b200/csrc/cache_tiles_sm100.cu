@@ -20,8 +20,9 @@
 // queries and first scores come under the last products and the output of the one before. Walks are short here (a window's,
 // a chunk's), and a unit's own start and end would be a third of them.
 //
-// Few units are divided along the keys: each CTA leaves its rows' outputs relative to their own maxima, and the last
-// one to arrive (or, over a prefix, the kernel over the sequences' own keys) adds them in the order of the splits.
+// Few units are divided along the keys: each CTA leaves its rows' outputs relative to their own maxima, and a kernel over
+// all rows adds them in the order of the splits. (The last CTA of a unit to arrive did that first: 256 rows on one SM took longer
+// than the launch.)
 #include "cache_tiles_sm100.cuh"
 
 #include <cuda_runtime.h>
@@ -62,7 +63,6 @@ struct Tail {
   uint32_t tmem_base_slot;
   uint32_t abort_flag;
   uint32_t patch_flag[2];  // the last unit of an even and of an odd count that had values taken out of a block
-  int is_last;
 };
 
 template <int D>
@@ -241,9 +241,9 @@ __device__ __noinline__ void patch_row(const TilesParams &p, int unit, int pos, 
   }
 }
 
-// A row's result, or its part of it, and what becomes of the parts of a unit that several CTAs share.
+// A row's result, or its part of it.
 template <int D>
-__device__ __forceinline__ void finish_row(const TilesParams &p, const Unit &u, Tail &t, uint32_t t_out, int row, int pos, int my_blocks, bool ok,
+__device__ __forceinline__ void finish_row(const TilesParams &p, const Unit &u, uint32_t t_out, int row, int pos, int my_blocks, bool ok,
                                            bool patch, float m_used, float l_run) {
   const bool live = row < p.rows;
   const bool parts = p.over_batch || u.active > 1;
@@ -258,7 +258,7 @@ __device__ __forceinline__ void finish_row(const TilesParams &p, const Unit &u, 
   const int in_group = p.by_group.take(&query);
   const int64_t norm_at = (static_cast<int64_t>(u.run) * p.group + in_group) * p.norm_pitch + query;
   // (a row whose every score is -inf has no softmax)
-  float inv = empty ? 0.0f : (m_used == -INFINITY ? NAN : 1.0f / l_run);
+  const float inv = empty ? 0.0f : (m_used == -INFINITY ? NAN : 1.0f / l_run);
   if (ok) {
 #pragma unroll 1
     for (int c = 0; c < D / 32; ++c) {
@@ -299,52 +299,33 @@ __device__ __forceinline__ void finish_row(const TilesParams &p, const Unit &u, 
     if (live && parts) p.part_sum[part_row0 + u.split * part_step] = make_float2(m_used, m_used == -INFINITY && l_run == l_run ? 0.0f : l_run);
     if (live && !parts && p.row_norm != nullptr) p.row_norm[norm_at] = make_float2(m_used, inv);
   }
-  if (p.over_batch || u.active == 1) return;
-  asm volatile("bar.sync 1, %0;" ::"n"(kSoftmaxWarps * 32) : "memory");
-  if (threadIdx.x == 0) {
-    __threadfence();
-    uint32_t *counter = &p.counters[u.run * p.row_pairs + u.pair];
-    const uint32_t before = atomicAdd(counter, 1u);
-    t.is_last = before + 1 == static_cast<uint32_t>(u.active);
-    if (t.is_last) *counter = 0;
-    __threadfence();
-  }
-  asm volatile("bar.sync 1, %0;" ::"n"(kSoftmaxWarps * 32) : "memory");
-  if (!t.is_last || !live) return;
-  float m = -INFINITY, l = 0.0f;
-  for (int s = 0; s < u.active; ++s) m = fmaxf(m, __ldcg(&p.part_sum[part_row0 + s * part_step]).x);
-  for (int s = 0; s < u.active; ++s) {
-    const float2 part = __ldcg(&p.part_sum[part_row0 + s * part_step]);
-    l += part.x == -INFINITY ? part.y : part.y * exp2f(part.x - m);
-  }
-  inv = empty ? 0.0f : (m == -INFINITY ? NAN : 1.0f / l);
-#pragma unroll 1
-  for (int c = 0; c < D / 32; ++c) {
-    float o[32] = {};
-    for (int s = 0; s < u.active; ++s) {
-      const float part_m = __ldcg(&p.part_sum[part_row0 + s * part_step]).x;
-      const float f = part_m == -INFINITY ? 0.0f : exp2f(part_m - m);
-      const float4 *src = reinterpret_cast<const float4 *>(p.part_out + (part_row0 + s * part_step) * D + c * 32);
-#pragma unroll
-      for (int g = 0; g < 8; ++g) {
-        const float4 x = __ldcg(src + g);
-        o[4 * g] = fmaf(x.x, f, o[4 * g]);
-        o[4 * g + 1] = fmaf(x.y, f, o[4 * g + 1]);
-        o[4 * g + 2] = fmaf(x.z, f, o[4 * g + 2]);
-        o[4 * g + 3] = fmaf(x.w, f, o[4 * g + 3]);
-      }
-    }
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      uint4 w;
-      w.x = pack16(o[g * 8 + 0] * inv, o[g * 8 + 1] * inv, p.is_bf16);
-      w.y = pack16(o[g * 8 + 2] * inv, o[g * 8 + 3] * inv, p.is_bf16);
-      w.z = pack16(o[g * 8 + 4] * inv, o[g * 8 + 5] * inv, p.is_bf16);
-      w.w = pack16(o[g * 8 + 6] * inv, o[g * 8 + 7] * inv, p.is_bf16);
-      *reinterpret_cast<uint4 *>(dst + c * 32 + g * 8) = empty ? make_uint4(0, 0, 0, 0) : w;
-    }
-  }
-  if (p.row_norm != nullptr) p.row_norm[norm_at] = make_float2(m, inv);
+}
+
+// The results of rows whose unit several CTAs shared: four columns a thread.
+template <int D, bool BF16>
+__global__ void __launch_bounds__(128) join_tiles_kernel(const __grid_constant__ TilesParams p, const Divisor by_rows, int64_t total) {
+  griddep_wait();
+  griddep_launch_dependents();
+  constexpr int kQuads = D / 4;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 128 + threadIdx.x;
+  if (at >= total) return;
+  const int col = static_cast<int>(at % kQuads) * 4;
+  int run = static_cast<int>(at / kQuads);
+  const int row = by_rows.take(&run), pair = row / kPairRows;
+  const Unit u(p, run + p.runs * p.splits * (p.row_pairs - 1 - pair));  // (its first split)
+  if (u.active == 1) return;
+  RowSum sum;
+  sum.clear();
+  const int64_t first = (static_cast<int64_t>(run) * p.row_pairs + pair) * p.splits * kPairRows + (row - u.row0);
+  add_parts<D>(u.active, p.part_sum, p.part_out, col, &sum, [&](int c) { return first + c * kPairRows; });
+  int query = row;
+  const int in_group = p.by_group.take(&query);
+  const bool empty = p.prefix_len == 0 && query + u.len - p.q_len < 0;  // sees no key: zeros
+  // (a row whose every score is -inf has no softmax)
+  const float inv = empty ? 0.0f : (sum.m == -INFINITY ? NAN : 1.0f / sum.l);
+  const uint2 w = make_uint2(pack_pair<BF16>(sum.o.x * inv, sum.o.y * inv), pack_pair<BF16>(sum.o.z * inv, sum.o.w * inv));
+  *reinterpret_cast<uint2 *>(p.out + row_offset(p, p.out_stride, u.head, u.seq, row) + col) = empty ? make_uint2(0, 0) : w;
+  if (p.row_norm != nullptr && col == 0) p.row_norm[(static_cast<int64_t>(run) * p.group + in_group) * p.norm_pitch + query] = make_float2(sum.m, inv);
 }
 
 template <int D>
@@ -477,7 +458,7 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
           tc_fence_after_sync();
         }
         const bool patch = *reinterpret_cast<volatile uint32_t *>(&t.patch_flag[count & 1]) == static_cast<uint32_t>(count);
-        finish_row<D>(p, u, t, t_out, row, pos, my_blocks, ok, patch, m_used, l_run);
+        finish_row<D>(p, u, t_out, row, pos, my_blocks, ok, patch, m_used, l_run);
         // The next unit's first product overwrites this output: it waits for probabilities that the tile's
         // four warps hand over only after these reads.
         tc_fence_before_sync();
@@ -794,9 +775,11 @@ cudaError_t launch(const CUtensorMap &tq, const CUtensorMap (&maps)[6], const Ti
 
 int cache_tiles_pairs(int rows) { return (rows + kPairRows - 1) / kPairRows; }
 
-int cache_tiles_splits(int64_t units, int keys, int most_units, int least_blocks) {
+int cache_tiles_positions(int group) { return kPairRows / group + 2; }
+
+int cache_tiles_splits(int64_t units, int keys, int least_blocks) {
   const int blocks = (keys + kBlockKv - 1) / kBlockKv;
-  if (units >= sm_count() || units > most_units) return 1;
+  if (units >= sm_count()) return 1;
   // One CTA an SM, and no more of them than SMs.
   const int wanted = static_cast<int>(std::min<int64_t>(sm_count() / units, std::max(1, blocks / least_blocks)));
   const int per_split = (blocks + wanted - 1) / wanted;
@@ -845,7 +828,13 @@ cudaError_t cache_tiles(TilesParams p, const CacheAttentionArgs &a, const char *
   if (!p.q_by_tma) tq = maps[0];
   const int64_t ctas = static_cast<int64_t>(p.runs) * p.row_pairs * p.splits;
   *why = "launching the tile kernel";
-  return a.head_dim == 64 ? launch<64>(tq, maps, p, ctas, a.stream) : launch<128>(tq, maps, p, ctas, a.stream);
+  cudaError_t e = a.head_dim == 64 ? launch<64>(tq, maps, p, ctas, a.stream) : launch<128>(tq, maps, p, ctas, a.stream);
+  if (e != cudaSuccess || p.over_batch || p.splits == 1) return e;
+  *why = "launching the kernel that adds the parts";
+  const int64_t total = static_cast<int64_t>(p.runs) * p.rows * (a.head_dim / 4);
+  auto join = a.head_dim == 64 ? (a.is_bf16 ? join_tiles_kernel<64, true> : join_tiles_kernel<64, false>)
+                               : (a.is_bf16 ? join_tiles_kernel<128, true> : join_tiles_kernel<128, false>);
+  return launch_overlapped(join, (total + 127) / 128, 128, 0, a.stream, p, Divisor::of(static_cast<uint32_t>(p.rows)), total);
 }
 
 }  // namespace flsm100

@@ -30,17 +30,17 @@ struct TilesParams {
   float scale_log2;
   float *part_out;   // (kv_head, split, rows, D) over a prefix, (run, pair, split, 256, D) else
   float2 *part_sum;  // the same without D: maximum in log2 units, sum
-  uint32_t *counters;
   float2 *row_norm;  // (run, query head of the group, norm_pitch): maximum and 1 / sum, or null
   int norm_pitch;
   uint32_t *status;
 };
 
 int cache_tiles_pairs(int rows);
-// `keys`: the most that a pair's rows see between them. At most `most_units` units may be divided, into parts of
-// `least_blocks` blocks of 128 keys at least.
-int cache_tiles_splits(int64_t units, int keys, int most_units, int least_blocks);
+int cache_tiles_positions(int group);  // the most that the rows of a pair lie on
+// `keys`: the most that a pair's rows see between them; a part has `least_blocks` blocks of 128 of them at least.
+int cache_tiles_splits(int64_t units, int keys, int least_blocks);
 size_t cache_tiles_part_rows(int64_t units, int splits);
+// Two launches where a pair's blocks are divided and the rows are not those of a whole batch over a prefix: the second adds the parts.
 cudaError_t cache_tiles(TilesParams p, const CacheAttentionArgs &a, const char **why);
 
 }  // namespace flsm100
