@@ -135,6 +135,20 @@ __device__ __forceinline__ int4 claimed_cta(const uint4 *answer) {
   return c;
 }
 
+// Zeros in the rows of `ATOMS` atoms of 128 that boxes of `rows` rows never fill: what lies there takes part in no result, but a
+// row's garbage would have its warp rescale when other garbage would not, and the results differ in their last bits.
+template <int ATOMS>
+__device__ __forceinline__ void clear_empty_places(uint8_t *atoms, int rows, int threads) {
+  const int pieces = (kBlockQ - rows) * (kAtomBytes / 16);  // of an atom
+#pragma unroll 1
+  for (int a = 0; a < ATOMS; ++a) {
+    for (int i = threadIdx.x; i < pieces; i += threads) {
+      *reinterpret_cast<uint4 *>(atoms + a * kBlockQ * kAtomBytes + rows * kAtomBytes + i * 16) = make_uint4(0, 0, 0, 0);
+    }
+  }
+  fence_proxy_async_smem();
+}
+
 // The tiles in shared and tensor memory.
 template <int D>
 struct TileLayout {

@@ -743,9 +743,13 @@ int prefix_splits(int64_t units, int keys) {
 
 size_t round_256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
 
-// From so many packed rows of a key-value head on a run takes the tiles of the tensor cores: up to there the tiles of 16
-// rows read the keys again from L2 at most three times.
-constexpr int kTilesFromRows = 64;
+// From so many packed rows of a key-value head on a run takes the tensor cores' tiles, as soon as there are two tiles of 16
+// rows that would each walk the keys (microseconds, 16-row tiles and tensor cores, 8 x 8 heads over 2000 keys: 20 rows 25.6 and
+// 24.3, 36 rows 32.5 and 24.7, 68 rows 46.6 and 25.9; one sequence: 36 rows 16.0 and 14.0).
+constexpr int kMostTileHeads = 128;
+constexpr int kTilesFromRows = 17;
+// With the keys' weights, for which the tensor cores compute the scores a second time and the others store them:
+constexpr int kWeightTilesFromRows = 64;
 
 int64_t score_pitch_of(int kv_len) { return (static_cast<int64_t>(kv_len) + kKeysAtOnce - 1) / kKeysAtOnce * kKeysAtOnce; }
 
@@ -760,8 +764,8 @@ int tile_rows_of(int rows) { return rows <= 8 ? 8 : 16; }
 struct CachePlan {
   int rows;         // packed rows of a run
   bool tiles;       // the sequences' own keys (and a prefix before them in the same walk) on the tile kernel
-  int tile_rows;    // of the few-row kernel: 8 or 16
-  int row_tiles;    // of so many, or pairs of 128
+  int tile_rows;    // of the few-row kernel: 8 or 16; of the tile kernel up to 128
+  int row_tiles;    // of so many, or pairs of them
   int splits;       // of a pair of tiles
   int ctas;         // of the few-row kernel
   bool prefix_apart;  // a kernel of its own over the prefix for the rows of the whole batch
@@ -777,7 +781,8 @@ CachePlan cache_plan(const CacheAttentionArgs &a) {
   const int group = a.heads / a.kv_heads;
   const int64_t d = a.head_dim;
   p.rows = group * a.q_len;
-  p.tiles = p.rows >= kTilesFromRows;
+  // (a tile holds whole queries, so their heads have to go into it)
+  p.tiles = p.rows >= (a.weights_out != nullptr ? kWeightTilesFromRows : kTilesFromRows) && group <= kMostTileHeads;
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t off = at;
@@ -790,15 +795,16 @@ CachePlan cache_plan(const CacheAttentionArgs &a) {
   size_t part_rows = 0;
   if (p.tiles) {
     most = std::min<int64_t>(a.kv_len, static_cast<int64_t>(a.window) + a.sinks + std::min(a.q_len, cache_tiles_positions(group)));
-    p.row_tiles = cache_tiles_pairs(p.rows);
+    p.tile_rows = cache_tile_rows(group);
+    p.row_tiles = cache_tiles_pairs(p.rows, p.tile_rows);
     p.splits = cache_tiles_splits(runs * p.row_tiles, static_cast<int>(std::min<int64_t>(most + a.prefix_len, INT32_MAX)), 4);
-    part_rows = p.splits > 1 ? cache_tiles_part_rows(runs * p.row_tiles, p.splits) : 0;
+    part_rows = p.splits > 1 ? cache_tiles_part_rows(runs * p.row_tiles, p.splits, p.tile_rows) : 0;
   } else {
     p.tile_rows = tile_rows_of(p.rows);
     p.row_tiles = (p.rows + p.tile_rows - 1) / p.tile_rows;
     const int64_t steps = (most + kStepKeys - 1) / kStepKeys, least = std::min<int64_t>(kLeastSteps, steps);  // of a unit, and of a CTA
     // (beside a prefix's tile kernel, whose CTAs hold their SMs for a while, in two rounds: the SMs it leaves free take more of them)
-    const bool beside_tiles = a.prefix_len > 0 && static_cast<int64_t>(a.batch) * p.rows >= kTilesFromRows;
+    const bool beside_tiles = a.prefix_len > 0 && static_cast<int64_t>(a.batch) * p.rows >= kTilesFromRows && p.rows <= kMostTileHeads;
     p.ctas = static_cast<int>(std::min<int64_t>((beside_tiles ? 2 : 1) * kCtasPerSm * sm_count(), (runs * p.row_tiles * steps + least - 1) / least));
     part_rows = static_cast<size_t>(p.ctas) * 2 * p.tile_rows;
   }
@@ -809,11 +815,12 @@ CachePlan cache_plan(const CacheAttentionArgs &a) {
   if (a.prefix_len > 0 && !p.tiles) {
     p.prefix_apart = true;
     p.prefix_rows = a.batch * p.rows;
-    p.prefix_tiles = p.prefix_rows >= kTilesFromRows;
+    p.prefix_tiles = p.prefix_rows >= kTilesFromRows && p.rows <= kMostTileHeads;
     if (p.prefix_tiles) {
       p.own_out = take(static_cast<size_t>(runs) * p.rows * d * 4);
       p.own_sum = take(static_cast<size_t>(runs) * p.rows * 8);
-      p.prefix_row_tiles = cache_tiles_pairs(p.prefix_rows);
+      p.prefix_tile_rows = cache_tile_rows(p.rows);
+      p.prefix_row_tiles = cache_tiles_pairs(p.prefix_rows, p.prefix_tile_rows);
       p.prefix_splits = cache_tiles_splits(static_cast<int64_t>(a.kv_heads) * p.prefix_row_tiles, a.prefix_len, kPrefixBlocks);
     } else {
       p.prefix_tile_rows = tile_rows_of(p.prefix_rows);
@@ -828,8 +835,8 @@ CachePlan cache_plan(const CacheAttentionArgs &a) {
     p.prefix_sum = take(static_cast<size_t>(a.kv_heads) * p.prefix_splits * p.prefix_rows * 8);
   }
   if (a.weights_out != nullptr && p.tiles) {
-    p.weights = cache_weights_plan(a, kCacheCounters);
-    p.row_norm = take(static_cast<size_t>(runs) * group * cache_weights_norm_pitch(a.q_len) * 8);
+    p.weights = cache_weights_plan(a, p.tile_rows, kCacheCounters);
+    p.row_norm = take(static_cast<size_t>(runs) * cache_weights_norm_pitch(p.rows, p.tile_rows) * 8);
     p.scores = take(p.weights.part_bytes);
   } else if (a.weights_out != nullptr) {
     p.scores = take(static_cast<size_t>(runs) * p.rows * score_pitch_of(a.kv_len) * 4);
@@ -919,13 +926,14 @@ cudaError_t cache_attention(const CacheAttentionArgs &a, const char **why, int *
   if (plan.tiles) {
     tiles.runs = a.batch * a.kv_heads;
     tiles.rows = plan.rows;
+    tiles.tile_rows = plan.tile_rows;
     tiles.row_pairs = plan.row_tiles;
     tiles.splits = plan.splits;
     tiles.part_out = floats(plan.part_out);
     tiles.part_sum = pairs(plan.part_sum);
     if (a.weights_out != nullptr) {
       tiles.row_norm = pairs(plan.row_norm);
-      tiles.norm_pitch = cache_weights_norm_pitch(a.q_len);
+      tiles.norm_pitch = cache_weights_norm_pitch(plan.rows, plan.tile_rows);
     }
     e = cache_tiles(tiles, a, why);
     *launches += e == cudaSuccess ? (plan.splits > 1 ? 2 : 1) : 0;
@@ -938,6 +946,10 @@ cudaError_t cache_attention(const CacheAttentionArgs &a, const char **why, int *
     w.q_len = a.q_len;
     w.kv_len = a.kv_len;
     w.runs = tiles.runs;
+    w.rows = plan.rows;
+    w.tile_rows = plan.tile_rows;
+    w.positions = plan.tile_rows / w.group;
+    w.by_positions = Divisor::of(static_cast<uint32_t>(w.positions));
     w.pairs = plan.weights.pairs;
     w.parts = plan.weights.parts;
     w.part_blocks = plan.weights.part_blocks;
@@ -978,6 +990,7 @@ cudaError_t cache_attention(const CacheAttentionArgs &a, const char **why, int *
       tiles.over_batch = true;
       tiles.runs = a.kv_heads;
       tiles.rows = plan.prefix_rows;
+      tiles.tile_rows = plan.prefix_tile_rows;
       tiles.row_pairs = plan.prefix_row_tiles;
       tiles.splits = plan.prefix_splits;
       tiles.part_out = floats(plan.prefix_out);

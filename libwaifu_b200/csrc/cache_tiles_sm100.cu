@@ -1,20 +1,20 @@
 // Attention over a key-value cache for many query rows (prompts, and the rows of a whole batch over a prefix that
 // it shares): both products on tcgen05, in the way of the two-tile attention kernel.
 //
-// A CTA owns two tiles of 128 rows of one key-value head. The rows are packed: row r is query r / group of query
+// A CTA owns two tiles of up to 128 rows of one key-value head. The rows are packed: row r is query r / group of query
 // head r % group of the ones that share the head, so that a block of keys is read once for all of them and a
 // tile's rows sit close together (under a window a tile walks its 128 / group positions and the window, not 128
 // and the window). Over a prefix, which all of a batch sees, the rows of every sequence are packed one after the other.
+// A tile holds whole queries (or whole sequences), as many as go into 128 rows, and so is a box of the queries' tensor.
 // K and V blocks of 128 keys arrive by TMA into one ring of slots. The walk is a list of blocks: those of a prefix, then the
 // sinks and the keys from the first window's start to the last query's position, one after the other and cut every 128
 // keys (a block that holds both comes in boxes of 16 rows, the sinks filled up to whole ones): 8192 tokens under a window of
 // 1024 keys and 16 sinks walk 9 blocks a unit so, and 10.4 in blocks at multiples of 128.
 //
-// So do the queries where a tile is a box of the tensor (a group, or a group and its queries, that divides 128); otherwise two
-// helping warps gather them. A block that some row does not see whole (past the sequence's end, at a window's edge, on
-// the diagonal) passes those warps before its product: they clear the values of keys that no
-// row sees and take infinities and NaN out of the others, because a probability of zero times such a value is not
-// zero. Rows that do see them have them added by hand at the end.
+// A block that some row does not see whole (past the sequence's end, at a window's edge, on the diagonal) passes two
+// helping warps before its product: they clear the values of keys that no row sees and take infinities and NaN out of the
+// others, because a probability of zero times such a value is not zero. Rows that do see them have them added by hand at
+// the end.
 //
 // A running CTA takes over units whose own CTA has not started (clusterlaunchcontrol.try_cancel): the next unit's keys,
 // queries and first scores come under the last products and the output of the one before. Walks are short here (a window's,
@@ -37,7 +37,6 @@ namespace flsm100 {
 
 namespace {
 
-constexpr int kPairRows = kTiles * kBlockQ;
 constexpr int kSoftmaxWarps = kTiles * kTileWarps;
 constexpr int kProducerWarp = kSoftmaxWarps;
 constexpr int kMmaWarp = kSoftmaxWarps + 1;
@@ -134,8 +133,8 @@ struct Unit {
     pair = p.row_pairs - 1 - at;
     seq = run;
     head = p.by_kv_heads.take(&seq);
-    row0 = pair * kPairRows;
-    const int last_row = min(row0 + kPairRows, p.rows) - 1;
+    row0 = pair * kTiles * p.tile_rows;
+    const int last_row = min(row0 + kTiles * p.tile_rows, p.rows) - 1;
     walk.prefix_len = p.prefix_len;
     walk.prefix_blocks = (p.prefix_len + kBlockKv - 1) / kBlockKv;
     walk.window = p.window;
@@ -161,7 +160,7 @@ struct Unit {
     if (p.over_batch) walk.dirty = Dirty{0, 0, INT32_MAX};
 #pragma unroll
     for (int i = 0; i < kTiles; ++i) {
-      const int first_row = row0 + i * kBlockQ, last = min(first_row + kBlockQ, p.rows) - 1;
+      const int first_row = row0 + i * p.tile_rows, last = min(first_row + p.tile_rows, p.rows) - 1;
       const int mine = p.over_batch ? total : min(total, walk.blocks_up_to(p.by_group.quotient(last) + len - p.q_len));
       blocks[i] = first_row >= p.rows ? 0 : max(0, min(walk.count, mine - walk.first));
     }
@@ -243,20 +242,19 @@ __device__ __noinline__ void patch_row(const TilesParams &p, int unit, int pos, 
 
 // A row's result, or its part of it.
 template <int D>
-__device__ __forceinline__ void finish_row(const TilesParams &p, const Unit &u, uint32_t t_out, int row, int pos, int my_blocks, bool ok,
-                                           bool patch, float m_used, float l_run) {
-  const bool live = row < p.rows;
+__device__ __forceinline__ void finish_row(const TilesParams &p, const Unit &u, uint32_t t_out, int tile, int in_tile, int pos, int my_blocks,
+                                           bool ok, bool patch, float m_used, float l_run) {
+  const int row = u.row0 + tile * p.tile_rows + in_tile;
+  const bool live = in_tile < p.tile_rows && row < p.rows;
   const bool parts = p.over_batch || u.active > 1;
-  // The index of this row's part of split s: (kv_head, split, rows) over a prefix, (unit, split, 256) else.
+  // The index of this row's part of split s: (kv_head, split, rows) over a prefix, (unit, split, rows of a pair) else.
   const int64_t part_row0 = p.over_batch ? static_cast<int64_t>(u.head) * p.splits * p.rows + row
-                                         : (static_cast<int64_t>(u.run) * p.row_pairs + u.pair) * p.splits * kPairRows + (row - u.row0);
-  const int64_t part_step = p.over_batch ? p.rows : kPairRows;
+                                         : (static_cast<int64_t>(u.run) * p.row_pairs + u.pair) * p.splits * kTiles * p.tile_rows + (row - u.row0);
+  const int64_t part_step = p.over_batch ? p.rows : kTiles * p.tile_rows;
   const bool empty = p.prefix_len == 0 && pos < 0;  // sees no key: zeros
   uint16_t *dst = live && !p.over_batch ? p.out + row_offset(p, p.out_stride, u.head, u.seq, row) : nullptr;
   float *part_dst = p.part_out + (part_row0 + u.split * part_step) * D;
-  int query = row;
-  const int in_group = p.by_group.take(&query);
-  const int64_t norm_at = (static_cast<int64_t>(u.run) * p.group + in_group) * p.norm_pitch + query;
+  const int64_t norm_at = static_cast<int64_t>(u.run) * p.norm_pitch + (u.pair * kTiles + tile) * kBlockQ + in_tile;
   // (a row whose every score is -inf has no softmax)
   const float inv = empty ? 0.0f : (m_used == -INFINITY ? NAN : 1.0f / l_run);
   if (ok) {
@@ -297,13 +295,14 @@ __device__ __forceinline__ void finish_row(const TilesParams &p, const Unit &u, 
     }
     // (the cubic's smallest exponentials keep a part that saw nothing from summing to zero)
     if (live && parts) p.part_sum[part_row0 + u.split * part_step] = make_float2(m_used, m_used == -INFINITY && l_run == l_run ? 0.0f : l_run);
-    if (live && !parts && p.row_norm != nullptr) p.row_norm[norm_at] = make_float2(m_used, inv);
+    // (of a tile's empty places zeros, whose rows then weigh nothing)
+    if (p.row_norm != nullptr && (!live || !parts)) p.row_norm[norm_at] = live ? make_float2(m_used, inv) : make_float2(0.0f, 0.0f);
   }
 }
 
 // The results of rows whose unit several CTAs shared: four columns a thread.
 template <int D, bool BF16>
-__global__ void __launch_bounds__(128) join_tiles_kernel(const __grid_constant__ TilesParams p, const Divisor by_rows, int64_t total) {
+__global__ void __launch_bounds__(128) join_tiles_kernel(const __grid_constant__ TilesParams p, const Divisor by_rows, const Divisor by_tile_rows, int64_t total) {
   griddep_wait();
   griddep_launch_dependents();
   constexpr int kQuads = D / 4;
@@ -311,21 +310,20 @@ __global__ void __launch_bounds__(128) join_tiles_kernel(const __grid_constant__
   if (at >= total) return;
   const int col = static_cast<int>(at % kQuads) * 4;
   int run = static_cast<int>(at / kQuads);
-  const int row = by_rows.take(&run), pair = row / kPairRows;
+  const int row = by_rows.take(&run), tile = by_tile_rows.quotient(row), pair = tile / kTiles;
   const Unit u(p, run + p.runs * p.splits * (p.row_pairs - 1 - pair));  // (its first split)
   if (u.active == 1) return;
   RowSum sum;
   sum.clear();
-  const int64_t first = (static_cast<int64_t>(run) * p.row_pairs + pair) * p.splits * kPairRows + (row - u.row0);
-  add_parts<D>(u.active, p.part_sum, p.part_out, col, &sum, [&](int c) { return first + c * kPairRows; });
-  int query = row;
-  const int in_group = p.by_group.take(&query);
-  const bool empty = p.prefix_len == 0 && query + u.len - p.q_len < 0;  // sees no key: zeros
+  const int pair_rows = kTiles * p.tile_rows;
+  const int64_t first = (static_cast<int64_t>(run) * p.row_pairs + pair) * p.splits * pair_rows + (row - u.row0);
+  add_parts<D>(u.active, p.part_sum, p.part_out, col, &sum, [&](int c) { return first + c * pair_rows; });
+  const bool empty = p.prefix_len == 0 && p.by_group.quotient(row) + u.len - p.q_len < 0;  // sees no key: zeros
   // (a row whose every score is -inf has no softmax)
   const float inv = empty ? 0.0f : (sum.m == -INFINITY ? NAN : 1.0f / sum.l);
   const uint2 w = make_uint2(pack_pair<BF16>(sum.o.x * inv, sum.o.y * inv), pack_pair<BF16>(sum.o.z * inv, sum.o.w * inv));
   *reinterpret_cast<uint2 *>(p.out + row_offset(p, p.out_stride, u.head, u.seq, row) + col) = empty ? make_uint2(0, 0) : w;
-  if (p.row_norm != nullptr && col == 0) p.row_norm[(static_cast<int64_t>(run) * p.group + in_group) * p.norm_pitch + query] = make_float2(sum.m, inv);
+  if (p.row_norm != nullptr && col == 0) p.row_norm[static_cast<int64_t>(run) * p.norm_pitch + tile * kBlockQ + row - tile * p.tile_rows] = make_float2(sum.m, inv);
 }
 
 template <int D>
@@ -361,7 +359,7 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       mbar_init(&t.slot_clean_bar[i], kHelpWarps);
     }
     for (int i = 0; i < kTiles; ++i) {
-      mbar_init(&t.q_full_bar[i], p.q_by_tma ? 1 : kHelpWarps);
+      mbar_init(&t.q_full_bar[i], 1);
       mbar_init(&t.q_empty_bar[i], 1);
       mbar_init(&t.s_full_bar[i], 1);
       for (int h = 0; h < kPParts; ++h) mbar_init(&t.p_full_bar[i][h], kTileWarps);
@@ -370,7 +368,7 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     fence_barrier_init();
   }
   if (warp == kProducerWarp && lane == 0) {
-    if (p.q_by_tma) tma_prefetch_desc(&tmap_q);
+    tma_prefetch_desc(&tmap_q);
     tma_prefetch_desc(&tmap_k);
     tma_prefetch_desc(&tmap_v);
   }
@@ -378,6 +376,7 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     tmem_alloc<1>(&t.tmem_base_slot, L::kTmemCols);
     tmem_relinquish<1>();
   }
+  clear_empty_places<L::kQAtoms * kTiles>(smem + L::kQOff, p.tile_rows, kThreads);
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
@@ -412,13 +411,13 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     for (int count = 1; ok && unit >= 0; ++count) {
       const Unit u(p, unit);
       if (u.split < u.active) {
-        const int tile_row0 = u.row0 + tile * kBlockQ;
+        const int tile_row0 = u.row0 + tile * p.tile_rows, tile_end = min(tile_row0 + p.tile_rows, p.rows);
         const int my_blocks = tile == 0 ? u.blocks[0] : u.blocks[1];
-        const int row = tile_row0 + static_cast<int>(quarter) * 32 + static_cast<int>(lane);
-        const int pos = p.by_group.quotient(min(row, p.rows - 1)) + u.len - p.q_len;
+        const int in_tile = static_cast<int>(quarter) * 32 + static_cast<int>(lane);
+        const int pos = p.by_group.quotient(max(0, min(tile_row0 + in_tile, tile_end - 1))) + u.len - p.q_len;
         // What every row of the tile sees.
         const int common_last = p.by_group.quotient(tile_row0) + u.len - p.q_len;
-        const int common_before = p.by_group.quotient(min(tile_row0 + kBlockQ, p.rows) - 1) + u.len - p.q_len - p.window;
+        const int common_before = p.by_group.quotient(max(0, tile_end - 1)) + u.len - p.q_len - p.window;
         float m_used = -INFINITY;
         float l_run = 0.0f;
         for (int j = 0; j < my_blocks && ok; ++j) {
@@ -458,7 +457,7 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
           tc_fence_after_sync();
         }
         const bool patch = *reinterpret_cast<volatile uint32_t *>(&t.patch_flag[count & 1]) == static_cast<uint32_t>(count);
-        finish_row<D>(p, u, t_out, row, pos, my_blocks, ok, patch, m_used, l_run);
+        finish_row<D>(p, u, t_out, tile, in_tile, pos, my_blocks, ok, patch, m_used, l_run);
         // The next unit's first product overwrites this output: it waits for probabilities that the tile's
         // four warps hand over only after these reads.
         tc_fence_before_sync();
@@ -507,15 +506,15 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
               }
             }
             // The queries behind the first block of keys, once the last scores of the unit before have been computed.
-            for (int q = 0; i == 0 && p.q_by_tma && q < kTiles && ok; ++q) {
+            for (int q = 0; i == 0 && q < kTiles && ok; ++q) {
               if ((q == 0 ? u.blocks[0] : u.blocks[1]) == 0) continue;
               if (!mbar_wait(&t.q_empty_bar[q], ((q_phase >> q) & 1) ^ 1, &abort_flag)) {
                 ok = false;
                 break;
               }
               q_phase ^= 1u << q;
-              mbar_arrive_expect_tx(&t.q_full_bar[q], L::kQBytes);
-              const int row = u.row0 + q * kBlockQ;
+              mbar_arrive_expect_tx(&t.q_full_bar[q], static_cast<uint32_t>(p.tile_rows) * D * 2);
+              const int row = u.row0 + q * p.tile_rows;
               const int seq = p.over_batch ? p.by_sequence_rows.quotient(row) : u.seq, query = p.over_batch ? 0 : p.by_group.quotient(row);
 #pragma unroll
               for (int a = 0; a < L::kQAtoms; ++a) {
@@ -648,47 +647,15 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         atomicCAS(p.status, 0u, kStatusAttentionTimeout);
       }
     } else {
-      // ------------------------------------------------------------------ queries, and values that are not seen by all
+      // ------------------------------------------------------------------ values that are not seen by all
       const int which = static_cast<int>(warp) - kHelpWarp;
       // A half whose exponent is all ones carries into its sign bit.
       const uint32_t exponent = p.is_bf16 ? 0x7F807F80u : 0x7C007C00u, carry = p.is_bf16 ? 0x00800080u : 0x04000400u;
       bool ok = true;
-      uint32_t q_phase = 0;  // bit i: of tile i's queries
       int n = 0;
       int unit = blockIdx.x;
       for (int count = 1; ok && unit >= 0; ++count) {
         const Unit u(p, unit);
-        if (!p.q_by_tma) {
-          // Half of each tile's rows, a few at a time: piece c of row r of an atom lies at c ^ (r & 7).
-          constexpr int kPieces = D / 8, kRowsAtOnce = 32 / kPieces;
-          const int c = static_cast<int>(lane) % kPieces;
-#pragma unroll 1
-          for (int i = 0; i < kTiles; ++i) {
-            if (ok && (i == 0 ? u.blocks[0] : u.blocks[1]) > 0) {
-              ok = __all_sync(0xffffffffu, mbar_wait(&t.q_empty_bar[i], ((q_phase >> i) & 1) ^ 1, &abort_flag));
-              q_phase ^= 1u << i;
-#pragma unroll 4
-              for (int k = 0; ok && k < kBlockQ / kHelpWarps / kRowsAtOnce; ++k) {
-                const int in_tile = which * (kBlockQ / kHelpWarps) + k * kRowsAtOnce + static_cast<int>(lane) / kPieces;
-                const int r = u.row0 + i * kBlockQ + in_tile;
-                cp_async_16(q_tile(i) + (c >> 3) * kBlockQ * kAtomBytes + in_tile * kAtomBytes + (((c & 7) ^ (in_tile & 7)) << 4),
-                            p.q + row_offset(p, p.q_stride, u.head, u.seq, min(r, p.rows - 1)) + c * 8, r < p.rows ? 16 : 0);
-              }
-            }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-          }
-#pragma unroll
-          for (int i = 0; i < kTiles; ++i) {
-            if (i == 0) {
-              asm volatile("cp.async.wait_group 1;" ::: "memory");
-            } else {
-              asm volatile("cp.async.wait_group 0;" ::: "memory");
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (ok && u.blocks[i] > 0 && lane == 0) mbar_arrive(&t.q_full_bar[i]);
-          }
-        }
         // (Every load is waited for and its slot given back, so that none is filled again before its turn here.)
         for (int j = 0; j < u.walk.count && ok; ++j) {
           const int nk = n + 2 * j, nv = nk + 1;
@@ -773,9 +740,11 @@ cudaError_t launch(const CUtensorMap &tq, const CUtensorMap (&maps)[6], const Ti
 
 }  // namespace
 
-int cache_tiles_pairs(int rows) { return (rows + kPairRows - 1) / kPairRows; }
+int cache_tile_rows(int whole) { return kBlockQ / whole * whole; }
 
-int cache_tiles_positions(int group) { return kPairRows / group + 2; }
+int cache_tiles_pairs(int rows, int tile_rows) { return (rows + kTiles * tile_rows - 1) / (kTiles * tile_rows); }
+
+int cache_tiles_positions(int group) { return kTiles * (kBlockQ / group); }
 
 int cache_tiles_splits(int64_t units, int keys, int least_blocks) {
   const int blocks = (keys + kBlockKv - 1) / kBlockKv;
@@ -786,24 +755,19 @@ int cache_tiles_splits(int64_t units, int keys, int least_blocks) {
   return (blocks + per_split - 1) / per_split;
 }
 
-size_t cache_tiles_part_rows(int64_t units, int splits) { return static_cast<size_t>(units) * splits * kPairRows; }
+size_t cache_tiles_part_rows(int64_t units, int splits, int tile_rows) { return static_cast<size_t>(units) * splits * kTiles * tile_rows; }
 
 cudaError_t cache_tiles(TilesParams p, const CacheAttentionArgs &a, const char **why) {
   CUtensorMap tq, maps[6];  // of q; of k and v, the same in boxes of 16 positions, of the prefix
   p.by_runs = Divisor::of(static_cast<uint32_t>(p.runs));
   p.by_splits = Divisor::of(static_cast<uint32_t>(p.splits));
-  // A tile's rows as a box: the heads of a group, a run of queries, and over a prefix a run of sequences.
-  const int per_query = p.group, per_sequence = p.group * p.q_len;
-  const bool whole_queries = !p.over_batch && per_query <= kBlockQ && kBlockQ % per_query == 0;
-  const bool whole_sequences = p.over_batch && per_sequence <= kBlockQ && kBlockQ % per_sequence == 0;
-  p.q_by_tma = whole_queries || whole_sequences;
-  if (p.q_by_tma) {
+  {  // A tile's rows as a box: the heads of a group, a run of queries, and over a prefix a run of sequences.
     const uint64_t dims[4] = {static_cast<uint64_t>(a.head_dim) * 2, static_cast<uint64_t>(a.heads), static_cast<uint64_t>(a.q_len),
                               static_cast<uint64_t>(a.batch)};
     auto bytes = [&](int64_t s, int extent) { return static_cast<uint64_t>(extent > 1 ? s : a.head_dim) * 2; };
     const uint64_t strides[3] = {bytes(a.q_stride[1], a.heads), bytes(a.q_stride[2], a.q_len), bytes(a.q_stride[0], a.batch)};
-    const uint32_t box[3] = {static_cast<uint32_t>(p.group), static_cast<uint32_t>(whole_sequences ? p.q_len : kBlockQ / per_query),
-                             static_cast<uint32_t>(whole_sequences ? kBlockQ / per_sequence : 1)};
+    const int queries = p.over_batch ? a.q_len : p.tile_rows / p.group;
+    const uint32_t box[3] = {static_cast<uint32_t>(p.group), static_cast<uint32_t>(queries), static_cast<uint32_t>(p.tile_rows / (p.group * queries))};
     if (!make_tmap(&tq, a.q, 4, dims, strides, box)) {
       *why = "cuTensorMapEncodeTiled refused q";
       return cudaErrorInvalidValue;
@@ -825,7 +789,6 @@ cudaError_t cache_tiles(TilesParams p, const CacheAttentionArgs &a, const char *
   // (the others are not used)
   if (!own) maps[0] = maps[2] = maps[4], maps[1] = maps[3] = maps[5];
   if (!prefix) maps[4] = maps[0], maps[5] = maps[1];
-  if (!p.q_by_tma) tq = maps[0];
   const int64_t ctas = static_cast<int64_t>(p.runs) * p.row_pairs * p.splits;
   *why = "launching the tile kernel";
   cudaError_t e = a.head_dim == 64 ? launch<64>(tq, maps, p, ctas, a.stream) : launch<128>(tq, maps, p, ctas, a.stream);
@@ -834,7 +797,7 @@ cudaError_t cache_tiles(TilesParams p, const CacheAttentionArgs &a, const char *
   const int64_t total = static_cast<int64_t>(p.runs) * p.rows * (a.head_dim / 4);
   auto join = a.head_dim == 64 ? (a.is_bf16 ? join_tiles_kernel<64, true> : join_tiles_kernel<64, false>)
                                : (a.is_bf16 ? join_tiles_kernel<128, true> : join_tiles_kernel<128, false>);
-  return launch_overlapped(join, (total + 127) / 128, 128, 0, a.stream, p, Divisor::of(static_cast<uint32_t>(p.rows)), total);
+  return launch_overlapped(join, (total + 127) / 128, 128, 0, a.stream, p, Divisor::of(static_cast<uint32_t>(p.rows)), Divisor::of(static_cast<uint32_t>(p.tile_rows)), total);
 }
 
 }  // namespace flsm100

@@ -3,8 +3,8 @@
 // The attention kernel has left each query row's maximum m and 1 / sum; a key's weight from a row is
 // exp2(score - m) / sum, and its scores are computed again: storing them would move heads x queries x keys x 4 bytes
 // twice, more than the product takes. Here the keys are the rows of the product, S^T = K Q^T: a CTA owns two tiles of 128
-// keys of one key-value head and walks the queries of the heads that share it 128 at a time, so a thread owns a key and adds up
-// over the columns of its row in tensor memory; nothing has to meet another thread. The scores of two blocks lie in
+// keys of one key-value head and walks the rows of the heads that share it, packed as the tile kernel packs them, up to
+// 128 at a time, so a thread owns a key and adds up over the columns of its row in tensor memory; nothing has to meet another thread. The scores of two blocks lie in
 // tensor memory at a time, so that a block's product runs under the exponentials of the one before it. The
 // walks of a key's tiles are divided over CTAs, whose sums the last one to arrive adds in their order.
 //
@@ -54,12 +54,11 @@ struct Layout : TileLayout<D> {
   static_assert(kSlots >= 2 && kSmemBytes <= 227 * 1024, "shared memory");
 };
 
-// Two tiles of keys and the blocks of queries that see some of them: those of the first head, of the second, ...
+// Two tiles of keys and the blocks of rows that see some of them.
 struct Unit {
   int run, head, seq, part, pair;
-  int key0, len, offset;        // query i sits at i + offset
-  int first_block, per_head;    // blocks of 128 queries of one head, from first_block on
-  int first, count, active;     // of this part, in the walk over all heads
+  int key0, len, offset;     // query i sits at i + offset
+  int first, count, active;  // blocks of this part
   __device__ __forceinline__ Unit(const WeightsParams &p, int at) {
     // The first keys, which most queries see, first.
     run = at % p.runs;
@@ -71,33 +70,15 @@ struct Unit {
     key0 = pair * kKeysPerCta;
     len = sequence_length(p.kv_lens, seq, p.kv_len);
     offset = len - p.q_len;
-    first_block = max(0, key0 - offset) / kBlockQ;
-    per_head = key0 < len ? max(0, (p.q_len + kBlockQ - 1) / kBlockQ - first_block) : 0;
-    const int total = p.group * per_head;
+    const int first_block = p.by_positions.quotient(max(0, key0 - offset)), blocks = p.by_positions.quotient(p.q_len + p.positions - 1);
+    const int total = key0 < len ? max(0, blocks - first_block) : 0;
     active = max(1, (total + p.part_blocks - 1) / p.part_blocks);
-    first = part * p.part_blocks;
-    count = max(0, min(p.part_blocks, total - first));
+    first = first_block + part * p.part_blocks;
+    count = max(0, min(p.part_blocks, total - part * p.part_blocks));
   }
-  // Does a query of the block from query0 on see a key of tile i?
-  __device__ __forceinline__ bool meets(int query0, int i) const {
-    return key0 + i * kBlockKv < len && query0 + kBlockQ - 1 + offset >= key0 + i * kBlockKv;
-  }
-};
-
-// Where a role's walk over a part's blocks stands.
-struct Place {
-  int head, query0, end;
-  __device__ __forceinline__ explicit Place(const Unit &u) {
-    head = u.per_head > 0 ? u.first / u.per_head : 0;
-    query0 = (u.first_block + u.first - head * u.per_head) * kBlockQ;
-    end = (u.first_block + u.per_head) * kBlockQ;
-  }
-  __device__ __forceinline__ void advance(const Unit &u) {
-    query0 += kBlockQ;
-    if (query0 == end) {
-      query0 = u.first_block * kBlockQ;
-      ++head;
-    }
+  // Does a query of block b see a key of tile i?
+  __device__ __forceinline__ bool meets(const WeightsParams &p, int b, int i) const {
+    return key0 + i * kBlockKv < len && (first + b + 1) * p.positions - 1 + offset >= key0 + i * kBlockKv;
   }
 };
 
@@ -142,6 +123,7 @@ cache_weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     tmem_alloc<1>(&t.tmem_base_slot, L::kTmemCols);
     tmem_relinquish<1>();
   }
+  clear_empty_places<L::kQAtoms * S>(smem + L::kQueriesOff, p.tile_rows, kThreads);  // (their maxima and 1 / sums are zeros too: they add nothing)
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
@@ -160,12 +142,11 @@ cache_weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     float sum = 0.0f;
     bool ok = true;
     int met = 0;
-    Place at(u);
-    for (int b = 0; b < u.count && ok; ++b, at.advance(u)) {
+    for (int b = 0; b < u.count && ok; ++b) {
       const int st = b % S;
       ok = __all_sync(0xffffffffu, mbar_wait(&t.slot_full_bar[st], (b / S) & 1, &abort_flag));
       if (!ok) break;
-      if (u.meets(at.query0, tile)) {
+      if (u.meets(p, b, tile)) {
         ok = __all_sync(0xffffffffu, mbar_wait(&t.s_full_bar[tile][met & 1], (met >> 1) & 1, &abort_flag));
         if (!ok) break;
         tc_fence_after_sync();
@@ -180,9 +161,9 @@ cache_weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         if (lane == 0) mbar_arrive(&t.s_empty_bar[tile][met & 1]);
         ++met;
         const float4 *norm = reinterpret_cast<const float4 *>(smem + L::kNormsOff + st * kNormBytes);  // two queries each
-        const int query0 = at.query0;
+        const int query0 = (u.first + b) * p.positions;
         float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (query0 + u.offset >= tile_last && query0 + kBlockQ <= p.q_len) {  // every query of the block sees every key of the tile
+        if (query0 + u.offset >= tile_last) {  // every row of the block sees every key of the tile
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
 #pragma unroll
@@ -193,15 +174,15 @@ cache_weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
             }
           }
         } else {
-          const int begin = key - u.offset - query0, end = p.q_len - query0;  // of the columns that see the key
+          const int begin = max(0, key - u.offset - query0) * p.group;  // the first column that sees the key
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
 #pragma unroll
             for (int i = 0; i < 32; i += 2) {
               const float4 n = norm[(c * 32 + i) / 2];
               const int col = c * 32 + i;
-              if (col >= begin && col < end) part[i & 3] = fmaf(fast_exp2(fmaf(__uint_as_float(sc[c][i]), p.scale_log2, -n.x)), n.y, part[i & 3]);
-              if (col + 1 >= begin && col + 1 < end) {
+              if (col >= begin) part[i & 3] = fmaf(fast_exp2(fmaf(__uint_as_float(sc[c][i]), p.scale_log2, -n.x)), n.y, part[i & 3]);
+              if (col + 1 >= begin) {
                 part[(i + 1) & 3] = fmaf(fast_exp2(fmaf(__uint_as_float(sc[c][i + 1]), p.scale_log2, -n.z)), n.w, part[(i + 1) & 3]);
               }
             }
@@ -253,21 +234,19 @@ cache_weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
           }
         }
       }
-      Place at(u);
-      for (int b = 0; b < u.count && ok; ++b, at.advance(u)) {
+      for (int b = 0; b < u.count && ok; ++b) {
         const int st = b % S;
         if (!mbar_wait(&t.slot_empty_bar[st], ((b / S) & 1) ^ 1, &abort_flag)) {
           ok = false;
           break;
         }
-        const int g = at.head, query0 = at.query0;
-        mbar_arrive_expect_tx(&t.slot_full_bar[st], L::kSlotBytes);
+        mbar_arrive_expect_tx(&t.slot_full_bar[st], static_cast<uint32_t>(p.tile_rows) * D * 2 + kNormBytes);
 #pragma unroll
         for (int a = 0; a < L::kQAtoms; ++a) {
-          tma_load_4d(smem + L::kQueriesOff + st * L::kQBytes + a * kBlockQ * kAtomBytes, &tmap_q, &t.slot_full_bar[st], a * kAtomBytes, query0,
-                      u.head * p.group + g, u.seq);
+          tma_load_4d(smem + L::kQueriesOff + st * L::kQBytes + a * kBlockQ * kAtomBytes, &tmap_q, &t.slot_full_bar[st], a * kAtomBytes, u.head * p.group,
+                      (u.first + b) * p.positions, u.seq);
         }
-        bulk_load_1d(smem + L::kNormsOff + st * kNormBytes, p.row_norm + (static_cast<int64_t>(u.run) * p.group + g) * p.norm_pitch + query0,
+        bulk_load_1d(smem + L::kNormsOff + st * kNormBytes, p.row_norm + static_cast<int64_t>(u.run) * p.norm_pitch + (u.first + b) * kBlockQ,
                      kNormBytes, &t.slot_full_bar[st]);
       }
       if (!ok) {
@@ -283,14 +262,13 @@ cache_weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     const uint64_t qdesc0 = umma_desc_sw128(smem_u32(smem + L::kQueriesOff));
     bool ok = u.count == 0 || mbar_wait(&t.k_full_bar, 0, &abort_flag);
     int met[kTiles] = {0, 0};
-    Place at(u);
-    for (int b = 0; b < u.count && ok; ++b, at.advance(u)) {
+    for (int b = 0; b < u.count && ok; ++b) {
       const int st = b % S;
       ok = mbar_wait(&t.slot_full_bar[st], (b / S) & 1, &abort_flag);
       const uint64_t qd = qdesc0 + static_cast<uint64_t>(st * (L::kQBytes >> 4));
 #pragma unroll
       for (int i = 0; i < kTiles; ++i) {
-        if (!ok || !u.meets(at.query0, i)) continue;
+        if (!ok || !u.meets(p, b, i)) continue;
         ok = mbar_wait(&t.s_empty_bar[i][met[i] & 1], ((met[i] >> 1) & 1) ^ 1, &abort_flag);
         if (!ok) continue;
         tc_fence_after_sync();
@@ -334,14 +312,14 @@ cudaError_t launch(const CUtensorMap &tq, const CUtensorMap &tk, const WeightsPa
 
 }  // namespace
 
-int cache_weights_norm_pitch(int q_len) { return (q_len + kBlockQ - 1) / kBlockQ * kBlockQ; }
+int cache_weights_norm_pitch(int rows, int tile_rows) { return (rows + kTiles * tile_rows - 1) / (kTiles * tile_rows) * kTiles * kBlockQ; }
 
-WeightsPlan cache_weights_plan(const CacheAttentionArgs &a, int most_units) {
+WeightsPlan cache_weights_plan(const CacheAttentionArgs &a, int tile_rows, int most_units) {
   WeightsPlan plan;
   const int64_t runs = static_cast<int64_t>(a.batch) * a.kv_heads;
   plan.pairs = (a.kv_len + kKeysPerCta - 1) / kKeysPerCta;
-  const int query_blocks = (a.q_len + kBlockQ - 1) / kBlockQ, group = a.heads / a.kv_heads;
-  const int64_t longest = static_cast<int64_t>(group) * query_blocks;  // blocks of the first keys' walk
+  const int positions = tile_rows / (a.heads / a.kv_heads);  // of a block
+  const int64_t longest = (a.q_len + positions - 1) / positions;  // blocks of the first keys' walk
   plan.part_blocks = static_cast<int>(longest);
   if (runs * plan.pairs <= most_units) {
     // The shortest parts (eight blocks at least) of which there are no more than SMs, for sequences that fill the cache: one
@@ -349,8 +327,8 @@ WeightsPlan cache_weights_plan(const CacheAttentionArgs &a, int most_units) {
     auto parts_of = [&](int64_t part) {
       int64_t sum = 0;
       for (int pair = 0; pair < plan.pairs; ++pair) {
-        const int64_t first = std::max<int64_t>(0, static_cast<int64_t>(pair) * kKeysPerCta - (a.kv_len - a.q_len)) / kBlockQ;
-        sum += (group * std::max<int64_t>(0, query_blocks - first) + part - 1) / part;
+        const int64_t first = std::max<int64_t>(0, static_cast<int64_t>(pair) * kKeysPerCta - (a.kv_len - a.q_len)) / positions;
+        sum += (std::max<int64_t>(0, longest - first) + part - 1) / part;
       }
       return sum * runs;
     };
@@ -373,7 +351,12 @@ WeightsPlan cache_weights_plan(const CacheAttentionArgs &a, int most_units) {
 
 cudaError_t cache_weights(const WeightsParams &p, const CacheAttentionArgs &a, const char **why) {
   CUtensorMap tq, tk;
-  if (!row_map(&tq, a.q, a.head_dim, a.q_len, a.heads, a.batch, a.q_stride[0], a.q_stride[1], a.q_stride[2], kBlockQ) ||
+  const uint64_t dims[4] = {static_cast<uint64_t>(a.head_dim) * 2, static_cast<uint64_t>(a.heads), static_cast<uint64_t>(a.q_len),
+                            static_cast<uint64_t>(a.batch)};
+  auto bytes = [&](int64_t s, int extent) { return static_cast<uint64_t>(extent > 1 ? s : a.head_dim) * 2; };
+  const uint64_t strides[3] = {bytes(a.q_stride[1], a.heads), bytes(a.q_stride[2], a.q_len), bytes(a.q_stride[0], a.batch)};
+  const uint32_t box[3] = {static_cast<uint32_t>(p.group), static_cast<uint32_t>(p.positions), 1};
+  if (!make_tmap(&tq, a.q, 4, dims, strides, box) ||
       !row_map(&tk, a.k, a.head_dim, a.kv_len, a.kv_heads, a.batch, a.k_stride[0], a.k_stride[1], a.k_stride[2], kBlockKv)) {
     *why = "cuTensorMapEncodeTiled refused q or k";
     return cudaErrorInvalidValue;

@@ -5,6 +5,7 @@
 #include <stdint.h>
 
 #include "cache_attention_sm100.cuh"
+#include "cache_common_sm100.cuh"
 
 namespace flsm100 {
 
@@ -14,10 +15,14 @@ struct WeightsParams {
   int kv_heads, group, q_len, kv_len;
   int runs;         // (sequence, key-value head)
   int pairs;        // of 128 keys
-  int parts;        // CTAs that divide a pair's blocks of queries, part_blocks each
+  int rows;         // packed rows of a run: query r / group of head r % group
+  int tile_rows;    // of a block of them: whole queries
+  int positions;    // tile_rows / group
+  Divisor by_positions;
+  int parts;        // CTAs that divide a pair's blocks of rows, part_blocks each
   int part_blocks;
   float scale_log2;
-  const float2 *row_norm;  // (run, query head of the group, norm_pitch): maximum in log2 units and 1 / sum
+  const float2 *row_norm;  // (run, norm_pitch), 128 to a block: a row's maximum in log2 units and 1 / sum
   int norm_pitch;
   float *part_sums;  // (run, pair, part, 256)
   uint32_t *counters;
@@ -33,9 +38,9 @@ struct WeightsPlan {
   int64_t ctas;
 };
 
-int cache_weights_norm_pitch(int q_len);  // whole blocks of queries
+int cache_weights_norm_pitch(int rows, int tile_rows);  // 128 to a block, and to an even number of them
 // At most `most_units` walks may be divided.
-WeightsPlan cache_weights_plan(const CacheAttentionArgs &a, int most_units);
+WeightsPlan cache_weights_plan(const CacheAttentionArgs &a, int tile_rows, int most_units);
 cudaError_t cache_weights(const WeightsParams &p, const CacheAttentionArgs &a, const char **why);
 
 }  // namespace flsm100
