@@ -920,7 +920,7 @@ cudaError_t cache_attention(const CacheAttentionArgs &a, const char **why, int *
   cudaError_t e;
   TilesParams tiles = {};
   fill_params(a, &tiles);
-  tiles.is_bf16 = a.is_bf16;
+
   tiles.status = a.status;
   tiles.prefix_len = a.prefix_len;
   if (plan.tiles) {

@@ -241,7 +241,7 @@ __device__ __noinline__ void patch_row(const TilesParams &p, int unit, int pos, 
 }
 
 // A row's result, or its part of it.
-template <int D>
+template <int D, bool BF16>
 __device__ __forceinline__ void finish_row(const TilesParams &p, const Unit &u, uint32_t t_out, int tile, int in_tile, int pos, int my_blocks,
                                            bool ok, bool patch, float m_used, float l_run) {
   const int row = u.row0 + tile * p.tile_rows + in_tile;
@@ -277,21 +277,17 @@ __device__ __forceinline__ void finish_row(const TilesParams &p, const Unit &u, 
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           uint4 w;
-          w.x = pack16(__uint_as_float(v[g * 8 + 0]) * inv, __uint_as_float(v[g * 8 + 1]) * inv, p.is_bf16);
-          w.y = pack16(__uint_as_float(v[g * 8 + 2]) * inv, __uint_as_float(v[g * 8 + 3]) * inv, p.is_bf16);
-          w.z = pack16(__uint_as_float(v[g * 8 + 4]) * inv, __uint_as_float(v[g * 8 + 5]) * inv, p.is_bf16);
-          w.w = pack16(__uint_as_float(v[g * 8 + 6]) * inv, __uint_as_float(v[g * 8 + 7]) * inv, p.is_bf16);
+          w.x = pack16(__uint_as_float(v[g * 8 + 0]) * inv, __uint_as_float(v[g * 8 + 1]) * inv, BF16);
+          w.y = pack16(__uint_as_float(v[g * 8 + 2]) * inv, __uint_as_float(v[g * 8 + 3]) * inv, BF16);
+          w.z = pack16(__uint_as_float(v[g * 8 + 4]) * inv, __uint_as_float(v[g * 8 + 5]) * inv, BF16);
+          w.w = pack16(__uint_as_float(v[g * 8 + 6]) * inv, __uint_as_float(v[g * 8 + 7]) * inv, BF16);
           *reinterpret_cast<uint4 *>(dst + c * 32 + g * 8) = empty ? make_uint4(0, 0, 0, 0) : w;
         }
       }
     }
     if (live && patch && m_used != -INFINITY && l_run == l_run) {
       const uint16_t *q = p.q + row_offset(p, p.q_stride, u.head, u.seq, row);
-      if (p.is_bf16) {
-        patch_row<D, true>(p, u.index, pos, q, m_used, l_run, dst, parts ? part_dst : nullptr);
-      } else {
-        patch_row<D, false>(p, u.index, pos, q, m_used, l_run, dst, parts ? part_dst : nullptr);
-      }
+      patch_row<D, BF16>(p, u.index, pos, q, m_used, l_run, dst, parts ? part_dst : nullptr);
     }
     // (the cubic's smallest exponentials keep a part that saw nothing from summing to zero)
     if (live && parts) p.part_sum[part_row0 + u.split * part_step] = make_float2(m_used, m_used == -INFINITY && l_run == l_run ? 0.0f : l_run);
@@ -326,7 +322,7 @@ __global__ void __launch_bounds__(128) join_tiles_kernel(const __grid_constant__
   if (p.row_norm != nullptr && col == 0) p.row_norm[static_cast<int64_t>(run) * p.norm_pitch + tile * kBlockQ + row - tile * p.tile_rows] = make_float2(sum.m, inv);
 }
 
-template <int D>
+template <int D, bool BF16>
 __global__ void __launch_bounds__(kThreads, 1)
 cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
                    const __grid_constant__ CUtensorMap tmap_k16, const __grid_constant__ CUtensorMap tmap_v16,
@@ -448,7 +444,7 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
               hide.sinks = p.sinks - hide.key0;
             }
           }
-          softmax_block<D, true>(p.scale_log2, p.is_bf16, t_scores, t_out, j == 0, hide, t.p_full_bar[tile], lane, &m_used, &l_run);
+          softmax_block<D, true>(p.scale_log2, BF16, t_scores, t_out, j == 0, hide, t.p_full_bar[tile], lane, &m_used, &l_run);
         }
         // The last product.
         if (ok && my_blocks > 0) {
@@ -457,7 +453,7 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
           tc_fence_after_sync();
         }
         const bool patch = *reinterpret_cast<volatile uint32_t *>(&t.patch_flag[count & 1]) == static_cast<uint32_t>(count);
-        finish_row<D>(p, u, t_out, tile, in_tile, pos, my_blocks, ok, patch, m_used, l_run);
+        finish_row<D, BF16>(p, u, t_out, tile, in_tile, pos, my_blocks, ok, patch, m_used, l_run);
         // The next unit's first product overwrites this output: it waits for probabilities that the tile's
         // four warps hand over only after these reads.
         tc_fence_before_sync();
@@ -547,7 +543,7 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       // ------------------------------------------------------------------ MMA issuer
       // The whole warp walks the loop and an elected lane issues.
       const bool issuer = elect_one();
-      const TileMmas<D> mma(p.is_bf16, true, tmem_base, smem_u32(q_tile(0)), issuer);
+      const TileMmas<D> mma(BF16, true, tmem_base, smem_u32(q_tile(0)), issuer);
       const uint64_t sdesc0 = umma_desc_sw128(smem_u32(slot(0)));
       bool ok = true;
       uint32_t clean_phase = 0;  // bit i: the parity of the next unclean values in slot i
@@ -650,7 +646,7 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       // ------------------------------------------------------------------ values that are not seen by all
       const int which = static_cast<int>(warp) - kHelpWarp;
       // A half whose exponent is all ones carries into its sign bit.
-      const uint32_t exponent = p.is_bf16 ? 0x7F807F80u : 0x7C007C00u, carry = p.is_bf16 ? 0x00800080u : 0x04000400u;
+      constexpr uint32_t exponent = BF16 ? 0x7F807F80u : 0x7C007C00u, carry = BF16 ? 0x00800080u : 0x04000400u;
       bool ok = true;
       int n = 0;
       int unit = blockIdx.x;
@@ -670,7 +666,7 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
           uint8_t *block = slot(nv % S) + lane * 16;
           const int x0 = u.walk.place0(j);
           uint32_t odd = 0;  // the sign bits of halves whose exponent is all ones
-#pragma unroll 4
+#pragma unroll 1  // (unrolled by four: 157 us instead of 151, 8192 tokens under a window; the kernel's instructions no longer fit so well)
           for (int r = which * 4; r < kBlockKv; r += kHelpWarps * 4) {  // four keys' 128 bytes of an atom
             const int x = x0 + r + static_cast<int>(lane >> 3);
             const bool hidden = u.walk.hidden(x), mixed = !hidden && u.walk.mixed(x);
@@ -692,8 +688,8 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
               for (int a = 0; a < L::kQAtoms; ++a) {
                 uint4 *at = reinterpret_cast<uint4 *>(block + a * kBlockKv * kAtomBytes + r * kAtomBytes);
                 const uint4 w = *at;
-                *at = p.is_bf16 ? without_nonfinite<true>(w) : without_nonfinite<false>(w);
-                taken = taken || (p.is_bf16 ? has_nonfinite<true>(w) : has_nonfinite<false>(w));
+                *at = without_nonfinite<BF16>(w);
+                taken = taken || has_nonfinite<BF16>(w);
               }
             }
           }
@@ -729,10 +725,10 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
   }
 }
 
-template <int D>
+template <int D, bool BF16>
 cudaError_t launch(const CUtensorMap &tq, const CUtensorMap (&maps)[6], const TilesParams &p, int64_t ctas, cudaStream_t stream) {
   using L = Layout<D>;
-  auto kernel = cache_tiles_kernel<D>;
+  auto kernel = cache_tiles_kernel<D, BF16>;
   static const cudaError_t attr_set = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmemBytes);
   if (attr_set != cudaSuccess) return attr_set;
   return launch_overlapped(kernel, ctas, kThreads, L::kSmemBytes, stream, tq, maps[0], maps[1], maps[2], maps[3], maps[4], maps[5], p);
@@ -791,7 +787,8 @@ cudaError_t cache_tiles(TilesParams p, const CacheAttentionArgs &a, const char *
   if (!prefix) maps[4] = maps[0], maps[5] = maps[1];
   const int64_t ctas = static_cast<int64_t>(p.runs) * p.row_pairs * p.splits;
   *why = "launching the tile kernel";
-  cudaError_t e = a.head_dim == 64 ? launch<64>(tq, maps, p, ctas, a.stream) : launch<128>(tq, maps, p, ctas, a.stream);
+  cudaError_t e = a.head_dim == 64 ? (a.is_bf16 ? launch<64, true>(tq, maps, p, ctas, a.stream) : launch<64, false>(tq, maps, p, ctas, a.stream))
+                                   : (a.is_bf16 ? launch<128, true>(tq, maps, p, ctas, a.stream) : launch<128, false>(tq, maps, p, ctas, a.stream));
   if (e != cudaSuccess || p.over_batch || p.splits == 1) return e;
   *why = "launching the kernel that adds the parts";
   const int64_t total = static_cast<int64_t>(p.runs) * p.rows * (a.head_dim / 4);

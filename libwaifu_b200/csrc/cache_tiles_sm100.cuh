@@ -14,7 +14,6 @@ struct TilesParams {
   uint16_t *out;
   int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3];
   const int32_t *kv_lens;
-  int is_bf16;
   int kv_heads, group, q_len, kv_len;
   int window, sinks;
   int prefix_len;   // keys that every row sees, walked first; 0 without
