@@ -49,34 +49,6 @@ constexpr int kIssueRegs = 96, kSoftmaxRegs = 200;
 static_assert(128 * kIssueRegs + kSoftmaxWarps * 32 * kSoftmaxRegs <= kThreads * 168, "no more than the block was launched with");
 constexpr int kMaxSlots = 6;
 
-struct Tail {
-  uint4 claim;         // the answer to the last try_cancel
-  uint64_t claim_bar;  // ... which has arrived
-  uint64_t unit_full_bar[2], unit_empty_bar[2];  // producer -> all: the next unit is in next_unit[slot]; all -> producer
-  int next_unit[2];                              // -1 when there is none left
-  uint64_t q_full_bar[kTiles], q_empty_bar[kTiles];
-  uint64_t slot_full_bar[kMaxSlots], slot_empty_bar[kMaxSlots], slot_clean_bar[kMaxSlots];
-  uint64_t s_full_bar[kTiles];     // MMA -> softmax: the tile's scores are in tensor memory
-  uint64_t p_full_bar[kTiles][2];  // softmax -> MMA: that part of the tile's probabilities is in tensor memory
-  uint64_t pv_done_bar[kTiles];    // MMA -> softmax: the last block is in the tile's output
-  uint32_t tmem_base_slot;
-  uint32_t abort_flag;
-  uint32_t patch_flag[2];  // the last unit of an even and of an odd count that had values taken out of a block
-};
-
-template <int D>
-struct Layout : TileLayout<D> {
-  using T = TileLayout<D>;
-  static constexpr int kRoom = (227 * 1024 - kTiles * T::kQBytes - static_cast<int>(sizeof(Tail))) / T::kSlotBytes;
-  static constexpr int kSlots = kRoom < kMaxSlots ? kRoom : kMaxSlots;
-  static_assert(kSlots >= 3, "K of the next block, V of this one and a load in flight");
-  static constexpr int kQOff = 0;
-  static constexpr int kSlotOff = kQOff + kTiles * T::kQBytes;
-  static constexpr int kTailOff = kSlotOff + kSlots * T::kSlotBytes;
-  static constexpr int kSmemBytes = kTailOff + static_cast<int>(sizeof(Tail));
-  static_assert(kSmemBytes <= 227 * 1024, "shared memory");
-};
-
 // The blocks of a walk that hold keys some row does not see: from one up to another (sinks, the windows' starts), and from one
 // on (the rows' own positions, the end).
 struct Dirty {
@@ -96,12 +68,15 @@ struct Walk {
   int window, sinks;
   Dirty dirty;              // (keys past a prefix's end come as zeros: its blocks never are)
 
-  __device__ __forceinline__ void find_dirty() {
+  // The blocks of own keys that some row at first .. last does not see whole.
+  __device__ __forceinline__ Dirty dirty_for(int first_row_pos, int last_row_pos) const {
     const int own = prefix_blocks - first;  // the walk's first own block, in this split
     auto block_of = [](int place) { return place < 0 ? 0 : place / kBlockKv; };
-    dirty.begin = own + block_of(pad > 0 ? sinks : sinks - begin);
-    dirty.end = own + (last_pos - window - begin + pad < 0 ? 0 : block_of(last_pos - window - begin + pad) + 1);
-    dirty.from = own + block_of(first_pos + 1 + pad - begin);
+    Dirty d;
+    d.begin = own + block_of(pad > 0 ? sinks : sinks - begin);
+    d.end = own + (last_row_pos - window - begin + pad < 0 ? 0 : block_of(last_row_pos - window - begin + pad) + 1);
+    d.from = own + block_of(first_row_pos + 1 + pad - begin);
+    return d;
   }
   __device__ __forceinline__ bool in_prefix(int j) const { return first + j < prefix_blocks; }
   __device__ __forceinline__ int place0(int j) const { return (first + j - prefix_blocks) * kBlockKv; }
@@ -117,6 +92,35 @@ struct Walk {
   __device__ __forceinline__ int blocks_up_to(int position) const {
     return prefix_blocks + (position < 0 ? 0 : (position - begin + pad) / kBlockKv + 1);
   }
+};
+
+struct Tail {
+  uint4 claim;         // the answer to the last try_cancel
+  uint64_t claim_bar;  // ... which has arrived
+  uint64_t unit_full_bar[2], unit_empty_bar[2];  // producer -> all: the next unit is in next_unit[slot]; all -> producer
+  int next_unit[2];                              // -1 when there is none left
+  uint64_t q_full_bar[kTiles], q_empty_bar[kTiles];
+  uint64_t slot_full_bar[kMaxSlots], slot_empty_bar[kMaxSlots], slot_clean_bar[kMaxSlots];
+  uint64_t s_full_bar[kTiles];     // MMA -> softmax: the tile's scores are in tensor memory
+  uint64_t p_full_bar[kTiles][2];  // softmax -> MMA: that part of the tile's probabilities is in tensor memory
+  uint64_t pv_done_bar[kTiles];    // MMA -> softmax: the last block is in the tile's output
+  uint32_t tmem_base_slot;
+  uint32_t abort_flag;
+  uint32_t patch_flag[2];  // the last unit of an even and of an odd count that had values taken out of a block
+  Walk walk[kSoftmaxWarps];  // of the unit that the warp works on
+};
+
+template <int D>
+struct Layout : TileLayout<D> {
+  using T = TileLayout<D>;
+  static constexpr int kRoom = (227 * 1024 - kTiles * T::kQBytes - static_cast<int>(sizeof(Tail))) / T::kSlotBytes;
+  static constexpr int kSlots = kRoom < kMaxSlots ? kRoom : kMaxSlots;
+  static_assert(kSlots >= 3, "K of the next block, V of this one and a load in flight");
+  static constexpr int kQOff = 0;
+  static constexpr int kSlotOff = kQOff + kTiles * T::kQBytes;
+  static constexpr int kTailOff = kSlotOff + kSlots * T::kSlotBytes;
+  static constexpr int kSmemBytes = kTailOff + static_cast<int>(sizeof(Tail));
+  static_assert(kSmemBytes <= 227 * 1024, "shared memory");
 };
 
 struct Unit {
@@ -156,8 +160,7 @@ struct Unit {
     active = p.splits == 1 ? 1 : max(1, (total + per_split - 1) / per_split);
     walk.first = split * per_split;
     walk.count = max(0, min(per_split, total - walk.first));  // (0 past the active splits)
-    walk.find_dirty();
-    if (p.over_batch) walk.dirty = Dirty{0, 0, INT32_MAX};
+    walk.dirty = p.over_batch ? Dirty{0, 0, INT32_MAX} : walk.dirty_for(walk.first_pos, walk.last_pos);
 #pragma unroll
     for (int i = 0; i < kTiles; ++i) {
       const int first_row = row0 + i * p.tile_rows, last = min(first_row + p.tile_rows, p.rows) - 1;
@@ -178,12 +181,31 @@ struct Todo {
 // Bits 0 .. n - 1.
 __device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u); }
 
-// Of a block's keys, the first of which is key0, the row sees those up to `last` that are behind `before`, and the first `sinks`.
+// Sets the scores of the keys of block j that the row at `pos` does not see to -inf, where there are any for its tile. What
+// it takes of the walk lies in shared memory: the softmax has no registers to spare for it.
 struct HideUnseen {
   bool edge;
-  int key0, last, before, sinks;
+  const Walk *walk;
+  int j, pos;
   __device__ __forceinline__ void operator()(uint32_t (&sc)[kBlockKv / 32][32]) const {
     if (!edge) return;
+    int key0, last, before, sinks;  // of the block's keys, from key0 on, the row sees those up to `last` behind `before`, and the first `sinks`
+    if (walk->in_prefix(j)) {
+      key0 = (walk->first + j) * kBlockKv;
+      last = walk->prefix_len - 1;
+      before = -1;
+      sinks = 0;
+    } else {
+      const int x0 = walk->place0(j);
+      key0 = x0 - walk->pad + walk->begin;
+      last = pos;
+      before = pos - walk->window;
+      sinks = walk->sinks - key0;
+      if (x0 < walk->pad) {  // sinks, and what follows them
+        before = max(before, walk->begin - 1);
+        sinks = walk->sinks - x0;
+      }
+    }
 #pragma unroll
     for (int c = 0; c < kBlockKv / 32; ++c) {
       const int base = key0 + c * 32;
@@ -405,55 +427,49 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     int unit = blockIdx.x;
 #pragma unroll 1
     for (int count = 1; ok && unit >= 0; ++count) {
-      const Unit u(p, unit);
-      if (u.split < u.active) {
-        const int tile_row0 = u.row0 + tile * p.tile_rows, tile_end = min(tile_row0 + p.tile_rows, p.rows);
-        const int my_blocks = tile == 0 ? u.blocks[0] : u.blocks[1];
-        const int in_tile = static_cast<int>(quarter) * 32 + static_cast<int>(lane);
-        const int pos = p.by_group.quotient(max(0, min(tile_row0 + in_tile, tile_end - 1))) + u.len - p.q_len;
-        // What every row of the tile sees.
-        const int common_last = p.by_group.quotient(tile_row0) + u.len - p.q_len;
-        const int common_before = p.by_group.quotient(max(0, tile_end - 1)) + u.len - p.q_len - p.window;
-        float m_used = -INFINITY;
-        float l_run = 0.0f;
-        for (int j = 0; j < my_blocks && ok; ++j) {
-          // (Scores of block j are issued behind the product of block j - 1: once they are here the tile's
-          // output is complete up to that block.)
-          ok = __all_sync(0xffffffffu, mbar_wait(&t.s_full_bar[tile], s_phase, &abort_flag));
-          if (!ok) break;
-          s_phase ^= 1;
-          tc_fence_after_sync();
-          HideUnseen hide;
-          if (u.walk.in_prefix(j)) {
-            hide.key0 = (u.walk.first + j) * kBlockKv;
-            hide.edge = hide.key0 + kBlockKv > p.prefix_len;
-            hide.last = p.prefix_len - 1;
-            hide.before = -1;
-            hide.sinks = 0;
-          } else {
-            const int x0 = u.walk.place0(j);
-            hide.key0 = x0 - u.walk.pad + u.walk.begin;
-            hide.last = pos;
-            if (x0 < u.walk.pad) {  // sinks, and what follows them
-              hide.edge = x0 + kBlockKv > p.sinks;
-              hide.before = max(pos - p.window, u.walk.begin - 1);
-              hide.sinks = p.sinks - x0;
-            } else {
-              hide.edge = hide.key0 + kBlockKv - 1 > common_last || (hide.key0 + kBlockKv - 1 >= p.sinks && hide.key0 <= common_before);
-              hide.before = pos - p.window;
-              hide.sinks = p.sinks - hide.key0;
-            }
-          }
-          softmax_block<D, true>(p.scale_log2, BF16, t_scores, t_out, j == 0, hide, t.p_full_bar[tile], lane, &m_used, &l_run);
+      // What the loop needs of the unit; the rest is worked out again behind it.
+      int my_blocks, pos;
+      Dirty edges;
+      bool active;
+      {
+        const Unit u(p, unit);
+        active = u.split < u.active;
+        my_blocks = tile == 0 ? u.blocks[0] : u.blocks[1];
+        const int tile_row0 = u.row0 + tile * p.tile_rows, tile_end = min(tile_row0 + p.tile_rows, p.rows), offset = u.len - p.q_len;
+        pos = p.by_group.quotient(max(0, min(tile_row0 + static_cast<int>(threadIdx.x % kBlockQ), tile_end - 1))) + offset;
+        const int first = p.by_group.quotient(tile_row0) + offset, last = p.by_group.quotient(max(0, tile_end - 1)) + offset;
+        edges = u.walk.dirty_for(first, last);
+        if (p.prefix_len > 0) {  // (no window there)
+          edges.end = u.walk.prefix_blocks - u.walk.first;
+          edges.begin = edges.end - (p.prefix_len % kBlockKv != 0 ? 1 : 0);
+          if (p.over_batch) edges.from = INT32_MAX;
         }
-        // The last product.
-        if (ok && my_blocks > 0) {
-          ok = __all_sync(0xffffffffu, mbar_wait(&t.pv_done_bar[tile], pv_phase, &abort_flag));
-          pv_phase ^= 1;
-          tc_fence_after_sync();
-        }
+        if (lane == 0) t.walk[warp] = u.walk;
+        __syncwarp();
+      }
+      float m_used = -INFINITY;
+      float l_run = 0.0f;
+      for (int j = 0; j < my_blocks && ok; ++j) {
+        // (Scores of block j are issued behind the product of block j - 1: once they are here the tile's
+        // output is complete up to that block.)
+        ok = __all_sync(0xffffffffu, mbar_wait(&t.s_full_bar[tile], s_phase, &abort_flag));
+        if (!ok) break;
+        s_phase ^= 1;
+        tc_fence_after_sync();
+        const HideUnseen hide{edges.has(j), &t.walk[warp], j, pos};
+        softmax_block<D, true>(p.scale_log2, BF16, t_scores, t_out, j == 0, hide, t.p_full_bar[tile], lane, &m_used, &l_run);
+      }
+      // The last product.
+      if (ok && my_blocks > 0) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&t.pv_done_bar[tile], pv_phase, &abort_flag));
+        pv_phase ^= 1;
+        tc_fence_after_sync();
+      }
+      if (active) {
+        asm volatile("" : "+r"(unit));  // (or what is worked out here would stay in registers from above)
+        const Unit u(p, unit);
         const bool patch = *reinterpret_cast<volatile uint32_t *>(&t.patch_flag[count & 1]) == static_cast<uint32_t>(count);
-        finish_row<D, BF16>(p, u, t_out, tile, in_tile, pos, my_blocks, ok, patch, m_used, l_run);
+        finish_row<D, BF16>(p, u, t_out, tile, static_cast<int>(threadIdx.x % kBlockQ), pos, my_blocks, ok, patch, m_used, l_run);
         // The next unit's first product overwrites this output: it waits for probabilities that the tile's
         // four warps hand over only after these reads.
         tc_fence_before_sync();
