@@ -44,8 +44,9 @@ __device__ __forceinline__ void store_32_bytes(void *dst, uint32_t a, uint32_t b
                : "memory");
 }
 
+// (Read past L1: a kernel that starts under the end of another may find a line there from before the lengths were written.)
 __device__ __forceinline__ int sequence_length(const int32_t *kv_lens, int seq, int kv_len) {
-  return kv_lens == nullptr ? kv_len : min(max(kv_lens[seq], 0), kv_len);
+  return kv_lens == nullptr ? kv_len : min(max(__ldcg(kv_lens + seq), 0), kv_len);
 }
 
 // Keys 0 .. sinks - 1 and begin .. end - 1, counted through.

@@ -748,8 +748,10 @@ size_t round_256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
 // 24.3, 36 rows 32.5 and 24.7, 68 rows 46.6 and 25.9; one sequence: 36 rows 16.0 and 14.0).
 constexpr int kMostTileHeads = 128;
 constexpr int kTilesFromRows = 17;
-// With the keys' weights, for which the tensor cores compute the scores a second time and the others store them:
+// With the keys' weights, for which the tensor cores compute the scores a second time and the few-row kernel stores them, from
+// so many (32 x 8 heads over 2000 keys: 36 rows 122 and 171 us, 68 rows 197 and 173), or where the scores took over 256 MiB.
 constexpr int kWeightTilesFromRows = 64;
+constexpr int64_t kMostScores = int64_t{64} << 20;
 
 int64_t score_pitch_of(int kv_len) { return (static_cast<int64_t>(kv_len) + kKeysAtOnce - 1) / kKeysAtOnce * kKeysAtOnce; }
 
@@ -782,7 +784,9 @@ CachePlan cache_plan(const CacheAttentionArgs &a) {
   const int64_t d = a.head_dim;
   p.rows = group * a.q_len;
   // (a tile holds whole queries, so their heads have to go into it)
-  p.tiles = p.rows >= (a.weights_out != nullptr ? kWeightTilesFromRows : kTilesFromRows) && group <= kMostTileHeads;
+  const int64_t scores = static_cast<int64_t>(a.batch) * a.kv_heads * p.rows * a.kv_len;
+  const bool many_rows = p.rows >= kTilesFromRows && (a.weights_out == nullptr || p.rows >= kWeightTilesFromRows || scores > kMostScores);
+  p.tiles = many_rows && group <= kMostTileHeads;
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t off = at;

@@ -8,7 +8,9 @@
 // tensor memory at a time, so that a block's product runs under the exponentials of the one before it. The
 // walks of a key's tiles are divided over CTAs, whose sums the last one to arrive adds in their order.
 //
-// What bounds it is the special-function unit: 16 exponentials a cycle and SM against 128 x 128 of them a tile and block.
+// What bounds it is the special-function unit: 16 exponentials a cycle and SM against 128 x 128 of them a tile and block, 23 of
+// the 37 us that 2 x 16 heads of 2048 queries and keys take. They are all the hardware's (2^-22), unlike the attention
+// kernel's, whose cubic (7.5e-5 in one of four) a row's sum carries.
 #include "cache_weights_sm100.cuh"
 
 #include <cuda_runtime.h>
@@ -323,7 +325,7 @@ WeightsPlan cache_weights_plan(const CacheAttentionArgs &a, int tile_rows, int m
   plan.part_blocks = static_cast<int>(longest);
   if (runs * plan.pairs <= most_units) {
     // The shortest parts (eight blocks at least) of which there are no more than SMs, for sequences that fill the cache: one
-    // round of CTAs (2 x 4 runs of 2048 keys and queries: parts of 14 blocks in three rounds 53 us, of 20 in one 31).
+    // round of CTAs (2 x 4 runs of 2048 keys, four heads and 2048 queries each: parts of 14 blocks in three rounds 53 us, of 20 in one 37).
     auto parts_of = [&](int64_t part) {
       int64_t sum = 0;
       for (int pair = 0; pair < plan.pairs; ++pair) {

@@ -9,8 +9,9 @@ weight x |value| over them, B the largest sum of |q k| / sqrt(D) behind a score,
   (2^-12 + n 2^-23) A     exponentials (a cubic good to 7.5e-5 in numerator and denominator) and the sums over keys.
 These are sums of the worst; over a whole result, where roundings are spread evenly, fl_attention's bound holds too: a
 relative L2 error of at most 5e-3.
-A key's weight W, added up over R queries: 2 (D + 4) 2^-23 B + 2^-20 + (n + R) 2^-23 of it (exponentials by the
-hardware's function, 2^-22), and 2^-23 of the total for the additions to what was there."""
+A key's weight W, added up over R queries: 2 (D + 4) 2^-23 B + 2^-20 + 2^-13 + (n + R) 2^-23 of it (exponentials by the
+hardware's function, 2^-22, but for the rows' sums, which may hold the cubic's 7.5e-5 < 2^-13), and 2^-23 of the total
+for the additions to what was there."""
 import numpy as np
 import pytest
 
@@ -95,6 +96,10 @@ WINDOW = [
     (1, 2, 2, 600, 600, 64, 1, 0, None),                   # every query sees itself alone
     (2, 4, 2, 300, 700, 128, 250, 40, [700, 511]),
     (1, 3, 3, 1100, 1100, 128, 300, 4, [1093]),
+    (1, 100, 1, 2, 300, 128, 77, 9, [291]),                # a tile of one query's 100 heads
+    (1, 150, 1, 3, 200, 64, 60, 5, [170]),                 # more heads than a tile holds
+    (3, 10, 2, 60, 70, 128, 9, 33, [70, 40, 0]),           # sinks beyond the window's start
+    (2, 4, 4, 40, 9000, 64, 5000, 300, [9000, 8000]),      # few units whose blocks are divided; sinks over whole blocks
 ]
 
 
@@ -124,6 +129,9 @@ PREFIX = [
     (2, 4, 4, 200, 260, 64, 300, [260, 150]),
     (3, 4, 1, 129, 140, 128, 513, [140, 129, 60]),
     (1, 2, 1, 1, 30, 128, 5000, None),
+    (30, 3, 1, 2, 50, 64, 1300, None),                   # 21 sequences of six rows to a tile
+    (2, 150, 1, 1, 33, 64, 290, [33, 2]),                # more heads than a tile holds
+    (2, 2, 1, 150, 200, 128, 3000, [200, 30]),           # few units whose walk over prefix and own keys is divided
 ]
 
 
@@ -149,6 +157,9 @@ WEIGHTS = [
     (2, 4, 1, 150, 150, 128, [150, 149]),
     (1, 6, 2, 333, 700, 64, [611]),
     (2, 2, 2, 700, 500, 128, [500, 130]),        # queries before every key
+    (2, 12, 2, 7, 1001, 128, [1001, 600]),       # stored scores of three tiles of rows
+    (1, 150, 1, 2, 130, 64, None),
+    (1, 2, 1, 200, 5000, 64, [4990]),            # keys whose queries' blocks are few
 ]
 
 
@@ -169,7 +180,7 @@ def test_weights(flint, oracle, N, H, Hk, L, S, D, lens, is_bf16, tokens):
     assert (got_w[:, :, S:] == 7.0).all()
     want, weights, size, score = C.attention(c.value("q"), c.value("k"), c.value("v"), lens)
     check_out(got, want, size, score, S, is_bf16, "weights' output")
-    tol = (2 * (D + 4) * 2.0 ** -23 * score.max() + 2.0 ** -20 + (S + H // Hk * L) * 2.0 ** -23) * weights + 2.0 ** -23 * (before + weights)
+    tol = (2 * (D + 4) * 2.0 ** -23 * score.max() + 2.0 ** -20 + 2.0 ** -13 + (S + H // Hk * L) * 2.0 ** -23) * weights + 2.0 ** -23 * (before + weights)
     off = np.abs(got_w[:, :, :S] - (before + weights)) / tol
     assert off.max() <= 1.0, f"{off.max():.2f} of the tolerance"
 
@@ -225,6 +236,65 @@ def test_a_length_outside_the_cache_counts_as_the_nearest(flint, oracle):
     check_out(got, want, size, score, 21, True, "lengths")
 
 
+@pytest.mark.parametrize("L", [1, 40])
+def test_offsets_past_32_bits(flint, oracle, L):
+    """Sequences of a cache that lie 3 GiB apart, the third past 2^31 elements from its start."""
+    import torch
+    F, O = flint, oracle
+    H, Hk, S, D, apart = 4, 2, 300, 64, 3 << 29
+    rng = np.random.default_rng(L)
+    store = torch.empty(2 * apart + Hk * S * D, dtype=torch.bfloat16, device="cuda")
+    q, k, v = (O.narrow(rng.standard_normal((3, h, n, D)).astype(np.float32), True) for h, n in ((H, L), (Hk, S), (Hk, S)))
+    at = {}
+    for name, a in (("k", k), ("v", v)):
+        for n in range(3):
+            store[n * apart:n * apart + Hk * S * D] = torch.from_numpy(a[n].reshape(-1).view(np.int16)).cuda().view(torch.bfloat16)
+        t = F.Tensor.from_device_ptr(store.data_ptr(), (3, Hk, S, D), F.DType.BFLOAT16, keepalive=store, stride=(apart, S * D, D, 1), numel=store.numel())
+        if name == "k":  # (v in storage of its own, as far apart)
+            store = torch.empty_like(store)
+        at[name] = t
+    torch.cuda.synchronize()
+    widen = lambda a: O.widen(a, True).astype(np.float64)  # noqa: E731
+    out = F.attention_window(dev(F, q, F.DType.BFLOAT16), at["k"], at["v"], 200, 3)
+    want, _, size, score = C.attention(widen(q), widen(k), widen(v), None, 200, 3)
+    check_out(widen(out.numpy()), want, size, score, 203, True, "far apart")
+    w, fresh = dev(F, rng.random((3, Hk, S)).astype(np.float32), F.DType.FLOAT), torch.empty(3, Hk, 100, D, dtype=torch.bfloat16, device="cuda")
+    ko = F.Tensor.from_device_ptr(fresh.data_ptr(), (3, Hk, 100, D), F.DType.BFLOAT16, keepalive=fresh)
+    F.cache_evict(at["k"], at["v"], w, 100, 10, k_out=ko)
+    kept = C.evict(w.numpy(), None, 100, 10)
+    F.synchronize()
+    assert np.array_equal(ko.numpy()[2, 1], k[2, 1, kept[2, 1]])
+
+
+def test_calls_from_two_threads(flint, oracle):
+    """Calls of different shapes at once: the workspace is theirs in turn."""
+    import threading
+    F = flint
+    cases = [Cache(F, oracle, 5, 2, 4, 2, 1, 3000, 128, True, [3000, 1111]), Cache(F, oracle, 6, 1, 6, 2, 150, 800, 64, False, [777])]
+    devices, results = [c.device() for c in cases], [[], []]
+    wants = [C.attention(c.value("q"), c.value("k"), c.value("v"), c.lens) for c in cases]
+    weights = [np.zeros((c.shape[0], c.shape[2], c.shape[4]), np.float32) for c in cases]
+
+    def work(i):
+        t = devices[i]
+        for _ in range(20):
+            w = dev(F, weights[i], F.DType.FLOAT)
+            out, w = F.attention_weights(t["q"], t["k"], t["v"], w, t["lens"])
+            results[i].append((out.numpy(), w.numpy()))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    F.synchronize()
+    for i, c in enumerate(cases):
+        want, _, size, score = wants[i]
+        assert len(results[i]) == 20
+        check_out(oracle.widen(results[i][0][0], c.is_bf16).astype(np.float64), want, size, score, c.shape[4], c.is_bf16, f"thread {i}")
+        assert all(np.array_equal(a, results[i][0][0]) and np.array_equal(b, results[i][0][1]) for a, b in results[i])
+
+
 EVICT = [
     # N, Hk, S, D, keep, recent, room, lens
     (1, 1, 1, 64, 1, 0, 1, None),
@@ -232,6 +302,8 @@ EVICT = [
     (2, 3, 3000, 128, 1025, 1025, 1025, [3000, 1026]),   # the recent ones alone
     (2, 1, 2500, 24, 1200, 0, 1300, [2500, 0]),          # none of them; a sequence without keys
     (1, 2, 100, 8, 100, 5, 100, None),                   # nothing to evict
+    (2, 1, 60000, 8, 777, 20, 777, [60000, 30011]),      # more weights than fit in shared memory
+    (1, 1, 30000, 8, 20000, 9000, 20000, None),          # ... or with a list beside them
 ]
 
 
