@@ -755,10 +755,22 @@ constexpr int64_t kMostScores = int64_t{64} << 20;
 
 int64_t score_pitch_of(int kv_len) { return (static_cast<int64_t>(kv_len) + kKeysAtOnce - 1) / kKeysAtOnce * kKeysAtOnce; }
 
-// The least blocks of 128 keys of a prefix that are worth a CTA of the tile kernel: a CTA of four takes some 11 us to begin and
-// to write its parts, and 2.3 us a block, while the kernel over the own keys has the other SMs (64 sequences behind 8192
-// keys: parts of four blocks 60 us, of eight 50; of sixteen 72 before the two overlapped).
+// The blocks of 128 keys of a prefix to a CTA of the tile kernel: it takes some 11 us to begin and to write its parts, and 2.3 us a
+// block, while the kernel over the own keys has the other SMs (64 sequences behind 8192 keys: parts of four blocks 60 us, of
+// eight 50; of sixteen 72 before the two overlapped).
 constexpr int kPrefixBlocks = 8;
+// A run's own blocks are divided into parts of so many where there are SMs for them.
+constexpr int kOwnBlocks = 4;
+// Up to two tiles of 16 rows over less than so many keys of all heads stay with the few-row kernel (24 rows of one head, 257
+// keys: 8.6 us, on the tensor cores 12.1, one launch more; 24 rows of eight heads over 5000 keys 26.2 and 20.7).
+constexpr int kFewPrefixRows = 32;
+constexpr int64_t kFewPrefixKeys = 16384;
+
+bool prefix_on_tiles(const CacheAttentionArgs &a, int rows) {  // of a run; the batch's together over the prefix
+  const int64_t together = static_cast<int64_t>(a.batch) * rows;
+  if (together < kTilesFromRows || rows > kMostTileHeads) return false;
+  return together > kFewPrefixRows || static_cast<int64_t>(a.kv_heads) * a.prefix_len >= kFewPrefixKeys;
+}
 
 int tile_rows_of(int rows) { return rows <= 8 ? 8 : 16; }
 
@@ -801,14 +813,14 @@ CachePlan cache_plan(const CacheAttentionArgs &a) {
     most = std::min<int64_t>(a.kv_len, static_cast<int64_t>(a.window) + a.sinks + std::min(a.q_len, cache_tiles_positions(group)));
     p.tile_rows = cache_tile_rows(group);
     p.row_tiles = cache_tiles_pairs(p.rows, p.tile_rows);
-    p.splits = cache_tiles_splits(runs * p.row_tiles, static_cast<int>(std::min<int64_t>(most + a.prefix_len, INT32_MAX)), 4);
+    p.splits = cache_tiles_splits(runs * p.row_tiles, static_cast<int>(std::min<int64_t>(most + a.prefix_len, INT32_MAX)), kOwnBlocks);
     part_rows = p.splits > 1 ? cache_tiles_part_rows(runs * p.row_tiles, p.splits, p.tile_rows) : 0;
   } else {
     p.tile_rows = tile_rows_of(p.rows);
     p.row_tiles = (p.rows + p.tile_rows - 1) / p.tile_rows;
     const int64_t steps = (most + kStepKeys - 1) / kStepKeys, least = std::min<int64_t>(kLeastSteps, steps);  // of a unit, and of a CTA
     // (beside a prefix's tile kernel, whose CTAs hold their SMs for a while, in two rounds: the SMs it leaves free take more of them)
-    const bool beside_tiles = a.prefix_len > 0 && static_cast<int64_t>(a.batch) * p.rows >= kTilesFromRows && p.rows <= kMostTileHeads;
+    const bool beside_tiles = a.prefix_len > 0 && prefix_on_tiles(a, p.rows);
     p.ctas = static_cast<int>(std::min<int64_t>((beside_tiles ? 2 : 1) * kCtasPerSm * sm_count(), (runs * p.row_tiles * steps + least - 1) / least));
     part_rows = static_cast<size_t>(p.ctas) * 2 * p.tile_rows;
   }
@@ -819,7 +831,7 @@ CachePlan cache_plan(const CacheAttentionArgs &a) {
   if (a.prefix_len > 0 && !p.tiles) {
     p.prefix_apart = true;
     p.prefix_rows = a.batch * p.rows;
-    p.prefix_tiles = p.prefix_rows >= kTilesFromRows && p.rows <= kMostTileHeads;
+    p.prefix_tiles = prefix_on_tiles(a, p.rows);
     if (p.prefix_tiles) {
       p.own_out = take(static_cast<size_t>(runs) * p.rows * d * 4);
       p.own_sum = take(static_cast<size_t>(runs) * p.rows * 8);

@@ -758,11 +758,11 @@ int cache_tiles_pairs(int rows, int tile_rows) { return (rows + kTiles * tile_ro
 
 int cache_tiles_positions(int group) { return kTiles * (kBlockQ / group); }
 
-int cache_tiles_splits(int64_t units, int keys, int least_blocks) {
+int cache_tiles_splits(int64_t units, int keys, int part_blocks) {
   const int blocks = (keys + kBlockKv - 1) / kBlockKv;
   if (units >= sm_count()) return 1;
   // One CTA an SM, and no more of them than SMs.
-  const int wanted = static_cast<int>(std::min<int64_t>(sm_count() / units, std::max(1, blocks / least_blocks)));
+  const int wanted = static_cast<int>(std::min<int64_t>(sm_count() / units, std::max(1, (blocks + part_blocks - 1) / part_blocks)));
   const int per_split = (blocks + wanted - 1) / wanted;
   return (blocks + per_split - 1) / per_split;
 }

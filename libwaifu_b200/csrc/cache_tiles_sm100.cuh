@@ -37,8 +37,9 @@ struct TilesParams {
 int cache_tile_rows(int whole);
 int cache_tiles_pairs(int rows, int tile_rows);
 int cache_tiles_positions(int group);  // the most that the rows of a pair lie on
-// `keys`: the most that a pair's rows see between them; a part has `least_blocks` blocks of 128 of them at least.
-int cache_tiles_splits(int64_t units, int keys, int least_blocks);
+// `keys`: the most that a pair's rows see between them; parts of about `part_blocks` blocks of 128 of them, longer ones where
+// there were more than SMs.
+int cache_tiles_splits(int64_t units, int keys, int part_blocks);
 size_t cache_tiles_part_rows(int64_t units, int splits, int tile_rows);
 // Two launches where a pair's blocks are divided and the rows are not those of a whole batch over a prefix: the second adds the parts.
 cudaError_t cache_tiles(TilesParams p, const CacheAttentionArgs &a, const char **why);
