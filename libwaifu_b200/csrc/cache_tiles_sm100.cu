@@ -106,7 +106,9 @@ struct Tail {
   uint64_t pv_done_bar[kTiles];    // MMA -> softmax: the last block is in the tile's output
   uint32_t tmem_base_slot;
   uint32_t abort_flag;
-  uint32_t patch_flag[2];  // the last unit of an even and of an odd count that had values taken out of a block
+  // The last unit of a count (mod 4) that had values taken out of a block. The helping warps may be two units ahead of the
+  // softmax (one without blocks between), so two places would not do.
+  uint32_t patch_flag[4];
   Walk walk[kSoftmaxWarps];  // of the unit that the warp works on
 };
 
@@ -365,7 +367,7 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
   }
   if (threadIdx.x == 0) {
     t.abort_flag = 0;
-    t.patch_flag[0] = t.patch_flag[1] = 0;
+    for (uint32_t &flag : t.patch_flag) flag = 0;
     mbar_init(&t.claim_bar, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&t.unit_full_bar[i], 1);
@@ -468,7 +470,7 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       if (active) {
         asm volatile("" : "+r"(unit));  // (or what is worked out here would stay in registers from above)
         const Unit u(p, unit);
-        const bool patch = *reinterpret_cast<volatile uint32_t *>(&t.patch_flag[count & 1]) == static_cast<uint32_t>(count);
+        const bool patch = *reinterpret_cast<volatile uint32_t *>(&t.patch_flag[count & 3]) == static_cast<uint32_t>(count);
         finish_row<D, BF16>(p, u, t_out, tile, static_cast<int>(threadIdx.x % kBlockQ), pos, my_blocks, ok, patch, m_used, l_run);
         // The next unit's first product overwrites this output: it waits for probabilities that the tile's
         // four warps hand over only after these reads.
@@ -709,7 +711,7 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
               }
             }
           }
-          if (taken) *reinterpret_cast<volatile uint32_t *>(&t.patch_flag[count & 1]) = static_cast<uint32_t>(count);
+          if (taken) *reinterpret_cast<volatile uint32_t *>(&t.patch_flag[count & 3]) = static_cast<uint32_t>(count);
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {

@@ -212,6 +212,25 @@ def test_what_is_not_seen_may_be_anything(flint, oracle, L, S, window, sinks, le
     assert np.isfinite(got).any()
 
 
+def test_values_that_some_see_beside_sequences_without_keys(flint, oracle):
+    """More sequences than the GPU runs at a time, two of three without keys: a NaN that some queries of each of the
+    others see reaches those queries, whichever sequences are worked on after one another."""
+    N, L, S, D = 900, 40, 96, 64
+    rng = np.random.default_rng(5)
+    lens = np.where(rng.integers(0, 3, N) > 0, 0, rng.integers(60, S + 1, N))
+    c = Cache(flint, oracle, 78, N, 1, 1, L, S, D, True, lens)
+    for n in range(N):
+        c.bits["v"][n, 0, max(lens[n] - 7, 0), n % D] = 0x7FC0
+    t = c.device()
+    want, _, size, score = C.attention(c.value("q"), c.value("k"), c.value("v"), lens, S, 0)
+    size = np.where(np.isfinite(size), size, 0.0)
+    for _ in range(3):
+        flint.attention_window(t["q"], t["k"], t["v"], S, 0, t["lens"], t["out"])
+        got = c.read(t["out"])
+        flint.synchronize()
+        check_out(got, want, size, score, S, True, "beside empty ones")
+
+
 @pytest.mark.parametrize("L", [1, 200])
 def test_peaked_scores_and_equal_results(flint, oracle, L):
     """Scores far apart, so that the running maximum moves; the same call twice gives the same bits."""
