@@ -673,9 +673,9 @@ __global__ void __launch_bounds__(128) join_prefix_kernel(const __grid_constant_
   const int head = p.by_kv_heads.take(&seq);
   RowSum sum;
   sum.clear();
-  const float2 own = p.own_sum[row];
+  const float2 own = __ldcg(&p.own_sum[row]);
   sum.raise(own.x);
-  sum.add(own, *reinterpret_cast<const float4 *>(p.own_out + static_cast<int64_t>(row) * D + col));
+  sum.add(own, __ldcg(reinterpret_cast<const float4 *>(p.own_out + static_cast<int64_t>(row) * D + col)));
   const int64_t first = static_cast<int64_t>(head) * p.prefix_splits * p.prefix_rows + static_cast<int64_t>(seq) * p.rows + r;
   add_parts<D>(p.prefix_splits, p.prefix_sum, p.prefix_out, col, &sum, [&](int c) { return first + static_cast<int64_t>(c) * p.prefix_rows; });
   const float inv = sum.m == -INFINITY ? NAN : 1.0f / sum.l;  // (a row whose every score is -inf has no softmax)
@@ -892,7 +892,8 @@ bool cache_attention_supported(const CacheAttentionArgs &a, const char **why) {
     return false;
   }
   const CachePlan plan = cache_plan(a);
-  if ((plan.tiles && static_cast<int64_t>(a.batch) * a.kv_heads * plan.row_tiles * plan.splits > most) || plan.weights.ctas > most ||
+  const int64_t steps = (static_cast<int64_t>(a.kv_len) + kStepKeys - 1) / kStepKeys * a.batch * a.kv_heads * plan.row_tiles;  // at most
+  if ((!plan.tiles && steps / plan.ctas >= most) || (plan.tiles && static_cast<int64_t>(a.batch) * a.kv_heads * plan.row_tiles * plan.splits > most) || plan.weights.ctas > most ||
       static_cast<int64_t>(a.batch) * a.kv_heads * ((static_cast<int64_t>(a.kv_len) + 255) / 256) > most) {
     *why = "more work than one launch indexes";
     return false;

@@ -2496,6 +2496,20 @@ bool views_overlap(const fl_tensor_view_impl_t &a, const fl_tensor_view_impl_t &
   return raw_ptr(a) < end(b) && raw_ptr(b) < end(a);
 }
 
+// Whether two views have elements in common, as far as their ends tell: views that take turns in memory do not.
+bool views_share(const fl_tensor_view_impl_t &a, const fl_tensor_view_impl_t &b) {
+  if (!views_overlap(a, b)) return false;
+  if (raw_ptr(a) == raw_ptr(b)) return true;
+  auto holds = [](const fl_tensor_view_impl_t &dense, const fl_tensor_view_impl_t &other) {
+    int64_t last = 0;
+    for (size_t i = 0; i < other.shape.size(); ++i) last += static_cast<int64_t>(other.shape[i] - 1) * other.stride[i];
+    const auto *from = raw_ptr(dense), *to = from + numel_of(dense) * dtype_size(dense.data->dtype);
+    const auto *first = raw_ptr(other), *end = first + last * dtype_size(other.data->dtype);
+    return is_contiguous(dense) && ((first >= from && first < to) || (end >= from && end < to));
+  };
+  return holds(a, b) || holds(b, a);
+}
+
 void check_lens(const fl_tensor_view_impl_t &lens, int batch, const char *what) {
   if (dtype_of(lens) != FL_DTYPE_INT32 || lens.shape != std::vector<int32_t>{batch} || !is_contiguous(lens)) {
     invalid(std::string(what) + " is not a contiguous <int32>(" + std::to_string(batch) + ")");
@@ -2563,6 +2577,9 @@ CacheAttentionArgs cache_attention_args(fl_operators_t operators, fl_tensor_view
   if (a.kv_len > kMaxCacheKeys) invalid("attention: more than 2^30 keys");
   for (const auto &t : all) check_rows(*t.view, t.name);
   for (const auto &t : all) check_not_repeated(*t.view, t.name);
+  for (int i = 0; i < 3; ++i) {
+    if (views_share(*all[i].view, out)) invalid(std::string("attention: out shares elements with ") + all[i].name);
+  }
   if (kv_lens_h) {
     const fl_tensor_view_impl_t &lens = deref(kv_lens_h);
     check_lens(lens, a.batch, "kv_lens");
@@ -2636,6 +2653,7 @@ int32_t fl_attention_shared_prefix(fl_operators_t operators, fl_tensor_view_t q,
     check_rows(pv, "the prefix's v");
     check_not_repeated(pk, "the prefix's k");
     check_not_repeated(pv, "the prefix's v");
+    if (views_share(pk, deref(out)) || views_share(pv, deref(out))) invalid("attention: out shares elements with the prefix");
     a.prefix_k = raw_ptr(pk);
     a.prefix_v = raw_ptr(pv);
     a.prefix_len = pk.shape[2];
@@ -2716,6 +2734,9 @@ int32_t fl_cache_evict(fl_operators_t operators, fl_tensor_view_t k_h, fl_tensor
     if (lens_out_h) {
       const fl_tensor_view_impl_t &lens = deref(lens_out_h);
       check_lens(lens, batch, "lens_out");
+      if (kv_lens_h && raw_ptr(lens) != raw_ptr(deref(kv_lens_h)) && views_overlap(lens, deref(kv_lens_h))) {
+        invalid("eviction: lens_out overlaps kv_lens without being the same view");
+      }
       a.lens_out = reinterpret_cast<int32_t *>(raw_ptr(lens));
     } else if (kv_lens_h) {
       invalid("eviction: kv_lens without lens_out, which takes the new lengths");
@@ -2729,14 +2750,14 @@ int32_t fl_cache_evict(fl_operators_t operators, fl_tensor_view_t k_h, fl_tensor
       if (device_of(*kept) != FL_DEVICE_CUDA) invalid("kept is not on the operators' device");
     }
     // What is written meets nothing that is read, and nothing else that is written (only lens_out may be kv_lens).
-    const fl_tensor_view_impl_t *written[4] = {&k_out, &v_out, &weights_out, kept};
+    const fl_tensor_view_impl_t *written[5] = {&k_out, &v_out, &weights_out, kept, lens_out_h ? &deref(lens_out_h) : nullptr};
     const fl_tensor_view_impl_t *read[3] = {&k, &v, &weights};
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 5; ++i) {
       if (!written[i]) continue;
       for (const fl_tensor_view_impl_t *r : read) {
         if (views_overlap(*written[i], *r)) invalid("eviction: an output overlaps k, v or weights");
       }
-      for (int j = i + 1; j < 4; ++j) {
+      for (int j = i + 1; j < 5; ++j) {
         if (written[j] && views_overlap(*written[i], *written[j])) invalid("eviction: two outputs overlap");
       }
     }

@@ -8,7 +8,7 @@ def at(F, shape, dtype, stride=None, address=1 << 20, room=1 << 40):
 
 
 def operands(F, dt, N=2, H=4, Hk=2, L=1, S=10, D=64, P=6):
-    t = {"q": at(F, (N, H, L, D), dt), "k": at(F, (N, Hk, S, D), dt), "v": at(F, (N, Hk, S, D), dt), "out": at(F, (N, H, L, D), dt),
+    t = {"q": at(F, (N, H, L, D), dt), "k": at(F, (N, Hk, S, D), dt), "v": at(F, (N, Hk, S, D), dt), "out": at(F, (N, H, L, D), dt, address=1 << 28),
          "pk": at(F, (1, Hk, P, D), dt), "pv": at(F, (1, Hk, P, D), dt), "lens": at(F, (N,), F.DType.INT32),
          "w": at(F, (N, Hk, S), F.DType.FLOAT), "wo": at(F, (N, Hk, S), F.DType.FLOAT, address=1 << 30)}
     return t
@@ -52,6 +52,7 @@ def test_what_attention_refuses(flint, no_device):
         (dict(k=at(F, (2, 2, 10, 64), bf, (1280, 640, 64, 2))), "k's last dimension"),
         (dict(k=at(F, (2, 2, 10, 64), bf, (0, 640, 64, 1))), "stride of 0"), (dict(out=at(F, (2, 4, 1, 64), bf, (0, 64, 64, 1))), "stride of 0"),
         (dict(v=at(F, (2, 2, 10, 64), bf, (1300, 650, 65, 1))), "multiple of 8"), (dict(q=at(F, (2, 4, 1, 64), bf, address=(1 << 20) + 2)), "16-byte"),
+        (dict(out=t["q"]), "out shares elements with q"), (dict(out=at(F, (2, 4, 1, 64), bf, address=(1 << 20) + 2304)), "shares elements with k"),
         (dict(lens=at(F, (3,), F.DType.INT32)), "kv_lens"), (dict(lens=at(F, (2,), F.DType.LONG)), "kv_lens"),
         (dict(lens=at(F, (2,), F.DType.INT32, (2,))), "kv_lens"),
     ]
@@ -63,7 +64,11 @@ def test_what_attention_refuses(flint, no_device):
 
     prefix = lambda **c: N.refused(L.fl_attention_shared_prefix, ops, *[{**t, **c}[n] for n in ("q", "pk", "pv", "k", "v", "lens", "out")])  # noqa: E731
     assert not prefix()[0]
-    for change, words in [(dict(pk=at(F, (2, 2, 6, 64), bf)), "(1, kv_heads, length, head_dim)"), (dict(pv=at(F, (1, 2, 7, 64), bf)), "disagree"),
+    between = dict(q=at(F, (2, 4, 1, 64), bf, (1024, 128, 128, 1)), out=at(F, (2, 4, 1, 64), bf, (1024, 128, 128, 1), (1 << 20) + 128))
+    far = dict(k=at(F, (2, 2, 10, 64), bf, address=1 << 29), v=at(F, (2, 2, 10, 64), bf, address=1 << 29))
+    assert not window(**between, **far)[0]  # q and out take turns in memory
+    for change, words in [(dict(out=at(F, (2, 4, 1, 64), bf, address=(1 << 20) + 512), **far), "shares elements with q"), (dict(out=at(F, (2, 4, 1, 64), bf), **far, q=at(F, (2, 4, 1, 64), bf, address=1 << 27)), "prefix"),
+                          (dict(pk=at(F, (2, 2, 6, 64), bf)), "(1, kv_heads, length, head_dim)"), (dict(pv=at(F, (1, 2, 7, 64), bf)), "disagree"),
                           (dict(pk=at(F, (1, 2, 0, 64), bf), pv=at(F, (1, 2, 0, 64), bf)), "empty prefix"), (dict(pk=at(F, (1, 2, 6, 64), half)), "type"),
                           (dict(pk=at(F, (1, 2, 6, 64), bf, (768, 384, 0, 1))), "stride of 0"), (dict(pv=at(F, (1, 2, 6, 64), bf, address=(1 << 20) + 8)), "16-byte")]:
         refusal, message = prefix(**change)
@@ -86,7 +91,7 @@ def test_what_eviction_refuses(flint, no_device):
     L = F.lib()
     bf, fl = F.DType.BFLOAT16, F.DType.FLOAT
     far = lambda i: (i + 2) << 32  # noqa: E731
-    t = {"k": at(F, (2, 2, 10, 24), bf), "v": at(F, (2, 2, 10, 24), bf), "w": at(F, (2, 2, 10), fl), "lens": at(F, (2,), F.DType.INT32),
+    t = {"k": at(F, (2, 2, 10, 24), bf), "v": at(F, (2, 2, 10, 24), bf), "w": at(F, (2, 2, 10), fl), "lens": at(F, (2,), F.DType.INT32, address=far(8)),
          "ko": at(F, (2, 2, 6, 24), bf, address=far(0)), "vo": at(F, (2, 2, 6, 24), bf, address=far(1)), "wo": at(F, (2, 2, 6), fl, address=far(2)),
          "lo": at(F, (2,), F.DType.INT32, address=far(3)), "kept": at(F, (2, 2, 5), F.DType.INT32, address=far(4))}
 
@@ -101,6 +106,8 @@ def test_what_eviction_refuses(flint, no_device):
             (dict(ko=at(F, (2, 2, 6, 24), F.DType.FLOAT16, address=far(0))), "one type"), (dict(w=at(F, (2, 2, 6), fl)), "weights"),
             (dict(wo=at(F, (2, 2, 10), fl, address=far(2))), "weights_out"), (dict(lo=None), "lens_out"), (dict(lens=at(F, (1,), F.DType.INT32)), "kv_lens"),
             (dict(kept=at(F, (2, 2, 6), F.DType.INT32, address=far(4))), "kept"), (dict(ko=at(F, (2, 2, 6, 24), bf, address=(1 << 20) + 16)), "overlaps k, v or weights"),
+            (dict(lo=at(F, (2,), F.DType.INT32, address=far(8) + 4)), "lens_out overlaps kv_lens"),
+            (dict(lo=at(F, (2,), F.DType.INT32, address=far(2) + 16)), "two outputs"),
             (dict(vo=t["ko"]), "two outputs"), (dict(ko=at(F, (2, 2, 6, 24), bf, (0, 144, 24, 1), far(0))), "stride of 0"),
             (dict(k=at(F, (2, 2, 10, 24), bf, (480, 240, 24, 1), (1 << 20) + 2)), "16-byte")]:
         refusal, message = evict(**change)
