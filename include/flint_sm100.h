@@ -414,7 +414,7 @@ FLAPI int32_t fl_attention_window(fl_operators_t operators, fl_tensor_view_t q, 
 /* A batch whose sequences share their beginning (a system prompt, a document, the prompt of several
  * samples): prefix_k and prefix_v (1, kv_heads, P, D), strides as k's, hold it once; k, v and kv_lens each
  * sequence's own keys behind it. Every query sees all P keys of the prefix and its own sequence's keys 0 .. p
- * (none for p < 0). The prefix's keys are read for all the batch's queries together. */
+ * (none for p < 0). Short queries of the whole batch walk the prefix together, in one pass over its keys. */
 FLAPI int32_t fl_attention_shared_prefix(fl_operators_t operators, fl_tensor_view_t q, fl_tensor_view_t prefix_k,
                                          fl_tensor_view_t prefix_v, fl_tensor_view_t k, fl_tensor_view_t v,
                                          fl_tensor_view_t kv_lens, fl_tensor_view_t out);
