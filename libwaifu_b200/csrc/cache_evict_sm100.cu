@@ -1,12 +1,14 @@
 // Eviction from a key-value cache by accumulated attention weight: which keys stay, and their rows gathered.
 //
-// One CTA per sequence and key-value head finds the weight of the last key that stays by its bits, eleven, eleven and ten
-// from the top (a histogram of the keys that agree so far, then the bin in which the wanted rank falls), and
-// lists the keys above it and the first of those equal to it in the order of their positions (a scan over the CTA).
-// The weights are read once, into shared memory as far as they fit, and only the keys of the bin found are looked at again.
-// Equal weights fall into one bin: the lanes of a warp that share the first one's count together. (16 x 8 heads of 8192 keys and
-// their rows 89.0 us; 90.5 with eight bits at a time over all keys and the lanes grouped by all their bins, which takes longer
-// the more bins there are.)
+// One CTA per sequence and key-value head finds the weight of the last key that stays by its bits, and lists the keys above it
+// and the first of those equal to it in the order of their positions (a scan over the CTA). A pass counts the keys in
+// 2048 bins that divide the range in question in equal parts, at first that from the lightest key to the heaviest, and goes on
+// with the bin in which the wanted rank falls, until that bin is one number or all of its keys stay: three passes at most. The
+// weights are read once, into shared memory as far as they fit. What bounds a CTA is its instructions, so the
+// passes are short: a key's bin, and one atomic without a result, which the hardware adds up for
+// the lanes that share a bin (16 x 8 heads of 8192 keys and their rows 85.8 us, all weights equal 83.0; with bins at fixed bits,
+// lanes grouped by votes and the keys of the bin found listed for the next pass 89.1; bit by bit over keys in registers, a
+// barrier a bit, 94.4).
 // The rows are then copied by a kernel over the whole GPU, sixteen bytes a thread. Both are bound by memory: a weight is
 // read once and a kept row once, and written once.
 #include "cache_attention_sm100.cuh"
@@ -38,19 +40,20 @@ struct SelectParams {
   const int32_t *kv_lens;
   int32_t *kept;
   int kv_heads, kv_len, out_len, keep, recent;
-  int cached_keys, listed_keys;  // room for so many in shared memory
+  int cached_keys;  // room for so many in shared memory
 };
 
 constexpr int kKeysPerThread = 4;  // of the scan
-constexpr int kMaxCachedWords = 48 * 1024;  // of shared memory: the keys' weights, and as many places for those of a bin
+constexpr int kMaxCachedKeys = 48 * 1024;  // in shared memory
 constexpr int kBins = 2048;
 
 __global__ void __launch_bounds__(kSelectThreads, 1) select_kept_kernel(const __grid_constant__ SelectParams p) {
   extern __shared__ __align__(16) uint32_t cache[];
   __shared__ uint32_t bins[kBins];
   __shared__ uint32_t warp_counts[kSelectThreads / 32];
+  __shared__ uint32_t warp_low[kSelectThreads / 32], warp_high[kSelectThreads / 32];
   __shared__ uint32_t found_bin;
-  __shared__ int found_rank, listed;
+  __shared__ int found_rank, found_keys;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   griddep_wait();
   griddep_launch_dependents();
@@ -67,34 +70,32 @@ __global__ void __launch_bounds__(kSelectThreads, 1) select_kept_kernel(const __
   const int cached = choose ? min(old, p.cached_keys) : 0;
   auto order_at = [&](int i) -> uint32_t { return i < cached ? cache[i] : order_of(weights[i]); };
   if (choose) {
+    uint32_t low = 0xffffffffu, high = 0u;
 #pragma unroll 4
-    for (int i = threadIdx.x; i < cached; i += kSelectThreads) cache[i] = order_of(weights[i]);
-    uint32_t *list = cache + cached;          // the keys that agree so far
-    const bool lists = p.listed_keys >= old;  // (there is room for all of them)
-    int keys = old;                           // to look at: all, then those listed
-    uint32_t mask = 0;
+    for (int i = threadIdx.x; i < old; i += kSelectThreads) {
+      const uint32_t o = order_of(weights[i]);
+      if (i < cached) cache[i] = o;
+      low = min(low, o);
+      high = max(high, o);
+    }
+    low = __reduce_min_sync(0xffffffffu, low);
+    high = __reduce_max_sync(0xffffffffu, high);
+    if (lane == 0) warp_low[warp] = low, warp_high[warp] = high;
+    __syncthreads();
+    low = __reduce_min_sync(0xffffffffu, warp_low[lane]);
+    high = __reduce_max_sync(0xffffffffu, warp_high[lane]);
+    // The bins of a pass divide [low, low + (width << shift)), which holds the wanted key, in equal parts: at first from the
+    // lightest key to the heaviest.
+    int shift = max(0, 21 - __clz(static_cast<int>(high - low)));
+    uint32_t width = kBins;
 #pragma unroll 1
-    for (int pass = 0; pass < 3; ++pass) {
-      const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
-      const uint32_t bits = pass == 2 ? 1023u : 2047u;
-      const bool from_list = lists && pass > 0;
+    while (true) {
       for (int i = threadIdx.x; i < kBins; i += kSelectThreads) bins[i] = 0;
-      if (threadIdx.x == 0) listed = 0;
       __syncthreads();
-      for (int base = 0; base < keys; base += kSelectThreads) {
-        const int i = base + threadIdx.x;
-        const uint32_t o = i < keys ? (from_list ? list[i] : order_at(i)) : 0u;
-        const uint32_t bin = i < keys && (o & mask) == last ? (o >> shift) & bits : kBins;
-        // The lanes that share their bin with the first one that has any count together, the others for themselves.
-        const uint32_t counted = __ballot_sync(0xffffffffu, bin < kBins);
-        if (counted == 0) continue;
-        const int leader = __ffs(static_cast<int>(counted)) - 1;
-        const uint32_t with_leader = __ballot_sync(0xffffffffu, bin == __shfl_sync(0xffffffffu, bin, leader));
-        if (lane == leader) {
-          atomicAdd(&bins[bin], static_cast<uint32_t>(__popc(with_leader)));
-        } else if (bin < kBins && !((with_leader >> lane) & 1u)) {
-          atomicAdd(&bins[bin], 1u);
-        }
+#pragma unroll 4
+      for (int i = threadIdx.x; i < old; i += kSelectThreads) {
+        const uint32_t bin = (order_at(i) - low) >> shift;  // (of a key below `low`, which the first pass has not, beyond the bins)
+        if (bin < width) atomicAdd(&bins[bin], 1u);
       }
       __syncthreads();
       // Two bins a thread, the highest first: the bin in which the rank falls, and what is left of the rank there.
@@ -114,30 +115,21 @@ __global__ void __launch_bounds__(kSelectThreads, 1) select_kept_kernel(const __
         const int second = rank > here[0] ? 1 : 0;
         found_bin = static_cast<uint32_t>(top - second);
         found_rank = second ? rank - here[0] : rank;
+        found_keys = here[second];
       }
       __syncthreads();
-      if (lists && pass < 2) {
-        // The keys of that bin, in any order; a list is compacted in place, each round's keys after all of them were read.
-        const uint32_t agreed = last | (found_bin << shift), agree_mask = mask | (bits << shift);
-        for (int base = 0; base < keys; base += kSelectThreads) {
-          const int i = base + threadIdx.x;
-          const uint32_t o = i < keys ? (from_list ? list[i] : order_at(i)) : 0u;
-          const bool agrees = i < keys && (o & agree_mask) == agreed;
-          const uint32_t votes = __ballot_sync(0xffffffffu, agrees);
-          if (from_list) __syncthreads();
-          int at = 0;
-          if (lane == 0 && votes != 0) at = atomicAdd(&listed, __popc(votes));
-          at = __shfl_sync(0xffffffffu, at, 0) + __popc(votes & ((1u << lane) - 1u));
-          if (agrees) list[at] = o;
-          if (from_list) __syncthreads();
-        }
-        __syncthreads();
-        keys = listed;
-      }
-      last |= found_bin << shift;
-      mask |= bits << shift;
       wanted = found_rank;
-      __syncthreads();  // (what was found and listed has been read)
+      low += found_bin << shift;
+      last = low;
+      if (shift == 0) break;
+      if (found_keys == wanted) {  // all that are left
+        last = low - 1;
+        wanted = 0;
+        break;
+      }
+      const int next_shift = max(0, shift - 11);
+      width = 1u << (shift - next_shift);
+      shift = next_shift;
     }
   }
   // Of the old keys those above `last` stay, and the first `wanted` that equal it; of the others all.
@@ -237,13 +229,12 @@ cudaError_t cache_evict(const CacheEvictArgs &a) {
   s.out_len = a.out_len;
   s.keep = a.keep;
   s.recent = a.recent;
-  static const cudaError_t attr_set = cudaFuncSetAttribute(select_kept_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxCachedWords * 4);
+  static const cudaError_t attr_set = cudaFuncSetAttribute(select_kept_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxCachedKeys * 4);
   if (attr_set != cudaSuccess) return attr_set;
   // (a cache that holds no more than stays has nothing to choose from)
-  s.cached_keys = a.kv_len <= a.keep ? 0 : std::min(a.kv_len, kMaxCachedWords);
-  s.listed_keys = 2 * static_cast<int64_t>(s.cached_keys) <= kMaxCachedWords ? s.cached_keys : 0;
+  s.cached_keys = a.kv_len <= a.keep ? 0 : std::min(a.kv_len, kMaxCachedKeys);
   cudaError_t e = launch_overlapped(select_kept_kernel, static_cast<int64_t>(a.batch) * a.kv_heads, kSelectThreads,
-                                    static_cast<size_t>(s.cached_keys + s.listed_keys) * 4, a.stream, s);
+                                    static_cast<size_t>(s.cached_keys) * 4, a.stream, s);
   if (e != cudaSuccess) return e;
 
   GatherParams g = {};

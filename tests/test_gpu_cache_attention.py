@@ -323,6 +323,8 @@ EVICT = [
     (1, 2, 100, 8, 100, 5, 100, None),                   # nothing to evict
     (2, 1, 60000, 8, 777, 20, 777, [60000, 30011]),      # more weights than fit in shared memory
     (1, 1, 30000, 8, 20000, 9000, 20000, None),          # ... or with a list beside them
+    (2, 1, 22000, 8, 9000, 300, 9000, [22000, 16684]),   # more than a CTA holds in registers, listed, and as many as it does
+    (1, 1, 16685, 8, 400, 300, 400, None),               # one more
 ]
 
 
