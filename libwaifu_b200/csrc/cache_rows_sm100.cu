@@ -693,19 +693,19 @@ __global__ void __launch_bounds__(kAddThreads) add_weights_kernel(const float *s
                                                                   Divisor by_chunks, Divisor by_kv_heads, int group, int q_len, int kv_len,
                                                                   const int32_t *kv_lens, const float *weights_in, int64_t in_seq,
                                                                   int64_t in_head, float *weights_out, int64_t out_seq, int64_t out_head) {
-  griddep_wait();
-  griddep_launch_dependents();
   int run = blockIdx.x;
   const int key = (by_chunks.take(&run) * kAddThreads + threadIdx.x) * kKeysAtOnce;
-  if (key >= kv_len) return;
+  // (The weights up to here and the lengths are complete: the kernel before has waited for what wrote them. They are read past L1.)
   int seq = run;
   const int head = by_kv_heads.take(&seq);
   const float *in = weights_in + seq * in_seq + head * in_head + key;
   float *out = weights_out + seq * out_seq + head * out_head + key;
   float before[kKeysAtOnce], sum[kKeysAtOnce] = {};
 #pragma unroll
-  for (int k = 0; k < kKeysAtOnce; ++k) before[k] = key + k < kv_len ? in[k] : 0.0f;
+  for (int k = 0; k < kKeysAtOnce; ++k) before[k] = key + k < kv_len ? __ldcg(in + k) : 0.0f;
   const int len = sequence_length(kv_lens, seq, kv_len);
+  griddep_wait();  // the scores, and the rows' maxima and sums
+  griddep_launch_dependents();
   if (key < len) {
     // Query i sees the keys up to i + len - q_len; the rows' scores of others were not written.
     const float *score = scores + static_cast<int64_t>(run) * rows * score_pitch + key;
