@@ -389,6 +389,7 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
   cp_async_wait_group<kStages - 2>();
   __syncthreads();  // the first unit's queries are there
   begin_unit();
+  __syncthreads();  // ... and have been read: behind two units of one step the third one's come to their place with the next load
 
   int stage = 0;
   for (int done = 0; done < count; ++done) {

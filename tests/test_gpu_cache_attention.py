@@ -426,3 +426,43 @@ def test_a_decoder_that_evicts(flint, oracle):
         check_out(widen(near.numpy()), want, size, score, 16, True, f"window of step {step}")
     F.synchronize()
     assert evictions == 1 and np.abs(weights.numpy()[:, :, :int(lens[0])] - book[:, :, :int(lens[0])]).max() < 1e-4  # 30 steps of float sums near 1
+
+
+SHORT_WALKS = [
+    # N, H, Hk, L, S, D, window, lens: units of one step of 64 keys, several to a CTA
+    (130, 8, 8, 1, 60, 64, 60, None),
+    (130, 8, 8, 1, 700, 128, 64, [700 - 5 * n for n in range(130)]),
+    (16, 8, 8, 1, 300, 128, 300, [300] + [40] * 15),
+    (200, 6, 3, 2, 64, 64, 64, [n * 37 % 65 for n in range(200)]),
+    (250, 35, 1, 1, 64, 64, 64, None),                               # three tiles of 16 rows, the last one partial
+    (200, 70, 2, 1, 40, 128, 40, [n * 13 % 41 for n in range(200)]),
+]
+
+
+@pytest.mark.parametrize("N,H,Hk,L,S,D,window,lens", SHORT_WALKS)
+def test_many_short_walks_one_after_the_other(flint, oracle, N, H, Hk, L, S, D, window, lens):
+    """A CTA of the few-row kernel goes through many units, whose queries take turns in two places: right, and the same
+    bits every time. (With the keys' weights the kernel takes up to 63 rows, in tiles of 16.)"""
+    F = flint
+    c = Cache(F, oracle, 21 + N + S, N, H, Hk, L, S, D, True, lens)
+    t = c.device()
+    weighed = window == S
+    zeros = np.zeros((N, Hk, S), np.float32)
+
+    def once():
+        if not weighed:
+            F.attention_window(t["q"], t["k"], t["v"], window, 0, t["lens"], t["out"])
+            return c.read(t["out"]), zeros
+        _, w = F.attention_weights(t["q"], t["k"], t["v"], dev(F, zeros, F.DType.FLOAT), t["lens"], out=t["out"])
+        return c.read(t["out"]), w.numpy()
+
+    got, got_w = once()
+    for _ in range(20):
+        again, again_w = once()
+        assert np.array_equal(got, again) and np.array_equal(got_w, again_w)
+    F.synchronize()
+    want, weights, size, score = C.attention(c.value("q"), c.value("k"), c.value("v"), lens, window, 0)
+    check_out(got, want, size, score, S, True, "short walks")
+    if weighed:
+        tol = (2 * (D + 4) * 2.0 ** -23 * score.max() + 2.0 ** -20 + 2.0 ** -13 + (S + H // Hk * L) * 2.0 ** -23) * weights
+        assert (np.abs(got_w - weights) <= tol).all()
