@@ -110,6 +110,20 @@ template <bool BF16>
 __device__ __forceinline__ bool has_nonfinite(uint4 w) {
   return (nonfinite_halves<BF16>(w.x) | nonfinite_halves<BF16>(w.y) | nonfinite_halves<BF16>(w.z) | nonfinite_halves<BF16>(w.w)) != 0;
 }
+// Zeros (of either sign) go on as such, through eight finite values: zero times an infinity or a NaN is a NaN, which stays.
+template <bool BF16>
+__device__ __forceinline__ uint32_t probe_nonfinite(uint4 w, uint32_t zeros) {
+  const uint32_t each[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (BF16) {
+      asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(zeros) : "r"(each[i]), "r"(0u));
+    } else {
+      asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(zeros) : "r"(each[i]), "r"(0u));
+    }
+  }
+  return zeros;
+}
 template <bool BF16>
 __device__ __forceinline__ uint4 without_nonfinite(uint4 w) {
   return make_uint4(w.x & ~nonfinite_halves<BF16>(w.x), w.y & ~nonfinite_halves<BF16>(w.y), w.z & ~nonfinite_halves<BF16>(w.z),

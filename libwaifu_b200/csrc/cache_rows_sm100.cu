@@ -487,15 +487,16 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
           lo[n][h] = transpose_8x8(lo[n][h]);
         }
       }
-      // Infinities and NaN in the values of a key that one row sees and another does not: zero times such a value is
-      // not zero, so they leave the tile, and the rows that see them get their products by hand.
-      if (differ) {
-        bool odd = false;
+      // Infinities and NaN in the values leave the tile, and the rows that see them get their products by hand: zero times
+      // such a value is not zero, whether the zero is the probability of a key that the row does not see or what rounding
+      // left of one that it does, and a negative rest would take an infinity back.
+      {
+        uint32_t odd = 0;
 #pragma unroll
         for (int i = 0; i < L::kTileBytes / 512; ++i) {
-          odd |= has_nonfinite<BF16>(*reinterpret_cast<const uint4 *>(v_tile + (i * 32 + lane) * 16));
+          odd = probe_nonfinite<BF16>(*reinterpret_cast<const uint4 *>(v_tile + (i * 32 + lane) * 16), odd);
         }
-        if (__any_sync(0xffffffffu, odd)) {
+        if (__any_sync(0xffffffffu, (odd & 0x7FFF7FFFu) != 0)) {
           for (int kk = 0; kk < kTileKeys; ++kk) {
             const int from = ((kk & 7) << 2) | (lane & 3);
             const int key = at0 + kk < total ? at.range.key(at0 + kk) : 0;

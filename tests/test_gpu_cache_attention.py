@@ -466,3 +466,58 @@ def test_many_short_walks_one_after_the_other(flint, oracle, N, H, Hk, L, S, D, 
     if weighed:
         tol = (2 * (D + 4) * 2.0 ** -23 * score.max() + 2.0 ** -20 + 2.0 ** -13 + (S + H // Hk * L) * 2.0 ** -23) * weights
         assert (np.abs(got_w - weights) <= tol).all()
+
+
+def put(c, name, at, value):
+    """A value (nan, inf or -inf) at a place of an operand."""
+    bits = {"nan": (0x7FC0, 0x7E00), "inf": (0x7F80, 0x7C00), "-inf": (0xFF80, 0xFC00)}[value]
+    c.bits[name][at] = bits[0] if c.is_bf16 else bits[1]
+
+
+@pytest.mark.parametrize("H,Hk,L,S", [(1, 1, 1, 1), (4, 2, 1, 100), (4, 2, 1, 3000), (6, 2, 4, 500), (4, 2, 40, 300)])
+@pytest.mark.parametrize("route", ["window", "prefix", "weights"])
+@pytest.mark.parametrize("is_bf16", [True, False])
+def test_seen_infinities_reach_the_result(flint, oracle, H, Hk, L, S, route, is_bf16):
+    """An infinity in a value that a query sees is its result's, whichever others see it too; both signs, or a NaN,
+    make a NaN. Scores are close, so that no weight rounds to zero."""
+    F, N, D, P = flint, 2, 64, 70
+    c = Cache(F, oracle, 91 + S + L, N, H, Hk, L, S, D, is_bf16, [S, max(S // 2, 1)], P=P if route == "prefix" else 0, spread=0.5)
+    last = S // 2 - 1 if S > 1 else 0  # seen by every query of the first sequence, by the last ones of the second
+    put(c, "v", (0, 0, 0, 3), "inf")
+    put(c, "v", (0, 0, S // 2, 4), "-inf")
+    put(c, "v", (0, Hk - 1, S // 3, 5), "inf")
+    put(c, "v", (0, Hk - 1, S // 2, 5), "-inf" if S > 1 else "inf")
+    put(c, "v", (0, 0, S // 4, 6), "nan")
+    put(c, "v", (1, 0, last, 7), "inf")
+    put(c, "v", (1, Hk - 1, last // 2, 63), "-inf")
+    if route == "prefix":
+        put(c, "prefix_v", (0, 0, 0, 8), "inf")
+        put(c, "prefix_v", (0, Hk - 1, P - 1, 9), "-inf")
+        put(c, "prefix_v", (0, 0, 64, 3), "-inf")
+    t = c.device()
+    if route == "window":
+        F.attention_window(t["q"], t["k"], t["v"], S, 0, t["lens"], t["out"])
+        got = c.read(t["out"])
+        F.attention_window(t["q"], t["k"], t["v"], max(S // 2, 1), 1, t["lens"], t["out"])
+        under = c.read(t["out"])
+        with np.errstate(invalid="ignore"):
+            want, _, size, score = C.attention(c.value("q"), c.value("k"), c.value("v"), c.lens, max(S // 2, 1), 1)
+        check_out(under, want, np.nan_to_num(size, posinf=0.0), score, S, is_bf16, "under a window")
+        with np.errstate(invalid="ignore"):
+            want, _, size, score = C.attention(c.value("q"), c.value("k"), c.value("v"), c.lens)
+    elif route == "prefix":
+        F.attention_shared_prefix(t["q"], t["prefix_k"], t["prefix_v"], t["k"], t["v"], t["lens"], t["out"])
+        got = c.read(t["out"])
+        with np.errstate(invalid="ignore"):
+            want, _, size, score = C.attention(c.value("q"), c.value("k"), c.value("v"), c.lens, prefix_k=c.value("prefix_k"), prefix_v=c.value("prefix_v"))
+    else:
+        w = dev(F, np.zeros((N, Hk, S), np.float32), F.DType.FLOAT)
+        F.attention_weights(t["q"], t["k"], t["v"], w, t["lens"], out=t["out"])
+        got = c.read(t["out"])
+        with np.errstate(invalid="ignore"):
+            want, weights, size, score = C.attention(c.value("q"), c.value("k"), c.value("v"), c.lens)
+        tol = (2 * (D + 4) * 2.0 ** -23 * score.max() + 2.0 ** -20 + 2.0 ** -13 + (S + H // Hk * L) * 2.0 ** -23) * weights
+        assert (np.abs(w.numpy() - weights) <= tol).all()  # values have no part in them
+    F.synchronize()
+    check_out(got, want, np.nan_to_num(size, posinf=0.0), score, S + P, is_bf16, route)
+    assert np.isinf(got).any()
