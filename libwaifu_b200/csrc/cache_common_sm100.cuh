@@ -106,10 +106,6 @@ __device__ __forceinline__ uint32_t nonfinite_halves(uint32_t w) {
   constexpr uint32_t kExponent = BF16 ? 0x7F807F80u : 0x7C007C00u;
   return __vcmpeq2(w & kExponent, kExponent);
 }
-template <bool BF16>
-__device__ __forceinline__ bool has_nonfinite(uint4 w) {
-  return (nonfinite_halves<BF16>(w.x) | nonfinite_halves<BF16>(w.y) | nonfinite_halves<BF16>(w.z) | nonfinite_halves<BF16>(w.w)) != 0;
-}
 // Zeros (of either sign) go on as such, through eight finite values: zero times an infinity or a NaN is a NaN, which stays.
 template <bool BF16>
 __device__ __forceinline__ uint32_t probe_nonfinite(uint4 w, uint32_t zeros) {

@@ -12,9 +12,9 @@
 // 1024 keys and 16 sinks walk 9 blocks a unit so, and 10.4 in blocks at multiples of 128.
 //
 // A block that some row does not see whole (past the sequence's end, at a window's edge, on the diagonal) passes two
-// helping warps before its product: they clear the values of keys that no row sees and take infinities and NaN out of the
-// others, because a probability of zero times such a value is not zero. Rows that do see them have them added by hand at
-// the end.
+// helping warps before its product: they clear the values of keys that no row sees and take infinities, NaN and values of
+// another size than any sum's out of the others, because what stands for a probability of zero times such a value is not
+// zero (TooLarge). Rows that do see them have them added by hand at the end.
 //
 // A running CTA takes over units whose own CTA has not started (clusterlaunchcontrol.try_cancel): the next unit's keys,
 // queries and first scores come under the last products and the output of the one before. Walks are short here (a window's,
@@ -231,34 +231,61 @@ __device__ __forceinline__ int64_t row_offset(const TilesParams &p, const int64_
   return seq * stride[0] + static_cast<int64_t>(head * p.group + g) * stride[1] + i * stride[2];
 }
 
-// Adds what a row sees of the infinities and NaN that were taken out of its blocks: rare, and as slow as it is plain.
+// The values that a key loses where some row of the tile does not see it: infinities and NaN, which a probability of zero does not
+// stop, and of bfloat16 what is 2^64 or more, because the cubic's probability of an unseen key is 2^-126 (no half, but a
+// bfloat16; to give it a zero cost 69.6 -> 72.5 us on prefix_extend). A mask of such halves, by a carry out of their exponents.
+template <bool BF16>
+struct TooLarge {
+  static constexpr uint32_t kExponent = BF16 ? 0x7F807F80u : 0x7C007C00u;
+  static constexpr uint32_t kCarry = BF16 ? 0x20802080u : 0x04000400u;  // from an exponent field of 191, of 31 on
+  // Into the sign bits.
+  static __device__ __forceinline__ uint32_t signs(uint32_t w) { return (w & kExponent) + kCarry; }
+  static __device__ __forceinline__ uint32_t halves(uint32_t w) { return ((signs(w) >> 15) & 0x00010001u) * 0xFFFFu; }
+  static __device__ __forceinline__ bool any(uint4 w) { return ((signs(w.x) | signs(w.y) | signs(w.z) | signs(w.w)) & 0x80008000u) != 0; }
+  static __device__ __forceinline__ uint4 without(uint4 w) {
+    return make_uint4(w.x & ~halves(w.x), w.y & ~halves(w.y), w.z & ~halves(w.z), w.w & ~halves(w.w));
+  }
+};
+
+// Adds what a row sees of the values that were taken out of its blocks, eight columns at a time: rare, and as slow as it is plain.
 template <int D, bool BF16>
 __device__ __noinline__ void patch_row(const TilesParams &p, int unit, int pos, const uint16_t *q, float m, float l, uint16_t *out, float *part) {
   const Unit u(p, unit);
-  for (int j = 0; j < u.walk.count; ++j) {
-    if (!u.walk.dirty.has(j)) continue;
-    for (int x = u.walk.place0(j); x < u.walk.place0(j) + kBlockKv; ++x) {
-      const int key = u.walk.key_at(x);
-      if (u.walk.hidden(x) || key > pos || !(key > pos - p.window || key < p.sinks)) continue;
-      const uint16_t *v = p.v + u.seq * p.v_stride[0] + u.head * p.v_stride[1] + key * p.v_stride[2];
-      const uint16_t *k = p.k + u.seq * p.k_stride[0] + u.head * p.k_stride[1] + key * p.k_stride[2];
-      bool odd = false;
-      for (int d = 0; d < D; d += 8) odd |= has_nonfinite<BF16>(*reinterpret_cast<const uint4 *>(v + d));
-      if (!odd) continue;
-      float s = 0.0f;
-      for (int d = 0; d < D; d += 2) {
-        const float2 x = widen_pair<BF16>(*reinterpret_cast<const uint32_t *>(q + d)), y = widen_pair<BF16>(*reinterpret_cast<const uint32_t *>(k + d));
-        s = fmaf(x.x, y.x, fmaf(x.y, y.y, s));
-      }
-      const float w = exp2f(s * p.scale_log2 - m);
-      for (int d = 0; d < D; ++d) {
-        const float x = widen_pair<BF16>(v[d]).x;
-        if (fabsf(x) < INFINITY) continue;
-        if (part != nullptr) {
-          part[d] += w * x;
-        } else {
-          out[d] = static_cast<uint16_t>(pack_pair<BF16>(widen_pair<BF16>(out[d]).x + w / l * x, 0.0f));
+  for (int c = 0; c < D; c += 8) {
+    float sum[8] = {};
+    bool found = false;
+    for (int j = 0; j < u.walk.count; ++j) {
+      if (!u.walk.dirty.has(j)) continue;
+      for (int x = u.walk.place0(j); x < u.walk.place0(j) + kBlockKv; ++x) {
+        const int key = u.walk.key_at(x);
+        if (u.walk.hidden(x) || !u.walk.mixed(x) || key > pos || !(key > pos - p.window || key < p.sinks)) continue;
+        const uint4 v = *reinterpret_cast<const uint4 *>(p.v + u.seq * p.v_stride[0] + u.head * p.v_stride[1] + key * p.v_stride[2] + c);
+        if (!TooLarge<BF16>::any(v)) continue;
+        found = true;
+        const uint16_t *k = p.k + u.seq * p.k_stride[0] + u.head * p.k_stride[1] + key * p.k_stride[2];
+        float s = 0.0f;
+        for (int d = 0; d < D; d += 2) {
+          const float2 a = widen_pair<BF16>(*reinterpret_cast<const uint32_t *>(q + d)), b = widen_pair<BF16>(*reinterpret_cast<const uint32_t *>(k + d));
+          s = fmaf(a.x, b.x, fmaf(a.y, b.y, s));
         }
+        const float w = exp2f(s * p.scale_log2 - m);
+        const uint32_t pairs[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t large = TooLarge<BF16>::halves(pairs[i]);
+          const float2 y = widen_pair<BF16>(pairs[i]);
+          if (large & 0xFFFFu) sum[2 * i] += w * y.x;
+          if (large >> 16) sum[2 * i + 1] += w * y.y;
+        }
+      }
+    }
+    if (!found) continue;
+    for (int i = 0; i < 8; ++i) {
+      if (sum[i] == 0.0f) continue;
+      if (part != nullptr) {
+        part[c + i] += sum[i];
+      } else {
+        out[c + i] = static_cast<uint16_t>(pack_pair<BF16>(widen_pair<BF16>(out[c + i]).x + sum[i] / l, 0.0f));
       }
     }
   }
@@ -662,9 +689,8 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       }
     } else {
       // ------------------------------------------------------------------ values that are not seen by all
+      using Large = TooLarge<BF16>;
       const int which = static_cast<int>(warp) - kHelpWarp;
-      // A half whose exponent is all ones carries into its sign bit.
-      constexpr uint32_t exponent = BF16 ? 0x7F807F80u : 0x7C007C00u, carry = BF16 ? 0x00800080u : 0x04000400u;
       bool ok = true;
       int n = 0;
       int unit = blockIdx.x;
@@ -683,7 +709,7 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
           }
           uint8_t *block = slot(nv % S) + lane * 16;
           const int x0 = u.walk.place0(j);
-          uint32_t odd = 0;  // the sign bits of halves whose exponent is all ones
+          uint32_t odd = 0;  // sign bits
 #pragma unroll 1  // (unrolled by four: 157 us instead of 151, 8192 tokens under a window; the kernel's instructions no longer fit so well)
           for (int r = which * 4; r < kBlockKv; r += kHelpWarps * 4) {  // four keys' 128 bytes of an atom
             const int x = x0 + r + static_cast<int>(lane >> 3);
@@ -694,7 +720,7 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
               if (hidden) *at = make_uint4(0, 0, 0, 0);
               if (mixed) {
                 const uint4 w = *at;
-                odd |= ((w.x & exponent) + carry) | ((w.y & exponent) + carry) | ((w.z & exponent) + carry) | ((w.w & exponent) + carry);
+                odd |= Large::signs(w.x) | Large::signs(w.y) | Large::signs(w.z) | Large::signs(w.w);
               }
             }
           }
@@ -706,8 +732,8 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
               for (int a = 0; a < L::kQAtoms; ++a) {
                 uint4 *at = reinterpret_cast<uint4 *>(block + a * kBlockKv * kAtomBytes + r * kAtomBytes);
                 const uint4 w = *at;
-                *at = without_nonfinite<BF16>(w);
-                taken = taken || has_nonfinite<BF16>(w);
+                *at = Large::without(w);
+                taken = taken || Large::any(w);
               }
             }
           }

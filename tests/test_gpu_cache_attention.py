@@ -521,3 +521,27 @@ def test_seen_infinities_reach_the_result(flint, oracle, H, Hk, L, S, route, is_
     F.synchronize()
     check_out(got, want, np.nan_to_num(size, posinf=0.0), score, S + P, is_bf16, route)
     assert np.isinf(got).any()
+
+
+@pytest.mark.parametrize("L,S,window,sinks,lens", [(1, 300, 100, 5, [300, 250]), (5, 300, 100, 5, [300, 103]), (40, 300, 300, 0, [300, 170]),
+                                                   (150, 500, 200, 20, [500, 490]), (60, 9000, 9000, 0, [9000, 4000])])
+def test_large_values_of_unseen_keys(flint, oracle, L, S, window, sinks, lens):
+    """Finite values far above the others in keys that some queries see and others do not: those others' results have
+    nothing of them. (2^-126, the least normal float, times 1e37 would be 0.1.)"""
+    c = Cache(flint, oracle, 55 + L, 2, 4, 2, L, S, 64, True, lens, spread=0.5)
+    large = oracle.narrow(np.array([1e37], np.float32), True)[0]
+    for n, length in enumerate(lens):
+        at = max(length - max(L // 2, 1) - 4, 0)
+        c.bits["v"][n, 0, at:at + 8, 7] = large           # the later queries see them
+        before = length - window - L // 2
+        if before > sinks + 8:
+            c.bits["v"][n, 1, before - 4:before + 4, 9] = large  # the earlier ones
+        c.bits["v"][n, 1, sinks:sinks + 8, 11] = large    # not in the sinks
+    t = c.device()
+    flint.attention_window(t["q"], t["k"], t["v"], window, sinks, t["lens"], t["out"])
+    got = c.read(t["out"])
+    flint.synchronize()
+    want, _, size, score = C.attention(c.value("q"), c.value("k"), c.value("v"), lens, window, sinks)
+    check_out(got, want, size, score, S, True, "large values")
+    small = np.abs(want).max(-1) < 100
+    assert np.linalg.norm(got[small] - want[small]) <= 5e-3 * np.linalg.norm(want[small])
