@@ -84,6 +84,34 @@ struct Unit {
   }
 };
 
+// A key's sum over this part's rows that came out as NaN. The columns of a block that hold no row are zeros, their 1 / sum too, but
+// zero times a key's infinity is a NaN. A row that sees such a key scores it -inf, or +inf or NaN, which make that row's own sum a NaN:
+// the key's weight from it is zero, or a NaN as are all weights from a row without a sum. (Looked at here, and not where the columns
+// are added up: a bound on each exponent that drops the NaN took 72.5 us where this takes 70.7, weights_prefill.)
+template <int D>
+__device__ __noinline__ float sum_without_empty_columns(const WeightsParams &p, const Unit &u, int key, const uint8_t *key_row, float sum) {
+  bool infinite = false;
+  for (int a = 0; a < D / kAtomElems; ++a) {  // (the pieces of a row lie in another order: here it is all the same)
+    const uint16_t *w = reinterpret_cast<const uint16_t *>(key_row + a * kBlockKv * kAtomBytes);
+    const int infinity = p.is_bf16 ? 0x7F80 : 0x7C00;
+    for (int d = 0; d < kAtomElems; ++d) {
+      const int magnitude = w[d] & 0x7FFF;
+      if (magnitude > infinity) return sum;
+      infinite |= magnitude == infinity;
+    }
+  }
+  if (!infinite) return sum;
+  for (int b = u.first; b < u.first + u.count; ++b) {
+    const int query0 = b * p.positions, from = max(0, key - u.offset - query0), to = min(p.positions, p.q_len - query0);
+    const float2 *norm = p.row_norm + static_cast<int64_t>(u.run) * p.norm_pitch + b * kBlockQ;
+    for (int c = from * p.group; c < to * p.group; ++c) {
+      const float inv = __ldcg(&norm[c]).y;
+      if (inv != inv) return sum;
+    }
+  }
+  return 0.0f;
+}
+
 template <int D>
 __global__ void __launch_bounds__(kThreads, 1)
 cache_weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
@@ -125,7 +153,7 @@ cache_weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     tmem_alloc<1>(&t.tmem_base_slot, L::kTmemCols);
     tmem_relinquish<1>();
   }
-  clear_empty_places<L::kQAtoms * S>(smem + L::kQueriesOff, p.tile_rows, kThreads);  // (their maxima and 1 / sums are zeros too: they add nothing)
+  clear_empty_places<L::kQAtoms * S>(smem + L::kQueriesOff, p.tile_rows, kThreads);  // (their maxima and 1 / sums are zeros too)
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
@@ -194,6 +222,9 @@ cache_weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&t.slot_empty_bar[st]);
+    }
+    if (ok && sum != sum && key < u.len && mbar_wait(&t.k_full_bar, 0, &abort_flag)) {
+      sum = sum_without_empty_columns<D>(p, u, key, smem + L::kKeysOff + tile * L::T::kSlotBytes + (in_cta % kBlockKv) * kAtomBytes, sum);
     }
     if (u.active > 1) {
       float *parts = p.part_sums + (static_cast<int64_t>(u.run) * p.pairs + u.pair) * p.parts * kKeysPerCta + in_cta;

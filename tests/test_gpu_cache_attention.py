@@ -545,3 +545,52 @@ def test_large_values_of_unseen_keys(flint, oracle, L, S, window, sinks, lens):
     check_out(got, want, size, score, S, True, "large values")
     small = np.abs(want).max(-1) < 100
     assert np.linalg.norm(got[small] - want[small]) <= 5e-3 * np.linalg.norm(want[small])
+
+
+@pytest.mark.parametrize("H,Hk,L,S,D", [(6, 2, 1, 300, 64), (6, 2, 150, 400, 64), (4, 1, 33, 300, 128), (14, 2, 100, 350, 128), (8, 2, 200, 600, 64)])
+@pytest.mark.parametrize("is_bf16", [True, False])
+def test_weights_of_keys_that_every_query_scores_minus_infinity(flint, oracle, H, Hk, L, S, D, is_bf16):
+    """Such keys weigh nothing, with blocks of rows that are full and that are not (groups of 3 and 7; a last block's end)."""
+    F = flint
+    c = Cache(F, oracle, 71 + L, 2, H, Hk, L, S, D, is_bf16, [S, S - 30], spread=0.5)
+    c.bits["q"][..., 9] &= 0x7FFF  # positive
+    _, _, _, score = C.attention(c.value("q"), c.value("k"), c.value("v"), c.lens)
+    tiny = c.bits["q"][..., 9] == 0
+    c.bits["q"][..., 9][tiny] = 0x3C00
+    at = [0, 100, S - 31 - L // 2, S - 1 - L // 2]
+    for n in range(2):
+        for h in range(Hk):
+            for j in at:
+                put(c, "k", (n, h, j, 9), "-inf")
+    t = c.device()
+    w = dev(F, np.zeros((2, Hk, S), np.float32), F.DType.FLOAT)
+    F.attention_weights(t["q"], t["k"], t["v"], w, t["lens"], out=t["out"])
+    got, got_w = c.read(t["out"]), w.numpy()
+    F.synchronize()
+    want, weights, size, _ = C.attention(c.value("q"), c.value("k"), c.value("v"), c.lens)
+    assert (got_w[:, :, at] == 0).all()
+    tol = (2 * (D + 4) * 2.0 ** -23 * score.max() + 2.0 ** -20 + 2.0 ** -13 + (S + H // Hk * L) * 2.0 ** -23) * weights
+    assert (np.abs(got_w - weights) <= tol).all()
+    check_out(got, want, size, score, S, is_bf16, "beside them")
+
+
+@pytest.mark.parametrize("H,Hk,L,S,D", [(6, 2, 1, 300, 64), (6, 2, 150, 400, 64), (8, 2, 200, 600, 64)])
+@pytest.mark.parametrize("odd", ["nan", "inf"])
+def test_weights_beside_scores_without_a_softmax(flint, oracle, H, Hk, L, S, D, odd):
+    """A key that some queries score NaN or +inf takes these queries' weights with it, and no others: those of every key
+    they see, one that everything scores -inf among them."""
+    F = flint
+    c = Cache(F, oracle, 72 + L, 2, H, Hk, L, S, D, True, [S, S - 30], spread=0.5)
+    c.bits["q"][..., 9] = c.bits["q"][..., 9] & 0x7FFF | 0x3800  # positive
+    put(c, "k", (0, 0, S - 1 - L // 2, 9), odd)
+    for h in range(Hk):
+        put(c, "k", (0, h, 50, 9), "-inf")
+    t = c.device()
+    w = dev(F, np.zeros((2, Hk, S), np.float32), F.DType.FLOAT)
+    F.attention_weights(t["q"], t["k"], t["v"], w, t["lens"], out=t["out"])
+    got, got_w = c.read(t["out"]), w.numpy()
+    F.synchronize()
+    with np.errstate(invalid="ignore"):
+        want, weights, _, _ = C.attention(c.value("q"), c.value("k"), c.value("v"), c.lens)
+    assert np.array_equal(np.isnan(got_w), np.isnan(weights)) and np.isnan(weights[0, 0]).all() and not np.isnan(weights[0, 1:]).any()
+    assert np.array_equal(np.isnan(got), np.isnan(want)) and (got_w[0, 1:, 50] == 0).all()
