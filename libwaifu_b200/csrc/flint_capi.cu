@@ -6,6 +6,7 @@
 
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <atomic>
 #include <cstdlib>
 #include <cstring>
@@ -2485,29 +2486,62 @@ uint32_t *cache_counters() {
   return g_dev.cache_counters;
 }
 
-// Whether the bytes two views reach meet.
-bool views_overlap(const fl_tensor_view_impl_t &a, const fl_tensor_view_impl_t &b) {
-  auto end = [](const fl_tensor_view_impl_t &v) {
-    int64_t last = 0;
-    for (size_t i = 0; i < v.shape.size(); ++i) last += static_cast<int64_t>(v.shape[i] - 1) * v.stride[i];
-    return raw_ptr(v) + (last + 1) * dtype_size(v.data->dtype);
-  };
-  if (numel_of(a) == 0 || numel_of(b) == 0) return false;
-  return raw_ptr(a) < end(b) && raw_ptr(b) < end(a);
+// Whether numbers 0 <= z_i <= most_i give sum of each_i z_i = total, each_i descending and positive. The search takes the terms in turn, each
+// where the rest can still make up the difference: for strides that lie in one another two or three values a term. Past a bound on its
+// steps the answer is yes.
+struct Term {
+  int64_t each, most;
+};
+bool can_sum(const Term *terms, int count, int64_t total, int64_t reach, int *steps) {
+  if (total < 0 || total > reach) return false;
+  if (count == 0 || total == 0) return true;
+  if (--*steps < 0) return true;
+  const int64_t each = terms->each, rest = reach - each * terms->most;
+  const int64_t first = total > rest ? (total - rest + each - 1) / each : 0, last = std::min(terms->most, total / each);
+  for (int64_t z = first; z <= last; ++z) {
+    if (can_sum(terms + 1, count - 1, total - z * each, rest, steps)) return true;
+  }
+  return false;
 }
 
-// Whether two views have elements in common, as far as their ends tell: views that take turns in memory do not.
-bool views_share(const fl_tensor_view_impl_t &a, const fl_tensor_view_impl_t &b) {
-  if (!views_overlap(a, b)) return false;
-  if (raw_ptr(a) == raw_ptr(b)) return true;
-  auto holds = [](const fl_tensor_view_impl_t &dense, const fl_tensor_view_impl_t &other) {
+// Whether two views have a byte in common; views that take turns in memory do not.
+bool views_overlap(const fl_tensor_view_impl_t &a, const fl_tensor_view_impl_t &b) {
+  if (numel_of(a) == 0 || numel_of(b) == 0) return false;
+  auto last_byte = [](const fl_tensor_view_impl_t &v) {
     int64_t last = 0;
-    for (size_t i = 0; i < other.shape.size(); ++i) last += static_cast<int64_t>(other.shape[i] - 1) * other.stride[i];
-    const auto *from = raw_ptr(dense), *to = from + numel_of(dense) * dtype_size(dense.data->dtype);
-    const auto *first = raw_ptr(other), *end = first + last * dtype_size(other.data->dtype);
-    return is_contiguous(dense) && ((first >= from && first < to) || (end >= from && end < to));
+    for (size_t i = 0; i < v.shape.size(); ++i) last += static_cast<int64_t>(v.shape[i] - 1) * v.stride[i];
+    return (last + 1) * dtype_size(dtype_of(v)) - 1;
   };
-  return holds(a, b) || holds(b, a);
+  const int64_t a_last = last_byte(a), b_last = last_byte(b);
+  // a's byte at x is b's at distance + ..., so x and what is left of b behind its own add up to distance + b_last.
+  const int64_t distance = raw_ptr(b) - raw_ptr(a);
+  if (distance > a_last || distance + b_last < 0) return false;
+  std::vector<Term> terms{{1, dtype_size(dtype_of(a)) - 1 + dtype_size(dtype_of(b)) - 1}};
+  for (const fl_tensor_view_impl_t *v : {&a, &b}) {
+    for (size_t i = 0; i < v->shape.size(); ++i) {
+      if (v->shape[i] > 1 && v->stride[i] > 0) terms.push_back({v->stride[i] * dtype_size(dtype_of(*v)), v->shape[i] - 1});
+    }
+  }
+  std::sort(terms.begin(), terms.end(), [](const Term &x, const Term &y) { return x.each > y.each; });
+  size_t used = 0;
+  for (size_t i = 1; i < terms.size(); ++i) {  // (alike ones together)
+    if (terms[i].each == terms[used].each) {
+      terms[used].most += terms[i].most;
+    } else {
+      terms[++used] = terms[i];
+    }
+  }
+  int steps = 1 << 14;
+  return can_sum(terms.data(), static_cast<int>(used) + 1, distance + b_last, a_last + b_last, &steps);
+}
+
+// Whether a view reads and writes just where another does.
+bool same_view(const fl_tensor_view_impl_t &a, const fl_tensor_view_impl_t &b) {
+  if (raw_ptr(a) != raw_ptr(b) || a.shape != b.shape || dtype_of(a) != dtype_of(b)) return false;
+  for (size_t i = 0; i < a.shape.size(); ++i) {
+    if (a.shape[i] > 1 && a.stride[i] != b.stride[i]) return false;
+  }
+  return true;
 }
 
 void check_lens(const fl_tensor_view_impl_t &lens, int batch, const char *what) {
@@ -2578,7 +2612,7 @@ CacheAttentionArgs cache_attention_args(fl_operators_t operators, fl_tensor_view
   for (const auto &t : all) check_rows(*t.view, t.name);
   for (const auto &t : all) check_not_repeated(*t.view, t.name);
   for (int i = 0; i < 3; ++i) {
-    if (views_share(*all[i].view, out)) invalid(std::string("attention: out shares elements with ") + all[i].name);
+    if (views_overlap(*all[i].view, out)) invalid(std::string("attention: out shares elements with ") + all[i].name);
   }
   if (kv_lens_h) {
     const fl_tensor_view_impl_t &lens = deref(kv_lens_h);
@@ -2653,7 +2687,7 @@ int32_t fl_attention_shared_prefix(fl_operators_t operators, fl_tensor_view_t q,
     check_rows(pv, "the prefix's v");
     check_not_repeated(pk, "the prefix's k");
     check_not_repeated(pv, "the prefix's v");
-    if (views_share(pk, deref(out)) || views_share(pv, deref(out))) invalid("attention: out shares elements with the prefix");
+    if (views_overlap(pk, deref(out)) || views_overlap(pv, deref(out))) invalid("attention: out shares elements with the prefix");
     a.prefix_k = raw_ptr(pk);
     a.prefix_v = raw_ptr(pv);
     a.prefix_len = pk.shape[2];
@@ -2674,8 +2708,7 @@ int32_t fl_attention_weights(fl_operators_t operators, fl_tensor_view_t q, fl_te
     check_weights(in, a.batch, a.kv_heads, a.kv_len, "weights");
     check_weights(to, a.batch, a.kv_heads, a.kv_len, "weights_out");
     check_not_repeated(to, "weights_out");
-    const bool in_place = raw_ptr(in) == raw_ptr(to) && in.stride == to.stride;
-    if (!in_place && views_overlap(in, to)) invalid("attention: weights and weights_out overlap without being the same view");
+    if (!same_view(in, to) && views_overlap(in, to)) invalid("attention: weights and weights_out overlap without being the same view");
     a.weights_in = reinterpret_cast<const float *>(raw_ptr(in));
     a.weights_out = reinterpret_cast<float *>(raw_ptr(to));
     for (int i = 0; i < 2; ++i) {
@@ -2734,7 +2767,7 @@ int32_t fl_cache_evict(fl_operators_t operators, fl_tensor_view_t k_h, fl_tensor
     if (lens_out_h) {
       const fl_tensor_view_impl_t &lens = deref(lens_out_h);
       check_lens(lens, batch, "lens_out");
-      if (kv_lens_h && raw_ptr(lens) != raw_ptr(deref(kv_lens_h)) && views_overlap(lens, deref(kv_lens_h))) {
+      if (kv_lens_h && !same_view(lens, deref(kv_lens_h)) && views_overlap(lens, deref(kv_lens_h))) {
         invalid("eviction: lens_out overlaps kv_lens without being the same view");
       }
       a.lens_out = reinterpret_cast<int32_t *>(raw_ptr(lens));

@@ -114,3 +114,86 @@ def test_what_eviction_refuses(flint, no_device):
         assert refusal and words in message, (change.keys(), message)
     assert evict(k=at(F, (2, 2, 10, 20), bf), v=at(F, (2, 2, 10, 20), bf), ko=at(F, (2, 2, 6, 20), bf, address=far(0)), vo=at(F, (2, 2, 6, 20), bf, address=far(1)))[0]
     assert not evict(k=at(F, (2, 2, 10, 24), bf, (0, 0, 24, 1)))[0]  # read with their true strides: inputs may repeat
+
+
+def test_outputs_that_take_turns_in_memory(flint, no_device):
+    """A cache that keeps keys and values side by side, (N, S, 2, kv_heads, D), is taken for both; one element in common is not."""
+    F, (N, ops) = flint, no_device
+    L = F.lib()
+    bf, fl = F.DType.BFLOAT16, F.DType.FLOAT
+    far = lambda i: (i + 2) << 32  # noqa: E731
+    side = lambda address, i, rows=6: at(F, (2, 2, rows, 24), bf, (2 * 48 * rows, 24, 96, 1), address + int(96 * i))  # noqa: E731  (keys 0, values 1)
+    t = {"k": at(F, (2, 2, 10, 24), bf), "v": at(F, (2, 2, 10, 24), bf), "w": at(F, (2, 2, 10), fl), "lens": at(F, (2,), F.DType.INT32, address=far(8)),
+         "ko": at(F, (2, 2, 6, 24), bf, address=far(0)), "vo": at(F, (2, 2, 6, 24), bf, address=far(1)), "wo": at(F, (2, 2, 6), fl, address=far(2)),
+         "lo": at(F, (2,), F.DType.INT32, address=far(3)), "kept": at(F, (2, 2, 5), F.DType.INT32, address=far(4))}
+
+    def evict(**c):
+        u = {**t, **c}
+        return N.refused(L.fl_cache_evict, ops, u["k"], u["v"], u["w"], u["lens"], 5, 2, u["ko"], u["vo"], u["wo"], u["lo"], u["kept"])
+
+    assert not evict(ko=side(far(0), 0), vo=side(far(0), 1))[0]
+    refusal, message = evict(ko=side(far(0), 0), vo=side(far(0), 0.5))
+    assert refusal and "two outputs" in message
+    # Both caches in one allocation, sequence by sequence.
+    old = lambda i: at(F, (2, 2, 10, 24), bf, (4096, 240, 24, 1), far(0) + 1024 * i)  # noqa: E731
+    new = lambda i: at(F, (2, 2, 6, 24), bf, (4096, 144, 24, 1), far(0) + 2048 + 1024 * i)  # noqa: E731
+    assert not evict(k=old(0), v=old(1), ko=new(0), vo=new(1))[0]
+    refusal, message = evict(k=old(0), v=old(1), ko=new(0), vo=new(-1))
+    assert refusal and "overlaps k, v or weights" in message
+    # Weights of two steps that take turns, head by head.
+    step = lambda i: at(F, (2, 2, 10), fl, (40, 20, 1), far(5) + i)  # noqa: E731
+    q = operands(F, bf)
+    weights = lambda w, wo: N.refused(L.fl_attention_weights, ops, q["q"], q["k"], q["v"], q["lens"], w, wo, q["out"])  # noqa: E731
+    assert not weights(step(0), step(40))[0] and not weights(step(40), step(40))[0]
+    refusal, message = weights(step(0), step(36))
+    assert refusal and "overlap" in message
+    one = at(F, (1, 2, 10), fl, (20, 10, 1), far(5)), at(F, (1, 2, 10), fl, (0, 10, 1), far(5))  # the same, a stride that is never used apart
+    single = operands(F, bf, N=1)
+    assert not N.refused(L.fl_attention_weights, ops, single["q"], single["k"], single["v"], None, *one, single["out"])[0]
+
+
+def test_an_output_that_shares_elements_with_neither_view_whole(flint, no_device):
+    """Strided views that meet in the middle alone: the one's ends lie between the other's elements."""
+    F, (N, ops) = flint, no_device
+    bf = F.DType.BFLOAT16
+    t = operands(F, bf, N=3, H=2, Hk=2)
+    k = at(F, (3, 2, 10, 64), bf, (4096, 1024, 64, 1), 1 << 24)
+    for delta, shares in ((0, True), (128, True), (1280, False), (3 * 4096 * 2, False), (-2 * 4096 * 2 + 128, True), (-2 * 4096 * 2 - 128, False)):
+        out = at(F, (3, 2, 1, 64), bf, (4096, 1024, 64, 1), (1 << 24) + delta)
+        refusal, message = N.refused(F.lib().fl_attention_window, ops, t["q"], k, t["v"], None, 5, 0, out)
+        assert refusal == shares and (not shares or "shares elements with k" in message), (delta, message)
+
+
+def test_shared_elements_against_sets_of_them(flint, no_device):
+    """Random layouts: refused exactly where a set of the one view's elements meets a set of the other's."""
+    import random
+    import numpy as np
+    F, (N, ops) = flint, no_device
+    bf, D, rng = F.DType.BFLOAT16, 64, random.Random(4)
+
+    def layout(shape, gaps):
+        order, strides, step = [0, 1, 2], [0, 0, 0], D
+        rng.shuffle(order)
+        for d in order:
+            strides[d] = step + rng.choice(gaps)
+            step = strides[d] * shape[d]
+        return strides
+
+    def elements(shape, strides, start):
+        grid = sum(np.arange(n).reshape([-1 if i == j else 1 for j in range(4)]) * s for i, (n, s) in enumerate(zip((*shape, D), (*strides, 1))))
+        return set((grid + start).ravel().tolist())
+
+    seen = {True: 0, False: 0}
+    for _ in range(300):
+        n, hk, l, s = rng.randint(1, 3), rng.randint(1, 3), rng.randint(1, 4), rng.randint(1, 5)
+        out, keys = (n, hk, l), (n, hk, s)
+        so, sk = layout(out, [0, 64, 256, 960]), layout(keys, [0, 64, 64, 192, 1032]) if rng.random() < 0.7 else [8 * rng.randint(1, 60) for _ in range(3)]
+        start = 1 << 20
+        delta = 8 * rng.randint(-200, 600)
+        t = {"q": at(F, (*out, D), bf, address=1 << 40), "v": at(F, (*keys, D), bf, address=1 << 41),
+             "k": at(F, (*keys, D), bf, (*sk, 1), 2 * start), "out": at(F, (*out, D), bf, (*so, 1), 2 * (start + delta))}
+        refusal, message = N.refused(F.lib().fl_attention_window, ops, t["q"], t["k"], t["v"], None, 5, 0, t["out"])
+        shares = not elements(keys, sk, start).isdisjoint(elements(out, so, start + delta))
+        assert refusal == shares and (not shares or "shares elements with k" in message), (out, so, keys, sk, delta, message)
+        seen[shares] += 1
+    assert min(seen.values()) > 50
