@@ -2634,6 +2634,10 @@ CacheAttentionArgs cache_attention_args(fl_operators_t operators, fl_tensor_view
   return a;
 }
 
+void check_lens_apart(fl_tensor_view_t kv_lens, fl_tensor_view_t out) {
+  if (kv_lens && views_overlap(deref(kv_lens), deref(out))) invalid("attention: out shares elements with kv_lens");
+}
+
 int32_t run_cache_attention(CacheAttentionArgs &a) {
   require_kernels();
   check_earlier_kernel_status();
@@ -2663,6 +2667,7 @@ int32_t fl_attention_window(fl_operators_t operators, fl_tensor_view_t q, fl_ten
     // (a window or first keys beyond the cache's length hide nothing)
     a.window = window < a.kv_len ? window : a.kv_len;
     a.sinks = sinks < a.kv_len ? sinks : a.kv_len;
+    check_lens_apart(kv_lens, out);
     return run_cache_attention(a);
   });
 }
@@ -2688,6 +2693,7 @@ int32_t fl_attention_shared_prefix(fl_operators_t operators, fl_tensor_view_t q,
     check_not_repeated(pk, "the prefix's k");
     check_not_repeated(pv, "the prefix's v");
     if (views_overlap(pk, deref(out)) || views_overlap(pv, deref(out))) invalid("attention: out shares elements with the prefix");
+    check_lens_apart(kv_lens, out);
     a.prefix_k = raw_ptr(pk);
     a.prefix_v = raw_ptr(pv);
     a.prefix_len = pk.shape[2];
@@ -2709,6 +2715,13 @@ int32_t fl_attention_weights(fl_operators_t operators, fl_tensor_view_t q, fl_te
     check_weights(to, a.batch, a.kv_heads, a.kv_len, "weights_out");
     check_not_repeated(to, "weights_out");
     if (!same_view(in, to) && views_overlap(in, to)) invalid("attention: weights and weights_out overlap without being the same view");
+    check_lens_apart(kv_lens, out);
+    if (views_overlap(in, deref(out))) invalid("attention: out shares elements with weights");
+    // (In place it is memory that the caller reads as sums of weights, so nothing else.)
+    const struct { fl_tensor_view_t view; const char *name; } others[5] = {{out, "out"}, {q, "q"}, {k, "k"}, {v, "v"}, {kv_lens, "kv_lens"}};
+    for (int i = 0; i < (same_view(in, to) ? 1 : 5); ++i) {
+      if (others[i].view && views_overlap(to, deref(others[i].view))) invalid(std::string("attention: weights_out shares elements with ") + others[i].name);
+    }
     a.weights_in = reinterpret_cast<const float *>(raw_ptr(in));
     a.weights_out = reinterpret_cast<float *>(raw_ptr(to));
     for (int i = 0; i < 2; ++i) {
@@ -2790,6 +2803,7 @@ int32_t fl_cache_evict(fl_operators_t operators, fl_tensor_view_t k_h, fl_tensor
       for (const fl_tensor_view_impl_t *r : read) {
         if (views_overlap(*written[i], *r)) invalid("eviction: an output overlaps k, v or weights");
       }
+      if (kv_lens_h && i != 4 && views_overlap(*written[i], deref(kv_lens_h))) invalid("eviction: an output overlaps kv_lens");
       for (int j = i + 1; j < 5; ++j) {
         if (written[j] && views_overlap(*written[i], *written[j])) invalid("eviction: two outputs overlap");
       }

@@ -197,3 +197,38 @@ def test_shared_elements_against_sets_of_them(flint, no_device):
         assert refusal == shares and (not shares or "shares elements with k" in message), (out, so, keys, sk, delta, message)
         seen[shares] += 1
     assert min(seen.values()) > 50
+
+
+def test_every_output_is_compared_with_every_input(flint, no_device):
+    F, (N, ops) = flint, no_device
+    L = F.lib()
+    bf, fl, i32 = F.DType.BFLOAT16, F.DType.FLOAT, F.DType.INT32
+    far = lambda i: (i + 2) << 32  # noqa: E731
+    q = {name: at(F, (2, h, n, 64), bf, address=far(i)) for i, (name, h, n) in enumerate((("q", 4, 1), ("k", 2, 10), ("v", 2, 10), ("out", 4, 1)))}
+    q.update(lens=at(F, (2,), i32, address=far(4)), w=at(F, (2, 2, 10), fl, address=far(5)), wo=at(F, (2, 2, 10), fl, address=far(6)))
+    over = lambda x, shift=16: (at(F, (2, 4, 1, 64), bf, address=x + shift))  # noqa: E731
+    weights = lambda **c: N.refused(L.fl_attention_weights, ops, *[{**q, **c}[n] for n in ("q", "k", "v", "lens", "w", "wo", "out")])  # noqa: E731
+    window = lambda **c: N.refused(L.fl_attention_window, ops, *[{**q, **c}[n] for n in ("q", "k", "v", "lens")], 5, 0, {**q, **c}["out"])  # noqa: E731
+    assert not weights()[0] and not window()[0]
+    refusal, message = window(lens=at(F, (2,), i32, address=far(3) + 16))
+    assert refusal and "out shares elements with kv_lens" in message
+    refusal, message = weights(out=over(far(5)))
+    assert refusal and "out shares elements with weights" in message
+    for i, name in enumerate(("q", "k", "v", "out", "kv_lens")):
+        refusal, message = weights(wo=at(F, (2, 2, 10), fl, address=far(i) + 4))
+        assert refusal and f"weights_out shares elements with {name}" in message, (name, message)
+    assert not weights(lens=None, wo=at(F, (2, 2, 10), fl, address=far(4)))[0]
+    t = {"k": at(F, (2, 2, 10, 24), bf), "v": at(F, (2, 2, 10, 24), bf), "w": at(F, (2, 2, 10), fl), "lens": at(F, (2,), i32, address=far(8) + 16),
+         "ko": at(F, (2, 2, 6, 24), bf, address=far(0)), "vo": at(F, (2, 2, 6, 24), bf, address=far(1)), "wo": at(F, (2, 2, 6), fl, address=far(2)),
+         "lo": at(F, (2,), i32, address=far(3)), "kept": at(F, (2, 2, 5), i32, address=far(4))}
+
+    def evict(**c):
+        u = {**t, **c}
+        return N.refused(L.fl_cache_evict, ops, u["k"], u["v"], u["w"], u["lens"], 5, 2, u["ko"], u["vo"], u["wo"], u["lo"], u["kept"])
+
+    for lo in (t["lo"], t["lens"]):
+        assert not evict(lo=lo)[0]
+        for name, view in (("ko", at(F, (2, 2, 6, 24), bf, address=far(8))), ("vo", at(F, (2, 2, 6, 24), bf, address=far(8))),
+                           ("wo", at(F, (2, 2, 6), fl, address=far(8))), ("kept", at(F, (2, 2, 5), i32, address=far(8)))):
+            refusal, message = evict(lo=lo, **{name: view})
+            assert refusal and "an output overlaps kv_lens" in message, (name, message)
