@@ -2535,6 +2535,37 @@ bool views_overlap(const fl_tensor_view_impl_t &a, const fl_tensor_view_impl_t &
   return can_sum(terms.data(), static_cast<int>(used) + 1, distance + b_last, a_last + b_last, &steps);
 }
 
+// No two elements of a written operand lie in one place.
+void check_written(const fl_tensor_view_impl_t &v, const char *what) {
+  if (numel_of(v) == 0) return;
+  std::vector<Term> terms;
+  for (size_t i = 0; i < v.shape.size(); ++i) {
+    if (v.shape[i] > 1) terms.push_back({v.stride[i], v.shape[i] - 1});  // (strides of 0 have been refused)
+  }
+  std::sort(terms.begin(), terms.end(), [](const Term &x, const Term &y) { return x.each > y.each; });
+  int64_t reach = 0;
+  bool nested = true;
+  for (size_t i = terms.size(); i-- > 0;) {
+    nested = nested && terms[i].each > reach;
+    reach += terms[i].each * terms[i].most;
+  }
+  if (nested) return;
+  // Two index vectors whose difference is positive in dimension k and anything in the others, both moved to begin at zero.
+  for (size_t k = 0; k < terms.size(); ++k) {
+    std::vector<Term> apart = terms;
+    int64_t total = -terms[k].each, whole = 0;
+    for (size_t i = 0; i < terms.size(); ++i) {
+      if (i != k) total += terms[i].each * terms[i].most;
+      apart[i].most = i == k ? terms[i].most - 1 : 2 * terms[i].most;
+      whole += apart[i].each * apart[i].most;
+    }
+    int steps = 1 << 14;
+    if (can_sum(apart.data(), static_cast<int>(apart.size()), total, whole, &steps)) {
+      invalid(std::string(what) + " has two elements in one place");
+    }
+  }
+}
+
 // Whether a view reads and writes just where another does.
 bool same_view(const fl_tensor_view_impl_t &a, const fl_tensor_view_impl_t &b) {
   if (raw_ptr(a) != raw_ptr(b) || a.shape != b.shape || dtype_of(a) != dtype_of(b)) return false;
@@ -2611,6 +2642,7 @@ CacheAttentionArgs cache_attention_args(fl_operators_t operators, fl_tensor_view
   if (a.kv_len > kMaxCacheKeys) invalid("attention: more than 2^30 keys");
   for (const auto &t : all) check_rows(*t.view, t.name);
   for (const auto &t : all) check_not_repeated(*t.view, t.name);
+  check_written(out, "out");
   for (int i = 0; i < 3; ++i) {
     if (views_overlap(*all[i].view, out)) invalid(std::string("attention: out shares elements with ") + all[i].name);
   }
@@ -2714,6 +2746,7 @@ int32_t fl_attention_weights(fl_operators_t operators, fl_tensor_view_t q, fl_te
     check_weights(in, a.batch, a.kv_heads, a.kv_len, "weights");
     check_weights(to, a.batch, a.kv_heads, a.kv_len, "weights_out");
     check_not_repeated(to, "weights_out");
+    check_written(to, "weights_out");
     if (!same_view(in, to) && views_overlap(in, to)) invalid("attention: weights and weights_out overlap without being the same view");
     check_lens_apart(kv_lens, out);
     if (views_overlap(in, deref(out))) invalid("attention: out shares elements with weights");
@@ -2771,6 +2804,9 @@ int32_t fl_cache_evict(fl_operators_t operators, fl_tensor_view_t k_h, fl_tensor
     check_weights(weights, batch, kv_heads, kv_len, "weights");
     check_weights(weights_out, batch, kv_heads, out_len, "weights_out");
     check_not_repeated(weights_out, "weights_out");
+    check_written(k_out, "k_out");
+    check_written(v_out, "v_out");
+    check_written(weights_out, "weights_out");
     CacheEvictArgs a = {};
     if (kv_lens_h) {
       const fl_tensor_view_impl_t &lens = deref(kv_lens_h);

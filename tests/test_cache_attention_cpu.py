@@ -232,3 +232,32 @@ def test_every_output_is_compared_with_every_input(flint, no_device):
                            ("wo", at(F, (2, 2, 6), fl, address=far(8))), ("kept", at(F, (2, 2, 5), i32, address=far(8)))):
             refusal, message = evict(lo=lo, **{name: view})
             assert refusal and "an output overlaps kv_lens" in message, (name, message)
+
+
+def test_outputs_whose_own_elements_meet(flint, no_device):
+    """Strides that lead to one place by two ways are refused in what is written, taken in what is read."""
+    F, (N, ops) = flint, no_device
+    L = F.lib()
+    bf, fl = F.DType.BFLOAT16, F.DType.FLOAT
+    far = lambda i: (i + 2) << 32  # noqa: E731
+    t = operands(F, bf, N=3, H=4, Hk=2, L=5)
+    shape = (3, 4, 5, 64)
+    window = lambda out, k=t["k"]: N.refused(L.fl_attention_window, ops, t["q"], k, t["v"], None, 5, 0, out)  # noqa: E731
+    for strides, meets in [((1280, 320, 64, 1), False), ((1280, 64, 256, 1), False), ((64, 192, 768, 1), False), ((1280, 320, 56, 1), True),
+                           ((1280, 256, 64, 1), True), ((1280, 64, 64, 1), True), ((128, 1024, 192, 1), True), ((128, 2048, 320, 1), False),
+                           ((3 * 64, 3 * 2 * 5 * 64, 2 * 64, 1), True)]:
+        refusal, message = window(at(F, shape, bf, strides, far(3)))
+        assert refusal == meets and (not meets or "two elements in one place" in message), (strides, message)
+    assert not window(at(F, shape, bf, address=far(3)), at(F, (3, 2, 10, 64), bf, (640, 320, 8, 1)))[0]
+    w = lambda strides: at(F, (3, 2, 10), fl, strides, far(5))  # noqa: E731
+    for strides, meets in [((20, 10, 1), False), ((10, 30, 1), False), ((10, 10, 1), True), ((20, 9, 1), True)]:
+        refusal, message = N.refused(L.fl_attention_weights, ops, t["q"], t["k"], t["v"], None, at(F, (3, 2, 10), fl, address=far(6)), w(strides), at(F, shape, bf, address=far(3)))
+        assert refusal == meets and (not meets or "two elements in one place" in message), (strides, message)
+    e = {"k": at(F, (2, 2, 10, 24), bf), "v": at(F, (2, 2, 10, 24), bf), "w": at(F, (2, 2, 10), fl), "ko": at(F, (2, 2, 6, 24), bf, address=far(0)),
+         "vo": at(F, (2, 2, 6, 24), bf, address=far(1)), "wo": at(F, (2, 2, 6), fl, address=far(2))}
+    for name, view in [("ko", at(F, (2, 2, 6, 24), bf, (288, 136, 24, 1), far(0))), ("vo", at(F, (2, 2, 6, 24), bf, (288, 144, 16, 1), far(1))),
+                       ("wo", at(F, (2, 2, 6), fl, (12, 5, 1), far(2)))]:
+        u = {**e, name: view}
+        refusal, message = N.refused(L.fl_cache_evict, ops, u["k"], u["v"], u["w"], None, 5, 2, u["ko"], u["vo"], u["wo"], None, None)
+        assert refusal and "two elements in one place" in message, (name, message)
+    assert not N.refused(L.fl_cache_evict, ops, e["k"], e["v"], e["w"], None, 5, 2, e["ko"], e["vo"], e["wo"], None, None)[0]
