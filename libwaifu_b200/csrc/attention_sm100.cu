@@ -781,7 +781,7 @@ attention2_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       ok = __all_sync(0xffffffffu, mbar_wait(&t.s_full_bar[tile], j & 1, &abort_flag));
       if (!ok) break;
       tc_fence_after_sync();
-      softmax_block<D, false>(p.scale_log2, p.is_bf16, t_scores, t_out, j == 0, HideBehind{j * kBlockKv, common_last, key_last}, t.p_full_bar[tile], lane, &m_used, &l_run);
+      softmax_block<D, false>(p.scale_log2, p.is_bf16, 0.0f, t_scores, t_out, j == 0, HideBehind{j * kBlockKv, common_last, key_last}, t.p_full_bar[tile], lane, &m_used, &l_run);
     }
     // The last product.
     if (ok && my_blocks > 0) {
@@ -1025,7 +1025,7 @@ attention2_units_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
         if (!ok) break;
         s_phase ^= 1;
         tc_fence_after_sync();
-        softmax_block<D, false>(p.scale_log2, p.is_bf16, t_scores, t_out, j == 0, HideBehind{j * kBlockKv, common_last, key_last}, t.p_full_bar[tile], lane, &m_used, &l_run);
+        softmax_block<D, false>(p.scale_log2, p.is_bf16, 0.0f, t_scores, t_out, j == 0, HideBehind{j * kBlockKv, common_last, key_last}, t.p_full_bar[tile], lane, &m_used, &l_run);
       }
       // The last product.
       if (ok && my_blocks > 0) {

@@ -167,11 +167,12 @@ struct TileLayout {
 // Block j of the keys for one query (a lane's row of the tile): its scores from tensor memory, the running
 // maximum and sum, and the probabilities back into tensor memory, part by part. `hide(scores)` sets those of the
 // keys the row does not see to -inf; `first` is the tile's first block, whose output need not be rescaled.
+// The probabilities, their sum and the output are 2^shift times what they are relative to *m_used_io.
 // Where a seen score that is NaN or +inf has to make the row NaN (CARRY_NAN), the maximum carries it into the sum: the
 // cubic exponential does not.
 template <int D, bool CARRY_NAN, typename Hide>
-__device__ __forceinline__ void softmax_block(float scale_log2, int is_bf16, uint32_t t_scores, uint32_t t_out, bool first, Hide &&hide,
-                                              uint64_t *p_full_bar, uint32_t lane, float *m_used_io, float *l_run_io) {
+__device__ __forceinline__ void softmax_block(float scale_log2, int is_bf16, float shift, uint32_t t_scores, uint32_t t_out, bool first,
+                                              Hide &&hide, uint64_t *p_full_bar, uint32_t lane, float *m_used_io, float *l_run_io) {
   constexpr int kPParts = kPartsOf<D>;
   constexpr int kChunks = kBlockKv / 32;
   static_assert(kChunks == 4, "four chunks of scores pack into the first two");
@@ -214,7 +215,7 @@ __device__ __forceinline__ void softmax_block(float scale_log2, int is_bf16, uin
   const float m_sub = (m_used == -INFINITY) ? 0.0f : m_used;
   // The probabilities, packed in place: pair i of the row's keys becomes column i of its P
   // (a slot whose scores have been used by then).
-  const uint64_t scale2 = f2_pack(scale_log2, scale_log2), neg_m2 = f2_pack(-m_sub, -m_sub);
+  const uint64_t scale2 = f2_pack(scale_log2, scale_log2), neg_m2 = f2_pack(shift - m_sub, shift - m_sub);
   uint64_t sums[2] = {0, 0};  // (pairs of float32 zeros)
   auto emit = [&](auto bf16_tag, int part) {
     constexpr int kBf16 = decltype(bf16_tag)::value ? 1 : 0;

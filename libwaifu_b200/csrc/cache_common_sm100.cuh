@@ -37,6 +37,12 @@ struct Divisor {
   }
 };
 
+// Half probabilities are 2^7 times what they are relative to a row's maximum, and the row's sum and output with them. The maximum lags by
+// 2^8 at most (see the kernels), so the largest is 2^15; the least that does not round to zero is 2^-32 instead of 2^-25. A
+// million keys below 2^-25 have up to 3 % of a row's weight, below 2^-32 less than a half's rounding. (bfloat16 has float's range.)
+template <bool BF16>
+constexpr float kProbabilityShift = BF16 ? 0.0f : 7.0f;
+
 // Eight 32-bit values to 32-byte aligned memory: a whole sector from one lane.
 __device__ __forceinline__ void store_32_bytes(void *dst, uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t e, uint32_t f, uint32_t g,
                                                uint32_t h) {

@@ -444,7 +444,7 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
         }
       }
       // The output and the sum are relative to a maximum that follows the rows' own only when one has grown by more
-      // than 2^8: until then the exponentials stay below what every type here holds, and no lane has to know another's.
+      // than 2^8: until then the exponentials stay below what every type here holds (2^15 in half), and no lane has to know another's.
       bool grown = false;
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
@@ -475,7 +475,8 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
       uint32_t hi[NB][2], lo[NB][2];
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
-        const float s0 = m[n][0] == -INFINITY ? 0.0f : m[n][0], s1 = m[n][1] == -INFINITY ? 0.0f : m[n][1];
+        constexpr float kShift = kProbabilityShift<BF16>;
+        const float s0 = m[n][0] == -INFINITY ? 0.0f : m[n][0] - kShift, s1 = m[n][1] == -INFINITY ? 0.0f : m[n][1] - kShift;
 #pragma unroll
         for (int i = 0; i < 4; ++i) sc[n][i] = exp2_approx(sc[n][i] - ((i & 1) ? s1 : s0));
         l[n][0] += sc[n][0] + sc[n][2];
@@ -547,7 +548,7 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
       for (int i = 0; i < 2; ++i) {
 #pragma unroll
         for (int x = 4; x <= 16; x <<= 1) l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], x);
-        if (lane < 4) warp_sum[warp][n * 8 + my_row + i] = make_float2(m[n][i], l[n][i]);
+        if (lane < 4) warp_sum[warp][n * 8 + my_row + i] = make_float2(m[n][i] - kProbabilityShift<BF16>, l[n][i]);
       }
     }
     __syncwarp();  // (every lane has read its stage)

@@ -291,10 +291,10 @@ __device__ __noinline__ void patch_row(const TilesParams &p, int unit, int pos, 
   }
 }
 
-// A row's result, or its part of it.
+// A row's result, or its part of it: output and sum are relative to m.
 template <int D, bool BF16>
 __device__ __forceinline__ void finish_row(const TilesParams &p, const Unit &u, uint32_t t_out, int tile, int in_tile, int pos, int my_blocks,
-                                           bool ok, bool patch, float m_used, float l_run) {
+                                           bool ok, bool patch, float m, float l_run) {
   const int row = u.row0 + tile * p.tile_rows + in_tile;
   const bool live = in_tile < p.tile_rows && row < p.rows;
   const bool parts = p.over_batch || u.active > 1;
@@ -307,7 +307,7 @@ __device__ __forceinline__ void finish_row(const TilesParams &p, const Unit &u, 
   float *part_dst = p.part_out + (part_row0 + u.split * part_step) * D;
   const int64_t norm_at = static_cast<int64_t>(u.run) * p.norm_pitch + (u.pair * kTiles + tile) * kBlockQ + in_tile;
   // (a row whose every score is -inf has no softmax)
-  const float inv = empty ? 0.0f : (m_used == -INFINITY ? NAN : 1.0f / l_run);
+  const float inv = empty ? 0.0f : (m == -INFINITY ? NAN : 1.0f / l_run);
   if (ok) {
 #pragma unroll 1
     for (int c = 0; c < D / 32; ++c) {
@@ -336,14 +336,14 @@ __device__ __forceinline__ void finish_row(const TilesParams &p, const Unit &u, 
         }
       }
     }
-    if (live && patch && m_used != -INFINITY && l_run == l_run) {
+    if (live && patch && m != -INFINITY && l_run == l_run) {
       const uint16_t *q = p.q + row_offset(p, p.q_stride, u.head, u.seq, row);
-      patch_row<D, BF16>(p, u.index, pos, q, m_used, l_run, dst, parts ? part_dst : nullptr);
+      patch_row<D, BF16>(p, u.index, pos, q, m, l_run, dst, parts ? part_dst : nullptr);
     }
     // (the cubic's smallest exponentials keep a part that saw nothing from summing to zero)
-    if (live && parts) p.part_sum[part_row0 + u.split * part_step] = make_float2(m_used, m_used == -INFINITY && l_run == l_run ? 0.0f : l_run);
+    if (live && parts) p.part_sum[part_row0 + u.split * part_step] = make_float2(m, m == -INFINITY && l_run == l_run ? 0.0f : l_run);
     // (of a tile's empty places zeros, whose rows then weigh nothing)
-    if (p.row_norm != nullptr && (!live || !parts)) p.row_norm[norm_at] = live ? make_float2(m_used, inv) : make_float2(0.0f, 0.0f);
+    if (p.row_norm != nullptr && (!live || !parts)) p.row_norm[norm_at] = live ? make_float2(m, inv) : make_float2(0.0f, 0.0f);
   }
 }
 
@@ -486,7 +486,7 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         s_phase ^= 1;
         tc_fence_after_sync();
         const HideUnseen hide{edges.has(j), &t.walk[warp], j, pos};
-        softmax_block<D, true>(p.scale_log2, BF16, t_scores, t_out, j == 0, hide, t.p_full_bar[tile], lane, &m_used, &l_run);
+        softmax_block<D, true>(p.scale_log2, BF16, kProbabilityShift<BF16>, t_scores, t_out, j == 0, hide, t.p_full_bar[tile], lane, &m_used, &l_run);
       }
       // The last product.
       if (ok && my_blocks > 0) {
@@ -498,7 +498,7 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         asm volatile("" : "+r"(unit));  // (or what is worked out here would stay in registers from above)
         const Unit u(p, unit);
         const bool patch = *reinterpret_cast<volatile uint32_t *>(&t.patch_flag[count & 3]) == static_cast<uint32_t>(count);
-        finish_row<D, BF16>(p, u, t_out, tile, static_cast<int>(threadIdx.x % kBlockQ), pos, my_blocks, ok, patch, m_used, l_run);
+        finish_row<D, BF16>(p, u, t_out, tile, static_cast<int>(threadIdx.x % kBlockQ), pos, my_blocks, ok, patch, m_used - kProbabilityShift<BF16>, l_run);
         // The next unit's first product overwrites this output: it waits for probabilities that the tile's
         // four warps hand over only after these reads.
         tc_fence_before_sync();

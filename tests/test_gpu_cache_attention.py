@@ -594,3 +594,38 @@ def test_weights_beside_scores_without_a_softmax(flint, oracle, H, Hk, L, S, D, 
         want, weights, _, _ = C.attention(c.value("q"), c.value("k"), c.value("v"), c.lens)
     assert np.array_equal(np.isnan(got_w), np.isnan(weights)) and np.isnan(weights[0, 0]).all() and not np.isnan(weights[0, 1:]).any()
     assert np.array_equal(np.isnan(got), np.isnan(want)) and (got_w[0, 1:, 50] == 0).all()
+
+
+@pytest.mark.parametrize("S,P", [(65536, 0), (700, 65536)])
+@pytest.mark.parametrize("is_bf16", [True, False])
+def test_many_light_keys_beside_a_heavy_one(flint, oracle, S, P, is_bf16):
+    """One key takes nearly all of the weight, and each of the others about 2^-26, below what a half holds, in a walk that
+    is not divided: together they are seen in the columns where the heavy key's value is zero. A half weight is off by
+    2^-32 at most of the largest, times values below 1."""
+    F, H, L, D = flint, 64, 600, 64
+    c = Cache(F, oracle, 61, 1, H, 1, L, S, D, is_bf16, None, P=P, spread=0.1)
+    keys, values = ("prefix_k", "prefix_v") if P else ("k", "v")
+    c.bits["q"][..., 0] = oracle.narrow(np.array([16.0], np.float32), is_bf16)[0]
+    for name in {keys, "k"}:
+        c.bits[name][..., 0] = 0
+    c.bits[keys][0, 0, 5, 0] = oracle.narrow(np.array([9.0], np.float32), is_bf16)[0]
+    for name in {values, "v"}:
+        c.bits[name] = oracle.narrow(np.abs(np.random.default_rng(2).standard_normal(c.bits[name].shape)).clip(0, 1).astype(np.float32), is_bf16)
+    c.bits[values][0, 0, 5] = 0
+    t = c.device()
+    if P:
+        F.attention_shared_prefix(t["q"], t["prefix_k"], t["prefix_v"], t["k"], t["v"], None, t["out"])
+    else:
+        F.attention_window(t["q"], t["k"], t["v"], S, 0, None, t["out"])
+    got = c.read(t["out"])
+    F.synchronize()
+    u = 2.0 ** (-8 if is_bf16 else -11)
+    q, k, v = c.value("q")[0], c.value("k")[0, 0], c.value("v")[0, 0]
+    for h, i in ((0, 0), (3, 77), (63, 599), (20, 300)):
+        seen_k, seen_v = k[:i + S - L + 1], v[:i + S - L + 1]
+        if P:
+            seen_k, seen_v = np.concatenate([c.value("prefix_k")[0, 0], seen_k]), np.concatenate([c.value("prefix_v")[0, 0], seen_v])
+        want, _, size, score = C.attend(q[h, i], seen_k, seen_v)
+        n = len(seen_k)
+        tol = u * want + (u + 2 * (D + 4) * 2.0 ** -23 * score + 2.0 ** -12 + n * 2.0 ** -23) * size + (0.0 if is_bf16 else n * 2.0 ** -32 + 2.0 ** -25)
+        assert (want > 4e-4).all() and (np.abs(got[0, h, i] - want) <= tol).all(), (np.abs(got[0, h, i] - want) / tol).max()
