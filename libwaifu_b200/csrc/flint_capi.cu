@@ -2640,6 +2640,7 @@ CacheAttentionArgs cache_attention_args(fl_operators_t operators, fl_tensor_view
   }
   if (a.kv_len <= 0) invalid("attention: no keys");
   if (a.kv_len > kMaxCacheKeys) invalid("attention: more than 2^30 keys");
+  if (a.q_len > kMaxCacheKeys) invalid("attention: more than 2^30 queries");  // (their positions less a window stay in 32 bits)
   for (const auto &t : all) check_rows(*t.view, t.name);
   for (const auto &t : all) check_not_repeated(*t.view, t.name);
   check_written(out, "out");

@@ -261,3 +261,14 @@ def test_outputs_whose_own_elements_meet(flint, no_device):
         refusal, message = N.refused(L.fl_cache_evict, ops, u["k"], u["v"], u["w"], None, 5, 2, u["ko"], u["vo"], u["wo"], None, None)
         assert refusal and "two elements in one place" in message, (name, message)
     assert not N.refused(L.fl_cache_evict, ops, e["k"], e["v"], e["w"], None, 5, 2, e["ko"], e["vo"], e["wo"], None, None)[0]
+
+
+def test_more_positions_than_32_bits_hold(flint, no_device):
+    """A query's position less a window of 2^30 keys has to be an int: 2^30 queries at most, and as many keys."""
+    F, (N, ops) = flint, no_device
+    bf = F.DType.BFLOAT16
+    kv = at(F, (1, 1, 1 << 30, 64), bf, (64, 64, 8, 1))
+    for queries in (1 << 30, (1 << 30) + 1):
+        q, out = (at(F, (1, 1, queries, 64), bf, (64, 64, step, 1), address=(i + 1) << 42) for i, step in enumerate((8, 64)))
+        refusal, message = N.refused(F.lib().fl_attention_window, ops, q, kv, kv, None, 1 << 30, 0, out)
+        assert refusal == (queries > 1 << 30) and (not refusal or "more than 2^30 queries" in message), message
