@@ -397,14 +397,19 @@ FLAPI int32_t fl_qk_norm_rope(fl_tensor_view_t qkv, fl_tensor_view_t q_weight, f
  * q and out (N, heads, L, D), k and v (N, kv_heads, S, D) with kv_heads dividing heads, <float16> or
  * <bfloat16>, one type; D 64 or 128. The last dimension is contiguous, the other strides are free (a
  * (N, S, kv_heads, D) cache transposed is taken as it is) but multiples of 8 elements, and every operand
- * starts on a 16-byte boundary; none repeats a dimension, and out shares no element with the others. S is the cache's room: sequence n holds
- * the first kv_lens[n] keys of it, kv_lens <int32>(N) on the device (a value below 0 or above S counts as
+ * starts on a 16-byte boundary; none repeats a dimension, no two elements of an output lie in one place,
+ * and out shares none with the others, kv_lens among them. S is the cache's room: sequence n holds the
+ * first kv_lens[n] keys of it, kv_lens <int32>(N) on the device (a value below 0 or above S counts as
  * the nearer of the two), or all S where kv_lens is NULL. Query i sits at position p = i + kv_lens[n] - L
  * (the queries' own keys are in the cache already) and sees keys 0 .. p as each entry point says; a query that
  * sees none (p < 0) gets zeros. Scores are scaled by 1 / sqrt(D); maximum, sum and output are held in float
- * and out is rounded once. Keys that no query of a sequence sees may hold anything, infinities and NaN
- * among it; in a key that some see they reach the queries that see it and no others. Lengths are read on
- * the device: no call waits for the GPU. These entry points have no counterpart in the reference. */
+ * and out is rounded once. The softmax's weights are rounded to the operands' type before they meet the
+ * values where there are many rows to a key-value head (heads / kv_heads times L: 17, with the keys' weights
+ * 64; over a shared prefix the batch's together), and enter as two such numbers each below that. Keys that
+ * no query of a sequence sees may hold anything, infinities and NaN among it; in a key that some see they
+ * reach the queries that see it and no others (an infinite value whose weight rounds to zero as a NaN). At
+ * most 2^30 keys, and 2^30 queries a sequence. Lengths are read on the device: no call waits for the GPU.
+ * These entry points have no counterpart in the reference. */
 
 /* A sliding window: query p sees key j <= p if j > p - window or j < sinks (the first keys, which stay
  * visible however far the window has moved). window >= 1 (S or more: no window), sinks >= 0. */
@@ -414,7 +419,9 @@ FLAPI int32_t fl_attention_window(fl_operators_t operators, fl_tensor_view_t q, 
 /* A batch whose sequences share their beginning (a system prompt, a document, the prompt of several
  * samples): prefix_k and prefix_v (1, kv_heads, P, D), strides as k's, hold it once; k, v and kv_lens each
  * sequence's own keys behind it. Every query sees all P keys of the prefix and its own sequence's keys 0 .. p
- * (none for p < 0). Short queries of the whole batch walk the prefix together, in one pass over its keys. */
+ * (none for p < 0). Sequences of up to 16 rows to a key-value head (heads / kv_heads times L) walk the prefix
+ * together: its keys are read once for up to 256 rows of the batch. Longer ones walk it each for itself, 256
+ * rows at a time (where heads / kv_heads is above 128 together again, 16 rows at a time). */
 FLAPI int32_t fl_attention_shared_prefix(fl_operators_t operators, fl_tensor_view_t q, fl_tensor_view_t prefix_k,
                                          fl_tensor_view_t prefix_v, fl_tensor_view_t k, fl_tensor_view_t v,
                                          fl_tensor_view_t kv_lens, fl_tensor_view_t out);
@@ -423,8 +430,8 @@ FLAPI int32_t fl_attention_shared_prefix(fl_operators_t operators, fl_tensor_vie
  *   weights_out[n, h, j] = weights[n, h, j] + the sum, over the query heads that share key-value head h and
  *                          the L queries, of the softmax weight of key j (0 where it is not seen)
  * weights and weights_out <float>(N, kv_heads, S), the last dimension contiguous; the same view, or views
- * that do not overlap. Keys past kv_lens[n] take their weights over unchanged. The sums are taken in a fixed
- * order. L >= 1. */
+ * without an element in common; neither shares one with out, nor weights_out with q, k, v or kv_lens. Keys
+ * past kv_lens[n] take their weights over unchanged. The sums are taken in a fixed order. L >= 1. */
 FLAPI int32_t fl_attention_weights(fl_operators_t operators, fl_tensor_view_t q, fl_tensor_view_t k, fl_tensor_view_t v,
                                    fl_tensor_view_t kv_lens, fl_tensor_view_t weights, fl_tensor_view_t weights_out,
                                    fl_tensor_view_t out);
@@ -436,8 +443,9 @@ FLAPI int32_t fl_attention_weights(fl_operators_t operators, fl_tensor_view_t q,
  * <float>(N, kv_heads, room), their positions to kept <int32>(N, kv_heads, keep), -1 past the last (NULL: not
  * wanted); min(kv_lens[n], keep) to lens_out <int32>(N), which may be kv_lens (NULL only without kv_lens).
  * Rows of k_out and v_out past the new length are left as they were; weights there become 0, as new keys
- * start. D is a multiple of 8 here; strides and alignment as above, k and v may repeat dimensions. The outputs overlap neither the
- * inputs nor each other: a program with many layers keeps one cache to spare and takes turns. */
+ * start. D is a multiple of 8 here; strides and alignment as above, k and v may repeat dimensions. The outputs
+ * share no element with the inputs, kv_lens among them, nor with each other (keys and values may lie side by
+ * side): a program with many layers keeps one cache to spare and takes turns. */
 FLAPI int32_t fl_cache_evict(fl_operators_t operators, fl_tensor_view_t k, fl_tensor_view_t v, fl_tensor_view_t weights,
                              fl_tensor_view_t kv_lens, int32_t keep, int32_t recent, fl_tensor_view_t k_out, fl_tensor_view_t v_out,
                              fl_tensor_view_t weights_out, fl_tensor_view_t lens_out, fl_tensor_view_t kept);

@@ -13,8 +13,8 @@
 
 namespace flsm100 {
 
-
-// Division by a number that the host knows, of numbers below 2^31: with 2^s >= d > 2^(s - 1) and m = ceil(2^(32 + s) / d) - 2^32 the
+// Division by a number that the host knows, of numbers below 2^31, by a multiplication (Granlund and Montgomery's division by invariant
+// integers): with 2^s >= d > 2^(s - 1) and m = ceil(2^(32 + s) / d) - 2^32 the
 // quotient is (n m / 2^32 + n) / 2^s, rounded down twice. A unit's place takes a dozen divisions, which at some 40
 // instructions each were a microsecond and more at the beginning of a kernel.
 struct Divisor {

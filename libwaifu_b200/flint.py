@@ -725,8 +725,8 @@ def attention_window(q: Tensor, k: Tensor, v: Tensor, window: int, sinks: int = 
 def attention_shared_prefix(q: Tensor, prefix_k: Tensor, prefix_v: Tensor, k: Tensor, v: Tensor,
                             kv_lens: Optional[Tensor] = None, out: Optional[Tensor] = None) -> Tensor:
     """Attention of a batch whose sequences share their beginning: every query sees all of prefix_k and
-    prefix_v (1, kv_heads, P, D), which short queries walk together, and its own sequence's keys as in
-    attention_window without a window."""
+    prefix_v (1, kv_heads, P, D), which sequences of up to 16 rows to a key-value head (heads / kv_heads times L)
+    walk together, and its own sequence's keys as in attention_window without a window."""
     if out is None:
         out = Tensor.empty(tuple(q.shape), q.dtype)
     check(lib().fl_attention_shared_prefix(operators(), q.raw(), prefix_k.raw(), prefix_v.raw(), k.raw(), v.raw(),

@@ -629,3 +629,37 @@ def test_many_light_keys_beside_a_heavy_one(flint, oracle, S, P, is_bf16):
         n = len(seen_k)
         tol = u * want + (u + 2 * (D + 4) * 2.0 ** -23 * score + 2.0 ** -12 + n * 2.0 ** -23) * size + (0.0 if is_bf16 else n * 2.0 ** -32 + 2.0 ** -25)
         assert (want > 4e-4).all() and (np.abs(got[0, h, i] - want) <= tol).all(), (np.abs(got[0, h, i] - want) / tol).max()
+
+
+@pytest.mark.parametrize("N,H,Hk,L,S,D,P,lens", [
+    (5, 17, 1, 1, 40, 64, 300, [40, 0, 7, 33, 12]),
+    (6, 8, 2, 5, 70, 128, 700, [70, 4, 5, 0, 61, 33]),
+    (4, 16, 2, 5, 90, 64, 515, [90, 90, 3, 64]),
+    (3, 127, 1, 1, 50, 128, 260, [50, 1, 0]),
+    (3, 8, 2, 16, 64, 64, 1000, [64, 15, 16]),
+])
+@pytest.mark.parametrize("is_bf16,tokens", [(True, True), (False, False)])
+def test_a_few_tokens_of_several_sequences_behind_a_prefix(flint, oracle, N, H, Hk, L, S, D, P, lens, is_bf16, tokens):
+    """17 to 127 rows to a key-value head: a speculated step, or many query heads to one of keys."""
+    test_shared_prefix(flint, oracle, N, H, Hk, L, S, D, P, lens, is_bf16, tokens)
+
+
+def test_eviction_into_a_cache_with_keys_beside_values(flint, oracle):
+    """(N, room, 2, kv_heads, D): the outputs take turns in memory, and rows past the new length stay as they were."""
+    F, N, Hk, S, D, keep, recent, room = flint, 2, 3, 700, 64, 333, 30, 400
+    rng = np.random.default_rng(8)
+    k, v = (rng.integers(0, 2 ** 16, (N, Hk, S, D), dtype=np.uint16) for _ in range(2))
+    w, lens, bf = rng.random((N, Hk, S)).astype(np.float32), [700, 250], F.DType.BFLOAT16
+    store = dev(F, np.full((N, room, 2, Hk, D), 0xABCD, np.uint16), bf)
+    ko, vo = (store.view_as((N, Hk, room, D), (room * 2 * Hk * D, D, 2 * Hk * D, 1), i * Hk * D) for i in range(2))
+    kept = dev(F, np.zeros((N, Hk, keep), np.int32), F.DType.INT32)
+    _, _, wo, lo = F.cache_evict(dev(F, k, bf), dev(F, v, bf), dev(F, w, F.DType.FLOAT), keep, recent, dev(F, np.asarray(lens, np.int32), F.DType.INT32), ko, vo, kept=kept)
+    got, want = store.numpy(), C.evict(w, lens, keep, recent)
+    F.synchronize()
+    assert np.array_equal(kept.numpy(), want) and np.array_equal(lo.numpy(), [333, 250])
+    for n in range(N):
+        for h in range(Hk):
+            at = want[n, h][want[n, h] >= 0]
+            for i, source in enumerate((k, v)):
+                assert np.array_equal(got[n, :len(at), i, h], source[n, h, at]) and (got[n, len(at):, i, h] == 0xABCD).all()
+            assert np.array_equal(wo.numpy()[n, h, :len(at)], w[n, h, at])
