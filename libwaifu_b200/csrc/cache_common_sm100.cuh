@@ -112,6 +112,7 @@ __device__ __forceinline__ uint32_t nonfinite_halves(uint32_t w) {
   constexpr uint32_t kExponent = BF16 ? 0x7F807F80u : 0x7C007C00u;
   return __vcmpeq2(w & kExponent, kExponent);
 }
+
 // Zeros (of either sign) go on as such, through eight finite values: zero times an infinity or a NaN is a NaN, which stays.
 template <bool BF16>
 __device__ __forceinline__ uint32_t probe_nonfinite(uint4 w, uint32_t zeros) {
@@ -126,6 +127,7 @@ __device__ __forceinline__ uint32_t probe_nonfinite(uint4 w, uint32_t zeros) {
   }
   return zeros;
 }
+
 template <bool BF16>
 __device__ __forceinline__ uint4 without_nonfinite(uint4 w) {
   return make_uint4(w.x & ~nonfinite_halves<BF16>(w.x), w.y & ~nonfinite_halves<BF16>(w.y), w.z & ~nonfinite_halves<BF16>(w.z),
