@@ -247,46 +247,57 @@ struct TooLarge {
   }
 };
 
-// Adds what a row sees of the values that were taken out of its blocks, eight columns at a time: rare, and as slow as it is plain.
+// Adds what a row sees of the values that were taken out of its blocks: rare, and as slow as it is plain.
 template <int D, bool BF16>
 __device__ __noinline__ void patch_row(const TilesParams &p, int unit, int pos, const uint16_t *q, float m, float l, uint16_t *out, float *part) {
   const Unit u(p, unit);
-  for (int c = 0; c < D; c += 8) {
-    float sum[8] = {};
-    bool found = false;
-    for (int j = 0; j < u.walk.count; ++j) {
-      if (!u.walk.dirty.has(j)) continue;
-      for (int x = u.walk.place0(j); x < u.walk.place0(j) + kBlockKv; ++x) {
-        const int key = u.walk.key_at(x);
-        if (u.walk.hidden(x) || !u.walk.mixed(x) || key > pos || !(key > pos - p.window || key < p.sinks)) continue;
-        const uint4 v = *reinterpret_cast<const uint4 *>(p.v + u.seq * p.v_stride[0] + u.head * p.v_stride[1] + key * p.v_stride[2] + c);
-        if (!TooLarge<BF16>::any(v)) continue;
-        found = true;
-        const uint16_t *k = p.k + u.seq * p.k_stride[0] + u.head * p.k_stride[1] + key * p.k_stride[2];
-        float s = 0.0f;
-        for (int d = 0; d < D; d += 2) {
-          const float2 a = widen_pair<BF16>(*reinterpret_cast<const uint32_t *>(q + d)), b = widen_pair<BF16>(*reinterpret_cast<const uint32_t *>(k + d));
-          s = fmaf(a.x, b.x, fmaf(a.y, b.y, s));
-        }
-        const float w = exp2f(s * p.scale_log2 - m);
-        const uint32_t pairs[4] = {v.x, v.y, v.z, v.w};
+  auto pieces_of = [](const uint16_t *row) { return reinterpret_cast<const uint4 *>(row); };  // eight values each
+  float sum[D];
+#pragma unroll
+  for (int d = 0; d < D; ++d) sum[d] = 0.0f;
+  for (int j = 0; j < u.walk.count; ++j) {
+    if (!u.walk.dirty.has(j)) continue;
+    for (int x = u.walk.place0(j); x < u.walk.place0(j) + kBlockKv; ++x) {
+      const int key = u.walk.key_at(x);
+      if (u.walk.hidden(x) || !u.walk.mixed(x) || key > pos || !(key > pos - p.window || key < p.sinks)) continue;
+      const uint4 *v = pieces_of(p.v + u.seq * p.v_stride[0] + u.head * p.v_stride[1] + key * p.v_stride[2]);
+      bool found = false;
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) found |= TooLarge<BF16>::any(v[c]);
+      if (!found) continue;
+      const uint4 *k = pieces_of(p.k + u.seq * p.k_stride[0] + u.head * p.k_stride[1] + key * p.k_stride[2]);
+      float s = 0.0f;
+#pragma unroll 4
+      for (int c = 0; c < D / 8; ++c) {
+        const uint4 a = pieces_of(q)[c], b = k[c];
+        const uint32_t as[4] = {a.x, a.y, a.z, a.w}, bs[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint32_t large = TooLarge<BF16>::halves(pairs[i]);
-          const float2 y = widen_pair<BF16>(pairs[i]);
-          if (large & 0xFFFFu) sum[2 * i] += w * y.x;
-          if (large >> 16) sum[2 * i + 1] += w * y.y;
+          const float2 y = widen_pair<BF16>(as[i]), z = widen_pair<BF16>(bs[i]);
+          s = fmaf(y.x, z.x, fmaf(y.y, z.y, s));
+        }
+      }
+      const float w = exp2f(s * p.scale_log2 - m);
+#pragma unroll 1
+      for (int c = 0; c < D / 8; ++c) {
+        const uint4 y = v[c];
+        const uint32_t ys[4] = {y.x, y.y, y.z, y.w};
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t large = TooLarge<BF16>::halves(ys[i]);
+          const float2 z = widen_pair<BF16>(ys[i]);
+          if (large & 0xFFFFu) sum[c * 8 + 2 * i] += w * z.x;
+          if (large >> 16) sum[c * 8 + 2 * i + 1] += w * z.y;
         }
       }
     }
-    if (!found) continue;
-    for (int i = 0; i < 8; ++i) {
-      if (sum[i] == 0.0f) continue;
-      if (part != nullptr) {
-        part[c + i] += sum[i];
-      } else {
-        out[c + i] = static_cast<uint16_t>(pack_pair<BF16>(widen_pair<BF16>(out[c + i]).x + sum[i] / l, 0.0f));
-      }
+  }
+#pragma unroll 1
+  for (int d = 0; d < D; ++d) {
+    if (sum[d] == 0.0f) continue;
+    if (part != nullptr) {
+      part[d] += sum[d];
+    } else {
+      out[d] = static_cast<uint16_t>(pack_pair<BF16>(widen_pair<BF16>(out[d]).x + sum[d] / l, 0.0f));
     }
   }
 }
